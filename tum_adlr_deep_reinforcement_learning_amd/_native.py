@@ -40,7 +40,9 @@ def needs_build():
     return any(os.path.getmtime(s) > t for s in SOURCES if os.path.exists(s))
 
 
-EXTRA_FLAGS = ["-fno-slp-vectorize"]  # packed-f32 pairing costs register moves here
+# -fno-slp-vectorize: packed-f32 pairing costs register moves here.  -packed-fp32-ops: no v_pk_{add,mul,fma}_f32 at
+# all (some of their forms are unreliable on this hardware; the host pass warns that it does not know the feature)
+EXTRA_FLAGS = ["-fno-slp-vectorize", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
 @contextlib.contextmanager
