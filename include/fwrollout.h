@@ -180,6 +180,71 @@ int fw_collect_policy(const fw_mlp_policy* p, const fw_collect_io* io, void* str
 int fw_vecnorm_pending_update(const double* pend, int64_t stride, int32_t cnt, int32_t d, int32_t has_ret,
                               double* rms, double* merged, void* stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * Operators of a policy with memory (ABI 13; no counterpart in the reference, whose policies are
+ * memoryless): linear attention with a decay per head over rollout columns, its single-token form
+ * for the collect step, and group norm with an activation.  Tensors hold float32, bfloat16 or
+ * float16 (FW_DT_*); states, statistics and sums are float32 or wider.
+ * --------------------------------------------------------------------------------------------- */
+#define FW_DT_F32 0
+#define FW_DT_BF16 1
+#define FW_DT_F16 2
+
+/* One [T][N][H][D] operand: element strides of T, N and H (any sign or order; 0 broadcasts an
+ * input), unit stride in D. */
+typedef struct fw_seq_tensor {
+  void* p;
+  int64_t st, sn, sh;
+} fw_seq_tensor;
+
+/* Linear attention with a decay per head.  Per sequence n and head h, g = exp(log_decay[h]):
+ *   S_t = (starts[t][n] ? 0 : g S_{t-1}) + k_t v_t^T        S_{-1} = state_in (NULL: zeros)
+ *   out_t = S_t^T q_t                                       state_out = S_{len-1}
+ * for t < len = clamp(lengths[n], 0, T) (NULL: T); out rows t >= len are written as zeros.
+ * state_in / state_out: float [N][H][Dk][Dv], contiguous; they may be the same buffer.
+ * log_decay: float [H] (<= 0 for a decay).  starts: uint8 with element strides, or NULL.
+ * Backward (fw_linattn_backward): given dout and dstate (the gradient of state_out, NULL: zeros) writes
+ * dq, dk, dv (rows t >= len: zeros) and dstate_in (may be NULL); q, k, v are read again, no state is
+ * kept from the forward call.  Limits: 1 <= Dk, Dv <= 128.  A non-finite input reaches exactly the
+ * outputs the recurrence would let it reach; there it comes out as an infinity or a NaN.
+ * workspace: fw_linattn_workspace_bytes(...) bytes of device memory (may be 0), used on `stream`. */
+typedef struct fw_linattn {
+  int64_t T, N;
+  int32_t H, Dk, Dv, dtype;
+  fw_seq_tensor q, k, v, out;
+  const float* log_decay;
+  const uint8_t* starts;
+  int64_t starts_st, starts_sn;
+  const int32_t* lengths;
+  const float* state_in;
+  float* state_out;
+  fw_seq_tensor dout, dq, dk, dv;
+  const float* dstate;
+  float* dstate_in;
+  void* workspace;
+  size_t workspace_bytes;
+} fw_linattn;
+size_t fw_linattn_workspace_bytes(int64_t T, int64_t N, int32_t H, int32_t Dk, int32_t Dv, int32_t backward);
+int fw_linattn_forward(const fw_linattn* a, void* stream);
+int fw_linattn_backward(const fw_linattn* a, void* stream);
+
+/* The recurrent form for one token per sequence (the same recurrence with T = 1):
+ *   state_out = (starts[n] ? 0 : g state) + k v^T,  out = state_out^T q
+ * q, k [N][H][Dk], v, out [N][H][Dv] with element strides (the st fields are not read); state, state_out
+ * float [N][H][Dk][Dv] contiguous, 16-byte aligned; state_out == state updates in place, any other overlap
+ * is not allowed.  starts: uint8 with element stride starts_sn, or NULL.  Limits as fw_linattn. */
+typedef struct fw_linattn_token {
+  int64_t N;
+  int32_t H, Dk, Dv, dtype;
+  fw_seq_tensor q, k, v, out;
+  const float* log_decay;
+  const uint8_t* starts;
+  int64_t starts_sn;
+  const float* state;
+  float* state_out;
+} fw_linattn_token;
+int fw_linattn_step(const fw_linattn_token* a, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

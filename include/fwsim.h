@@ -36,7 +36,7 @@
 extern "C" {
 #endif
 
-#define FWSIM_ABI_VERSION 12
+#define FWSIM_ABI_VERSION 13
 
 /* ---- error codes ---------------------------------------------------------- */
 #define FW_OK 0

@@ -17,12 +17,12 @@ LIB_DIR = os.path.join(PKG, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libfwsim.so")
 HEADER = os.path.join(ROOT, "include", "fwsim.h")
 HEADERS = [HEADER, os.path.join(ROOT, "include", "fwrollout.h")]
-UNITS = [os.path.join(CSRC, "fw_kernels.hip"), os.path.join(CSRC, "fw_rollout.hip")]
-SOURCES = UNITS + [os.path.join(CSRC, "fw_device.hpp"), os.path.join(CSRC, "fw_quad.hpp"), os.path.join(CSRC, "fw_stats.hpp"), os.path.join(CSRC, "fw_x8_consts.inc")] + HEADERS
+UNITS = [os.path.join(CSRC, f) for f in ("fw_kernels.hip", "fw_rollout.hip", "fw_sequence.hip")]
+SOURCES = UNITS + [os.path.join(CSRC, "fw_seq_common.hpp"), os.path.join(CSRC, "fw_device.hpp"), os.path.join(CSRC, "fw_quad.hpp"), os.path.join(CSRC, "fw_stats.hpp"), os.path.join(CSRC, "fw_x8_consts.inc")] + HEADERS
 ARCH = os.environ.get("FWSIM_ARCH", "gfx950")
 
 _lib = None
-ABI_VERSION = 12  # include/fwsim.h FWSIM_ABI_VERSION
+ABI_VERSION = 13  # include/fwsim.h FWSIM_ABI_VERSION
 
 
 class FwError(RuntimeError):
@@ -71,7 +71,7 @@ def build(force=False, verbose=False, out=None, extra=None):
     """Compile csrc/*.hip into lib/libfwsim.so (cross-compiles without a GPU).
 
     fw_kernels.hip is compiled as N_PARTS translation units in parallel (the step kernels' template
-    instances dominate the compile time), then linked with fw_rollout.hip.  Holds a file lock around
+    instances dominate the compile time), then linked with the other units.  Holds a file lock around
     the staleness check and the compile, and writes through per-process temporary files, so parallel
     callers never see a partial library."""
     out = out or LIB_PATH
@@ -157,6 +157,10 @@ SIGNATURES = {
     "fw_vecnorm_merge_update": (_c.c_int, [_vp, _i32, _i32, _i32, _vp, _vp, _vp]),
     "fw_collect_policy": (_c.c_int, [_vp, _vp, _vp]),
     "fw_vecnorm_pending_update": (_c.c_int, [_vp, _i64, _i32, _i32, _i32, _vp, _vp, _vp]),
+    "fw_linattn_workspace_bytes": (_c.c_size_t, [_i64, _i64, _i32, _i32, _i32, _i32]),
+    "fw_linattn_forward": (_c.c_int, [_vp, _vp]),
+    "fw_linattn_backward": (_c.c_int, [_vp, _vp]),
+    "fw_linattn_step": (_c.c_int, [_vp, _vp]),
 }
 
 
@@ -190,6 +194,25 @@ class FwCollectIO(ctypes.Structure):  # include/fwrollout.h fw_collect_io
                 ("act_rows", _vp), ("val_rows", _vp), ("logp_rows", _vp), ("rew_rows", _vp), ("start_rows", _vp),
                 ("n", _i64), ("pend", _vp), ("pend_stride", _i64), ("pend_cnt", _i32), ("has_ret", _i32),
                 ("merged", _vp), ("rms_prev", _vp)]
+
+
+class FwSeqTensor(ctypes.Structure):  # include/fwrollout.h fw_seq_tensor
+    _fields_ = [("p", _vp), ("st", _i64), ("sn", _i64), ("sh", _i64)]
+
+
+class FwLinattn(ctypes.Structure):  # include/fwrollout.h fw_linattn
+    _fields_ = [("T", _i64), ("N", _i64), ("H", _i32), ("Dk", _i32), ("Dv", _i32), ("dtype", _i32)] + \
+               [(k, FwSeqTensor) for k in ("q", "k", "v", "out")] + \
+               [("log_decay", _vp), ("starts", _vp), ("starts_st", _i64), ("starts_sn", _i64), ("lengths", _vp),
+                ("state_in", _vp), ("state_out", _vp)] + \
+               [(k, FwSeqTensor) for k in ("dout", "dq", "dk", "dv")] + \
+               [("dstate", _vp), ("dstate_in", _vp), ("workspace", _vp), ("workspace_bytes", _c.c_size_t)]
+
+
+class FwLinattnToken(ctypes.Structure):  # include/fwrollout.h fw_linattn_token
+    _fields_ = [("N", _i64), ("H", _i32), ("Dk", _i32), ("Dv", _i32), ("dtype", _i32)] + \
+               [(k, FwSeqTensor) for k in ("q", "k", "v", "out")] + \
+               [("log_decay", _vp), ("starts", _vp), ("starts_sn", _i64), ("state", _vp), ("state_out", _vp)]
 
 
 def load(path=None):

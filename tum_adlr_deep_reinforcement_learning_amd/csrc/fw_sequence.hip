@@ -1,0 +1,611 @@
+// fw_sequence.hip -- linear attention with a decay per head over rollout columns (include/fwrollout.h):
+//
+//   k_scan        one wave runs one sequence, head and slice of value columns through time in blocks of C tokens
+//   k_scan_join   joins the states of time segments when there are few sequences
+//   k_token       the single-token form: reads the state once, writes it once
+//
+// The mathematics.  With g = exp(log_decay) and S the state before a block of C tokens,
+//   out_t = g^(t+1) S^T q_t + sum_{s<=t} g^(t-s) (q_t . k_s) v_s        S <- g^C S + sum_s g^(C-1-s) k_s v_s^T
+// and an episode start at x cuts every product whose span crosses it (s < x <= t).  The gradients are the same scan:
+//   dq = scan(dout, v, k);  dk = reversed scan(v, dout, q);  dv = reversed scan(k, q, dout)
+// with the states transposed where the roles of k and v change, so one kernel serves all four, and the backward
+// pass keeps nothing of the forward pass.
+#include <algorithm>
+
+#include "fw_seq_common.hpp"
+
+using namespace fwseq;
+
+namespace {
+
+constexpr int MAXDIM = 128;
+constexpr int SCAN_WAVES = 4;  // waves per block; each is on its own (no barrier, no LDS)
+
+struct Operand {
+  const void* p;
+  int64_t st, sn, sh;
+};
+struct State {  // element (n, h, seg, k, v) at p + n sn + h sh + seg sg + k sk + v sv
+  float* p;
+  int64_t sn, sh, sg;
+  int32_t sk, sv;
+};
+struct Pass {
+  Operand q, k, v, o;  // o.p NULL: only the state is wanted
+  State in, out;       // p NULL: zeros / not wanted
+};
+struct ScanArgs {
+  Pass pass[2];
+  int32_t n_pass, Dk, Dv, H, rev, n_slice, n_seg, run_seg;  // segments [0, run_seg) in processing order
+  int64_t T, N, seg_len;
+  const float* log_decay;
+  const uint8_t* starts;
+  int64_t starts_st, starts_sn;
+  const int32_t* lengths;
+  float* factor;  // [n_pass][N][H][n_seg]: what a segment multiplies a state with, or NULL
+};
+
+enum { FULL, GUARD, SCALAR };  // D fills the tiles; whole vectors in or out; element by element
+
+// NE contiguous elements at column `col` of a row of D; a column outside is read from column 0 (the caller drops it)
+template <typename T, int NE, int MODE>
+__device__ __forceinline__ void load_cols(const T* row, int col, int D, float* x) {
+  if constexpr (MODE == SCALAR) {
+#pragma unroll
+    for (int i = 0; i < NE; i++) x[i] = to_f32(row[col + i < D ? col + i : 0]);
+  } else {
+    constexpr int P = vec_elems<T>(NE);
+#pragma unroll
+    for (int i = 0; i < NE; i += P) load_vec<T, P>(row + (MODE == FULL || col + i < D ? col + i : 0), x + i);
+  }
+}
+template <typename T, int NE, int MODE>
+__device__ __forceinline__ void store_cols(T* row, int col, int D, const float* x) {
+  if constexpr (MODE == SCALAR) {
+#pragma unroll
+    for (int i = 0; i < NE; i++)
+      if (col + i < D) row[col + i] = from_f32<T>(x[i]);
+  } else {
+    constexpr int P = vec_elems<T>(NE);
+#pragma unroll
+    for (int i = 0; i < NE; i += P)
+      if (MODE == FULL || col + i < D) store_vec<T, P>(row + col + i, x + i);
+  }
+}
+
+__device__ __forceinline__ f32x4 mma(float a, float b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
+}
+
+// One wave; lane = 16 g + r.  Operands of a 16x16x4 product: A row r, B column r, depth g; result: column r, rows
+// 4 g + i.  Depths and rows may be numbered at will as long as both operands agree, and the numbering below makes
+// every result register the operand register of the product that needs it, so nothing moves between lanes:
+//   tokens       depth step j of lane group g is token 4 g + j  (block of C = 16)
+//   key columns  4 KT g + e, e = KT i + a: row 4 g + i of state tile a
+//   value cols   VT r + f (operand tile f), 4 VT g + VT i + f (result)
+// S[a][f] = state tile (k columns a, v columns f); P[i] = weight x (k_s . q_t) for s = 4 g + i, t = r;
+// O[f] = out^T: value columns down the rows, tokens along the columns.
+template <typename T, int KT, int VT, int MODE>
+__global__ __launch_bounds__(64 * SCAN_WAVES) void k_scan(ScanArgs A) {
+  constexpr int C = 16, TPL = 4;
+  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+  // unit = (((seg N + n) H + h) n_slice + slice) n_pass + pass
+  int64_t u = (int64_t)blockIdx.x * SCAN_WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int pi = (int)(u % A.n_pass);
+  u /= A.n_pass;
+  const int slice = (int)(u % A.n_slice);
+  u /= A.n_slice;
+  const int h = (int)(u % A.H);
+  u /= A.H;
+  const int64_t n = u % A.N;
+  const int seg = (int)(u / A.N);  // in processing order
+  if (seg >= A.run_seg) return;
+  const Pass& p = A.pass[pi];
+  const int Dk = A.Dk, Dv = A.Dv, v0 = slice * 16 * VT;
+  const bool rev = A.rev;
+  const int64_t seg0 = (rev ? A.n_seg - 1 - seg : seg) * A.seg_len;  // the segment's tokens: [seg0, seg1)
+  const int64_t seg1 = min(seg0 + A.seg_len, A.T);
+  int64_t len = A.T;
+  if (A.lengths) len = max((int64_t)0, min(A.T, (int64_t)A.lengths[n]));
+  const int64_t L = max((int64_t)0, min(len, seg1) - seg0);  // of which the first L are live
+
+  const T* qb = (const T*)p.q.p + n * p.q.sn + h * p.q.sh + seg0 * p.q.st;
+  const T* kb = (const T*)p.k.p + n * p.k.sn + h * p.k.sh + seg0 * p.k.st;
+  const T* vb = (const T*)p.v.p + n * p.v.sn + h * p.v.sh + seg0 * p.v.st + v0;
+  T* ob = (T*)p.o.p + n * p.o.sn + h * p.o.sh + seg0 * p.o.st + v0;
+  const bool want_out = p.o.p != nullptr;
+  const uint8_t* xb = A.starts ? A.starts + n * A.starts_sn + seg0 * A.starts_st : nullptr;
+  const float ld = A.log_decay[h];
+  auto power = [&](int m) { return m == 0 ? 1.0f : expf(ld * (float)m); };
+
+  f32x4 S[KT][VT];
+#pragma unroll
+  for (int a = 0; a < KT; a++)
+#pragma unroll
+    for (int f = 0; f < VT; f++) {
+      S[a][f] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (p.in.p) {
+        const float* s = p.in.p + n * p.in.sn + h * p.in.sh + seg * p.in.sg;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const int dk = KT * (4 * g + i) + a, dv = v0 + VT * r + f;
+          if (dk < Dk && dv < Dv) S[a][f][i] = s[(int64_t)dk * p.in.sk + (int64_t)dv * p.in.sv];
+        }
+      }
+    }
+
+  // weights of a whole block; a reversed pass carries g x the state of the token behind it, so that its final
+  // state is the gradient of the initial one and its first weight is 1
+  float wp[4], wi, wu[TPL], em1 = 0.f;
+  int cur = 0;
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const int d = rev ? 4 * g + i - r : r - 4 * g - i;
+    wp[i] = d >= 0 ? power(d) : 0.f;
+  }
+  bool fresh = false;    // an episode start among the segment's live tokens
+  int64_t done = 0;      // tokens processed
+  int single = 0;        // blocks of one token still to go (see below)
+  while (done < L) {
+    const int c = single ? 1 : (int)min((int64_t)C, L - done);
+    const int64_t t0 = rev ? L - done - c : done;
+    if (c != cur) {
+      cur = c;
+      wi = power(rev ? max(c - 1 - r, 0) : r + 1);
+#pragma unroll
+      for (int j = 0; j < TPL; j++) {
+        const int s = TPL * g + j;
+        wu[j] = s < c ? power(rev ? s + 1 : c - 1 - s) : 0.f;
+      }
+      em1 = expm1f(ld * (float)c);
+    }
+    uint32_t M = 0;  // bit s: an episode starts at token s of the block
+    if (xb) M = (uint32_t)__ballot(lane < c && xb[(t0 + (lane < c ? lane : 0)) * A.starts_st] != 0);
+    fresh |= M != 0;
+
+    // rows behind the block are read from its last token and dropped by zeros
+    float V[TPL][VT], K2[TPL][KT];
+    float bad = 0.f;
+#pragma unroll
+    for (int j = 0; j < TPL; j++) {
+      const int s = TPL * g + j;
+      const int64_t row = t0 + min(s, c - 1);
+      load_cols<T, VT, MODE>(vb + row * p.v.st, VT * r, Dv - v0, V[j]);
+      load_cols<T, KT, MODE>(kb + row * p.k.st, KT * r, Dk, K2[j]);
+#pragma unroll
+      for (int f = 0; f < VT; f++) {
+        bad += V[j][f];
+        if (s >= c) V[j][f] = 0.f;
+      }
+    }
+    // A masked product is a product with 0, which keeps a value away only while that value is finite.  A block with
+    // an infinity or a NaN among its values is therefore run token by token: nothing is masked then.
+    if (c > 1 && __any(!(fabsf(bad) < __builtin_huge_valf()))) {
+      single = c;
+      continue;
+    }
+
+    if (want_out) {
+      float Q[4 * KT], K1[4 * KT];
+      load_cols<T, 4 * KT, MODE>(qb + (t0 + min(r, c - 1)) * p.q.st, 4 * KT * g, Dk, Q);
+      load_cols<T, 4 * KT, MODE>(kb + (t0 + min(r, c - 1)) * p.k.st, 4 * KT * g, Dk, K1);
+      if constexpr (MODE != FULL)
+#pragma unroll
+        for (int e = 0; e < 4 * KT; e++)
+          if (4 * KT * g + e >= Dk) Q[e] = 0.f;
+      f32x4 P{0.f, 0.f, 0.f, 0.f};
+      f32x4 O[VT];
+#pragma unroll
+      for (int f = 0; f < VT; f++) O[f] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int a = 0; a < KT; a++) {
+          P = mma(K1[KT * i + a], Q[KT * i + a], P);
+#pragma unroll
+          for (int f = 0; f < VT; f++) O[f] = mma(S[a][f][i], Q[KT * i + a], O[f]);
+        }
+      // weights and masks: select, never multiply by 0
+      const bool blocked = M != 0 && (rev ? (M >> r) >> 1 : M & ((2u << r) - 1)) != 0;
+#pragma unroll
+      for (int f = 0; f < VT; f++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) O[f][i] = blocked ? 0.f : O[f][i] * wi;
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const int s = 4 * g + i;
+        bool keep = rev ? s >= r && s < c : s <= r;
+        if (M != 0) keep = keep && ((M >> min(s, r)) >> 1 & ((1u << abs(s - r)) - 1)) == 0;
+        P[i] = keep ? P[i] * wp[i] : 0.f;
+      }
+#pragma unroll
+      for (int j = 0; j < TPL; j++)
+#pragma unroll
+        for (int f = 0; f < VT; f++) O[f] = mma(V[j][f], P[j], O[f]);
+      if (r < c) {
+        float x[4 * VT];
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+          for (int f = 0; f < VT; f++) x[VT * i + f] = O[f][i];
+        store_cols<T, 4 * VT, MODE>(ob + (t0 + r) * p.o.st, 4 * VT * g, Dv - v0, x);
+      }
+    }
+
+    // the state: g^c S as S + S (g^c - 1), whose rounding does not add up over the blocks of a long memory
+#pragma unroll
+    for (int a = 0; a < KT; a++)
+#pragma unroll
+      for (int f = 0; f < VT; f++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) S[a][f][i] = M != 0 ? 0.f : fmaf(S[a][f][i], em1, S[a][f][i]);
+#pragma unroll
+    for (int j = 0; j < TPL; j++) {
+      const int s = TPL * g + j;
+      bool keep = s < c;
+      if (M != 0) keep = keep && (rev ? M & ((2u << s) - 1) : (M >> s) >> 1) == 0;
+#pragma unroll
+      for (int a = 0; a < KT; a++) {
+        const float kw = keep ? K2[j][a] * wu[j] : 0.f;
+#pragma unroll
+        for (int f = 0; f < VT; f++) S[a][f] = mma(kw, V[j][f], S[a][f]);
+      }
+    }
+    done += c;
+    if (single) single--;
+  }
+
+  if (p.out.p && (seg == A.n_seg - 1 || p.out.sg)) {
+    float* s = p.out.p + n * p.out.sn + h * p.out.sh + seg * p.out.sg;
+#pragma unroll
+    for (int a = 0; a < KT; a++)
+#pragma unroll
+      for (int f = 0; f < VT; f++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const int dk = KT * (4 * g + i) + a, dv = v0 + VT * r + f;
+          if (dk < Dk && dv < Dv) s[(int64_t)dk * p.out.sk + (int64_t)dv * p.out.sv] = S[a][f][i];
+        }
+  }
+  if (A.factor && slice == 0 && lane == 0)
+    A.factor[((pi * A.N + n) * A.H + h) * A.n_seg + seg] = fresh ? 0.f : (L == 0 ? 1.f : expf(ld * (float)L));
+  if (want_out) {  // rows behind the sequence's end
+    const float z[4 * VT] = {};
+    for (int64_t t = L + r; t < seg1 - seg0; t += 16)
+      store_cols<T, 4 * VT, MODE>(ob + t * p.o.st, 4 * VT * g, Dv - v0, z);
+  }
+}
+
+// ws[seg] holds what segment seg adds to a state; rewritten as the state that enters segment seg:
+//   c_0 = in;  c_{s+1} = factor_s c_s + ws_s
+// One thread per state element; the loads of all segments are independent of the recurrence.
+struct JoinArgs {
+  State in[2];  // p NULL: zeros
+  float* ws;    // [n_pass][N][H][n_seg][Dk][Dv]
+  const float* factor;
+  int64_t N;
+  int32_t n_pass, H, n_seg, Dk, Dv;
+};
+__global__ __launch_bounds__(256) void k_scan_join(JoinArgs A) {
+  const int64_t E = (int64_t)A.Dk * A.Dv, total = A.n_pass * A.N * A.H * E;
+  const int64_t x = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (x >= total) return;
+  const int64_t row = x / E, e = x - row * E;  // row = (pass N + n) H + h
+  const int h = (int)(row % A.H);
+  const int64_t n = (row / A.H) % A.N;
+  const int pi = (int)(row / A.H / A.N);
+  const State& in = A.in[pi];
+  float c = in.p ? in.p[n * in.sn + h * in.sh + (e / A.Dv) * in.sk + (e % A.Dv) * in.sv] : 0.f;
+  float* w = A.ws + row * A.n_seg * E + e;
+  const float* f = A.factor + row * A.n_seg;
+  constexpr int PF = 8;
+  for (int s0 = 0; s0 < A.n_seg; s0 += PF) {
+    float add[PF], fac[PF];
+#pragma unroll
+    for (int k = 0; k < PF; k++) {
+      const bool have = s0 + k < A.n_seg - 1;  // the last segment adds to nothing
+      add[k] = have ? w[(s0 + k) * E] : 0.f;
+      fac[k] = have ? f[s0 + k] : 0.f;
+    }
+#pragma unroll
+    for (int k = 0; k < PF; k++)
+      if (s0 + k < A.n_seg) {
+        w[(s0 + k) * E] = c;
+        c = fac[k] != 0.f ? fmaf(fac[k], c, add[k]) : add[k];
+      }
+  }
+}
+
+// ------------------------------------------------------------------ the single-token form
+struct TokenArgs {
+  Operand q, k, v, o;
+  const float* log_decay;
+  const uint8_t* starts;
+  int64_t starts_sn, N;
+  const float* in;
+  float* out;
+  int32_t H, Dk, Dv;
+};
+
+// One wave per (n, h).  LV lanes (a power of two) cover a state row in vectors of 4, 64 / LV rows per access.
+template <typename T, bool VEC>
+__global__ __launch_bounds__(256) void k_token(TokenArgs A, int lv_log2) {
+  const int lane = threadIdx.x & 63;
+  const int64_t u = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (u >= A.N * A.H) return;
+  const int h = (int)(u % A.H);
+  const int64_t n = u / A.H;
+  const int LV = 1 << lv_log2, rows = 64 >> lv_log2;
+  const int c = (lane & (LV - 1)) * 4, rr = lane >> lv_log2;
+  const T* q = (const T*)A.q.p + n * A.q.sn + h * A.q.sh;
+  const T* k = (const T*)A.k.p + n * A.k.sn + h * A.k.sh;
+  const T* v = (const T*)A.v.p + n * A.v.sn + h * A.v.sh;
+  T* o = (T*)A.o.p + n * A.o.sn + h * A.o.sh;
+  const bool start = A.starts && A.starts[n * A.starts_sn] != 0;
+  const float em1 = expm1f(A.log_decay[h]);
+  const float* sin = A.in + u * A.Dk * A.Dv;
+  float* sout = A.out + u * A.Dk * A.Dv;
+  float vv[4], acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < 4; i++) vv[i] = c + i < A.Dv ? to_f32(v[c + i]) : 0.f;
+  if (c < A.Dv)
+    for (int d = rr; d < A.Dk; d += rows) {
+      const float kd = to_f32(k[d]), qd = to_f32(q[d]);
+      float s[4] = {0.f, 0.f, 0.f, 0.f};
+      if (!start) {
+        if constexpr (VEC)
+          load_vec<float, 4>(sin + d * A.Dv + c, s);
+        else
+          for (int i = 0; i < 4; i++)
+            if (c + i < A.Dv) s[i] = sin[d * A.Dv + c + i];
+      }
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        s[i] = fmaf(kd, vv[i], fmaf(s[i], em1, s[i]));
+        acc[i] = fmaf(qd, s[i], acc[i]);
+      }
+      if constexpr (VEC)
+        store_vec<float, 4>(sout + d * A.Dv + c, s);
+      else
+        for (int i = 0; i < 4; i++)
+          if (c + i < A.Dv) sout[d * A.Dv + c + i] = s[i];
+    }
+  for (int m = LV; m < 64; m <<= 1)
+#pragma unroll
+    for (int i = 0; i < 4; i++) acc[i] += __shfl_xor(acc[i], m);
+  if (rr == 0)
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+      if (c + i < A.Dv) o[c + i] = from_f32<T>(acc[i]);
+}
+
+// ------------------------------------------------------------------ host side
+int tiles(int d) { return d <= 16 ? 1 : d <= 32 ? 2 : d <= 64 ? 4 : 8; }
+
+// Time segments: with fewer than SEG_WAVES waves the card is not full, so the time axis is cut, at the price of
+// reading k and v twice and of a state per segment.
+constexpr int SEG_WAVES = 1024;
+constexpr int SEG_MIN = 128;  // tokens
+struct Plan {
+  int64_t seg_len;
+  int n_seg;
+};
+Plan plan(int64_t T, int64_t N, int H, int Dv) {
+  const int slices = (tiles(Dv) + 3) / 4;
+  const int64_t waves = std::max<int64_t>(1, N * H * slices);
+  int64_t segs = std::min<int64_t>(SEG_WAVES / waves, T / SEG_MIN);
+  if (segs < 2) return {std::max<int64_t>(T, 1), 1};
+  const int64_t len = ((T + segs - 1) / segs + 63) / 64 * 64;
+  return {len, (int)((T + len - 1) / len)};
+}
+size_t plan_floats(const Plan& pl, int n_pass, int64_t N, int H, int Dk, int Dv) {
+  if (pl.n_seg < 2) return 0;
+  return (size_t)n_pass * N * H * pl.n_seg * ((size_t)Dk * Dv + 1);
+}
+
+template <typename T>
+bool aligned(const Operand& o, int D) {
+  const int per16 = 16 / sizeof(T);
+  return D % per16 == 0 && (uintptr_t)o.p % 16 == 0 && o.st % per16 == 0 && o.sn % per16 == 0 && o.sh % per16 == 0;
+}
+
+template <typename T, int KT, int VT>
+int launch_mode(const ScanArgs& A, int mode, hipStream_t s) {
+  const int64_t units = A.n_pass * (int64_t)A.n_slice * A.H * A.N * A.run_seg;
+  const int64_t blocks = (units + SCAN_WAVES - 1) / SCAN_WAVES;
+  if (blocks > INT32_MAX) return fw::set_error(FW_E_INVALID, "linear attention: too many sequences for one call");
+  const dim3 grid((unsigned)blocks), block(64 * SCAN_WAVES);
+  if (mode == FULL)
+    hipLaunchKernelGGL((k_scan<T, KT, VT, FULL>), grid, block, 0, s, A);
+  else if (mode == GUARD)
+    hipLaunchKernelGGL((k_scan<T, KT, VT, GUARD>), grid, block, 0, s, A);
+  else
+    hipLaunchKernelGGL((k_scan<T, KT, VT, SCALAR>), grid, block, 0, s, A);
+  FW_HIP(hipGetLastError());
+  return FW_OK;
+}
+
+template <typename T>
+int launch_scan(const ScanArgs& A, hipStream_t s) {
+  const int kt = tiles(A.Dk), vt = std::min(tiles(A.Dv), 4);
+  bool vec = true;
+  for (int i = 0; i < A.n_pass; i++)
+    for (const Operand* o : {&A.pass[i].q, &A.pass[i].k}) vec = vec && aligned<T>(*o, A.Dk);
+  for (int i = 0; i < A.n_pass; i++)
+    for (const Operand* o : {&A.pass[i].v, &A.pass[i].o}) vec = vec && aligned<T>(*o, A.Dv);
+  const int mode = !vec ? SCALAR : A.Dk == 16 * kt && A.Dv % (16 * vt) == 0 ? FULL : GUARD;
+  switch (kt * 8 + vt) {
+#define FW_CASE(K, V) \
+  case K * 8 + V: return launch_mode<T, K, V>(A, mode, s)
+    FW_CASE(1, 1); FW_CASE(1, 2); FW_CASE(1, 4);
+    FW_CASE(2, 1); FW_CASE(2, 2); FW_CASE(2, 4);
+    FW_CASE(4, 1); FW_CASE(4, 2); FW_CASE(4, 4);
+    FW_CASE(8, 1); FW_CASE(8, 2); FW_CASE(8, 4);
+#undef FW_CASE
+  }
+  return fw::set_error(FW_E_INVALID, "linear attention: head sizes 1..128");
+}
+
+int launch_scan_dt(int dtype, const ScanArgs& A, hipStream_t s) {
+  if (dtype == FW_DT_F32) return launch_scan<float>(A, s);
+  if (dtype == FW_DT_BF16) return launch_scan<bf16>(A, s);
+  return launch_scan<f16>(A, s);
+}
+
+// n_pass passes of the same direction and sizes, cut into time segments where the plan says so
+int run_passes(int dtype, ScanArgs A, const Plan& pl, float* ws, hipStream_t s) {
+  A.seg_len = pl.seg_len;
+  A.n_seg = A.run_seg = pl.n_seg;
+  A.n_slice = (tiles(A.Dv) + 3) / 4;
+  if (pl.n_seg < 2) return launch_scan_dt(dtype, A, s);
+  const int64_t E = (int64_t)A.Dk * A.Dv;
+  float* factor = ws + A.n_pass * A.N * A.H * pl.n_seg * E;
+  ScanArgs B = A;  // what each segment adds, from its keys and values alone
+  JoinArgs J{};
+  B.run_seg = pl.n_seg - 1;
+  B.factor = factor;
+  for (int i = 0; i < A.n_pass; i++) {
+    const State seg{ws + i * A.N * A.H * pl.n_seg * E, A.H * pl.n_seg * E, pl.n_seg * E, E, A.Dv, 1};
+    B.pass[i].o.p = nullptr;
+    B.pass[i].in.p = nullptr;
+    B.pass[i].out = seg;
+    J.in[i] = A.pass[i].in;
+    A.pass[i].in = seg;
+    A.pass[i].out.sg = 0;
+  }
+  if (int rc = launch_scan_dt(dtype, B, s)) return rc;
+  J.ws = ws;
+  J.factor = factor;
+  J.N = A.N;
+  J.n_pass = A.n_pass;
+  J.H = A.H;
+  J.n_seg = pl.n_seg;
+  J.Dk = A.Dk;
+  J.Dv = A.Dv;
+  const int64_t blocks = (A.n_pass * A.N * A.H * E + 255) / 256;
+  hipLaunchKernelGGL(k_scan_join, dim3((unsigned)blocks), dim3(256), 0, s, J);
+  FW_HIP(hipGetLastError());
+  return launch_scan_dt(dtype, A, s);
+}
+
+int check(const fw_linattn* a, const char* who) {
+  auto bad = [&](const char* m) { return fw::set_error(FW_E_INVALID, std::string(who) + ": " + m); };
+  if (!a) return bad("NULL arguments");
+  if (a->T < 0 || a->N < 0 || a->H < 1) return bad("T and N must be >= 0, H >= 1");
+  if (a->Dk < 1 || a->Dk > MAXDIM || a->Dv < 1 || a->Dv > MAXDIM) return bad("head sizes must be 1..128");
+  if (a->dtype < FW_DT_F32 || a->dtype > FW_DT_F16) return bad("dtype must be float32, bfloat16 or float16");
+  if (a->T > 0 && a->N > 0 && (!a->q.p || !a->k.p || !a->v.p)) return bad("NULL q, k or v");
+  if (!a->log_decay) return bad("NULL log_decay");
+  return FW_OK;
+}
+bool room(const fw_linattn* a, bool backward) {
+  const size_t need = fw_linattn_workspace_bytes(a->T, a->N, a->H, a->Dk, a->Dv, backward);
+  return need == 0 || (a->workspace && a->workspace_bytes >= need);
+}
+Operand in(const fw_seq_tensor& t) { return {t.p, t.st, t.sn, t.sh}; }
+ScanArgs base(const fw_linattn* a, bool rev) {
+  ScanArgs A{};
+  A.H = a->H;
+  A.rev = rev;
+  A.T = a->T;
+  A.N = a->N;
+  A.log_decay = a->log_decay;
+  A.starts = a->starts;
+  A.starts_st = a->starts_st;
+  A.starts_sn = a->starts_sn;
+  A.lengths = a->lengths;
+  return A;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t fw_linattn_workspace_bytes(int64_t T, int64_t N, int32_t H, int32_t Dk, int32_t Dv, int32_t backward) {
+  if (T < 1 || N < 1 || H < 1 || Dk < 1 || Dk > MAXDIM || Dv < 1 || Dv > MAXDIM) return 0;
+  if (!backward) return sizeof(float) * plan_floats(plan(T, N, H, Dv), 1, N, H, Dk, Dv);
+  // dq, dk and dv run one after another in the same room
+  return sizeof(float) * std::max(plan_floats(plan(T, N, H, Dk), 1, N, H, Dv, Dk),
+                                  plan_floats(plan(T, N, H, Dv), 1, N, H, Dk, Dv));
+}
+
+int fw_linattn_forward(const fw_linattn* a, void* stream) {
+  if (int rc = check(a, "fw_linattn_forward")) return rc;
+  if (a->N == 0) return FW_OK;
+  if (a->T > 0 && !a->out.p) return fw::set_error(FW_E_INVALID, "fw_linattn_forward: NULL out");
+  if (!room(a, false)) return fw::set_error(FW_E_INVALID, "fw_linattn_forward: workspace too small");
+  ScanArgs A = base(a, false);
+  A.n_pass = 1;
+  A.Dk = a->Dk;
+  A.Dv = a->Dv;
+  const int64_t E = (int64_t)a->Dk * a->Dv;
+  A.pass[0] = Pass{in(a->q), in(a->k), in(a->v), in(a->out),
+                   State{const_cast<float*>(a->state_in), a->H * E, E, 0, a->Dv, 1},
+                   State{a->state_out, a->H * E, E, 0, a->Dv, 1}};
+  return run_passes(a->dtype, A, plan(a->T, a->N, a->H, a->Dv), (float*)a->workspace, (hipStream_t)stream);
+}
+
+int fw_linattn_backward(const fw_linattn* a, void* stream) {
+  if (int rc = check(a, "fw_linattn_backward")) return rc;
+  if (a->N == 0) return FW_OK;
+  if (a->T > 0 && (!a->dout.p || !a->dq.p || !a->dk.p || !a->dv.p))
+    return fw::set_error(FW_E_INVALID, "fw_linattn_backward: NULL dout, dq, dk or dv");
+  if (!room(a, true)) return fw::set_error(FW_E_INVALID, "fw_linattn_backward: workspace too small");
+  const int64_t E = (int64_t)a->Dk * a->Dv;
+  hipStream_t s = (hipStream_t)stream;
+  float* ws = (float*)a->workspace;
+  auto straight = [&](const float* p) { return State{const_cast<float*>(p), a->H * E, E, 0, a->Dv, 1}; };
+  auto turned = [&](const float* p) { return State{const_cast<float*>(p), a->H * E, E, 0, 1, a->Dv}; };
+  const State none{};
+  const Plan pk = plan(a->T, a->N, a->H, a->Dk), pv = plan(a->T, a->N, a->H, a->Dv);
+  ScanArgs A = base(a, false);
+  A.n_pass = 1;
+  A.Dk = a->Dv;
+  A.Dv = a->Dk;
+  A.pass[0] = Pass{in(a->dout), in(a->v), in(a->k), in(a->dq), turned(a->state_in), none};
+  if (int rc = run_passes(a->dtype, A, pk, ws, s)) return rc;
+  A.rev = 1;
+  A.pass[0] = Pass{in(a->v), in(a->dout), in(a->q), in(a->dk), turned(a->dstate), none};
+  if (int rc = run_passes(a->dtype, A, pk, ws, s)) return rc;
+  A.Dk = a->Dk;
+  A.Dv = a->Dv;
+  A.pass[0] = Pass{in(a->k), in(a->q), in(a->dout), in(a->dv), straight(a->dstate), straight(a->dstate_in)};
+  return run_passes(a->dtype, A, pv, ws, s);
+}
+
+int fw_linattn_step(const fw_linattn_token* a, void* stream) {
+  auto bad = [&](const char* m) { return fw::set_error(FW_E_INVALID, std::string("fw_linattn_step: ") + m); };
+  if (!a) return bad("NULL arguments");
+  if (a->N < 0 || a->H < 1) return bad("N must be >= 0, H >= 1");
+  if (a->Dk < 1 || a->Dk > MAXDIM || a->Dv < 1 || a->Dv > MAXDIM) return bad("head sizes must be 1..128");
+  if (a->dtype < FW_DT_F32 || a->dtype > FW_DT_F16) return bad("dtype must be float32, bfloat16 or float16");
+  if (a->N == 0) return FW_OK;
+  if (!a->q.p || !a->k.p || !a->v.p || !a->out.p || !a->log_decay || !a->state || !a->state_out) return bad("NULL buffer");
+  if ((uintptr_t)a->state % 16 || (uintptr_t)a->state_out % 16) return bad("states must be 16-byte aligned");
+  TokenArgs A{in(a->q), in(a->k), in(a->v), in(a->out), a->log_decay, a->starts, a->starts_sn, a->N,
+              a->state, a->state_out, a->H, a->Dk, a->Dv};
+  int lv = 0;
+  while ((4 << lv) < a->Dv) lv++;
+  const int64_t blocks = (a->N * a->H + 3) / 4;
+  if (blocks > INT32_MAX) return bad("too many sequences for one call");
+  const dim3 grid((unsigned)blocks), block(256);
+  const bool vec = a->Dv % 4 == 0;
+  hipStream_t s = (hipStream_t)stream;
+#define FW_TOKEN(T)                                                                    \
+  if (vec)                                                                             \
+    hipLaunchKernelGGL((k_token<T, true>), grid, block, 0, s, A, lv);                  \
+  else                                                                                 \
+    hipLaunchKernelGGL((k_token<T, false>), grid, block, 0, s, A, lv)
+  if (a->dtype == FW_DT_F32) {
+    FW_TOKEN(float);
+  } else if (a->dtype == FW_DT_BF16) {
+    FW_TOKEN(bf16);
+  } else {
+    FW_TOKEN(f16);
+  }
+#undef FW_TOKEN
+  FW_HIP(hipGetLastError());
+  return FW_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,226 @@
+"""Operators of a policy with memory, in the layouts of the rollout slab (time-major, heads and channels last).
+
+  linear_attention       a decaying key-value memory per head over whole rollout columns [T][N], with resets at the
+                         episode starts, ragged lengths, a state carried in and out, and gradients
+  linear_attention_step  the same recurrence for one token per environment (the collect step)
+  group_norm_act         group norm with an activation over channels-last rows or maps, with gradients
+
+Every function launches on the current stream of its tensors' device, takes its workspace from torch's allocator on
+that stream and never synchronises.  Tensors are float32, bfloat16 or float16; states, statistics, sums and the
+gradients of parameters are float32.  There is no CPU path: CPU tensors are refused.
+
+The reference's policies are memoryless; these have no counterpart there.
+"""
+import ctypes
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _native
+
+_DT = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # include/fwrollout.h FW_DT_*
+MAX_HEAD = 128
+
+
+def _ptr(t):
+    return t.data_ptr() if t is not None else None
+
+
+def _stream(device):
+    return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+def _operand(s, t, step=False):
+    """Fills an fw_seq_tensor from a [T][N][H][D] (or [N][H][D]) tensor with unit stride in D."""
+    st = t.stride()
+    s.p = t.data_ptr()
+    if step:
+        s.st, s.sn, s.sh = 0, st[0], st[1]
+    else:
+        s.st, s.sn, s.sh = st[0], st[1], st[2]
+
+
+def _dense(t):
+    """Unit stride in the last dimension (a copy otherwise; broadcast leading dimensions stay views)."""
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _heads(who, q, k, v, dims):
+    lay = "[T, N, H, D]" if dims == 4 else "[N, H, D]"
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        if not isinstance(t, torch.Tensor) or t.dim() != dims:
+            raise ValueError("%s: %s must be a %s tensor" % (who, name, lay))
+        if t.device.type != "cuda":
+            raise ValueError("%s: %s must be on the GPU (no CPU path exists)" % (who, name))
+        if t.dtype not in _DT or t.dtype != q.dtype or t.device != q.device:
+            raise ValueError("%s: q, k and v must share a device and one of float32, bfloat16, float16" % who)
+    if q.shape != k.shape or q.shape[:-1] != v.shape[:-1]:
+        raise ValueError("%s: q and k must have the same shape, v the same up to its last dimension; got %s %s %s"
+                         % (who, tuple(q.shape), tuple(k.shape), tuple(v.shape)))
+    if not (1 <= q.shape[-1] <= MAX_HEAD and 1 <= v.shape[-1] <= MAX_HEAD):
+        raise ValueError("%s: head sizes must be 1..%d" % (who, MAX_HEAD))
+    if q.shape[-2] < 1:
+        raise ValueError("%s: at least one head" % who)
+
+
+def _decay(who, log_decay, H, device):
+    if not isinstance(log_decay, torch.Tensor) or log_decay.shape != (H,) or log_decay.dtype != torch.float32 or \
+            log_decay.device != device:
+        raise ValueError("%s: log_decay must be a float32 [H] tensor on the operands' device" % who)
+    if log_decay.requires_grad and torch.is_grad_enabled():
+        raise ValueError("%s: log_decay is a fixed schedule and has no gradient; detach it" % who)
+    return log_decay.contiguous()
+
+
+def _starts(who, x, shape, device):
+    if x is None:
+        return None
+    if not isinstance(x, torch.Tensor) or x.shape != shape or x.dtype not in (torch.uint8, torch.bool) or \
+            x.device != device:
+        raise ValueError("%s: episode_starts must be a uint8 or bool %s tensor on the operands' device"
+                         % (who, list(shape)))
+    return x
+
+
+def _state(who, x, shape, device, name):
+    if not isinstance(x, torch.Tensor) or x.shape != shape or x.dtype != torch.float32 or x.device != device:
+        raise ValueError("%s: %s must be a float32 %s tensor on the operands' device" % (who, name, list(shape)))
+    return x
+
+
+def _linattn_args(q, k, v, log_decay, starts, lengths):
+    a = _native.FwLinattn()
+    a.T, a.N, a.H, a.Dk = q.shape
+    a.Dv, a.dtype = v.shape[3], _DT[q.dtype]
+    _operand(a.q, q)
+    _operand(a.k, k)
+    _operand(a.v, v)
+    a.log_decay = log_decay.data_ptr()
+    if starts is not None:
+        a.starts = starts.data_ptr()
+        a.starts_st, a.starts_sn = starts.stride()
+    a.lengths = _ptr(lengths)
+    return a
+
+
+def _workspace(lib, a, device, backward):
+    n = lib.fw_linattn_workspace_bytes(a.T, a.N, a.H, a.Dk, a.Dv, backward)
+    ws = torch.empty(n, dtype=torch.uint8, device=device) if n else None
+    a.workspace, a.workspace_bytes = _ptr(ws), n
+    return ws  # referenced until the launches are queued; the allocator reuses it in stream order
+
+
+def _linattn_forward(q, k, v, log_decay, state, starts, lengths):
+    lib = _native.load()
+    a = _linattn_args(q, k, v, log_decay, starts, lengths)
+    out = torch.empty(v.shape, dtype=v.dtype, device=v.device)
+    final = torch.empty((a.N, a.H, a.Dk, a.Dv), dtype=torch.float32, device=v.device)
+    _operand(a.out, out)
+    a.state_in, a.state_out = _ptr(state), final.data_ptr()
+    with torch.cuda.device(q.device):
+        ws = _workspace(lib, a, q.device, 0)  # noqa: F841
+        _native.check(lib.fw_linattn_forward(ctypes.byref(a), _stream(q.device)), "fw_linattn_forward")
+    return out, final
+
+
+class _LinearAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, log_decay, state, starts, lengths):
+        out, final = _linattn_forward(q, k, v, log_decay, state, starts, lengths)
+        ctx.save_for_backward(q, k, v, log_decay, state, starts, lengths)
+        ctx.set_materialize_grads(False)
+        return out, final
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout, dfinal):
+        q, k, v, log_decay, state, starts, lengths = ctx.saved_tensors
+        lib = _native.load()
+        a = _linattn_args(q, k, v, log_decay, starts, lengths)
+        dout = _dense(dout) if dout is not None else torch.zeros(v.shape, dtype=v.dtype, device=v.device)
+        dfinal = dfinal.contiguous() if dfinal is not None else None
+        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+        for s, t in ((a.dout, dout), (a.dq, dq), (a.dk, dk), (a.dv, dv)):
+            _operand(s, t)
+        dstate = torch.empty_like(state) if state is not None and ctx.needs_input_grad[4] else None
+        a.state_in, a.dstate, a.dstate_in = _ptr(state), _ptr(dfinal), _ptr(dstate)
+        with torch.cuda.device(q.device):
+            ws = _workspace(lib, a, q.device, 1)  # noqa: F841
+            _native.check(lib.fw_linattn_backward(ctypes.byref(a), _stream(q.device)), "fw_linattn_backward")
+        return dq, dk, dv, None, dstate, None, None
+
+
+def linear_attention(q, k, v, log_decay, initial_state=None, episode_starts=None, lengths=None):
+    """Linear attention with a decay per head over the columns of a rollout; returns (out, final_state).
+
+    With ``g = exp(log_decay[h])``, per column n and head h::
+
+        S_t = (0 if episode_starts[t, n] else g S_{t-1}) + k_t v_t^T,   S_{-1} = initial_state (None: zeros)
+        out_t = S_t^T q_t,                                              final_state = S_{len-1}
+
+    q, k [T, N, H, Dk] and v [T, N, H, Dv] (head sizes 1..128) share a dtype; any strides, broadcast views too
+    (a q and k shared by the heads: ``expand`` them, and their gradient is summed).  Batch-major data is passed as
+    ``x.transpose(0, 1)``.  log_decay: float32 [H], <= 0, without a gradient.  initial_state, final_state: float32
+    [N, H, Dk, Dv].  episode_starts: uint8 or bool [T, N].  lengths: int [N]; rows behind a column's length are not
+    read, come out as zeros and get zero gradients (values are clamped to 0..T).  out has v's shape and dtype.
+
+    Differentiable in q, k, v and initial_state; nothing but the inputs is kept for the backward pass, which is
+    deterministic.  A non-finite input reaches the outputs that the recurrence lets it reach, and no others."""
+    _heads("linear_attention", q, k, v, 4)
+    T, N, H, Dk = q.shape
+    dev = q.device
+    log_decay = _decay("linear_attention", log_decay, H, dev)
+    starts = _starts("linear_attention", episode_starts, (T, N), dev)
+    state = None
+    if initial_state is not None:
+        state = _state("linear_attention", initial_state, (N, H, Dk, v.shape[3]), dev, "initial_state").contiguous()
+    if lengths is not None:
+        if not isinstance(lengths, torch.Tensor) or lengths.shape != (N,) or lengths.device != dev or \
+                lengths.dtype not in (torch.int32, torch.int64):
+            raise ValueError("linear_attention: lengths must be an int32 or int64 [N] tensor on the operands' device")
+        lengths = lengths.clamp(0, T).to(torch.int32).contiguous() if lengths.dtype == torch.int64 \
+            else lengths.contiguous()
+    q, k, v = _dense(q), _dense(k), _dense(v)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or
+                                    (state is not None and state.requires_grad)):
+        return _LinearAttention.apply(q, k, v, log_decay, state, starts, lengths)
+    return _linattn_forward(q, k, v, log_decay, state, starts, lengths)
+
+
+def linear_attention_step(q, k, v, log_decay, state, episode_starts=None, state_out=None):
+    """One token per environment of ``linear_attention``: q, k [N, H, Dk], v [N, H, Dv] -> out [N, H, Dv].
+
+    ``state`` (float32 [N, H, Dk, Dv], contiguous) is read once and the new state written once, in place or into
+    ``state_out``, which must not overlap it otherwise.  A row with episode_starts [N] set begins from zeros.  Has no
+    gradient (the training form is ``linear_attention``): inputs that require one are refused outside
+    ``torch.no_grad()``."""
+    who = "linear_attention_step"
+    _heads(who, q, k, v, 3)
+    N, H, Dk = q.shape
+    dev = q.device
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, state) if isinstance(t, torch.Tensor)):
+        raise ValueError("%s has no gradient: use linear_attention, or torch.no_grad()" % who)
+    log_decay = _decay(who, log_decay, H, dev)
+    starts = _starts(who, episode_starts, (N,), dev)
+    shape = (N, H, Dk, v.shape[2])
+    new = state if state_out is None else state_out
+    for name, t in (("state", state), ("state_out", new)):
+        _state(who, t, shape, dev, name)
+        if not t.is_contiguous() or t.data_ptr() % 16:
+            raise ValueError("%s: %s must be contiguous and 16-byte aligned" % (who, name))
+    b = new.numel() * 4
+    if new.data_ptr() != state.data_ptr() and abs(new.data_ptr() - state.data_ptr()) < b:
+        raise ValueError("%s: state_out overlaps state" % who)
+    q, k, v = _dense(q), _dense(k), _dense(v)
+    out = torch.empty(v.shape, dtype=v.dtype, device=dev)
+    a = _native.FwLinattnToken()
+    a.N, a.H, a.Dk, a.Dv, a.dtype = N, H, Dk, v.shape[2], _DT[q.dtype]
+    for s, t in ((a.q, q), (a.k, k), (a.v, v), (a.out, out)):
+        _operand(s, t, step=True)
+    a.log_decay = log_decay.data_ptr()
+    if starts is not None:
+        a.starts, a.starts_sn = starts.data_ptr(), starts.stride(0)
+    a.state, a.state_out = state.data_ptr(), new.data_ptr()
+    with torch.cuda.device(dev):
+        _native.check(_native.load().fw_linattn_step(ctypes.byref(a), _stream(dev)), "fw_linattn_step")
+    return out
