@@ -245,6 +245,38 @@ typedef struct fw_linattn_token {
 } fw_linattn_token;
 int fw_linattn_step(const fw_linattn_token* a, void* stream);
 
+/* Group norm with an activation, channels last.  Per sample n and group of C / G channels, over its L rows:
+ *   m = mean, r = 1 / sqrt(var + eps),  z = weight (x - m) r + bias,  y = act(z)
+ * x, y, dy, dx: [N][L][C] of dtype with element strides sn, sl and unit channel stride; weight, bias [C] of wdtype
+ * (dtype or float32), either may be NULL (1 / 0).  Statistics are float32, by deviations from the mean.
+ * Backward: dx, and dweight, dbias [C] of wdtype (either may be NULL), summed in a fixed order.
+ * stats: float [N][G][2] (m, r), written by the forward call and read by the backward call; it is needed where
+ * fw_group_norm_stats says 1 (elsewhere NULL: the statistics are rebuilt from x, which is in registers anyway). */
+#define FW_ACT_NONE 0
+#define FW_ACT_RELU 1
+#define FW_ACT_SILU 2
+#define FW_ACT_GELU 3 /* z Phi(z), by erf */
+#define FW_ACT_TANH 4
+typedef struct fw_rows {
+  void* p;
+  int64_t sn, sl;
+} fw_rows;
+typedef struct fw_group_norm {
+  int64_t N, L;
+  int32_t C, G, dtype, wdtype, act, pad;
+  double eps;
+  fw_rows x, y, dy, dx;
+  const void *weight, *bias;
+  void *dweight, *dbias;
+  float* stats;
+  void* workspace;
+  size_t workspace_bytes;
+} fw_group_norm;
+int fw_group_norm_stats(const fw_group_norm* a);
+size_t fw_group_norm_workspace_bytes(const fw_group_norm* a, int32_t backward);
+int fw_group_norm_forward(const fw_group_norm* a, void* stream);
+int fw_group_norm_backward(const fw_group_norm* a, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

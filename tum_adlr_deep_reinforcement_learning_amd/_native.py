@@ -17,7 +17,7 @@ LIB_DIR = os.path.join(PKG, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libfwsim.so")
 HEADER = os.path.join(ROOT, "include", "fwsim.h")
 HEADERS = [HEADER, os.path.join(ROOT, "include", "fwrollout.h")]
-UNITS = [os.path.join(CSRC, f) for f in ("fw_kernels.hip", "fw_rollout.hip", "fw_sequence.hip")]
+UNITS = [os.path.join(CSRC, f) for f in ("fw_kernels.hip", "fw_rollout.hip", "fw_sequence.hip", "fw_groupnorm.hip")]
 SOURCES = UNITS + [os.path.join(CSRC, "fw_seq_common.hpp"), os.path.join(CSRC, "fw_device.hpp"), os.path.join(CSRC, "fw_quad.hpp"), os.path.join(CSRC, "fw_stats.hpp"), os.path.join(CSRC, "fw_x8_consts.inc")] + HEADERS
 ARCH = os.environ.get("FWSIM_ARCH", "gfx950")
 
@@ -161,6 +161,10 @@ SIGNATURES = {
     "fw_linattn_forward": (_c.c_int, [_vp, _vp]),
     "fw_linattn_backward": (_c.c_int, [_vp, _vp]),
     "fw_linattn_step": (_c.c_int, [_vp, _vp]),
+    "fw_group_norm_stats": (_c.c_int, [_vp]),
+    "fw_group_norm_workspace_bytes": (_c.c_size_t, [_vp, _i32]),
+    "fw_group_norm_forward": (_c.c_int, [_vp, _vp]),
+    "fw_group_norm_backward": (_c.c_int, [_vp, _vp]),
 }
 
 
@@ -213,6 +217,17 @@ class FwLinattnToken(ctypes.Structure):  # include/fwrollout.h fw_linattn_token
     _fields_ = [("N", _i64), ("H", _i32), ("Dk", _i32), ("Dv", _i32), ("dtype", _i32)] + \
                [(k, FwSeqTensor) for k in ("q", "k", "v", "out")] + \
                [("log_decay", _vp), ("starts", _vp), ("starts_sn", _i64), ("state", _vp), ("state_out", _vp)]
+
+
+class FwRows(ctypes.Structure):  # include/fwrollout.h fw_rows
+    _fields_ = [("p", _vp), ("sn", _i64), ("sl", _i64)]
+
+
+class FwGroupNorm(ctypes.Structure):  # include/fwrollout.h fw_group_norm
+    _fields_ = [("N", _i64), ("L", _i64), ("C", _i32), ("G", _i32), ("dtype", _i32), ("wdtype", _i32), ("act", _i32),
+                ("pad", _i32), ("eps", _c.c_double)] + [(k, FwRows) for k in ("x", "y", "dy", "dx")] + \
+               [(k, _vp) for k in ("weight", "bias", "dweight", "dbias", "stats", "workspace")] + \
+               [("workspace_bytes", _c.c_size_t)]
 
 
 def load(path=None):

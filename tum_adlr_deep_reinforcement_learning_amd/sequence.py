@@ -224,3 +224,116 @@ def linear_attention_step(q, k, v, log_decay, state, episode_starts=None, state_
     with torch.cuda.device(dev):
         _native.check(_native.load().fw_linattn_step(ctypes.byref(a), _stream(dev)), "fw_linattn_step")
     return out
+
+
+# ------------------------------------------------------------------ group norm
+_ACT = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "tanh": 4}  # include/fwrollout.h FW_ACT_*
+
+
+def _rows(s, t):
+    s.p, s.sn, s.sl = t.data_ptr(), t.stride(0), t.stride(1)
+
+
+def _norm_args(x, groups, weight, bias, eps, act):
+    a = _native.FwGroupNorm()
+    a.N, a.L, a.C = x.shape
+    a.G, a.dtype, a.act, a.eps = groups, _DT[x.dtype], act, eps
+    p = weight if weight is not None else bias
+    a.wdtype = _DT[p.dtype] if p is not None else 0
+    a.weight, a.bias = _ptr(weight), _ptr(bias)
+    _rows(a.x, x)
+    return a
+
+
+def _norm_workspace(lib, a, device, backward):
+    n = lib.fw_group_norm_workspace_bytes(ctypes.byref(a), backward)
+    ws = torch.empty(n, dtype=torch.uint8, device=device) if n else None
+    a.workspace, a.workspace_bytes = _ptr(ws), n
+    return ws
+
+
+def _norm_forward(x, groups, weight, bias, eps, act, keep):
+    lib = _native.load()
+    a = _norm_args(x, groups, weight, bias, eps, act)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    _rows(a.y, y)
+    stats = None
+    if keep and lib.fw_group_norm_stats(ctypes.byref(a)):
+        stats = torch.empty((a.N, groups, 2), dtype=torch.float32, device=x.device)
+        a.stats = stats.data_ptr()
+    with torch.cuda.device(x.device):
+        ws = _norm_workspace(lib, a, x.device, 0)  # noqa: F841
+        _native.check(lib.fw_group_norm_forward(ctypes.byref(a), _stream(x.device)), "fw_group_norm_forward")
+    return y, stats
+
+
+class _GroupNormAct(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, groups, eps, act):
+        y, stats = _norm_forward(x, groups, weight, bias, eps, act, True)
+        ctx.save_for_backward(x, weight, bias, stats)
+        ctx.conf = (groups, eps, act)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, weight, bias, stats = ctx.saved_tensors
+        groups, eps, act = ctx.conf
+        lib = _native.load()
+        dy = _dense(dy)
+        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        dw = torch.empty_like(weight) if weight is not None and ctx.needs_input_grad[1] else None
+        db = torch.empty_like(bias) if bias is not None and ctx.needs_input_grad[2] else None
+        if x.numel() == 0:
+            return (dx,) + tuple(t.zero_() if t is not None else None for t in (dw, db)) + (None, None, None)
+        a = _norm_args(x, groups, weight, bias, eps, act)
+        _rows(a.dy, dy)
+        _rows(a.dx, dx)
+        a.dweight, a.dbias, a.stats = _ptr(dw), _ptr(db), _ptr(stats)
+        with torch.cuda.device(x.device):
+            ws = _norm_workspace(lib, a, x.device, 1)  # noqa: F841
+            _native.check(lib.fw_group_norm_backward(ctypes.byref(a), _stream(x.device)), "fw_group_norm_backward")
+        return dx, dw, db, None, None, None
+
+
+def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, activation="silu"):
+    """``activation(group_norm(x))``, channels last: x [N, ..., C] of float32, bfloat16 or float16.
+
+    The C channels form ``num_groups`` groups of neighbours; the statistics of a sample's group run over its channels
+    and over every dimension between the first and the last (none of them: per row, as for a policy's features).
+    weight, bias: [C] in x's dtype or float32 (both the same), or None.  activation: "none", "relu", "silu", "gelu" (by
+    erf) or "tanh".  Returns a contiguous tensor of x's shape and dtype.  Any strides with unit channel stride are
+    read in place.  Differentiable in x, weight and bias; deterministic."""
+    if not isinstance(x, torch.Tensor) or x.dim() < 2:
+        raise ValueError("group_norm_act: x must be an [N, ..., C] tensor")
+    if x.device.type != "cuda":
+        raise ValueError("group_norm_act: x must be on the GPU (no CPU path exists)")
+    if x.dtype not in _DT:
+        raise ValueError("group_norm_act: x must be float32, bfloat16 or float16")
+    C, groups = x.shape[-1], int(num_groups)
+    if groups < 1 or C < 1 or C % groups:
+        raise ValueError("group_norm_act: %d channels do not form %d groups" % (C, groups))
+    if activation not in _ACT:
+        raise ValueError("group_norm_act: activation must be one of %s" % ", ".join(_ACT))
+    if not float(eps) >= 0.0:
+        raise ValueError("group_norm_act: eps must be >= 0")
+    for name, p in (("weight", weight), ("bias", bias)):
+        if p is not None and (not isinstance(p, torch.Tensor) or p.shape != (C,) or p.device != x.device or
+                              p.dtype not in (x.dtype, torch.float32)):
+            raise ValueError("group_norm_act: %s must be a [C] tensor of x's dtype or float32 on its device" % name)
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise ValueError("group_norm_act: weight and bias must share a dtype")
+    shape = x.shape
+    rows = 1
+    for d in shape[1:-1]:
+        rows *= d
+    x = _dense(x.reshape(shape[0], rows, C))
+    weight = weight.contiguous() if weight is not None else None
+    bias = bias.contiguous() if bias is not None else None
+    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or
+                                    (bias is not None and bias.requires_grad)):
+        y = _GroupNormAct.apply(x, weight, bias, groups, float(eps), _ACT[activation])
+    else:
+        y = _norm_forward(x, groups, weight, bias, float(eps), _ACT[activation], False)[0]
+    return y.view(shape)
