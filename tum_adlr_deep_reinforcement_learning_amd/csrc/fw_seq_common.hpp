@@ -24,7 +24,9 @@ int set_error(int code, const std::string& msg);
 namespace fwseq {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 struct bf16 {  // storage only; arithmetic is in float
@@ -52,6 +54,13 @@ template <>
 __device__ __forceinline__ f16 from_f32<f16>(float x) {
   return f16{(_Float16)x};
 }
+
+// two floats as a pair of bfloat16 (to nearest), and the halves of a pair as floats
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{lo, hi}), bf16x2));
+}
+__device__ __forceinline__ float lo_f32(uint32_t p) { return __uint_as_float(p << 16); }
+__device__ __forceinline__ float hi_f32(uint32_t p) { return __uint_as_float(p & 0xffff0000u); }
 
 // n elements moved as one access of up to 16 bytes
 template <typename T, int N>

@@ -11,6 +11,7 @@
 // with the states transposed where the roles of k and v change, so one kernel serves all four, and the backward
 // pass keeps nothing of the forward pass.
 #include <algorithm>
+#include <type_traits>
 
 #include "fw_seq_common.hpp"
 
@@ -33,16 +34,42 @@ struct State {  // element (n, h, seg, k, v) at p + n sn + h sh + seg sg + k sk 
 struct Pass {
   Operand q, k, v, o;  // o.p NULL: only the state is wanted
   State in, out;       // p NULL: zeros / not wanted
+  int32_t rev;         // runs from the last token to the first
 };
 struct ScanArgs {
-  Pass pass[2];
-  int32_t n_pass, Dk, Dv, H, rev, n_slice, n_seg, run_seg;  // segments [0, run_seg) in processing order
+  Pass pass[3];
+  int32_t n_pass, Dk, Dv, H, n_slice, n_seg, run_seg;  // segments [0, run_seg) in processing order
   int64_t T, N, seg_len;
   const float* log_decay;
   const uint8_t* starts;
   int64_t starts_st, starts_sn;
   const int32_t* lengths;
   float* factor;  // [n_pass][N][H][n_seg]: what a segment multiplies a state with, or NULL
+};
+
+// What one wave works on: unit = (((seg N + n) H + h) n_slice + slice) n_pass + pass, so that the waves of a block share
+// rows (slices and passes the same ones, heads neighbouring ones).
+struct Unit {
+  int pass, slice, h, seg;  // seg in processing order
+  int64_t n, seg0, seg1, L;  // the segment's tokens [seg0, seg1), of which the first L are live
+  __device__ __forceinline__ bool decode(const ScanArgs& A) {
+    int64_t u = (int64_t)blockIdx.x * SCAN_WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    pass = (int)(u % A.n_pass);
+    u /= A.n_pass;
+    slice = (int)(u % A.n_slice);
+    u /= A.n_slice;
+    h = (int)(u % A.H);
+    u /= A.H;
+    n = u % A.N;
+    seg = (int)(u / A.N);
+    if (seg >= A.run_seg) return false;
+    seg0 = (A.pass[pass].rev ? A.n_seg - 1 - seg : seg) * A.seg_len;
+    seg1 = min(seg0 + A.seg_len, A.T);
+    int64_t len = A.T;
+    if (A.lengths) len = max((int64_t)0, min(A.T, (int64_t)A.lengths[n]));
+    L = max((int64_t)0, min(len, seg1) - seg0);
+    return true;
+  }
 };
 
 enum { FULL, GUARD, SCALAR };  // D fills the tiles; whole vectors in or out; element by element
@@ -89,26 +116,13 @@ template <typename T, int KT, int VT, int MODE>
 __global__ __launch_bounds__(64 * SCAN_WAVES) void k_scan(ScanArgs A) {
   constexpr int C = 16, TPL = 4;
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-  // unit = (((seg N + n) H + h) n_slice + slice) n_pass + pass
-  int64_t u = (int64_t)blockIdx.x * SCAN_WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int pi = (int)(u % A.n_pass);
-  u /= A.n_pass;
-  const int slice = (int)(u % A.n_slice);
-  u /= A.n_slice;
-  const int h = (int)(u % A.H);
-  u /= A.H;
-  const int64_t n = u % A.N;
-  const int seg = (int)(u / A.N);  // in processing order
-  if (seg >= A.run_seg) return;
-  const Pass& p = A.pass[pi];
+  Unit U;
+  if (!U.decode(A)) return;
+  const Pass& p = A.pass[U.pass];
+  const int64_t n = U.n, seg0 = U.seg0, seg1 = U.seg1, L = U.L;
+  const int h = U.h, seg = U.seg, slice = U.slice;
+  const bool rev = p.rev;
   const int Dk = A.Dk, Dv = A.Dv, v0 = slice * 16 * VT;
-  const bool rev = A.rev;
-  const int64_t seg0 = (rev ? A.n_seg - 1 - seg : seg) * A.seg_len;  // the segment's tokens: [seg0, seg1)
-  const int64_t seg1 = min(seg0 + A.seg_len, A.T);
-  int64_t len = A.T;
-  if (A.lengths) len = max((int64_t)0, min(A.T, (int64_t)A.lengths[n]));
-  const int64_t L = max((int64_t)0, min(len, seg1) - seg0);  // of which the first L are live
-
   const T* qb = (const T*)p.q.p + n * p.q.sn + h * p.q.sh + seg0 * p.q.st;
   const T* kb = (const T*)p.k.p + n * p.k.sn + h * p.k.sh + seg0 * p.k.st;
   const T* vb = (const T*)p.v.p + n * p.v.sn + h * p.v.sh + seg0 * p.v.st + v0;
@@ -268,11 +282,326 @@ __global__ __launch_bounds__(64 * SCAN_WAVES) void k_scan(ScanArgs A) {
         }
   }
   if (A.factor && slice == 0 && lane == 0)
-    A.factor[((pi * A.N + n) * A.H + h) * A.n_seg + seg] = fresh ? 0.f : (L == 0 ? 1.f : expf(ld * (float)L));
+    A.factor[((U.pass * A.N + n) * A.H + h) * A.n_seg + seg] = fresh ? 0.f : (L == 0 ? 1.f : expf(ld * (float)L));
   if (want_out) {  // rows behind the sequence's end
     const float z[4 * VT] = {};
     for (int64_t t = L + r; t < seg1 - seg0; t += 16)
       store_cols<T, 4 * VT, MODE>(ob + t * p.o.st, 4 * VT * g, Dv - v0, z);
+  }
+}
+
+
+// ------------------------------------------------------------------ bfloat16
+// The same scan on the 16x16x32 product of bfloat16: blocks of C = 32 tokens, depth 8 g + j of lane group g.
+//   tokens       8 g + j: key tile kt holds token 8 g + 4 kt + i in row 4 g + i, query tile qt token 16 qt + r in column r
+//   key columns  4 KT g + e as above, eight e to a product (KT = 1: four, the rest zeros)
+// Products of the inputs are exact in the float32 accumulators.  What is not an input is split into bfloat16 terms:
+// weighted scores and the state into two (2^-16 of a term, below the output's own half step), the weighted keys that
+// enter the state into three (exact to float32: the state is a float32 result).
+__device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+// NE elements of a row, packed in pairs
+template <int NE, int MODE>
+__device__ __forceinline__ void load_raw(const bf16* row, int col, int D, uint32_t* x) {
+  if constexpr (MODE == SCALAR || NE == 1) {
+#pragma unroll
+    for (int i = 0; i < NE; i++) {
+      const uint32_t e = row[MODE == FULL || col + i < D ? col + i : 0].u;
+      if (i & 1)
+        x[i / 2] |= e << 16;
+      else
+        x[i / 2] = e;
+    }
+  } else {
+    constexpr int P = NE < 8 ? NE : 8;
+#pragma unroll
+    for (int i = 0; i < NE; i += P) {
+      struct alignas(2 * P) V {
+        uint32_t e[P / 2];
+      };
+      const V v = *(const V*)(row + (MODE == FULL || col + i < D ? col + i : 0));
+#pragma unroll
+      for (int k = 0; k < P / 2; k++) x[i / 2 + k] = v.e[k];
+    }
+  }
+}
+// element a of two rows as a pair
+__device__ __forceinline__ uint32_t pair(const uint32_t* x0, const uint32_t* x1, int a) {
+  return __builtin_amdgcn_perm(x1[a / 2], x0[a / 2], a & 1 ? 0x07060302u : 0x05040100u);
+}
+
+template <int KT, int VT>
+struct Block16 {  // a block's operands as loaded
+  static constexpr int KW = (KT + 1) / 2, VW = (VT + 1) / 2, QW = 2 * KT;
+  uint32_t k2[8][KW], v[8][VW], q[2][QW], k1[2][QW];
+};
+
+template <int KT, int VT, int MODE>
+__global__ __launch_bounds__(64 * SCAN_WAVES, 1) void k_scan16(ScanArgs A) {
+  constexpr int C = 32, TPL = 8, NS = KT < 2 ? 1 : KT / 2;
+  using B16 = Block16<KT, VT>;
+  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+  Unit U;
+  if (!U.decode(A)) return;
+  const Pass& p = A.pass[U.pass];
+  const int64_t n = U.n, seg0 = U.seg0, seg1 = U.seg1, L = U.L;
+  const int h = U.h, seg = U.seg;
+  const bool rev = p.rev;
+  const int Dk = A.Dk, Dv = A.Dv, v0 = U.slice * 16 * VT;
+  const bf16* qb = (const bf16*)p.q.p + n * p.q.sn + h * p.q.sh + seg0 * p.q.st;
+  const bf16* kb = (const bf16*)p.k.p + n * p.k.sn + h * p.k.sh + seg0 * p.k.st;
+  const bf16* vb = (const bf16*)p.v.p + n * p.v.sn + h * p.v.sh + seg0 * p.v.st + v0;
+  bf16* ob = (bf16*)p.o.p + n * p.o.sn + h * p.o.sh + seg0 * p.o.st + v0;
+  const bool want_out = p.o.p != nullptr;
+  const uint8_t* xb = A.starts ? A.starts + n * A.starts_sn + seg0 * A.starts_st : nullptr;
+  const float ld = A.log_decay[h];
+  auto power = [&](int m) { return m == 0 ? 1.0f : expf(ld * (float)m); };
+
+  f32x4 S[KT][VT];
+#pragma unroll
+  for (int a = 0; a < KT; a++)
+#pragma unroll
+    for (int f = 0; f < VT; f++) {
+      S[a][f] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (p.in.p) {
+        const float* s = p.in.p + n * p.in.sn + h * p.in.sh + seg * p.in.sg;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const int dk = KT * (4 * g + i) + a, dv = v0 + VT * r + f;
+          if (dk < Dk && dv < Dv) S[a][f][i] = s[(int64_t)dk * p.in.sk + (int64_t)dv * p.in.sv];
+        }
+      }
+    }
+
+  float wp[2][2][4], wi[2], wu[TPL], em1 = 0.f;
+  int cur = 0;
+#pragma unroll
+  for (int kt = 0; kt < 2; kt++)
+#pragma unroll
+    for (int qt = 0; qt < 2; qt++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const int d = (16 * qt + r - 8 * g - 4 * kt - i) * (rev ? -1 : 1);
+        wp[kt][qt][i] = d >= 0 ? power(d) : 0.f;
+      }
+
+  auto fetch = [&](B16& b, int64_t t0, int c) {  // rows behind the block are read from its last token
+#pragma unroll
+    for (int j = 0; j < TPL; j++) {
+      const int64_t row = t0 + (c == C ? TPL * g + j : min(TPL * g + j, c - 1));
+      load_raw<VT, MODE>(vb + row * p.v.st, VT * r, Dv - v0, b.v[j]);
+      load_raw<KT, MODE>(kb + row * p.k.st, KT * r, Dk, b.k2[j]);
+    }
+    if (want_out) {
+#pragma unroll
+      for (int z = 0; z < 2; z++) {
+        const int kr = 8 * (r >> 2) + 4 * z + (r & 3), qr = 16 * z + r;
+        load_raw<4 * KT, MODE>(qb + (t0 + (c == C ? qr : min(qr, c - 1))) * p.q.st, 4 * KT * g, Dk, b.q[z]);
+        load_raw<4 * KT, MODE>(kb + (t0 + (c == C ? kr : min(kr, c - 1))) * p.k.st, 4 * KT * g, Dk, b.k1[z]);
+      }
+    }
+  };
+
+  bool fresh = false, loaded = false;
+  int64_t done = 0;
+  int single = 0;
+  B16 b, nb;
+  while (done < L) {
+    const int c = single ? 1 : (int)min((int64_t)C, L - done);
+    const int64_t t0 = rev ? L - done - c : done;
+    if (!loaded) fetch(b, t0, c);
+    loaded = !single && done + c < L;
+    if (loaded) {  // the next block's operands, while this one is computed
+      const int c2 = (int)min((int64_t)C, L - done - c);
+      fetch(nb, rev ? t0 - c2 : t0 + c, c2);
+    }
+    if (c != cur) {
+      cur = c;
+#pragma unroll
+      for (int qt = 0; qt < 2; qt++) wi[qt] = power(rev ? max(c - 1 - 16 * qt - r, 0) : 16 * qt + r + 1);
+#pragma unroll
+      for (int j = 0; j < TPL; j++) {
+        const int s = TPL * g + j;
+        wu[j] = s < c ? power(rev ? s + 1 : c - 1 - s) : 0.f;
+      }
+      em1 = expm1f(ld * (float)c);
+    }
+    uint32_t M = 0;
+    if (xb) M = (uint32_t)__ballot(lane < c && xb[(t0 + (lane < c ? lane : 0)) * A.starts_st] != 0);
+
+    u32x4 V[VT];  // tile f: tokens 8 g .. 8 g + 7 of value column VT r + f
+#pragma unroll
+    for (int f = 0; f < VT; f++)
+#pragma unroll
+      for (int m = 0; m < 4; m++) {
+        V[f][m] = pair(b.v[2 * m], b.v[2 * m + 1], f);
+        if (c < C) {
+          if (TPL * g + 2 * m >= c) V[f][m] = 0;
+          else if (TPL * g + 2 * m + 1 >= c) V[f][m] &= 0xffffu;
+        }
+      }
+    if (c > 1) {  // an infinity or a NaN among the values: token by token (see k_scan); 0 x value is 0 or NaN
+      f32x4 bad{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int f = 0; f < VT; f++) bad = mma(V[f], u32x4{0, 0, 0, 0}, bad);
+      if (__any(!(bad[0] + bad[1] + bad[2] + bad[3] == 0.f))) {
+        single = c;
+        loaded = false;
+        continue;
+      }
+    }
+    fresh |= M != 0;
+
+    if (want_out) {
+      f32x4 O[VT][2], P[2][2];
+#pragma unroll
+      for (int qt = 0; qt < 2; qt++) {
+#pragma unroll
+        for (int f = 0; f < VT; f++) O[f][qt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int kt = 0; kt < 2; kt++) P[kt][qt] = f32x4{0.f, 0.f, 0.f, 0.f};
+      }
+#pragma unroll
+      for (int s = 0; s < NS; s++) {
+        u32x4 Q[2], K1[2];
+#pragma unroll
+        for (int z = 0; z < 2; z++)
+#pragma unroll
+          for (int m = 0; m < 4; m++) {
+            Q[z][m] = 4 * s + m < B16::QW ? b.q[z][4 * s + m] : 0;
+            K1[z][m] = 4 * s + m < B16::QW ? b.k1[z][4 * s + m] : 0;
+            if constexpr (MODE != FULL) {
+              const int e = 4 * KT * g + 8 * s + 2 * m;
+              if (e >= Dk) Q[z][m] = 0;
+              else if (e + 1 >= Dk) Q[z][m] &= 0xffffu;
+            }
+          }
+#pragma unroll
+        for (int kt = 0; kt < 2; kt++)
+#pragma unroll
+          for (int qt = 0; qt < 2; qt++) P[kt][qt] = mma(K1[kt], Q[qt], P[kt][qt]);
+#pragma unroll
+        for (int f = 0; f < VT; f++) {
+          u32x4 hi{0, 0, 0, 0}, lo{0, 0, 0, 0};
+#pragma unroll
+          for (int m = 0; m < (KT < 2 ? 2 : 4); m++) {
+            const int e = 8 * s + 2 * m;
+            const float x0 = S[e % KT][f][e / KT], x1 = S[(e + 1) % KT][f][(e + 1) / KT];
+            hi[m] = pack_bf16(x0, x1);
+            lo[m] = pack_bf16(x0 - lo_f32(hi[m]), x1 - hi_f32(hi[m]));
+          }
+#pragma unroll
+          for (int qt = 0; qt < 2; qt++) {
+            O[f][qt] = mma(hi, Q[qt], O[f][qt]);
+            O[f][qt] = mma(lo, Q[qt], O[f][qt]);
+          }
+        }
+      }
+      u32x4 Ph[2], Pl[2];
+#pragma unroll
+      for (int qt = 0; qt < 2; qt++) {
+        const int t = 16 * qt + r;
+        const bool blocked = M != 0 && (rev ? (M >> t) >> 1 : M & ((2u << t) - 1)) != 0;
+#pragma unroll
+        for (int f = 0; f < VT; f++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) O[f][qt][i] = blocked ? 0.f : O[f][qt][i] * wi[qt];
+#pragma unroll
+        for (int kt = 0; kt < 2; kt++) {
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            const int s = 8 * g + 4 * kt + i;
+            bool keep = rev ? s >= t && s < c : s <= t;
+            if (M != 0) keep = keep && ((M >> min(s, t)) >> 1 & ((1u << abs(s - t)) - 1)) == 0;
+            P[kt][qt][i] = keep ? P[kt][qt][i] * wp[kt][qt][i] : 0.f;
+          }
+#pragma unroll
+          for (int m = 0; m < 2; m++) {
+            const float x0 = P[kt][qt][2 * m], x1 = P[kt][qt][2 * m + 1];
+            const uint32_t hi = pack_bf16(x0, x1);
+            Ph[qt][2 * kt + m] = hi;
+            Pl[qt][2 * kt + m] = pack_bf16(x0 - lo_f32(hi), x1 - hi_f32(hi));
+          }
+        }
+      }
+#pragma unroll
+      for (int f = 0; f < VT; f++)
+#pragma unroll
+        for (int qt = 0; qt < 2; qt++) {
+          O[f][qt] = mma(V[f], Ph[qt], O[f][qt]);
+          O[f][qt] = mma(V[f], Pl[qt], O[f][qt]);
+        }
+#pragma unroll
+      for (int qt = 0; qt < 2; qt++)
+        if (16 * qt + r < c) {
+          float x[4 * VT];
+#pragma unroll
+          for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int f = 0; f < VT; f++) x[VT * i + f] = O[f][qt][i];
+          store_cols<bf16, 4 * VT, MODE>(ob + (t0 + 16 * qt + r) * p.o.st, 4 * VT * g, Dv - v0, x);
+        }
+    }
+
+#pragma unroll
+    for (int a = 0; a < KT; a++)
+#pragma unroll
+      for (int f = 0; f < VT; f++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) S[a][f][i] = M != 0 ? 0.f : fmaf(S[a][f][i], em1, S[a][f][i]);
+    bool keep[TPL];
+#pragma unroll
+    for (int j = 0; j < TPL; j++) {
+      const int s = TPL * g + j;
+      keep[j] = s < c;
+      if (M != 0) keep[j] = keep[j] && (rev ? M & ((2u << s) - 1) : (M >> s) >> 1) == 0;
+    }
+#pragma unroll
+    for (int a = 0; a < KT; a++) {
+      u32x4 t0, t1, t2;
+#pragma unroll
+      for (int m = 0; m < 4; m++) {
+        const uint32_t kk = pair(b.k2[2 * m], b.k2[2 * m + 1], a);
+        // selects, so that nothing masked gets through
+        float x0 = keep[2 * m] ? lo_f32(kk) * wu[2 * m] : 0.f, x1 = keep[2 * m + 1] ? hi_f32(kk) * wu[2 * m + 1] : 0.f;
+        t0[m] = pack_bf16(x0, x1);
+        x0 -= lo_f32(t0[m]);
+        x1 -= hi_f32(t0[m]);
+        t1[m] = pack_bf16(x0, x1);
+        t2[m] = pack_bf16(x0 - lo_f32(t1[m]), x1 - hi_f32(t1[m]));
+      }
+#pragma unroll
+      for (int f = 0; f < VT; f++) {
+        S[a][f] = mma(t0, V[f], S[a][f]);
+        S[a][f] = mma(t1, V[f], S[a][f]);
+        S[a][f] = mma(t2, V[f], S[a][f]);
+      }
+    }
+    done += c;
+    if (single) single--;
+    if (loaded) b = nb;
+  }
+
+  if (p.out.p && (seg == A.n_seg - 1 || p.out.sg)) {
+    float* s = p.out.p + n * p.out.sn + h * p.out.sh + seg * p.out.sg;
+#pragma unroll
+    for (int a = 0; a < KT; a++)
+#pragma unroll
+      for (int f = 0; f < VT; f++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const int dk = KT * (4 * g + i) + a, dv = v0 + VT * r + f;
+          if (dk < Dk && dv < Dv) s[(int64_t)dk * p.out.sk + (int64_t)dv * p.out.sv] = S[a][f][i];
+        }
+  }
+  if (A.factor && U.slice == 0 && lane == 0)
+    A.factor[((U.pass * A.N + n) * A.H + h) * A.n_seg + seg] = fresh ? 0.f : (L == 0 ? 1.f : expf(ld * (float)L));
+  if (want_out) {
+    const float z[4 * VT] = {};
+    for (int64_t t = L + r; t < seg1 - seg0; t += 16)
+      store_cols<bf16, 4 * VT, MODE>(ob + t * p.o.st, 4 * VT * g, Dv - v0, z);
   }
 }
 
@@ -415,12 +744,19 @@ int launch_mode(const ScanArgs& A, int mode, hipStream_t s) {
   const int64_t blocks = (units + SCAN_WAVES - 1) / SCAN_WAVES;
   if (blocks > INT32_MAX) return fw::set_error(FW_E_INVALID, "linear attention: too many sequences for one call");
   const dim3 grid((unsigned)blocks), block(64 * SCAN_WAVES);
+  auto kernel = [&](auto m) {
+    constexpr int MODE = decltype(m)::value;
+    if constexpr (std::is_same_v<T, bf16>)
+      return k_scan16<KT, VT, MODE>;
+    else
+      return k_scan<T, KT, VT, MODE>;
+  };
   if (mode == FULL)
-    hipLaunchKernelGGL((k_scan<T, KT, VT, FULL>), grid, block, 0, s, A);
+    hipLaunchKernelGGL(kernel(std::integral_constant<int, FULL>()), grid, block, 0, s, A);
   else if (mode == GUARD)
-    hipLaunchKernelGGL((k_scan<T, KT, VT, GUARD>), grid, block, 0, s, A);
+    hipLaunchKernelGGL(kernel(std::integral_constant<int, GUARD>()), grid, block, 0, s, A);
   else
-    hipLaunchKernelGGL((k_scan<T, KT, VT, SCALAR>), grid, block, 0, s, A);
+    hipLaunchKernelGGL(kernel(std::integral_constant<int, SCALAR>()), grid, block, 0, s, A);
   FW_HIP(hipGetLastError());
   return FW_OK;
 }
@@ -503,10 +839,9 @@ bool room(const fw_linattn* a, bool backward) {
   return need == 0 || (a->workspace && a->workspace_bytes >= need);
 }
 Operand in(const fw_seq_tensor& t) { return {t.p, t.st, t.sn, t.sh}; }
-ScanArgs base(const fw_linattn* a, bool rev) {
+ScanArgs base(const fw_linattn* a) {
   ScanArgs A{};
   A.H = a->H;
-  A.rev = rev;
   A.T = a->T;
   A.N = a->N;
   A.log_decay = a->log_decay;
@@ -534,14 +869,14 @@ int fw_linattn_forward(const fw_linattn* a, void* stream) {
   if (a->N == 0) return FW_OK;
   if (a->T > 0 && !a->out.p) return fw::set_error(FW_E_INVALID, "fw_linattn_forward: NULL out");
   if (!room(a, false)) return fw::set_error(FW_E_INVALID, "fw_linattn_forward: workspace too small");
-  ScanArgs A = base(a, false);
+  ScanArgs A = base(a);
   A.n_pass = 1;
   A.Dk = a->Dk;
   A.Dv = a->Dv;
   const int64_t E = (int64_t)a->Dk * a->Dv;
   A.pass[0] = Pass{in(a->q), in(a->k), in(a->v), in(a->out),
                    State{const_cast<float*>(a->state_in), a->H * E, E, 0, a->Dv, 1},
-                   State{a->state_out, a->H * E, E, 0, a->Dv, 1}};
+                   State{a->state_out, a->H * E, E, 0, a->Dv, 1}, 0};
   return run_passes(a->dtype, A, plan(a->T, a->N, a->H, a->Dv), (float*)a->workspace, (hipStream_t)stream);
 }
 
@@ -558,18 +893,17 @@ int fw_linattn_backward(const fw_linattn* a, void* stream) {
   auto turned = [&](const float* p) { return State{const_cast<float*>(p), a->H * E, E, 0, 1, a->Dv}; };
   const State none{};
   const Plan pk = plan(a->T, a->N, a->H, a->Dk), pv = plan(a->T, a->N, a->H, a->Dv);
-  ScanArgs A = base(a, false);
+  ScanArgs A = base(a);
   A.n_pass = 1;
   A.Dk = a->Dv;
   A.Dv = a->Dk;
-  A.pass[0] = Pass{in(a->dout), in(a->v), in(a->k), in(a->dq), turned(a->state_in), none};
+  A.pass[0] = Pass{in(a->dout), in(a->v), in(a->k), in(a->dq), turned(a->state_in), none, 0};
   if (int rc = run_passes(a->dtype, A, pk, ws, s)) return rc;
-  A.rev = 1;
-  A.pass[0] = Pass{in(a->v), in(a->dout), in(a->q), in(a->dk), turned(a->dstate), none};
+  A.pass[0] = Pass{in(a->v), in(a->dout), in(a->q), in(a->dk), turned(a->dstate), none, 1};
   if (int rc = run_passes(a->dtype, A, pk, ws, s)) return rc;
   A.Dk = a->Dk;
   A.Dv = a->Dv;
-  A.pass[0] = Pass{in(a->k), in(a->q), in(a->dout), in(a->dv), straight(a->dstate), straight(a->dstate_in)};
+  A.pass[0] = Pass{in(a->k), in(a->q), in(a->dout), in(a->dv), straight(a->dstate), straight(a->dstate_in), 1};
   return run_passes(a->dtype, A, pv, ws, s);
 }
 
