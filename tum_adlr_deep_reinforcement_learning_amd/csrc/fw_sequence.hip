@@ -47,22 +47,21 @@ struct ScanArgs {
   float* factor;  // [n_pass][N][H][n_seg]: what a segment multiplies a state with, or NULL
 };
 
-// What one wave works on: unit = (((seg N + n) H + h) n_slice + slice) n_pass + pass, so that the waves of a block share
+// What one wave works on: unit = ((n H + h) n_slice + slice) n_pass + pass of segment blockIdx.y, so that the waves of a block share
 // rows (slices and passes the same ones, heads neighbouring ones).
 struct Unit {
   int pass, slice, h, seg;  // seg in processing order
   int64_t n, seg0, seg1, L;  // the segment's tokens [seg0, seg1), of which the first L are live
   __device__ __forceinline__ bool decode(const ScanArgs& A) {
-    int64_t u = (int64_t)blockIdx.x * SCAN_WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    pass = (int)(u % A.n_pass);
-    u /= A.n_pass;
-    slice = (int)(u % A.n_slice);
-    u /= A.n_slice;
-    h = (int)(u % A.H);
-    u /= A.H;
-    n = u % A.N;
-    seg = (int)(u / A.N);
-    if (seg >= A.run_seg) return false;
+    uint32_t u = blockIdx.x * SCAN_WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    pass = (int)(u % (uint32_t)A.n_pass);
+    u /= (uint32_t)A.n_pass;
+    slice = (int)(u % (uint32_t)A.n_slice);
+    u /= (uint32_t)A.n_slice;
+    h = (int)(u % (uint32_t)A.H);
+    n = u / (uint32_t)A.H;
+    seg = blockIdx.y;
+    if (n >= A.N) return false;
     seg0 = (A.pass[pass].rev ? A.n_seg - 1 - seg : seg) * A.seg_len;
     seg1 = min(seg0 + A.seg_len, A.T);
     int64_t len = A.T;
@@ -292,160 +291,273 @@ __global__ __launch_bounds__(64 * SCAN_WAVES) void k_scan(ScanArgs A) {
 
 
 // ------------------------------------------------------------------ bfloat16
-// The same scan on the 16x16x32 product of bfloat16: blocks of C = 32 tokens, depth 8 g + j of lane group g.
-//   tokens       8 g + j: key tile kt holds token 8 g + 4 kt + i in row 4 g + i, query tile qt token 16 qt + r in column r
-//   key columns  4 KT g + e as above, eight e to a product (KT = 1: four, the rest zeros)
+// The same scan on the 16x16x32 product of bfloat16, in blocks of C = 32 tokens.  A block's rows are copied to LDS by
+// the load unit while the block before is computed (no registers, no waiting but for the copy itself), in processing
+// order, so that a reversed pass is causal too: its rows run from the last token to the first.
+//   rows         key tile z: row 16 z + r; query tile z: row 16 z + r; as depth j = 4 z + i of lane group g: row
+//                16 z + 4 g + i -- the result registers of the score product are the operand of the value product
+//   key columns  depth 8 s + j of lane group g: 4 KT g + 8 s + j; state tile a: 4 KT g + 4 a + i down its rows
+//   value cols   tile f: 4 VT (r >> 2) + 4 f + (r & 3) across, 4 VT g + 4 f + i down: a lane stores 4 VT neighbours
+// Operands with tokens as depth (keys and values of the state's product, values of the output's) are read from LDS by
+// the transposing read: 4 lanes x 4 columns of one row each become 4 rows x 1 column per lane.
 // Products of the inputs are exact in the float32 accumulators.  What is not an input is split into bfloat16 terms:
-// weighted scores and the state into two (2^-16 of a term, below the output's own half step), the weighted keys that
-// enter the state into three (exact to float32: the state is a float32 result).
+// weighted scores and the state into two (2^-16 of a term, far below the output's own half step), the weighted keys
+// that enter the state into three (exact to float32: the state is a float32 result).
 __device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
-// NE elements of a row, packed in pairs
-template <int NE, int MODE>
-__device__ __forceinline__ void load_raw(const bf16* row, int col, int D, uint32_t* x) {
-  if constexpr (MODE == SCALAR || NE == 1) {
-#pragma unroll
-    for (int i = 0; i < NE; i++) {
-      const uint32_t e = row[MODE == FULL || col + i < D ? col + i : 0].u;
-      if (i & 1)
-        x[i / 2] |= e << 16;
-      else
-        x[i / 2] = e;
-    }
-  } else {
-    constexpr int P = NE < 8 ? NE : 8;
-#pragma unroll
-    for (int i = 0; i < NE; i += P) {
-      struct alignas(2 * P) V {
-        uint32_t e[P / 2];
-      };
-      const V v = *(const V*)(row + (MODE == FULL || col + i < D ? col + i : 0));
-#pragma unroll
-      for (int k = 0; k < P / 2; k++) x[i / 2 + k] = v.e[k];
-    }
-  }
-}
-// element a of two rows as a pair
-__device__ __forceinline__ uint32_t pair(const uint32_t* x0, const uint32_t* x1, int a) {
-  return __builtin_amdgcn_perm(x1[a / 2], x0[a / 2], a & 1 ? 0x07060302u : 0x05040100u);
-}
+// 32 rows of 16 NT columns in LDS, as 16-byte chunks; chunk c of a row is stored at c ^ turn(row), so that neither the
+// row-wise nor the column-wise reads meet in a bank
+template <int NT>
+struct Tile {
+  static constexpr int CH = 2 * NT, BYTES = 32 * 16 * CH, RI = 64 / CH, NI = 32 / RI;  // RI rows per copy instruction
+  __device__ static __forceinline__ int turn(int row) { return (row / (CH >= 8 ? 1 : 8 / CH)) & ((CH < 8 ? CH : 8) - 1); }
+  __device__ static __forceinline__ int at(int row, int chunk) { return (row * CH + (chunk ^ turn(row))) * 16; }
 
-template <int KT, int VT>
-struct Block16 {  // a block's operands as loaded
-  static constexpr int KW = (KT + 1) / 2, VW = (VT + 1) / 2, QW = 2 * KT;
-  uint32_t k2[8][KW], v[8][VW], q[2][QW], k1[2][QW];
-};
-
-template <int KT, int VT, int MODE>
-__global__ __launch_bounds__(64 * SCAN_WAVES, 1) void k_scan16(ScanArgs A) {
-  constexpr int C = 32, TPL = 8, NS = KT < 2 ? 1 : KT / 2;
-  using B16 = Block16<KT, VT>;
-  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-  Unit U;
-  if (!U.decode(A)) return;
-  const Pass& p = A.pass[U.pass];
-  const int64_t n = U.n, seg0 = U.seg0, seg1 = U.seg1, L = U.L;
-  const int h = U.h, seg = U.seg;
-  const bool rev = p.rev;
-  const int Dk = A.Dk, Dv = A.Dv, v0 = U.slice * 16 * VT;
-  const bf16* qb = (const bf16*)p.q.p + n * p.q.sn + h * p.q.sh + seg0 * p.q.st;
-  const bf16* kb = (const bf16*)p.k.p + n * p.k.sn + h * p.k.sh + seg0 * p.k.st;
-  const bf16* vb = (const bf16*)p.v.p + n * p.v.sn + h * p.v.sh + seg0 * p.v.st + v0;
-  bf16* ob = (bf16*)p.o.p + n * p.o.sn + h * p.o.sh + seg0 * p.o.st + v0;
-  const bool want_out = p.o.p != nullptr;
-  const uint8_t* xb = A.starts ? A.starts + n * A.starts_sn + seg0 * A.starts_st : nullptr;
-  const float ld = A.log_decay[h];
-  auto power = [&](int m) { return m == 0 ? 1.0f : expf(ld * (float)m); };
-
-  f32x4 S[KT][VT];
+  // copies rows 0..31 of a block of c rows; row u is token u, or c - 1 - u when reversed; rows behind the block repeat
+  // its last one.  Chunks outside D are left as they are (zeros).  base: the block's first token.
+  template <int MODE>
+  __device__ static __forceinline__ void fetch(char* lds, const bf16* base, int64_t st, int D, int c, bool rev, int lane) {
+    const int row0 = lane / CH, pc = lane % CH;
+    if constexpr (MODE == SCALAR) {
+#pragma unroll 1
+      for (int i = 0; i < NI; i++) {
+        const int row = i * RI + row0, col = (pc ^ turn(row)) * 8, u = min(row, c - 1);
+        const bf16* x = base + (int64_t)(rev ? c - 1 - u : u) * st;
+        u32x4 v;
 #pragma unroll
-  for (int a = 0; a < KT; a++)
+        for (int m = 0; m < 4; m++) {
+          const uint32_t lo = col + 2 * m < D ? x[col + 2 * m].u : 0, hi = col + 2 * m + 1 < D ? x[col + 2 * m + 1].u : 0;
+          v[m] = lo | hi << 16;
+        }
+        *(u32x4*)(lds + (i * 64 + lane) * 16) = v;
+      }
+    } else {
 #pragma unroll
-    for (int f = 0; f < VT; f++) {
-      S[a][f] = f32x4{0.f, 0.f, 0.f, 0.f};
-      if (p.in.p) {
-        const float* s = p.in.p + n * p.in.sn + h * p.in.sh + seg * p.in.sg;
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-          const int dk = KT * (4 * g + i) + a, dv = v0 + VT * r + f;
-          if (dk < Dk && dv < Dv) S[a][f][i] = s[(int64_t)dk * p.in.sk + (int64_t)dv * p.in.sv];
+      for (int i = 0; i < NI; i++) {
+        const int row = i * RI + row0, col = (pc ^ turn(row)) * 8;
+        if (MODE == FULL || col < D) {
+          const char* from;
+          if (c == 32) {  // uniform base + 32-bit lane offset (the launcher saw that 32 rows fit)
+            const int first = rev ? 32 - RI - i * RI : i * RI;
+            from = (const char*)(base + first * st) + (uint32_t)((rev ? RI - 1 - row0 : row0) * (int)st + col) * 2u;
+          } else {
+            const int u = min(row, c - 1);
+            from = (const char*)base + (uint32_t)((rev ? c - 1 - u : u) * (int)st + col) * 2u;
+          }
+          __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
+                                           (__attribute__((address_space(3))) void*)(lds + i * 1024), 16, 0, 0);
         }
       }
     }
+  }
 
-  float wp[2][2][4], wi[2], wu[TPL], em1 = 0.f;
+  // depth step s of rows 16 z + r: columns 4 NT g + 8 s ..
+  __device__ static __forceinline__ u32x4 across(const char* lds, int z, int s, int r, int g) {
+    if constexpr (NT == 1) {
+      const u32x2 v = *(const u32x2*)(lds + at(16 * z + r, g >> 1) + 8 * (g & 1));
+      return u32x4{v[0], v[1], 0, 0};
+    } else {
+      return *(const u32x4*)(lds + at(16 * z + r, NT * g / 2 + s));
+    }
+  }
+  // tile t with the rows as depth
+  __device__ static __forceinline__ u32x4 down(const char* lds, int t, int r, int g) {
+    u32x4 v;
+#pragma unroll
+    for (int z = 0; z < 2; z++) {
+      const int byte = 8 * NT * (r & 3) + 8 * t, row = 16 * z + 4 * g + (r >> 2);
+      const auto x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          (__attribute__((address_space(3))) s16x4*)(lds + at(row, byte >> 4) + (byte & 8)));
+      const u32x2 y = __builtin_bit_cast(u32x2, x);
+      v[2 * z] = y[0];
+      v[2 * z + 1] = y[1];
+    }
+    return v;
+  }
+};
+
+// the same value, but not known to be: keeps what a rare branch computes from it inside that branch
+__device__ __forceinline__ int here(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
+template <int KT, int VT, int MODE>
+__global__ __launch_bounds__(64 * SCAN_WAVES, 2) void k_scan16(ScanArgs A) {
+  constexpr int C = 32, NS = KT < 2 ? 1 : KT / 2;
+  using K = Tile<KT>;
+  using V = Tile<VT>;
+  __shared__ alignas(16) char smem[SCAN_WAVES][2 * K::BYTES + V::BYTES];
+  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+  char* const lq = smem[__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)];
+  char* const lk = lq + K::BYTES;
+  char* const lv = lk + K::BYTES;
+  Unit U;
+  if (!U.decode(A)) return;
+  const Pass& p = A.pass[U.pass];
+  const int64_t n = U.n, L = U.L;
+  const int h = U.h, seg = U.seg;
+  const bool rev = p.rev;
+  const int Dk = A.Dk, Dv = A.Dv, v0 = U.slice * 16 * VT;
+  const bf16* qb = (const bf16*)p.q.p + n * p.q.sn + h * p.q.sh + U.seg0 * p.q.st;
+  const bf16* kb = (const bf16*)p.k.p + n * p.k.sn + h * p.k.sh + U.seg0 * p.k.st;
+  const bf16* vb = (const bf16*)p.v.p + n * p.v.sn + h * p.v.sh + U.seg0 * p.v.st + v0;
+  bf16* ob = (bf16*)p.o.p + n * p.o.sn + h * p.o.sh + U.seg0 * p.o.st + v0;
+  const bool want_out = p.o.p != nullptr;
+  const uint8_t* xb = A.starts ? A.starts + n * A.starts_sn + U.seg0 * A.starts_st : nullptr;
+  float ld = A.log_decay[h];
+  ld = ld < -1e30f ? -1e30f : ld;  // g^0 = 1 for g = 0 too
+  auto power = [&](int m) { return expf(ld * (float)m); };
+
+  auto fetch = [&](int64_t t0, int c) {
+    V::template fetch<MODE>(lv, vb + t0 * p.v.st, p.v.st, Dv - v0, c, rev, lane);
+    K::template fetch<MODE>(lk, kb + t0 * p.k.st, p.k.st, Dk, c, rev, lane);
+    if (want_out) K::template fetch<MODE>(lq, qb + t0 * p.q.st, p.q.st, Dk, c, rev, lane);
+  };
+  if constexpr (MODE == GUARD) {
+    for (int i = lane * 16; i < 2 * K::BYTES + V::BYTES; i += 1024) *(u32x4*)(lq + i) = u32x4{0, 0, 0, 0};
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  }
+  bool loaded = L > 0;
+  if (loaded) {
+    const int c = (int)min((int64_t)C, L);
+    fetch(rev ? L - c : 0, c);
+  }
+
+  f32x4 S[KT][VT];
+  if (p.in.p) {  // outside Dk x Dv: the last row or column, which nothing reads
+    const float* s = p.in.p + n * p.in.sn + h * p.in.sh + seg * p.in.sg;
+#pragma unroll
+    for (int a = 0; a < KT; a++)
+#pragma unroll
+      for (int f = 0; f < VT; f++)
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+          S[a][f][i] = s[min(4 * KT * g + 4 * a + i, Dk - 1) * p.in.sk +
+                         min(v0 + 4 * VT * (r >> 2) + 4 * f + (r & 3), Dv - 1) * p.in.sv];
+  } else {
+#pragma unroll
+    for (int a = 0; a < KT; a++)
+#pragma unroll
+      for (int f = 0; f < VT; f++) S[a][f] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  // Weights.  A reversed pass carries g x the state of the row before: its first weight is 1, and its final state is
+  // the gradient of the initial one.
+  const int e = rev ? 0 : 1;
+  float wd[4], wo[4], wi[2], wu[2][4], em1 = 0.f;  // scores on and off the diagonal tile; state out; state in
   int cur = 0;
 #pragma unroll
-  for (int kt = 0; kt < 2; kt++)
+  for (int i = 0; i < 4; i++) {
+    wd[i] = r >= 4 * g + i ? power(r - 4 * g - i) : 0.f;
+    wo[i] = power(16 + r - 4 * g - i);
+  }
 #pragma unroll
-    for (int qt = 0; qt < 2; qt++)
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        const int d = (16 * qt + r - 8 * g - 4 * kt - i) * (rev ? -1 : 1);
-        wp[kt][qt][i] = d >= 0 ? power(d) : 0.f;
-      }
+  for (int z = 0; z < 2; z++) wi[z] = power(16 * z + r + e);
 
-  auto fetch = [&](B16& b, int64_t t0, int c) {  // rows behind the block are read from its last token
+  bool fresh = false;  // an episode start among the live tokens
+  int64_t done = 0;
+  int single = 0;           // blocks of one token still to go
+  uint32_t held[2][2 * VT];  // the outputs of the block before, stored once the next block's rows are there
+  int64_t held_t = 0;
+  int held_c = 0;
+  auto flush = [&] {
 #pragma unroll
-    for (int j = 0; j < TPL; j++) {
-      const int64_t row = t0 + (c == C ? TPL * g + j : min(TPL * g + j, c - 1));
-      load_raw<VT, MODE>(vb + row * p.v.st, VT * r, Dv - v0, b.v[j]);
-      load_raw<KT, MODE>(kb + row * p.k.st, KT * r, Dk, b.k2[j]);
-    }
-    if (want_out) {
+    for (int z = 0; z < 2; z++) {
+      const int u = 16 * z + r;
+      if (u < held_c) {
+        bf16* o = ob + (held_t + (rev ? held_c - 1 - u : u)) * p.o.st;
+        const int col = 4 * VT * g, D = Dv - v0;
+        if constexpr (MODE == SCALAR) {
 #pragma unroll
-      for (int z = 0; z < 2; z++) {
-        const int kr = 8 * (r >> 2) + 4 * z + (r & 3), qr = 16 * z + r;
-        load_raw<4 * KT, MODE>(qb + (t0 + (c == C ? qr : min(qr, c - 1))) * p.q.st, 4 * KT * g, Dk, b.q[z]);
-        load_raw<4 * KT, MODE>(kb + (t0 + (c == C ? kr : min(kr, c - 1))) * p.k.st, 4 * KT * g, Dk, b.k1[z]);
+          for (int k = 0; k < 4 * VT; k++)
+            if (col + k < D) o[col + k].u = (uint16_t)(held[z][k / 2] >> 16 * (k & 1));
+        } else {
+          constexpr int P = VT == 1 ? 2 : 4;
+          typedef uint32_t W __attribute__((ext_vector_type(P)));
+#pragma unroll
+          for (int k = 0; k < 2 * VT; k += P)
+            if (MODE == FULL || col + 2 * k < D) {
+              W w;
+#pragma unroll
+              for (int x = 0; x < P; x++) w[x] = held[z][k + x];
+              *(W*)(o + col + 2 * k) = w;
+            }
+        }
       }
     }
   };
 
-  bool fresh = false, loaded = false;
-  int64_t done = 0;
-  int single = 0;
-  B16 b, nb;
   while (done < L) {
     const int c = single ? 1 : (int)min((int64_t)C, L - done);
     const int64_t t0 = rev ? L - done - c : done;
-    if (!loaded) fetch(b, t0, c);
+    if (!loaded) {
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+      fetch(t0, c);
+    }
+    uint32_t M = 0;  // bit u: an episode starts at row u
+    if (xb) {
+      const int u = min(lane, c - 1);
+      M = (uint32_t)__ballot(lane < c && xb[(t0 + (rev ? c - 1 - u : u)) * A.starts_st] != 0);
+    }
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    u32x4 vf[VT], k2[KT], kf[2][NS], qf[2][NS];
+#pragma unroll
+    for (int f = 0; f < VT; f++) vf[f] = V::down(lv, f, r, g);
+#pragma unroll
+    for (int a = 0; a < KT; a++) k2[a] = K::down(lk, a, r, g);
+    if (want_out)
+#pragma unroll
+      for (int z = 0; z < 2; z++)
+#pragma unroll
+        for (int s = 0; s < NS; s++) {
+          kf[z][s] = K::across(lk, z, s, r, g);
+          qf[z][s] = K::across(lq, z, s, r, g);
+        }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (want_out) flush();
+    held_c = 0;
     loaded = !single && done + c < L;
-    if (loaded) {  // the next block's operands, while this one is computed
+    if (loaded) {
       const int c2 = (int)min((int64_t)C, L - done - c);
-      fetch(nb, rev ? t0 - c2 : t0 + c, c2);
+      fetch(rev ? t0 - c2 : t0 + c, c2);
     }
     if (c != cur) {
       cur = c;
+      const int g4 = here(4 * g);
 #pragma unroll
-      for (int qt = 0; qt < 2; qt++) wi[qt] = power(rev ? max(c - 1 - 16 * qt - r, 0) : 16 * qt + r + 1);
+      for (int z = 0; z < 2; z++)
 #pragma unroll
-      for (int j = 0; j < TPL; j++) {
-        const int s = TPL * g + j;
-        wu[j] = s < c ? power(rev ? s + 1 : c - 1 - s) : 0.f;
-      }
+        for (int i = 0; i < 4; i++) wu[z][i] = power(max(c - e - (16 * z + g4 + i), 0));
       em1 = expm1f(ld * (float)c);
     }
-    uint32_t M = 0;
-    if (xb) M = (uint32_t)__ballot(lane < c && xb[(t0 + (lane < c ? lane : 0)) * A.starts_st] != 0);
 
-    u32x4 V[VT];  // tile f: tokens 8 g .. 8 g + 7 of value column VT r + f
+    // Masks.  A start at row u of a forward pass cuts every span that contains row u but not from it on; in a reversed
+    // pass the cut lies behind row u, that is at row u + 1.
+    const uint64_t cut = rev ? (uint64_t)M << 1 : (uint64_t)M;
+    if (M != 0 || c < C) {
+      const int g4 = here(4 * g);
 #pragma unroll
-    for (int f = 0; f < VT; f++)
+      for (int z = 0; z < 2; z++)
 #pragma unroll
-      for (int m = 0; m < 4; m++) {
-        V[f][m] = pair(b.v[2 * m], b.v[2 * m + 1], f);
-        if (c < C) {
-          if (TPL * g + 2 * m >= c) V[f][m] = 0;
-          else if (TPL * g + 2 * m + 1 >= c) V[f][m] &= 0xffffu;
+        for (int m = 0; m < 2; m++) {
+          const int u = 16 * z + g4 + 2 * m;
+          const uint32_t live = (u < c ? 0xffffu : 0u) | (u + 1 < c ? 0xffff0000u : 0u);
+          const uint32_t open = ((cut >> u) >> 1 ? 0u : 0xffffu) | ((cut >> (u + 1)) >> 1 ? 0u : 0xffff0000u);
+#pragma unroll
+          for (int f = 0; f < VT; f++) vf[f][2 * z + m] &= live;
+#pragma unroll
+          for (int a = 0; a < KT; a++) k2[a][2 * z + m] &= live & open;
         }
-      }
-    if (c > 1) {  // an infinity or a NaN among the values: token by token (see k_scan); 0 x value is 0 or NaN
+    }
+    // A masked product is a product with 0, which keeps a value away only while that value is finite.  A block with an
+    // infinity or a NaN among its values is therefore run token by token: nothing is masked then.
+    if (c > 1) {
       f32x4 bad{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int f = 0; f < VT; f++) bad = mma(V[f], u32x4{0, 0, 0, 0}, bad);
+      for (int f = 0; f < VT; f++) bad = mma(vf[f], u32x4{0, 0, 0, 0}, bad);  // 0 or NaN
       if (__any(!(bad[0] + bad[1] + bad[2] + bad[3] == 0.f))) {
         single = c;
         loaded = false;
@@ -455,134 +567,123 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, 1) void k_scan16(ScanArgs A) {
     fresh |= M != 0;
 
     if (want_out) {
-      f32x4 O[VT][2], P[2][2];
+      const f32x4 zero{0.f, 0.f, 0.f, 0.f};
+      f32x4 O[VT][2], P[3];  // score tiles (key, query): (0, 0), (0, 1), (1, 1)
 #pragma unroll
-      for (int qt = 0; qt < 2; qt++) {
+      for (int z = 0; z < 2; z++)
 #pragma unroll
-        for (int f = 0; f < VT; f++) O[f][qt] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int f = 0; f < VT; f++) O[f][z] = zero;
 #pragma unroll
-        for (int kt = 0; kt < 2; kt++) P[kt][qt] = f32x4{0.f, 0.f, 0.f, 0.f};
-      }
+      for (int x = 0; x < 3; x++) P[x] = zero;
 #pragma unroll
       for (int s = 0; s < NS; s++) {
-        u32x4 Q[2], K1[2];
-#pragma unroll
-        for (int z = 0; z < 2; z++)
-#pragma unroll
-          for (int m = 0; m < 4; m++) {
-            Q[z][m] = 4 * s + m < B16::QW ? b.q[z][4 * s + m] : 0;
-            K1[z][m] = 4 * s + m < B16::QW ? b.k1[z][4 * s + m] : 0;
-            if constexpr (MODE != FULL) {
-              const int e = 4 * KT * g + 8 * s + 2 * m;
-              if (e >= Dk) Q[z][m] = 0;
-              else if (e + 1 >= Dk) Q[z][m] &= 0xffffu;
-            }
-          }
-#pragma unroll
-        for (int kt = 0; kt < 2; kt++)
-#pragma unroll
-          for (int qt = 0; qt < 2; qt++) P[kt][qt] = mma(K1[kt], Q[qt], P[kt][qt]);
+        P[0] = mma(kf[0][s], qf[0][s], P[0]);
+        P[1] = mma(kf[0][s], qf[1][s], P[1]);
+        P[2] = mma(kf[1][s], qf[1][s], P[2]);
 #pragma unroll
         for (int f = 0; f < VT; f++) {
           u32x4 hi{0, 0, 0, 0}, lo{0, 0, 0, 0};
 #pragma unroll
           for (int m = 0; m < (KT < 2 ? 2 : 4); m++) {
-            const int e = 8 * s + 2 * m;
-            const float x0 = S[e % KT][f][e / KT], x1 = S[(e + 1) % KT][f][(e + 1) / KT];
+            const float x0 = S[2 * s + m / 2][f][2 * (m & 1)], x1 = S[2 * s + m / 2][f][2 * (m & 1) + 1];
             hi[m] = pack_bf16(x0, x1);
             lo[m] = pack_bf16(x0 - lo_f32(hi[m]), x1 - hi_f32(hi[m]));
           }
 #pragma unroll
-          for (int qt = 0; qt < 2; qt++) {
-            O[f][qt] = mma(hi, Q[qt], O[f][qt]);
-            O[f][qt] = mma(lo, Q[qt], O[f][qt]);
+          for (int z = 0; z < 2; z++) {
+            O[f][z] = mma(hi, qf[z][s], O[f][z]);
+            O[f][z] = mma(lo, qf[z][s], O[f][z]);
           }
         }
       }
-      u32x4 Ph[2], Pl[2];
 #pragma unroll
-      for (int qt = 0; qt < 2; qt++) {
-        const int t = 16 * qt + r;
-        const bool blocked = M != 0 && (rev ? (M >> t) >> 1 : M & ((2u << t) - 1)) != 0;
+      for (int z = 0; z < 2; z++)
+#pragma unroll
+        for (int f = 0; f < VT; f++) O[f][z] *= wi[z];
+#pragma unroll
+      for (int i = 0; i < 4; i++) {  // select, never multiply by 0
+        P[0][i] = r >= 4 * g + i ? P[0][i] * wd[i] : 0.f;
+        P[1][i] = P[1][i] * wo[i];
+        P[2][i] = r >= 4 * g + i ? P[2][i] * wd[i] : 0.f;
+      }
+      if (M != 0) {
+        const int g4 = here(4 * g), rr = here(r);
+#pragma unroll
+        for (int z = 0; z < 2; z++)
+          if (cut & ((2ull << (16 * z + rr)) - 1))
+#pragma unroll
+            for (int f = 0; f < VT; f++) O[f][z] = zero;
+#pragma unroll
+        for (int x = 0; x < 3; x++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            const int s = (x == 2 ? 16 : 0) + g4 + i, t = (x == 0 ? 0 : 16) + rr;
+            if (s < t && ((cut >> s) >> 1 & ((1ull << (t - s)) - 1)) != 0) P[x][i] = 0.f;
+          }
+      }
+      u32x2 Ph[3], Pl[3];
+#pragma unroll
+      for (int x = 0; x < 3; x++)
+#pragma unroll
+        for (int m = 0; m < 2; m++) {
+          const float x0 = P[x][2 * m], x1 = P[x][2 * m + 1];
+          Ph[x][m] = pack_bf16(x0, x1);
+          Pl[x][m] = pack_bf16(x0 - lo_f32(Ph[x][m]), x1 - hi_f32(Ph[x][m]));
+        }
+#pragma unroll
+      for (int f = 0; f < VT; f++) {
+        O[f][0] = mma(vf[f], u32x4{Ph[0][0], Ph[0][1], 0, 0}, O[f][0]);
+        O[f][1] = mma(vf[f], u32x4{Ph[1][0], Ph[1][1], Ph[2][0], Ph[2][1]}, O[f][1]);
+        O[f][0] = mma(vf[f], u32x4{Pl[0][0], Pl[0][1], 0, 0}, O[f][0]);
+        O[f][1] = mma(vf[f], u32x4{Pl[1][0], Pl[1][1], Pl[2][0], Pl[2][1]}, O[f][1]);
+      }
+#pragma unroll
+      for (int z = 0; z < 2; z++)
 #pragma unroll
         for (int f = 0; f < VT; f++)
 #pragma unroll
-          for (int i = 0; i < 4; i++) O[f][qt][i] = blocked ? 0.f : O[f][qt][i] * wi[qt];
-#pragma unroll
-        for (int kt = 0; kt < 2; kt++) {
-#pragma unroll
-          for (int i = 0; i < 4; i++) {
-            const int s = 8 * g + 4 * kt + i;
-            bool keep = rev ? s >= t && s < c : s <= t;
-            if (M != 0) keep = keep && ((M >> min(s, t)) >> 1 & ((1u << abs(s - t)) - 1)) == 0;
-            P[kt][qt][i] = keep ? P[kt][qt][i] * wp[kt][qt][i] : 0.f;
-          }
-#pragma unroll
-          for (int m = 0; m < 2; m++) {
-            const float x0 = P[kt][qt][2 * m], x1 = P[kt][qt][2 * m + 1];
-            const uint32_t hi = pack_bf16(x0, x1);
-            Ph[qt][2 * kt + m] = hi;
-            Pl[qt][2 * kt + m] = pack_bf16(x0 - lo_f32(hi), x1 - hi_f32(hi));
-          }
-        }
-      }
-#pragma unroll
-      for (int f = 0; f < VT; f++)
-#pragma unroll
-        for (int qt = 0; qt < 2; qt++) {
-          O[f][qt] = mma(V[f], Ph[qt], O[f][qt]);
-          O[f][qt] = mma(V[f], Pl[qt], O[f][qt]);
-        }
-#pragma unroll
-      for (int qt = 0; qt < 2; qt++)
-        if (16 * qt + r < c) {
-          float x[4 * VT];
-#pragma unroll
-          for (int i = 0; i < 4; i++)
-#pragma unroll
-            for (int f = 0; f < VT; f++) x[VT * i + f] = O[f][qt][i];
-          store_cols<bf16, 4 * VT, MODE>(ob + (t0 + 16 * qt + r) * p.o.st, 4 * VT * g, Dv - v0, x);
-        }
+          for (int m = 0; m < 2; m++) held[z][2 * f + m] = pack_bf16(O[f][z][2 * m], O[f][z][2 * m + 1]);
+      held_t = t0;
+      held_c = c;
     }
 
+    // the state: g^c S as S + S (g^c - 1), whose rounding does not add up over the blocks of a long memory
+    if (M != 0) {
 #pragma unroll
-    for (int a = 0; a < KT; a++)
+      for (int a = 0; a < KT; a++)
 #pragma unroll
-      for (int f = 0; f < VT; f++)
+        for (int f = 0; f < VT; f++) S[a][f] = f32x4{0.f, 0.f, 0.f, 0.f};
+    } else {
 #pragma unroll
-        for (int i = 0; i < 4; i++) S[a][f][i] = M != 0 ? 0.f : fmaf(S[a][f][i], em1, S[a][f][i]);
-    bool keep[TPL];
+      for (int a = 0; a < KT; a++)
 #pragma unroll
-    for (int j = 0; j < TPL; j++) {
-      const int s = TPL * g + j;
-      keep[j] = s < c;
-      if (M != 0) keep[j] = keep[j] && (rev ? M & ((2u << s) - 1) : (M >> s) >> 1) == 0;
+        for (int f = 0; f < VT; f++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) S[a][f][i] = fmaf(S[a][f][i], em1, S[a][f][i]);
     }
 #pragma unroll
     for (int a = 0; a < KT; a++) {
-      u32x4 t0, t1, t2;
+      u32x4 k0, k1, kl;
 #pragma unroll
       for (int m = 0; m < 4; m++) {
-        const uint32_t kk = pair(b.k2[2 * m], b.k2[2 * m + 1], a);
-        // selects, so that nothing masked gets through
-        float x0 = keep[2 * m] ? lo_f32(kk) * wu[2 * m] : 0.f, x1 = keep[2 * m + 1] ? hi_f32(kk) * wu[2 * m + 1] : 0.f;
-        t0[m] = pack_bf16(x0, x1);
-        x0 -= lo_f32(t0[m]);
-        x1 -= hi_f32(t0[m]);
-        t1[m] = pack_bf16(x0, x1);
-        t2[m] = pack_bf16(x0 - lo_f32(t1[m]), x1 - hi_f32(t1[m]));
+        float x0 = lo_f32(k2[a][m]) * wu[m / 2][2 * (m & 1)], x1 = hi_f32(k2[a][m]) * wu[m / 2][2 * (m & 1) + 1];
+        k0[m] = pack_bf16(x0, x1);
+        x0 -= lo_f32(k0[m]);
+        x1 -= hi_f32(k0[m]);
+        k1[m] = pack_bf16(x0, x1);
+        kl[m] = pack_bf16(x0 - lo_f32(k1[m]), x1 - hi_f32(k1[m]));
       }
 #pragma unroll
       for (int f = 0; f < VT; f++) {
-        S[a][f] = mma(t0, V[f], S[a][f]);
-        S[a][f] = mma(t1, V[f], S[a][f]);
-        S[a][f] = mma(t2, V[f], S[a][f]);
+        S[a][f] = mma(k0, vf[f], S[a][f]);
+        S[a][f] = mma(k1, vf[f], S[a][f]);
+        S[a][f] = mma(kl, vf[f], S[a][f]);
       }
     }
     done += c;
     if (single) single--;
-    if (loaded) b = nb;
   }
+  if (want_out) flush();
 
   if (p.out.p && (seg == A.n_seg - 1 || p.out.sg)) {
     float* s = p.out.p + n * p.out.sn + h * p.out.sh + seg * p.out.sg;
@@ -592,15 +693,15 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, 1) void k_scan16(ScanArgs A) {
       for (int f = 0; f < VT; f++)
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-          const int dk = KT * (4 * g + i) + a, dv = v0 + VT * r + f;
-          if (dk < Dk && dv < Dv) s[(int64_t)dk * p.out.sk + (int64_t)dv * p.out.sv] = S[a][f][i];
+          const int dk = 4 * KT * g + 4 * a + i, dv = v0 + 4 * VT * (r >> 2) + 4 * f + (r & 3);
+          if (dk < Dk && dv < Dv) s[dk * p.out.sk + dv * p.out.sv] = S[a][f][i];
         }
   }
   if (A.factor && U.slice == 0 && lane == 0)
     A.factor[((U.pass * A.N + n) * A.H + h) * A.n_seg + seg] = fresh ? 0.f : (L == 0 ? 1.f : expf(ld * (float)L));
-  if (want_out) {
+  if (want_out) {  // rows behind the sequence's end
     const float z[4 * VT] = {};
-    for (int64_t t = L + r; t < seg1 - seg0; t += 16)
+    for (int64_t t = L + r; t < U.seg1 - U.seg0; t += 16)
       store_cols<bf16, 4 * VT, MODE>(ob + t * p.o.st, 4 * VT * g, Dv - v0, z);
   }
 }
@@ -735,15 +836,18 @@ size_t plan_floats(const Plan& pl, int n_pass, int64_t N, int H, int Dk, int Dv)
 template <typename T>
 bool aligned(const Operand& o, int D) {
   const int per16 = 16 / sizeof(T);
-  return D % per16 == 0 && (uintptr_t)o.p % 16 == 0 && o.st % per16 == 0 && o.sn % per16 == 0 && o.sh % per16 == 0;
+  // (a block's rows are addressed by 32-bit offsets)
+  return D % per16 == 0 && (uintptr_t)o.p % 16 == 0 && o.st % per16 == 0 && o.sn % per16 == 0 && o.sh % per16 == 0 &&
+         o.st >= 0 && o.st < (int64_t)1 << 24;
 }
 
 template <typename T, int KT, int VT>
 int launch_mode(const ScanArgs& A, int mode, hipStream_t s) {
-  const int64_t units = A.n_pass * (int64_t)A.n_slice * A.H * A.N * A.run_seg;
+  const int64_t units = A.n_pass * (int64_t)A.n_slice * A.H * A.N;
   const int64_t blocks = (units + SCAN_WAVES - 1) / SCAN_WAVES;
-  if (blocks > INT32_MAX) return fw::set_error(FW_E_INVALID, "linear attention: too many sequences for one call");
-  const dim3 grid((unsigned)blocks), block(64 * SCAN_WAVES);
+  if (blocks > INT32_MAX / SCAN_WAVES)
+    return fw::set_error(FW_E_INVALID, "linear attention: too many sequences for one call");
+  const dim3 grid((unsigned)blocks, A.run_seg), block(64 * SCAN_WAVES);
   auto kernel = [&](auto m) {
     constexpr int MODE = decltype(m)::value;
     if constexpr (std::is_same_v<T, bf16>)
