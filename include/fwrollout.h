@@ -224,7 +224,8 @@ typedef struct fw_linattn {
   void* workspace;
   size_t workspace_bytes;
 } fw_linattn;
-size_t fw_linattn_workspace_bytes(int64_t T, int64_t N, int32_t H, int32_t Dk, int32_t Dv, int32_t backward);
+size_t fw_linattn_workspace_bytes(int64_t T, int64_t N, int32_t H, int32_t Dk, int32_t Dv, int32_t dtype,
+                                  int32_t backward);
 int fw_linattn_forward(const fw_linattn* a, void* stream);
 int fw_linattn_backward(const fw_linattn* a, void* stream);
 

@@ -157,7 +157,7 @@ SIGNATURES = {
     "fw_vecnorm_merge_update": (_c.c_int, [_vp, _i32, _i32, _i32, _vp, _vp, _vp]),
     "fw_collect_policy": (_c.c_int, [_vp, _vp, _vp]),
     "fw_vecnorm_pending_update": (_c.c_int, [_vp, _i64, _i32, _i32, _i32, _vp, _vp, _vp]),
-    "fw_linattn_workspace_bytes": (_c.c_size_t, [_i64, _i64, _i32, _i32, _i32, _i32]),
+    "fw_linattn_workspace_bytes": (_c.c_size_t, [_i64, _i64, _i32, _i32, _i32, _i32, _i32]),
     "fw_linattn_forward": (_c.c_int, [_vp, _vp]),
     "fw_linattn_backward": (_c.c_int, [_vp, _vp]),
     "fw_linattn_step": (_c.c_int, [_vp, _vp]),

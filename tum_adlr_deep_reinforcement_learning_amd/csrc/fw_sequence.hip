@@ -35,10 +35,11 @@ struct Pass {
   Operand q, k, v, o;  // o.p NULL: only the state is wanted
   State in, out;       // p NULL: zeros / not wanted
   int32_t rev;         // runs from the last token to the first
+  int32_t Dk, Dv;
 };
 struct ScanArgs {
   Pass pass[3];
-  int32_t n_pass, Dk, Dv, H, n_slice, n_seg, run_seg;  // segments [0, run_seg) in processing order
+  int32_t n_pass, H, n_slice, n_seg, run_seg;  // segments [0, run_seg) in processing order
   int64_t T, N, seg_len;
   const float* log_decay;
   const uint8_t* starts;
@@ -117,11 +118,11 @@ __global__ __launch_bounds__(64 * SCAN_WAVES) void k_scan(ScanArgs A) {
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
   Unit U;
   if (!U.decode(A)) return;
-  const Pass& p = A.pass[U.pass];
+  const Pass p = A.pass[U.pass];
   const int64_t n = U.n, seg0 = U.seg0, seg1 = U.seg1, L = U.L;
   const int h = U.h, seg = U.seg, slice = U.slice;
   const bool rev = p.rev;
-  const int Dk = A.Dk, Dv = A.Dv, v0 = slice * 16 * VT;
+  const int Dk = p.Dk, Dv = p.Dv, v0 = slice * 16 * VT;
   const T* qb = (const T*)p.q.p + n * p.q.sn + h * p.q.sh + seg0 * p.q.st;
   const T* kb = (const T*)p.k.p + n * p.k.sn + h * p.k.sh + seg0 * p.k.st;
   const T* vb = (const T*)p.v.p + n * p.v.sn + h * p.v.sh + seg0 * p.v.st + v0;
@@ -301,8 +302,8 @@ __global__ __launch_bounds__(64 * SCAN_WAVES) void k_scan(ScanArgs A) {
 // Operands with tokens as depth (keys and values of the state's product, values of the output's) are read from LDS by
 // the transposing read: 4 lanes x 4 columns of one row each become 4 rows x 1 column per lane.
 // Products of the inputs are exact in the float32 accumulators.  What is not an input is split into bfloat16 terms:
-// weighted scores and the state into two (2^-16 of a term, far below the output's own half step), the weighted keys
-// that enter the state into three (exact to float32: the state is a float32 result).
+// weighted scores and the state into two (2^-16 of a term, far below the output's own half step), the weighted operand
+// of the state's product into three (exact to float32: the state is a float32 result).
 __device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
@@ -317,7 +318,7 @@ struct Tile {
 
   // copies rows 0..31 of a block of c rows; row u is token u, or c - 1 - u when reversed; rows behind the block repeat
   // its last one.  Chunks outside D are left as they are (zeros).  base: the block's first token.
-  template <int MODE>
+  template <int MODE, bool WHOLE>
   __device__ static __forceinline__ void fetch(char* lds, const bf16* base, int64_t st, int D, int c, bool rev, int lane) {
     const int row0 = lane / CH, pc = lane % CH;
     if constexpr (MODE == SCALAR) {
@@ -339,7 +340,7 @@ struct Tile {
         const int row = i * RI + row0, col = (pc ^ turn(row)) * 8;
         if (MODE == FULL || col < D) {
           const char* from;
-          if (c == 32) {  // uniform base + 32-bit lane offset (the launcher saw that 32 rows fit)
+          if constexpr (WHOLE) {  // c = 32: uniform base + 32-bit lane offset (the launcher saw that 32 rows fit)
             const int first = rev ? 32 - RI - i * RI : i * RI;
             from = (const char*)(base + first * st) + (uint32_t)((rev ? RI - 1 - row0 : row0) * (int)st + col) * 2u;
           } else {
@@ -396,11 +397,11 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, 2) void k_scan16(ScanArgs A) {
   char* const lv = lk + K::BYTES;
   Unit U;
   if (!U.decode(A)) return;
-  const Pass& p = A.pass[U.pass];
+  const Pass p = A.pass[U.pass];
   const int64_t n = U.n, L = U.L;
   const int h = U.h, seg = U.seg;
   const bool rev = p.rev;
-  const int Dk = A.Dk, Dv = A.Dv, v0 = U.slice * 16 * VT;
+  const int Dk = p.Dk, Dv = p.Dv, v0 = U.slice * 16 * VT;
   const bf16* qb = (const bf16*)p.q.p + n * p.q.sn + h * p.q.sh + U.seg0 * p.q.st;
   const bf16* kb = (const bf16*)p.k.p + n * p.k.sn + h * p.k.sh + U.seg0 * p.k.st;
   const bf16* vb = (const bf16*)p.v.p + n * p.v.sn + h * p.v.sh + U.seg0 * p.v.st + v0;
@@ -412,9 +413,16 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, 2) void k_scan16(ScanArgs A) {
   auto power = [&](int m) { return expf(ld * (float)m); };
 
   auto fetch = [&](int64_t t0, int c) {
-    V::template fetch<MODE>(lv, vb + t0 * p.v.st, p.v.st, Dv - v0, c, rev, lane);
-    K::template fetch<MODE>(lk, kb + t0 * p.k.st, p.k.st, Dk, c, rev, lane);
-    if (want_out) K::template fetch<MODE>(lq, qb + t0 * p.q.st, p.q.st, Dk, c, rev, lane);
+    auto go = [&](auto whole) {
+      constexpr bool W = decltype(whole)::value;
+      V::template fetch<MODE, W>(lv, vb + t0 * p.v.st, p.v.st, Dv - v0, c, rev, lane);
+      K::template fetch<MODE, W>(lk, kb + t0 * p.k.st, p.k.st, Dk, c, rev, lane);
+      if (want_out) K::template fetch<MODE, W>(lq, qb + t0 * p.q.st, p.q.st, Dk, c, rev, lane);
+    };
+    if (c == C)
+      go(std::true_type());
+    else
+      go(std::false_type());
   };
   if constexpr (MODE == GUARD) {
     for (int i = lane * 16; i < 2 * K::BYTES + V::BYTES; i += 1024) *(u32x4*)(lq + i) = u32x4{0, 0, 0, 0};
@@ -427,16 +435,24 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, 2) void k_scan16(ScanArgs A) {
   }
 
   f32x4 S[KT][VT];
-  if (p.in.p) {  // outside Dk x Dv: the last row or column, which nothing reads
+  // element (a, f, i) of this lane, outside Dk x Dv the last row or column (which nothing reads)
+  auto row_of = [&](int a, int i) {
+    const int dk = 4 * KT * g + 4 * a + i;
+    return MODE == FULL ? dk : min(dk, Dk - 1);
+  };
+  auto col_of = [&](int f) {
+    const int dv = v0 + 4 * VT * (r >> 2) + 4 * f + (r & 3);
+    return MODE == FULL ? dv : min(dv, Dv - 1);
+  };
+  if (p.in.p) {
     const float* s = p.in.p + n * p.in.sn + h * p.in.sh + seg * p.in.sg;
+    const int sk = p.in.sk, sv = p.in.sv;
 #pragma unroll
     for (int a = 0; a < KT; a++)
 #pragma unroll
       for (int f = 0; f < VT; f++)
 #pragma unroll
-        for (int i = 0; i < 4; i++)
-          S[a][f][i] = s[min(4 * KT * g + 4 * a + i, Dk - 1) * p.in.sk +
-                         min(v0 + 4 * VT * (r >> 2) + 4 * f + (r & 3), Dv - 1) * p.in.sv];
+        for (int i = 0; i < 4; i++) S[a][f][i] = s[(uint32_t)(row_of(a, i) * sk + col_of(f) * sv)];
   } else {
 #pragma unroll
     for (int a = 0; a < KT; a++)
@@ -460,35 +476,6 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, 2) void k_scan16(ScanArgs A) {
   bool fresh = false;  // an episode start among the live tokens
   int64_t done = 0;
   int single = 0;           // blocks of one token still to go
-  uint32_t held[2][2 * VT];  // the outputs of the block before, stored once the next block's rows are there
-  int64_t held_t = 0;
-  int held_c = 0;
-  auto flush = [&] {
-#pragma unroll
-    for (int z = 0; z < 2; z++) {
-      const int u = 16 * z + r;
-      if (u < held_c) {
-        bf16* o = ob + (held_t + (rev ? held_c - 1 - u : u)) * p.o.st;
-        const int col = 4 * VT * g, D = Dv - v0;
-        if constexpr (MODE == SCALAR) {
-#pragma unroll
-          for (int k = 0; k < 4 * VT; k++)
-            if (col + k < D) o[col + k].u = (uint16_t)(held[z][k / 2] >> 16 * (k & 1));
-        } else {
-          constexpr int P = VT == 1 ? 2 : 4;
-          typedef uint32_t W __attribute__((ext_vector_type(P)));
-#pragma unroll
-          for (int k = 0; k < 2 * VT; k += P)
-            if (MODE == FULL || col + 2 * k < D) {
-              W w;
-#pragma unroll
-              for (int x = 0; x < P; x++) w[x] = held[z][k + x];
-              *(W*)(o + col + 2 * k) = w;
-            }
-        }
-      }
-    }
-  };
 
   while (done < L) {
     const int c = single ? 1 : (int)min((int64_t)C, L - done);
@@ -503,27 +490,6 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, 2) void k_scan16(ScanArgs A) {
       M = (uint32_t)__ballot(lane < c && xb[(t0 + (rev ? c - 1 - u : u)) * A.starts_st] != 0);
     }
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-    u32x4 vf[VT], k2[KT], kf[2][NS], qf[2][NS];
-#pragma unroll
-    for (int f = 0; f < VT; f++) vf[f] = V::down(lv, f, r, g);
-#pragma unroll
-    for (int a = 0; a < KT; a++) k2[a] = K::down(lk, a, r, g);
-    if (want_out)
-#pragma unroll
-      for (int z = 0; z < 2; z++)
-#pragma unroll
-        for (int s = 0; s < NS; s++) {
-          kf[z][s] = K::across(lk, z, s, r, g);
-          qf[z][s] = K::across(lq, z, s, r, g);
-        }
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    if (want_out) flush();
-    held_c = 0;
-    loaded = !single && done + c < L;
-    if (loaded) {
-      const int c2 = (int)min((int64_t)C, L - done - c);
-      fetch(rev ? t0 - c2 : t0 + c, c2);
-    }
     if (c != cur) {
       cur = c;
       const int g4 = here(4 * g);
@@ -534,6 +500,51 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, 2) void k_scan16(ScanArgs A) {
       em1 = expm1f(ld * (float)c);
     }
 
+    const f32x4 zero{0.f, 0.f, 0.f, 0.f};
+    f32x4 O[VT][2], P[3];  // score tiles (key, query): (0, 0), (0, 1), (1, 1)
+    if (want_out) {
+#pragma unroll
+      for (int z = 0; z < 2; z++)
+#pragma unroll
+        for (int f = 0; f < VT; f++) O[f][z] = zero;
+#pragma unroll
+      for (int x = 0; x < 3; x++) P[x] = zero;
+#pragma unroll
+      for (int s = 0; s < NS; s++) {
+        if (s == 2) asm volatile("" ::: "memory");  // bounds the operands in registers at a time
+        const u32x4 kf[2] = {K::across(lk, 0, s, r, g), K::across(lk, 1, s, r, g)};
+        const u32x4 qf[2] = {K::across(lq, 0, s, r, g), K::across(lq, 1, s, r, g)};
+        P[0] = mma(kf[0], qf[0], P[0]);
+        P[1] = mma(kf[0], qf[1], P[1]);
+        P[2] = mma(kf[1], qf[1], P[2]);
+#pragma unroll
+        for (int f = 0; f < VT; f++) {
+          u32x4 hi{0, 0, 0, 0}, lo{0, 0, 0, 0};
+#pragma unroll
+          for (int m = 0; m < (KT < 2 ? 2 : 4); m++) {
+            const float x0 = S[2 * s + m / 2][f][2 * (m & 1)], x1 = S[2 * s + m / 2][f][2 * (m & 1) + 1];
+            hi[m] = pack_bf16(x0, x1);
+            lo[m] = pack_bf16(x0 - lo_f32(hi[m]), x1 - hi_f32(hi[m]));
+          }
+#pragma unroll
+          for (int z = 0; z < 2; z++) {
+            O[f][z] = mma(hi, qf[z], O[f][z]);
+            O[f][z] = mma(lo, qf[z], O[f][z]);
+          }
+        }
+      }
+    }
+    u32x4 vf[VT], k2[KT];
+#pragma unroll
+    for (int f = 0; f < VT; f++) vf[f] = V::down(lv, f, r, g);
+#pragma unroll
+    for (int a = 0; a < KT; a++) k2[a] = K::down(lk, a, r, g);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // every read of the block is done: its room is free
+    loaded = !single && done + c < L;
+    if (loaded) {
+      const int c2 = (int)min((int64_t)C, L - done - c);
+      fetch(rev ? t0 - c2 : t0 + c, c2);
+    }
     // Masks.  A start at row u of a forward pass cuts every span that contains row u but not from it on; in a reversed
     // pass the cut lies behind row u, that is at row u + 1.
     const uint64_t cut = rev ? (uint64_t)M << 1 : (uint64_t)M;
@@ -552,12 +563,12 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, 2) void k_scan16(ScanArgs A) {
           for (int a = 0; a < KT; a++) k2[a][2 * z + m] &= live & open;
         }
     }
+    f32x4 bad = zero;
+#pragma unroll
+    for (int f = 0; f < VT; f++) bad = mma(vf[f], u32x4{0, 0, 0, 0}, bad);  // 0 or NaN
     // A masked product is a product with 0, which keeps a value away only while that value is finite.  A block with an
     // infinity or a NaN among its values is therefore run token by token: nothing is masked then.
     if (c > 1) {
-      f32x4 bad{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int f = 0; f < VT; f++) bad = mma(vf[f], u32x4{0, 0, 0, 0}, bad);  // 0 or NaN
       if (__any(!(bad[0] + bad[1] + bad[2] + bad[3] == 0.f))) {
         single = c;
         loaded = false;
@@ -567,35 +578,6 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, 2) void k_scan16(ScanArgs A) {
     fresh |= M != 0;
 
     if (want_out) {
-      const f32x4 zero{0.f, 0.f, 0.f, 0.f};
-      f32x4 O[VT][2], P[3];  // score tiles (key, query): (0, 0), (0, 1), (1, 1)
-#pragma unroll
-      for (int z = 0; z < 2; z++)
-#pragma unroll
-        for (int f = 0; f < VT; f++) O[f][z] = zero;
-#pragma unroll
-      for (int x = 0; x < 3; x++) P[x] = zero;
-#pragma unroll
-      for (int s = 0; s < NS; s++) {
-        P[0] = mma(kf[0][s], qf[0][s], P[0]);
-        P[1] = mma(kf[0][s], qf[1][s], P[1]);
-        P[2] = mma(kf[1][s], qf[1][s], P[2]);
-#pragma unroll
-        for (int f = 0; f < VT; f++) {
-          u32x4 hi{0, 0, 0, 0}, lo{0, 0, 0, 0};
-#pragma unroll
-          for (int m = 0; m < (KT < 2 ? 2 : 4); m++) {
-            const float x0 = S[2 * s + m / 2][f][2 * (m & 1)], x1 = S[2 * s + m / 2][f][2 * (m & 1) + 1];
-            hi[m] = pack_bf16(x0, x1);
-            lo[m] = pack_bf16(x0 - lo_f32(hi[m]), x1 - hi_f32(hi[m]));
-          }
-#pragma unroll
-          for (int z = 0; z < 2; z++) {
-            O[f][z] = mma(hi, qf[z][s], O[f][z]);
-            O[f][z] = mma(lo, qf[z][s], O[f][z]);
-          }
-        }
-      }
 #pragma unroll
       for (int z = 0; z < 2; z++)
 #pragma unroll
@@ -638,13 +620,28 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, 2) void k_scan16(ScanArgs A) {
         O[f][1] = mma(vf[f], u32x4{Pl[1][0], Pl[1][1], Pl[2][0], Pl[2][1]}, O[f][1]);
       }
 #pragma unroll
-      for (int z = 0; z < 2; z++)
+      for (int z = 0; z < 2; z++) {
+        const int u = 16 * z + r, col = 4 * VT * g, D = Dv - v0;
+        if (u < c) {
+          bf16* o = ob + (t0 + (rev ? c - 1 - u : u)) * p.o.st;
+          uint32_t x[2 * VT];
 #pragma unroll
-        for (int f = 0; f < VT; f++)
+          for (int f = 0; f < VT; f++)
 #pragma unroll
-          for (int m = 0; m < 2; m++) held[z][2 * f + m] = pack_bf16(O[f][z][2 * m], O[f][z][2 * m + 1]);
-      held_t = t0;
-      held_c = c;
+            for (int m = 0; m < 2; m++) x[2 * f + m] = pack_bf16(O[f][z][2 * m], O[f][z][2 * m + 1]);
+          if constexpr (MODE == SCALAR) {
+#pragma unroll
+            for (int k = 0; k < 4 * VT; k++)
+              if (col + k < D) o[col + k].u = (uint16_t)(x[k / 2] >> 16 * (k & 1));
+          } else if constexpr (VT == 1) {
+            if (MODE == FULL || col < D) *(u32x2*)(o + col) = u32x2{x[0], x[1]};
+          } else {
+#pragma unroll
+            for (int k = 0; k < 2 * VT; k += 4)
+              if (MODE == FULL || col + 2 * k < D) *(u32x4*)(o + col + 2 * k) = u32x4{x[k], x[k + 1], x[k + 2], x[k + 3]};
+          }
+        }
+      }
     }
 
     // the state: g^c S as S + S (g^c - 1), whose rounding does not add up over the blocks of a long memory
@@ -653,49 +650,59 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, 2) void k_scan16(ScanArgs A) {
       for (int a = 0; a < KT; a++)
 #pragma unroll
         for (int f = 0; f < VT; f++) S[a][f] = f32x4{0.f, 0.f, 0.f, 0.f};
-    } else {
-#pragma unroll
-      for (int a = 0; a < KT; a++)
-#pragma unroll
-        for (int f = 0; f < VT; f++)
-#pragma unroll
-          for (int i = 0; i < 4; i++) S[a][f][i] = fmaf(S[a][f][i], em1, S[a][f][i]);
     }
-#pragma unroll
-    for (int a = 0; a < KT; a++) {
-      u32x4 k0, k1, kl;
-#pragma unroll
-      for (int m = 0; m < 4; m++) {
-        float x0 = lo_f32(k2[a][m]) * wu[m / 2][2 * (m & 1)], x1 = hi_f32(k2[a][m]) * wu[m / 2][2 * (m & 1) + 1];
-        k0[m] = pack_bf16(x0, x1);
-        x0 -= lo_f32(k0[m]);
-        x1 -= hi_f32(k0[m]);
-        k1[m] = pack_bf16(x0, x1);
-        kl[m] = pack_bf16(x0 - lo_f32(k1[m]), x1 - hi_f32(k1[m]));
-      }
-#pragma unroll
-      for (int f = 0; f < VT; f++) {
-        S[a][f] = mma(k0, vf[f], S[a][f]);
-        S[a][f] = mma(k1, vf[f], S[a][f]);
-        S[a][f] = mma(kl, vf[f], S[a][f]);
-      }
-    }
-    done += c;
-    if (single) single--;
-  }
-  if (want_out) flush();
-
-  if (p.out.p && (seg == A.n_seg - 1 || p.out.sg)) {
-    float* s = p.out.p + n * p.out.sn + h * p.out.sh + seg * p.out.sg;
 #pragma unroll
     for (int a = 0; a < KT; a++)
 #pragma unroll
       for (int f = 0; f < VT; f++)
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-          const int dk = 4 * KT * g + 4 * a + i, dv = v0 + 4 * VT * (r >> 2) + 4 * f + (r & 3);
-          if (dk < Dk && dv < Dv) s[dk * p.out.sk + dv * p.out.sv] = S[a][f][i];
-        }
+        for (int i = 0; i < 4; i++) S[a][f][i] = fmaf(S[a][f][i], em1, S[a][f][i]);
+    // the weights go to the operand of fewer tiles
+    auto weigh = [&](u32x4 x, u32x4(&t)[3]) {
+#pragma unroll
+      for (int m = 0; m < 4; m++) {
+        float x0 = lo_f32(x[m]) * wu[m / 2][2 * (m & 1)], x1 = hi_f32(x[m]) * wu[m / 2][2 * (m & 1) + 1];
+        t[0][m] = pack_bf16(x0, x1);
+        x0 -= lo_f32(t[0][m]);
+        x1 -= hi_f32(t[0][m]);
+        t[1][m] = pack_bf16(x0, x1);
+        t[2][m] = pack_bf16(x0 - lo_f32(t[1][m]), x1 - hi_f32(t[1][m]));
+      }
+    };
+    u32x4 t[3];
+    if constexpr (KT < VT) {
+#pragma unroll
+      for (int a = 0; a < KT; a++) {
+        weigh(k2[a], t);
+#pragma unroll
+        for (int x = 0; x < 3; x++)
+#pragma unroll
+          for (int f = 0; f < VT; f++) S[a][f] = mma(t[x], vf[f], S[a][f]);
+      }
+    } else {
+#pragma unroll
+      for (int f = 0; f < VT; f++) {
+        weigh(vf[f], t);
+#pragma unroll
+        for (int x = 0; x < 3; x++)
+#pragma unroll
+          for (int a = 0; a < KT; a++) S[a][f] = mma(k2[a], t[x], S[a][f]);
+      }
+    }
+    done += c;
+    if (single) single--;
+  }
+  if (p.out.p && (seg == A.n_seg - 1 || p.out.sg)) {
+    float* s = p.out.p + n * p.out.sn + h * p.out.sh + seg * p.out.sg;
+    const int sk = p.out.sk, sv = p.out.sv;
+#pragma unroll
+    for (int f = 0; f < VT; f++)
+      if (MODE == FULL || v0 + 4 * VT * (r >> 2) + 4 * f + (r & 3) < Dv)
+#pragma unroll
+        for (int a = 0; a < KT; a++)
+#pragma unroll
+          for (int i = 0; i < 4; i++)
+            if (MODE == FULL || 4 * KT * g + 4 * a + i < Dk) s[(uint32_t)(row_of(a, i) * sk + col_of(f) * sv)] = S[a][f][i];
   }
   if (A.factor && U.slice == 0 && lane == 0)
     A.factor[((U.pass * A.N + n) * A.H + h) * A.n_seg + seg] = fresh ? 0.f : (L == 0 ? 1.f : expf(ld * (float)L));
@@ -811,26 +818,33 @@ __global__ __launch_bounds__(256) void k_token(TokenArgs A, int lv_log2) {
 
 // ------------------------------------------------------------------ host side
 int tiles(int d) { return d <= 16 ? 1 : d <= 32 ? 2 : d <= 64 ? 4 : 8; }
+// value tiles of one wave: the state is KT x VT tiles of registers
+int slice_tiles(int dtype, int Dk, int Dv) { return std::min(tiles(Dv), dtype == FW_DT_BF16 && tiles(Dk) == 8 ? 2 : 4); }
+int slices(int dtype, int Dk, int Dv) {
+  const int vt = slice_tiles(dtype, Dk, Dv);
+  return (tiles(Dv) + vt - 1) / vt;
+}
 
 // Time segments: with fewer than SEG_WAVES waves the card is not full, so the time axis is cut, at the price of
 // reading k and v twice and of a state per segment.
-constexpr int SEG_WAVES = 1024;
+constexpr int SEG_WAVES = 2048;
 constexpr int SEG_MIN = 128;  // tokens
 struct Plan {
   int64_t seg_len;
   int n_seg;
 };
-Plan plan(int64_t T, int64_t N, int H, int Dv) {
-  const int slices = (tiles(Dv) + 3) / 4;
-  const int64_t waves = std::max<int64_t>(1, N * H * slices);
-  int64_t segs = std::min<int64_t>(SEG_WAVES / waves, T / SEG_MIN);
+Plan plan(int dtype, int64_t T, int64_t N, int H, int Dk, int Dv, bool backward) {
+  int64_t waves = N * H * slices(dtype, Dk, Dv);
+  if (backward) waves += 2 * N * H * slices(dtype, Dv, Dk);
+  const int64_t segs = std::min<int64_t>(SEG_WAVES / std::max<int64_t>(1, waves), T / SEG_MIN);
   if (segs < 2) return {std::max<int64_t>(T, 1), 1};
-  const int64_t len = ((T + segs - 1) / segs + 63) / 64 * 64;
+  const int64_t len = ((T + segs - 1) / segs + 31) / 32 * 32;
   return {len, (int)((T + len - 1) / len)};
 }
-size_t plan_floats(const Plan& pl, int n_pass, int64_t N, int H, int Dk, int Dv) {
+// a state per segment and what a segment multiplies a state with; the backward pass has two directions of them
+size_t plan_floats(const Plan& pl, int dirs, int64_t N, int H, int Dk, int Dv) {
   if (pl.n_seg < 2) return 0;
-  return (size_t)n_pass * N * H * pl.n_seg * ((size_t)Dk * Dv + 1);
+  return (size_t)dirs * N * H * pl.n_seg * ((size_t)Dk * Dv + 1);
 }
 
 template <typename T>
@@ -866,66 +880,67 @@ int launch_mode(const ScanArgs& A, int mode, hipStream_t s) {
 }
 
 template <typename T>
-int launch_scan(const ScanArgs& A, hipStream_t s) {
-  const int kt = tiles(A.Dk), vt = std::min(tiles(A.Dv), 4);
-  bool vec = true;
-  for (int i = 0; i < A.n_pass; i++)
-    for (const Operand* o : {&A.pass[i].q, &A.pass[i].k}) vec = vec && aligned<T>(*o, A.Dk);
-  for (int i = 0; i < A.n_pass; i++)
-    for (const Operand* o : {&A.pass[i].v, &A.pass[i].o}) vec = vec && aligned<T>(*o, A.Dv);
-  const int mode = !vec ? SCALAR : A.Dk == 16 * kt && A.Dv % (16 * vt) == 0 ? FULL : GUARD;
+int launch_scan(ScanArgs A, int kt, int vt, hipStream_t s) {
+  int mode = FULL;
+  for (int i = 0; i < A.n_pass; i++) {
+    const Pass& p = A.pass[i];
+    bool vec = aligned<T>(p.q, p.Dk) && aligned<T>(p.k, p.Dk) && aligned<T>(p.v, p.Dv) && aligned<T>(p.o, p.Dv);
+    mode = std::max<int>(mode, !vec ? SCALAR : p.Dk == 16 * kt && p.Dv % (16 * vt) == 0 ? FULL : GUARD);
+  }
   switch (kt * 8 + vt) {
 #define FW_CASE(K, V) \
   case K * 8 + V: return launch_mode<T, K, V>(A, mode, s)
     FW_CASE(1, 1); FW_CASE(1, 2); FW_CASE(1, 4);
     FW_CASE(2, 1); FW_CASE(2, 2); FW_CASE(2, 4);
     FW_CASE(4, 1); FW_CASE(4, 2); FW_CASE(4, 4);
-    FW_CASE(8, 1); FW_CASE(8, 2); FW_CASE(8, 4);
+    FW_CASE(8, 1); FW_CASE(8, 2);
+    case 8 * 8 + 4:
+      if constexpr (!std::is_same_v<T, bf16>) return launch_mode<T, 8, 4>(A, mode, s);
 #undef FW_CASE
   }
   return fw::set_error(FW_E_INVALID, "linear attention: head sizes 1..128");
 }
 
-int launch_scan_dt(int dtype, const ScanArgs& A, hipStream_t s) {
-  if (dtype == FW_DT_F32) return launch_scan<float>(A, s);
-  if (dtype == FW_DT_BF16) return launch_scan<bf16>(A, s);
-  return launch_scan<f16>(A, s);
+// Passes of equal tile counts go in one launch.
+int launch_passes(int dtype, ScanArgs A, const Pass* pass, int n_pass, hipStream_t s) {
+  for (int i = 0; i < n_pass; i += A.n_pass) {
+    const int kt = tiles(pass[i].Dk), vt = slice_tiles(dtype, pass[i].Dk, pass[i].Dv);
+    A.n_slice = slices(dtype, pass[i].Dk, pass[i].Dv);
+    A.n_pass = 0;
+    while (i + A.n_pass < n_pass && tiles(pass[i + A.n_pass].Dk) == kt && tiles(pass[i + A.n_pass].Dv) == tiles(pass[i].Dv)) {
+      A.pass[A.n_pass] = pass[i + A.n_pass];
+      A.n_pass++;
+    }
+    const int rc = dtype == FW_DT_F32    ? launch_scan<float>(A, kt, vt, s)
+                   : dtype == FW_DT_BF16 ? launch_scan<bf16>(A, kt, vt, s)
+                                         : launch_scan<f16>(A, kt, vt, s);
+    if (rc) return rc;
+  }
+  return FW_OK;
 }
 
-// n_pass passes of the same direction and sizes, cut into time segments where the plan says so
-int run_passes(int dtype, ScanArgs A, const Plan& pl, float* ws, hipStream_t s) {
-  A.seg_len = pl.seg_len;
-  A.n_seg = A.run_seg = pl.n_seg;
-  A.n_slice = (tiles(A.Dv) + 3) / 4;
-  if (pl.n_seg < 2) return launch_scan_dt(dtype, A, s);
-  const int64_t E = (int64_t)A.Dk * A.Dv;
-  float* factor = ws + A.n_pass * A.N * A.H * pl.n_seg * E;
-  ScanArgs B = A;  // what each segment adds, from its keys and values alone
+// The states that enter the segments, for each of `dirs` directions: what the segments add (add[d]: keys and values
+// alone), joined along time from in[d].  Leaves them in ws as [dirs][N][H][n_seg][Dk][Dv].
+int segment_states(int dtype, ScanArgs A, const Pass* add, const State* in, int dirs, float* ws, hipStream_t s) {
+  const int Dk = add[0].Dk, Dv = add[0].Dv;
+  const int64_t E = (int64_t)Dk * Dv;
+  A.factor = ws + dirs * A.N * A.H * A.n_seg * E;
+  A.run_seg = A.n_seg - 1;  // the last segment adds to nothing
+  if (int rc = launch_passes(dtype, A, add, dirs, s)) return rc;
   JoinArgs J{};
-  B.run_seg = pl.n_seg - 1;
-  B.factor = factor;
-  for (int i = 0; i < A.n_pass; i++) {
-    const State seg{ws + i * A.N * A.H * pl.n_seg * E, A.H * pl.n_seg * E, pl.n_seg * E, E, A.Dv, 1};
-    B.pass[i].o.p = nullptr;
-    B.pass[i].in.p = nullptr;
-    B.pass[i].out = seg;
-    J.in[i] = A.pass[i].in;
-    A.pass[i].in = seg;
-    A.pass[i].out.sg = 0;
-  }
-  if (int rc = launch_scan_dt(dtype, B, s)) return rc;
+  for (int d = 0; d < dirs; d++) J.in[d] = in[d];
   J.ws = ws;
-  J.factor = factor;
+  J.factor = A.factor;
   J.N = A.N;
-  J.n_pass = A.n_pass;
+  J.n_pass = dirs;
   J.H = A.H;
-  J.n_seg = pl.n_seg;
-  J.Dk = A.Dk;
-  J.Dv = A.Dv;
-  const int64_t blocks = (A.n_pass * A.N * A.H * E + 255) / 256;
+  J.n_seg = A.n_seg;
+  J.Dk = Dk;
+  J.Dv = Dv;
+  const int64_t blocks = (dirs * A.N * A.H * E + 255) / 256;
   hipLaunchKernelGGL(k_scan_join, dim3((unsigned)blocks), dim3(256), 0, s, J);
   FW_HIP(hipGetLastError());
-  return launch_scan_dt(dtype, A, s);
+  return FW_OK;
 }
 
 int check(const fw_linattn* a, const char* who) {
@@ -939,15 +954,17 @@ int check(const fw_linattn* a, const char* who) {
   return FW_OK;
 }
 bool room(const fw_linattn* a, bool backward) {
-  const size_t need = fw_linattn_workspace_bytes(a->T, a->N, a->H, a->Dk, a->Dv, backward);
+  const size_t need = fw_linattn_workspace_bytes(a->T, a->N, a->H, a->Dk, a->Dv, a->dtype, backward);
   return need == 0 || (a->workspace && a->workspace_bytes >= need);
 }
 Operand in(const fw_seq_tensor& t) { return {t.p, t.st, t.sn, t.sh}; }
-ScanArgs base(const fw_linattn* a) {
+ScanArgs base(const fw_linattn* a, const Plan& pl) {
   ScanArgs A{};
   A.H = a->H;
   A.T = a->T;
   A.N = a->N;
+  A.seg_len = pl.seg_len;
+  A.n_seg = A.run_seg = pl.n_seg;
   A.log_decay = a->log_decay;
   A.starts = a->starts;
   A.starts_st = a->starts_st;
@@ -955,33 +972,46 @@ ScanArgs base(const fw_linattn* a) {
   A.lengths = a->lengths;
   return A;
 }
+// a state tensor [N][H][Dk][Dv], read as it lies or with the roles of k and v exchanged
+State straight(const fw_linattn* a, const float* p) {
+  const int64_t E = (int64_t)a->Dk * a->Dv;
+  return {const_cast<float*>(p), a->H * E, E, 0, a->Dv, 1};
+}
+State turned(State s) {
+  std::swap(s.sk, s.sv);
+  return s;
+}
+State segments(const fw_linattn* a, float* ws, int dir, int n_seg) {
+  const int64_t E = (int64_t)a->Dk * a->Dv;
+  return {ws + dir * a->N * a->H * n_seg * E, a->H * n_seg * E, n_seg * E, E, a->Dv, 1};
+}
 
 }  // namespace
 
 extern "C" {
 
-size_t fw_linattn_workspace_bytes(int64_t T, int64_t N, int32_t H, int32_t Dk, int32_t Dv, int32_t backward) {
+size_t fw_linattn_workspace_bytes(int64_t T, int64_t N, int32_t H, int32_t Dk, int32_t Dv, int32_t dtype, int32_t backward) {
   if (T < 1 || N < 1 || H < 1 || Dk < 1 || Dk > MAXDIM || Dv < 1 || Dv > MAXDIM) return 0;
-  if (!backward) return sizeof(float) * plan_floats(plan(T, N, H, Dv), 1, N, H, Dk, Dv);
-  // dq, dk and dv run one after another in the same room
-  return sizeof(float) * std::max(plan_floats(plan(T, N, H, Dk), 1, N, H, Dv, Dk),
-                                  plan_floats(plan(T, N, H, Dv), 1, N, H, Dk, Dv));
+  return sizeof(float) * plan_floats(plan(dtype, T, N, H, Dk, Dv, backward), backward ? 2 : 1, N, H, Dk, Dv);
 }
 
 int fw_linattn_forward(const fw_linattn* a, void* stream) {
   if (int rc = check(a, "fw_linattn_forward")) return rc;
   if (a->N == 0) return FW_OK;
   if (a->T > 0 && !a->out.p) return fw::set_error(FW_E_INVALID, "fw_linattn_forward: NULL out");
+  const Plan pl = plan(a->dtype, a->T, a->N, a->H, a->Dk, a->Dv, false);
   if (!room(a, false)) return fw::set_error(FW_E_INVALID, "fw_linattn_forward: workspace too small");
-  ScanArgs A = base(a);
-  A.n_pass = 1;
-  A.Dk = a->Dk;
-  A.Dv = a->Dv;
-  const int64_t E = (int64_t)a->Dk * a->Dv;
-  A.pass[0] = Pass{in(a->q), in(a->k), in(a->v), in(a->out),
-                   State{const_cast<float*>(a->state_in), a->H * E, E, 0, a->Dv, 1},
-                   State{a->state_out, a->H * E, E, 0, a->Dv, 1}, 0};
-  return run_passes(a->dtype, A, plan(a->T, a->N, a->H, a->Dv), (float*)a->workspace, (hipStream_t)stream);
+  hipStream_t s = (hipStream_t)stream;
+  float* ws = (float*)a->workspace;
+  const ScanArgs A = base(a, pl);
+  Pass p{in(a->q), in(a->k), in(a->v), in(a->out), straight(a, a->state_in), straight(a, a->state_out), 0, a->Dk, a->Dv};
+  if (pl.n_seg > 1) {
+    const State seg = segments(a, ws, 0, pl.n_seg);
+    const Pass add{p.q, p.k, p.v, Operand{}, State{}, seg, 0, a->Dk, a->Dv};
+    if (int rc = segment_states(a->dtype, A, &add, &p.in, 1, ws, s)) return rc;
+    p.in = seg;
+  }
+  return launch_passes(a->dtype, A, &p, 1, s);
 }
 
 int fw_linattn_backward(const fw_linattn* a, void* stream) {
@@ -989,26 +1019,25 @@ int fw_linattn_backward(const fw_linattn* a, void* stream) {
   if (a->N == 0) return FW_OK;
   if (a->T > 0 && (!a->dout.p || !a->dq.p || !a->dk.p || !a->dv.p))
     return fw::set_error(FW_E_INVALID, "fw_linattn_backward: NULL dout, dq, dk or dv");
+  const Plan pl = plan(a->dtype, a->T, a->N, a->H, a->Dk, a->Dv, true);
   if (!room(a, true)) return fw::set_error(FW_E_INVALID, "fw_linattn_backward: workspace too small");
-  const int64_t E = (int64_t)a->Dk * a->Dv;
   hipStream_t s = (hipStream_t)stream;
   float* ws = (float*)a->workspace;
-  auto straight = [&](const float* p) { return State{const_cast<float*>(p), a->H * E, E, 0, a->Dv, 1}; };
-  auto turned = [&](const float* p) { return State{const_cast<float*>(p), a->H * E, E, 0, 1, a->Dv}; };
-  const State none{};
-  const Plan pk = plan(a->T, a->N, a->H, a->Dk), pv = plan(a->T, a->N, a->H, a->Dv);
-  ScanArgs A = base(a);
-  A.n_pass = 1;
-  A.Dk = a->Dv;
-  A.Dv = a->Dk;
-  A.pass[0] = Pass{in(a->dout), in(a->v), in(a->k), in(a->dq), turned(a->state_in), none, 0};
-  if (int rc = run_passes(a->dtype, A, pk, ws, s)) return rc;
-  A.pass[0] = Pass{in(a->v), in(a->dout), in(a->q), in(a->dk), turned(a->dstate), none, 1};
-  if (int rc = run_passes(a->dtype, A, pk, ws, s)) return rc;
-  A.Dk = a->Dk;
-  A.Dv = a->Dv;
-  A.pass[0] = Pass{in(a->k), in(a->q), in(a->dout), in(a->dv), straight(a->dstate), straight(a->dstate_in), 1};
-  return run_passes(a->dtype, A, pv, ws, s);
+  const ScanArgs A = base(a, pl);
+  State S = straight(a, a->state_in), R = straight(a, a->dstate);  // forward states; reversed ones
+  if (pl.n_seg > 1) {
+    const State in_[2] = {S, R};
+    S = segments(a, ws, 0, pl.n_seg);
+    R = segments(a, ws, 1, pl.n_seg);
+    const Pass add[2] = {{in(a->q), in(a->k), in(a->v), Operand{}, State{}, S, 0, a->Dk, a->Dv},
+                         {in(a->k), in(a->q), in(a->dout), Operand{}, State{}, R, 1, a->Dk, a->Dv}};
+    if (int rc = segment_states(a->dtype, A, add, in_, 2, ws, s)) return rc;
+  }
+  const Pass main[3] = {
+      {in(a->dout), in(a->v), in(a->k), in(a->dq), turned(S), State{}, 0, a->Dv, a->Dk},
+      {in(a->v), in(a->dout), in(a->q), in(a->dk), turned(R), State{}, 1, a->Dv, a->Dk},
+      {in(a->k), in(a->q), in(a->dout), in(a->dv), R, straight(a, a->dstate_in), 1, a->Dk, a->Dv}};
+  return launch_passes(a->dtype, A, main, 3, s);
 }
 
 int fw_linattn_step(const fw_linattn_token* a, void* stream) {

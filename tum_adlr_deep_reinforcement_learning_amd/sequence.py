@@ -104,7 +104,7 @@ def _linattn_args(q, k, v, log_decay, starts, lengths):
 
 
 def _workspace(lib, a, device, backward):
-    n = lib.fw_linattn_workspace_bytes(a.T, a.N, a.H, a.Dk, a.Dv, backward)
+    n = lib.fw_linattn_workspace_bytes(a.T, a.N, a.H, a.Dk, a.Dv, a.dtype, backward)
     ws = torch.empty(n, dtype=torch.uint8, device=device) if n else None
     a.workspace, a.workspace_bytes = _ptr(ws), n
     return ws  # referenced until the launches are queued; the allocator reuses it in stream order
