@@ -26,10 +26,13 @@ struct Operand {
   const void* p;
   int64_t st, sn, sh;
 };
-struct State {  // element (n, h, seg, k, v) at p + n sn + h sh + seg sg + k sk + v sv
+// Element (n, h, seg, k, v) at p + n sn + h sh + seg sg + (k / 4) k4 + (k % 4) k1 + (v / 4) v4 + (v % 4) v1: a caller's
+// [Dk][Dv] or a segment's [Dk / 4][Dv][4] (four keys of a value column together: what a lane holds), either of them as
+// it lies or with the roles of k and v exchanged.
+struct State {
   float* p;
   int64_t sn, sh, sg;
-  int32_t sk, sv;
+  int32_t k4, k1, v4, v1;
 };
 struct Pass {
   Operand q, k, v, o;  // o.p NULL: only the state is wanted
@@ -72,7 +75,64 @@ struct Unit {
   }
 };
 
+
 enum { FULL, GUARD, SCALAR };  // D fills the tiles; whole vectors in or out; element by element
+
+// The state as a wave holds it: lane 16 g + r, key column 4 KT g + e, value column dv(f), in S[e % KT][f][e / KT] (WIDE)
+// or S[e / 4][f][e % 4].  Four keys move as one access where they lie together.
+template <int MODE, bool WIDE, int KT, int VT, typename Col>
+__device__ __forceinline__ void load_state(f32x4 (&S)[KT][VT], const State& st, const float* s, int Dk, int Dv, int g,
+                                           Col dv) {
+  auto set = [&](int e, int f, float x) {
+    if (WIDE)
+      S[e % KT][f][e / KT] = x;
+    else
+      S[e / 4][f][e % 4] = x;
+  };
+  const bool four = st.k1 == 1 && ((uintptr_t)s | (st.k4 | st.v4 | st.v1) * 4) % 16 == 0;
+#pragma unroll
+  for (int f = 0; f < VT; f++) {  // outside Dk x Dv: the last row or column, which nothing reads
+    const int v = MODE == FULL ? dv(f) : min(dv(f), Dv - 1);
+    const float* c = s + (v >> 2) * st.v4 + (v & 3) * st.v1;
+    if (four) {
+#pragma unroll
+      for (int x = 0; x < KT; x++) {
+        const int q = MODE == FULL ? KT * g + x : min(KT * g + x, (Dk - 1) >> 2);
+        const f32x4 y = *(const f32x4*)(c + q * st.k4);
+#pragma unroll
+        for (int i = 0; i < 4; i++) set(4 * x + i, f, y[i]);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4 * KT; e++) {
+        const int k = MODE == FULL ? 4 * KT * g + e : min(4 * KT * g + e, Dk - 1);
+        set(e, f, c[(k >> 2) * st.k4 + (k & 3) * st.k1]);
+      }
+    }
+  }
+}
+template <int MODE, bool WIDE, int KT, int VT, typename Col>
+__device__ __forceinline__ void store_state(const f32x4 (&S)[KT][VT], const State& st, float* s, int Dk, int Dv, int g,
+                                            Col dv) {
+  auto at = [&](int e, int f) { return WIDE ? S[e % KT][f][e / KT] : S[e / 4][f][e % 4]; };
+#pragma unroll
+  for (int f = 0; f < VT; f++)
+    if (MODE == FULL || dv(f) < Dv) {
+      float* c = s + (dv(f) >> 2) * st.v4 + (dv(f) & 3) * st.v1;
+      if (st.sg) {  // a segment's state
+#pragma unroll
+        for (int x = 0; x < KT; x++)
+          if (MODE == FULL || 4 * (KT * g + x) < Dk)
+            *(f32x4*)(c + (KT * g + x) * st.k4) = f32x4{at(4 * x, f), at(4 * x + 1, f), at(4 * x + 2, f), at(4 * x + 3, f)};
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4 * KT; e++) {
+          const int k = 4 * KT * g + e;
+          if (MODE == FULL || k < Dk) c[(k >> 2) * st.k4 + (k & 3) * st.k1] = at(e, f);
+        }
+      }
+    }
+}
 
 // NE contiguous elements at column `col` of a row of D; a column outside is read from column 0 (the caller drops it)
 template <typename T, int NE, int MODE>
@@ -136,17 +196,9 @@ __global__ __launch_bounds__(64 * SCAN_WAVES) void k_scan(ScanArgs A) {
 #pragma unroll
   for (int a = 0; a < KT; a++)
 #pragma unroll
-    for (int f = 0; f < VT; f++) {
-      S[a][f] = f32x4{0.f, 0.f, 0.f, 0.f};
-      if (p.in.p) {
-        const float* s = p.in.p + n * p.in.sn + h * p.in.sh + seg * p.in.sg;
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-          const int dk = KT * (4 * g + i) + a, dv = v0 + VT * r + f;
-          if (dk < Dk && dv < Dv) S[a][f][i] = s[(int64_t)dk * p.in.sk + (int64_t)dv * p.in.sv];
-        }
-      }
-    }
+    for (int f = 0; f < VT; f++) S[a][f] = f32x4{0.f, 0.f, 0.f, 0.f};
+  auto column = [&](int f) { return v0 + VT * r + f; };
+  if (p.in.p) load_state<MODE, true>(S, p.in, p.in.p + n * p.in.sn + h * p.in.sh + seg * p.in.sg, Dk, Dv, g, column);
 
   // weights of a whole block; a reversed pass carries g x the state of the token behind it, so that its final
   // state is the gradient of the initial one and its first weight is 1
@@ -269,18 +321,8 @@ __global__ __launch_bounds__(64 * SCAN_WAVES) void k_scan(ScanArgs A) {
     if (single) single--;
   }
 
-  if (p.out.p && (seg == A.n_seg - 1 || p.out.sg)) {
-    float* s = p.out.p + n * p.out.sn + h * p.out.sh + seg * p.out.sg;
-#pragma unroll
-    for (int a = 0; a < KT; a++)
-#pragma unroll
-      for (int f = 0; f < VT; f++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-          const int dk = KT * (4 * g + i) + a, dv = v0 + VT * r + f;
-          if (dk < Dk && dv < Dv) s[(int64_t)dk * p.out.sk + (int64_t)dv * p.out.sv] = S[a][f][i];
-        }
-  }
+  if (p.out.p && (seg == A.n_seg - 1 || p.out.sg))
+    store_state<MODE, true>(S, p.out, p.out.p + n * p.out.sn + h * p.out.sh + seg * p.out.sg, Dk, Dv, g, column);
   if (A.factor && slice == 0 && lane == 0)
     A.factor[((U.pass * A.N + n) * A.H + h) * A.n_seg + seg] = fresh ? 0.f : (L == 0 ? 1.f : expf(ld * (float)L));
   if (want_out) {  // rows behind the sequence's end
@@ -435,30 +477,12 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, 2) void k_scan16(ScanArgs A) {
   }
 
   f32x4 S[KT][VT];
-  // element (a, f, i) of this lane, outside Dk x Dv the last row or column (which nothing reads)
-  auto row_of = [&](int a, int i) {
-    const int dk = 4 * KT * g + 4 * a + i;
-    return MODE == FULL ? dk : min(dk, Dk - 1);
-  };
-  auto col_of = [&](int f) {
-    const int dv = v0 + 4 * VT * (r >> 2) + 4 * f + (r & 3);
-    return MODE == FULL ? dv : min(dv, Dv - 1);
-  };
-  if (p.in.p) {
-    const float* s = p.in.p + n * p.in.sn + h * p.in.sh + seg * p.in.sg;
-    const int sk = p.in.sk, sv = p.in.sv;
 #pragma unroll
-    for (int a = 0; a < KT; a++)
+  for (int a = 0; a < KT; a++)
 #pragma unroll
-      for (int f = 0; f < VT; f++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) S[a][f][i] = s[(uint32_t)(row_of(a, i) * sk + col_of(f) * sv)];
-  } else {
-#pragma unroll
-    for (int a = 0; a < KT; a++)
-#pragma unroll
-      for (int f = 0; f < VT; f++) S[a][f] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
+    for (int f = 0; f < VT; f++) S[a][f] = f32x4{0.f, 0.f, 0.f, 0.f};
+  auto column = [&](int f) { return v0 + 4 * VT * (r >> 2) + 4 * f + (r & 3); };
+  if (p.in.p) load_state<MODE, false>(S, p.in, p.in.p + n * p.in.sn + h * p.in.sh + seg * p.in.sg, Dk, Dv, g, column);
 
   // Weights.  A reversed pass carries g x the state of the row before: its first weight is 1, and its final state is
   // the gradient of the initial one.
@@ -692,18 +716,8 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, 2) void k_scan16(ScanArgs A) {
     done += c;
     if (single) single--;
   }
-  if (p.out.p && (seg == A.n_seg - 1 || p.out.sg)) {
-    float* s = p.out.p + n * p.out.sn + h * p.out.sh + seg * p.out.sg;
-    const int sk = p.out.sk, sv = p.out.sv;
-#pragma unroll
-    for (int f = 0; f < VT; f++)
-      if (MODE == FULL || v0 + 4 * VT * (r >> 2) + 4 * f + (r & 3) < Dv)
-#pragma unroll
-        for (int a = 0; a < KT; a++)
-#pragma unroll
-          for (int i = 0; i < 4; i++)
-            if (MODE == FULL || 4 * KT * g + 4 * a + i < Dk) s[(uint32_t)(row_of(a, i) * sk + col_of(f) * sv)] = S[a][f][i];
-  }
+  if (p.out.p && (seg == A.n_seg - 1 || p.out.sg))
+    store_state<MODE, false>(S, p.out, p.out.p + n * p.out.sn + h * p.out.sh + seg * p.out.sg, Dk, Dv, g, column);
   if (A.factor && U.slice == 0 && lane == 0)
     A.factor[((U.pass * A.N + n) * A.H + h) * A.n_seg + seg] = fresh ? 0.f : (L == 0 ? 1.f : expf(ld * (float)L));
   if (want_out) {  // rows behind the sequence's end
@@ -715,40 +729,47 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, 2) void k_scan16(ScanArgs A) {
 
 // ws[seg] holds what segment seg adds to a state; rewritten as the state that enters segment seg:
 //   c_0 = in;  c_{s+1} = factor_s c_s + ws_s
-// One thread per state element; the loads of all segments are independent of the recurrence.
+// One thread per four keys of a value column; the loads of all segments are independent of the recurrence.
 struct JoinArgs {
   State in[2];  // p NULL: zeros
-  float* ws;    // [n_pass][N][H][n_seg][Dk][Dv]
+  float* ws;    // [dirs][N][H][n_seg][ceil(Dk / 4)][Dv][4]
   const float* factor;
   int64_t N;
-  int32_t n_pass, H, n_seg, Dk, Dv;
+  int32_t dirs, H, n_seg, Dk, Dv;
 };
 __global__ __launch_bounds__(256) void k_scan_join(JoinArgs A) {
-  const int64_t E = (int64_t)A.Dk * A.Dv, total = A.n_pass * A.N * A.H * E;
-  const int64_t x = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (x >= total) return;
-  const int64_t row = x / E, e = x - row * E;  // row = (pass N + n) H + h
-  const int h = (int)(row % A.H);
-  const int64_t n = (row / A.H) % A.N;
-  const int pi = (int)(row / A.H / A.N);
-  const State& in = A.in[pi];
-  float c = in.p ? in.p[n * in.sn + h * in.sh + (e / A.Dv) * in.sk + (e % A.Dv) * in.sv] : 0.f;
-  float* w = A.ws + row * A.n_seg * E + e;
-  const float* f = A.factor + row * A.n_seg;
+  const uint32_t E = (uint32_t)((A.Dk + 3) / 4 * A.Dv), x = blockIdx.x * 256 + threadIdx.x;
+  const uint32_t row = x / E, e = x - row * E;  // row = (dir N + n) H + h
+  if (row >= (uint32_t)(A.dirs * A.N * A.H)) return;
+  const uint32_t h = row % (uint32_t)A.H, n = row / (uint32_t)A.H % (uint32_t)A.N;
+  const State& in = A.in[row / (uint32_t)A.H / (uint32_t)A.N];
+  f32x4 c{0.f, 0.f, 0.f, 0.f};
+  if (in.p) {
+    const int k4 = (int)(e / A.Dv), v = (int)(e % A.Dv);
+    const float* s = in.p + n * in.sn + h * in.sh + k4 * in.k4 + (v >> 2) * in.v4 + (v & 3) * in.v1;
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+      if (4 * k4 + i < A.Dk) c[i] = s[i * in.k1];
+  }
+  f32x4* w = (f32x4*)A.ws + (int64_t)row * A.n_seg * E + e;
+  const float* f = A.factor + (int64_t)row * A.n_seg;
   constexpr int PF = 8;
   for (int s0 = 0; s0 < A.n_seg; s0 += PF) {
-    float add[PF], fac[PF];
+    f32x4 add[PF];
+    float fac[PF];
 #pragma unroll
-    for (int k = 0; k < PF; k++) {
-      const bool have = s0 + k < A.n_seg - 1;  // the last segment adds to nothing
-      add[k] = have ? w[(s0 + k) * E] : 0.f;
-      fac[k] = have ? f[s0 + k] : 0.f;
-    }
+    for (int k = 0; k < PF; k++)
+      if (s0 + k < A.n_seg - 1) {  // the last segment adds to nothing
+        add[k] = w[(int64_t)(s0 + k) * E];
+        fac[k] = f[s0 + k];
+      }
 #pragma unroll
     for (int k = 0; k < PF; k++)
       if (s0 + k < A.n_seg) {
-        w[(s0 + k) * E] = c;
-        c = fac[k] != 0.f ? fmaf(fac[k], c, add[k]) : add[k];
+        w[(int64_t)(s0 + k) * E] = c;
+        if (s0 + k < A.n_seg - 1)
+#pragma unroll
+          for (int i = 0; i < 4; i++) c[i] = fac[k] != 0.f ? fmaf(fac[k], c[i], add[k][i]) : add[k][i];
       }
   }
 }
@@ -833,18 +854,18 @@ struct Plan {
   int64_t seg_len;
   int n_seg;
 };
-Plan plan(int dtype, int64_t T, int64_t N, int H, int Dk, int Dv, bool backward) {
-  int64_t waves = N * H * slices(dtype, Dk, Dv);
-  if (backward) waves += 2 * N * H * slices(dtype, Dv, Dk);
+Plan plan(int dtype, int64_t T, int64_t N, int H, int Dk, int Dv) {
+  const int64_t waves = N * H * slices(dtype, Dk, Dv);
   const int64_t segs = std::min<int64_t>(SEG_WAVES / std::max<int64_t>(1, waves), T / SEG_MIN);
   if (segs < 2) return {std::max<int64_t>(T, 1), 1};
   const int64_t len = ((T + segs - 1) / segs + 31) / 32 * 32;
   return {len, (int)((T + len - 1) / len)};
 }
+int quads(int Dk) { return (Dk + 3) / 4 * 4; }
 // a state per segment and what a segment multiplies a state with; the backward pass has two directions of them
 size_t plan_floats(const Plan& pl, int dirs, int64_t N, int H, int Dk, int Dv) {
   if (pl.n_seg < 2) return 0;
-  return (size_t)dirs * N * H * pl.n_seg * ((size_t)Dk * Dv + 1);
+  return (size_t)dirs * N * H * pl.n_seg * ((size_t)quads(Dk) * Dv + 1);
 }
 
 template <typename T>
@@ -920,10 +941,10 @@ int launch_passes(int dtype, ScanArgs A, const Pass* pass, int n_pass, hipStream
 }
 
 // The states that enter the segments, for each of `dirs` directions: what the segments add (add[d]: keys and values
-// alone), joined along time from in[d].  Leaves them in ws as [dirs][N][H][n_seg][Dk][Dv].
+// alone), joined along time from in[d].  Leaves them in ws (see segments()).
 int segment_states(int dtype, ScanArgs A, const Pass* add, const State* in, int dirs, float* ws, hipStream_t s) {
   const int Dk = add[0].Dk, Dv = add[0].Dv;
-  const int64_t E = (int64_t)Dk * Dv;
+  const int64_t E = (int64_t)quads(Dk) * Dv;
   A.factor = ws + dirs * A.N * A.H * A.n_seg * E;
   A.run_seg = A.n_seg - 1;  // the last segment adds to nothing
   if (int rc = launch_passes(dtype, A, add, dirs, s)) return rc;
@@ -932,12 +953,12 @@ int segment_states(int dtype, ScanArgs A, const Pass* add, const State* in, int 
   J.ws = ws;
   J.factor = A.factor;
   J.N = A.N;
-  J.n_pass = dirs;
+  J.dirs = dirs;
   J.H = A.H;
   J.n_seg = A.n_seg;
   J.Dk = Dk;
   J.Dv = Dv;
-  const int64_t blocks = (dirs * A.N * A.H * E + 255) / 256;
+  const int64_t blocks = (dirs * A.N * A.H * E / 4 + 255) / 256;  // N H < SEG_WAVES
   hipLaunchKernelGGL(k_scan_join, dim3((unsigned)blocks), dim3(256), 0, s, J);
   FW_HIP(hipGetLastError());
   return FW_OK;
@@ -972,18 +993,18 @@ ScanArgs base(const fw_linattn* a, const Plan& pl) {
   A.lengths = a->lengths;
   return A;
 }
-// a state tensor [N][H][Dk][Dv], read as it lies or with the roles of k and v exchanged
 State straight(const fw_linattn* a, const float* p) {
   const int64_t E = (int64_t)a->Dk * a->Dv;
-  return {const_cast<float*>(p), a->H * E, E, 0, a->Dv, 1};
+  return {const_cast<float*>(p), a->H * E, E, 0, 4 * a->Dv, a->Dv, 4, 1};
 }
 State turned(State s) {
-  std::swap(s.sk, s.sv);
+  std::swap(s.k4, s.v4);
+  std::swap(s.k1, s.v1);
   return s;
 }
 State segments(const fw_linattn* a, float* ws, int dir, int n_seg) {
-  const int64_t E = (int64_t)a->Dk * a->Dv;
-  return {ws + dir * a->N * a->H * n_seg * E, a->H * n_seg * E, n_seg * E, E, a->Dv, 1};
+  const int64_t E = (int64_t)quads(a->Dk) * a->Dv;
+  return {ws + dir * a->N * a->H * n_seg * E, a->H * n_seg * E, n_seg * E, E, 4 * a->Dv, 1, 16, 4};
 }
 
 }  // namespace
@@ -992,14 +1013,14 @@ extern "C" {
 
 size_t fw_linattn_workspace_bytes(int64_t T, int64_t N, int32_t H, int32_t Dk, int32_t Dv, int32_t dtype, int32_t backward) {
   if (T < 1 || N < 1 || H < 1 || Dk < 1 || Dk > MAXDIM || Dv < 1 || Dv > MAXDIM) return 0;
-  return sizeof(float) * plan_floats(plan(dtype, T, N, H, Dk, Dv, backward), backward ? 2 : 1, N, H, Dk, Dv);
+  return sizeof(float) * plan_floats(plan(dtype, T, N, H, Dk, Dv), backward ? 2 : 1, N, H, Dk, Dv);
 }
 
 int fw_linattn_forward(const fw_linattn* a, void* stream) {
   if (int rc = check(a, "fw_linattn_forward")) return rc;
   if (a->N == 0) return FW_OK;
   if (a->T > 0 && !a->out.p) return fw::set_error(FW_E_INVALID, "fw_linattn_forward: NULL out");
-  const Plan pl = plan(a->dtype, a->T, a->N, a->H, a->Dk, a->Dv, false);
+  const Plan pl = plan(a->dtype, a->T, a->N, a->H, a->Dk, a->Dv);
   if (!room(a, false)) return fw::set_error(FW_E_INVALID, "fw_linattn_forward: workspace too small");
   hipStream_t s = (hipStream_t)stream;
   float* ws = (float*)a->workspace;
@@ -1019,7 +1040,7 @@ int fw_linattn_backward(const fw_linattn* a, void* stream) {
   if (a->N == 0) return FW_OK;
   if (a->T > 0 && (!a->dout.p || !a->dq.p || !a->dk.p || !a->dv.p))
     return fw::set_error(FW_E_INVALID, "fw_linattn_backward: NULL dout, dq, dk or dv");
-  const Plan pl = plan(a->dtype, a->T, a->N, a->H, a->Dk, a->Dv, true);
+  const Plan pl = plan(a->dtype, a->T, a->N, a->H, a->Dk, a->Dv);
   if (!room(a, true)) return fw::set_error(FW_E_INVALID, "fw_linattn_backward: workspace too small");
   hipStream_t s = (hipStream_t)stream;
   float* ws = (float*)a->workspace;
