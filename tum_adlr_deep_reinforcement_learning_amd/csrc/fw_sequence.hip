@@ -78,6 +78,27 @@ struct Unit {
 
 enum { FULL, GUARD, SCALAR };  // D fills the tiles; whole vectors in or out; element by element
 
+// Element j of the result on lane x of four is element x of lane j's argument.
+template <int CTRL>
+__device__ __forceinline__ float quad_perm(float x) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, true));
+}
+__device__ __forceinline__ f32x4 quad_turn(f32x4 y, int x) {
+#pragma unroll
+  for (int j = 0; j < 4; j += 2) {  // lanes 1 apart
+    const float t = quad_perm<0xB1>(x & 1 ? y[j] : y[j + 1]);
+    y[j] = x & 1 ? t : y[j];
+    y[j + 1] = x & 1 ? y[j + 1] : t;
+  }
+#pragma unroll
+  for (int j = 0; j < 2; j++) {  // lanes 2 apart
+    const float t = quad_perm<0x4E>(x & 2 ? y[j] : y[j + 2]);
+    y[j] = x & 2 ? t : y[j];
+    y[j + 2] = x & 2 ? y[j + 2] : t;
+  }
+  return y;
+}
+
 // The state as a wave holds it: lane 16 g + r, key column 4 KT g + e, value column dv(f), in S[e % KT][f][e / KT] (WIDE)
 // or S[e / 4][f][e % 4].  Four keys move as one access where they lie together.
 template <int MODE, bool WIDE, int KT, int VT, typename Col>
@@ -89,6 +110,20 @@ __device__ __forceinline__ void load_state(f32x4 (&S)[KT][VT], const State& st, 
     else
       S[e / 4][f][e % 4] = x;
   };
+  // a segment's state with the roles exchanged: four lanes' columns by four keys lie together, row by row
+  if (!WIDE && st.sg && st.v1 == 1) {
+    const int x = threadIdx.x & 3;
+#pragma unroll
+    for (int f = 0; f < VT; f++) {
+      const int v4 = MODE == FULL ? dv(f) >> 2 : min(dv(f) >> 2, (Dv - 1) >> 2);
+#pragma unroll
+      for (int a = 0; a < KT; a++) {
+        const int k = 4 * KT * g + 4 * a + x;
+        S[a][f] = quad_turn(*(const f32x4*)(s + v4 * st.v4 + (MODE == FULL ? k : min(k, Dk - 1)) * st.k1), x);
+      }
+    }
+    return;
+  }
   const bool four = st.k1 == 1 && ((uintptr_t)s | (st.k4 | st.v4 | st.v1) * 4) % 16 == 0;
 #pragma unroll
   for (int f = 0; f < VT; f++) {  // outside Dk x Dv: the last row or column, which nothing reads
@@ -340,7 +375,8 @@ __global__ __launch_bounds__(64 * SCAN_WAVES) void k_scan(ScanArgs A) {
 //   rows         key tile z: row 16 z + r; query tile z: row 16 z + r; as depth j = 4 z + i of lane group g: row
 //                16 z + 4 g + i -- the result registers of the score product are the operand of the value product
 //   key columns  depth 8 s + j of lane group g: 4 KT g + 8 s + j; state tile a: 4 KT g + 4 a + i down its rows
-//   value cols   tile f: 4 VT (r >> 2) + 4 f + (r & 3) across, 4 VT g + 4 f + i down: a lane stores 4 VT neighbours
+//   value cols   tile f: VC (r >> 2) + 32 (f / 2) + 4 (f % 2) + (r & 3) across, VC = min(4 VT, 8), and so VC g + 32 (f / 2)
+//                + 4 (f % 2) + i down: a lane has VC neighbours together
 // Operands with tokens as depth (keys and values of the state's product, values of the output's) are read from LDS by
 // the transposing read: 4 lanes x 4 columns of one row each become 4 rows x 1 column per lane.
 // Products of the inputs are exact in the float32 accumulators.  What is not an input is split into bfloat16 terms:
@@ -350,12 +386,15 @@ __device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
-// 32 rows of 16 NT columns in LDS, as 16-byte chunks; chunk c of a row is stored at c ^ turn(row), so that neither the
-// row-wise nor the column-wise reads meet in a bank
-template <int NT>
+// 32 rows of 16 NT columns in LDS, as 16-byte chunks; chunk c of a row is stored at c ^ turn(row), so that the 16 lanes
+// that are served together meet in no bank: 16 rows of one chunk (across), or 4 rows of 4 half chunks (down)
+template <int NT, bool VALUES>
 struct Tile {
   static constexpr int CH = 2 * NT, BYTES = 32 * 16 * CH, RI = 64 / CH, NI = 32 / RI;  // RI rows per copy instruction
-  __device__ static __forceinline__ int turn(int row) { return (row / (CH >= 8 ? 1 : 8 / CH)) & ((CH < 8 ? CH : 8) - 1); }
+  __device__ static __forceinline__ int turn(int row) {
+    if (VALUES && NT == 4) return (row >> 1 & 1) * 4;
+    return (row / (16 / CH)) & (CH - 1);
+  }
   __device__ static __forceinline__ int at(int row, int chunk) { return (row * CH + (chunk ^ turn(row))) * 16; }
 
   // copies rows 0..31 of a block of c rows; row u is token u, or c - 1 - u when reversed; rows behind the block repeat
@@ -396,6 +435,27 @@ struct Tile {
     }
   }
 
+  // the rows from LDS to memory, numbered as in fetch
+  template <int MODE>
+  __device__ static __forceinline__ void put(const char* lds, bf16* base, int64_t st, int D, int c, bool rev, int lane) {
+    const int row0 = lane / CH, pc = lane % CH;
+#pragma unroll
+    for (int i = 0; i < NI; i++) {
+      const int row = i * RI + row0, col = (pc ^ turn(row)) * 8;
+      const u32x4 v = *(const u32x4*)(lds + (i * 64 + lane) * 16);
+      if (row < c && (MODE == FULL || col < D)) {
+        const int64_t u = rev ? c - 1 - row : row;
+        if constexpr (MODE == SCALAR) {
+#pragma unroll
+          for (int k = 0; k < 8; k++)
+            if (col + k < D) base[u * st + col + k].u = (uint16_t)(v[k / 2] >> 16 * (k & 1));
+        } else {
+          *(u32x4*)((char*)base + (uint32_t)((int)u * (int)st + col) * 2u) = v;
+        }
+      }
+    }
+  }
+
   // depth step s of rows 16 z + r: columns 4 NT g + 8 s ..
   __device__ static __forceinline__ u32x4 across(const char* lds, int z, int s, int r, int g) {
     if constexpr (NT == 1) {
@@ -410,7 +470,8 @@ struct Tile {
     u32x4 v;
 #pragma unroll
     for (int z = 0; z < 2; z++) {
-      const int byte = 8 * NT * (r & 3) + 8 * t, row = 16 * z + 4 * g + (r >> 2);
+      const int byte = (VALUES && NT == 4 ? 16 * (r & 3) + 64 * (t >> 1) + 8 * (t & 1) : 8 * NT * (r & 3) + 8 * t);
+      const int row = 16 * z + 4 * g + (r >> 2);
       const auto x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
           (__attribute__((address_space(3))) s16x4*)(lds + at(row, byte >> 4) + (byte & 8)));
       const u32x2 y = __builtin_bit_cast(u32x2, x);
@@ -430,13 +491,16 @@ __device__ __forceinline__ int here(int x) {
 template <int KT, int VT, int MODE>
 __global__ __launch_bounds__(64 * SCAN_WAVES, 2) void k_scan16(ScanArgs A) {
   constexpr int C = 32, NS = KT < 2 ? 1 : KT / 2;
-  using K = Tile<KT>;
-  using V = Tile<VT>;
-  __shared__ alignas(16) char smem[SCAN_WAVES][2 * K::BYTES + V::BYTES];
+  using K = Tile<KT, false>;
+  using V = Tile<VT, true>;
+  constexpr int VC = VT == 1 ? 4 : 8;
+  using Out = Tile<VT, false>;
+  __shared__ alignas(16) char smem[SCAN_WAVES][2 * K::BYTES + V::BYTES + Out::BYTES];
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
   char* const lq = smem[__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)];
   char* const lk = lq + K::BYTES;
   char* const lv = lk + K::BYTES;
+  char* const lo_ = lv + V::BYTES;
   Unit U;
   if (!U.decode(A)) return;
   const Pass p = A.pass[U.pass];
@@ -481,7 +545,7 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, 2) void k_scan16(ScanArgs A) {
   for (int a = 0; a < KT; a++)
 #pragma unroll
     for (int f = 0; f < VT; f++) S[a][f] = f32x4{0.f, 0.f, 0.f, 0.f};
-  auto column = [&](int f) { return v0 + 4 * VT * (r >> 2) + 4 * f + (r & 3); };
+  auto column = [&](int f) { return v0 + VC * (r >> 2) + 32 * (f >> 1) + 4 * (f & 1) + (r & 3); };
   if (p.in.p) load_state<MODE, false>(S, p.in, p.in.p + n * p.in.sn + h * p.in.sh + seg * p.in.sg, Dk, Dv, g, column);
 
   // Weights.  A reversed pass carries g x the state of the row before: its first weight is 1, and its final state is
@@ -643,29 +707,24 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, 2) void k_scan16(ScanArgs A) {
         O[f][0] = mma(vf[f], u32x4{Pl[0][0], Pl[0][1], 0, 0}, O[f][0]);
         O[f][1] = mma(vf[f], u32x4{Pl[1][0], Pl[1][1], Pl[2][0], Pl[2][1]}, O[f][1]);
       }
+      // through LDS, so that neighbouring lanes store neighbouring columns
 #pragma unroll
       for (int z = 0; z < 2; z++) {
-        const int u = 16 * z + r, col = 4 * VT * g, D = Dv - v0;
-        if (u < c) {
-          bf16* o = ob + (t0 + (rev ? c - 1 - u : u)) * p.o.st;
-          uint32_t x[2 * VT];
+        uint32_t x[2 * VT];
 #pragma unroll
-          for (int f = 0; f < VT; f++)
+        for (int f = 0; f < VT; f++)
 #pragma unroll
-            for (int m = 0; m < 2; m++) x[2 * f + m] = pack_bf16(O[f][z][2 * m], O[f][z][2 * m + 1]);
-          if constexpr (MODE == SCALAR) {
+          for (int m = 0; m < 2; m++) x[2 * f + m] = pack_bf16(O[f][z][2 * m], O[f][z][2 * m + 1]);
+        if constexpr (VT == 1) {
+          *(u32x2*)(lo_ + Out::at(16 * z + r, g >> 1) + 8 * (g & 1)) = u32x2{x[0], x[1]};
+        } else {
 #pragma unroll
-            for (int k = 0; k < 4 * VT; k++)
-              if (col + k < D) o[col + k].u = (uint16_t)(x[k / 2] >> 16 * (k & 1));
-          } else if constexpr (VT == 1) {
-            if (MODE == FULL || col < D) *(u32x2*)(o + col) = u32x2{x[0], x[1]};
-          } else {
-#pragma unroll
-            for (int k = 0; k < 2 * VT; k += 4)
-              if (MODE == FULL || col + 2 * k < D) *(u32x4*)(o + col + 2 * k) = u32x4{x[k], x[k + 1], x[k + 2], x[k + 3]};
-          }
+          for (int k = 0; k < VT / 2; k++)
+            *(u32x4*)(lo_ + Out::at(16 * z + r, g + 4 * k)) = u32x4{x[4 * k], x[4 * k + 1], x[4 * k + 2], x[4 * k + 3]};
         }
       }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      Out::template put<MODE>(lo_, ob + t0 * p.o.st, p.o.st, Dv - v0, c, rev, lane);
     }
 
     // the state: g^c S as S + S (g^c - 1), whose rounding does not add up over the blocks of a long memory
@@ -721,9 +780,10 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, 2) void k_scan16(ScanArgs A) {
   if (A.factor && U.slice == 0 && lane == 0)
     A.factor[((U.pass * A.N + n) * A.H + h) * A.n_seg + seg] = fresh ? 0.f : (L == 0 ? 1.f : expf(ld * (float)L));
   if (want_out) {  // rows behind the sequence's end
-    const float z[4 * VT] = {};
-    for (int64_t t = L + r; t < U.seg1 - U.seg0; t += 16)
-      store_cols<bf16, 4 * VT, MODE>(ob + t * p.o.st, 4 * VT * g, Dv - v0, z);
+    for (int i = 0; i < Out::NI; i++) *(u32x4*)(lo_ + (i * 64 + lane) * 16) = u32x4{0, 0, 0, 0};
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    for (int64_t t = L; t < U.seg1 - U.seg0; t += C)
+      Out::template put<MODE>(lo_, ob + t * p.o.st, p.o.st, Dv - v0, (int)min((int64_t)C, U.seg1 - U.seg0 - t), false, lane);
   }
 }
 
