@@ -169,18 +169,108 @@ __device__ __forceinline__ void store_state(const f32x4 (&S)[KT][VT], const Stat
     }
 }
 
-// NE contiguous elements at column `col` of a row of D; a column outside is read from column 0 (the caller drops it)
-template <typename T, int NE, int MODE>
-__device__ __forceinline__ void load_cols(const T* row, int col, int D, float* x) {
-  if constexpr (MODE == SCALAR) {
-#pragma unroll
-    for (int i = 0; i < NE; i++) x[i] = to_f32(row[col + i < D ? col + i : 0]);
-  } else {
-    constexpr int P = vec_elems<T>(NE);
-#pragma unroll
-    for (int i = 0; i < NE; i += P) load_vec<T, P>(row + (MODE == FULL || col + i < D ? col + i : 0), x + i);
-  }
+// Each active lane copies 16 bytes (or 1) from base + off to its own place behind `lds`: lane x 16 (x 4) bytes.  base and
+// lds are the same on all lanes.  There is no result to wait for by register: the reader waits on the count of memory
+// operations.  Written as asm because a copy known to the compiler makes it wait for ALL copies before any LDS read; the
+// five wait states are those between a VALU write of the base and its use (the compiler does not look into asm).
+__device__ __forceinline__ uint64_t uniform(const void* p) {
+  const uint64_t x = (uint64_t)p;
+  return (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32 |
+         (uint32_t)__builtin_amdgcn_readfirstlane((int)x);
 }
+__device__ __forceinline__ uint32_t lds_address(const char* lds) {
+  return __builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)lds);
+}
+__device__ __forceinline__ void copy16(const void* base, uint32_t off, char* lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds_address(lds)), "v"(off),
+               "s"(uniform(base))
+               : "memory");
+}
+__device__ __forceinline__ void copy1(const void* base, uint32_t off, char* lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_ubyte %1, %2" ::"s"(lds_address(lds)), "v"(off),
+               "s"(uniform(base))
+               : "memory");
+}
+
+// ROWS rows of 16 NT columns in LDS, as 16-byte chunks; chunk c of a row is stored at c ^ turn(row), so that the 16
+// lanes that are served together meet in no bank: 16 rows of one chunk, or (TRANSPOSED) 4 rows of 4 half chunks
+template <typename T, int NT, int ROWS, bool TRANSPOSED = false>
+struct Tile {
+  static constexpr int PER = 16 / sizeof(T), CH = 16 * NT / PER, BYTES = ROWS * CH * 16;
+  static constexpr int RI = 64 / CH, NI = (ROWS + RI - 1) / RI;  // RI rows per copy instruction
+  __device__ static __forceinline__ int turn(int row) {
+    if (TRANSPOSED && NT == 4) return (row >> 1 & 1) * 4;
+    return (CH >= 16 ? row : row / (16 / CH)) & ((CH < 16 ? CH : 16) - 1);
+  }
+  __device__ static __forceinline__ int at(int row, int chunk) { return (row * CH + (chunk ^ turn(row))) * 16; }
+
+  // copies the rows of a block of c rows; row u is token u, or c - 1 - u when reversed; rows behind the block repeat
+  // its last one.  Chunks outside D are left as they are (zeros).  base: the block's first token.
+  template <int MODE, bool WHOLE>
+  __device__ static __forceinline__ void fetch(char* lds, const T* base, int64_t st, int D, int c, bool rev, int lane) {
+    const int row0 = lane / CH, pc = lane % CH;
+    if constexpr (MODE == SCALAR) {
+#pragma unroll 1
+      for (int i = 0; i < NI; i++) {
+        const int row = i * RI + row0, col = (pc ^ turn(row)) * PER, u = min(row, c - 1);
+        const T* x = base + (int64_t)(rev ? c - 1 - u : u) * st;
+        Pack<T, PER> v;
+#pragma unroll
+        for (int m = 0; m < PER; m++) v.e[m] = col + m < D ? x[col + m] : T{};
+        if (row < ROWS) *(Pack<T, PER>*)(lds + (i * 64 + lane) * 16) = v;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < NI; i++) {
+        const int row = i * RI + row0, col = (pc ^ turn(row)) * PER;
+        if ((RI <= ROWS || row < ROWS) && (MODE == FULL || col < D)) {
+          // uniform base + 32-bit lane offset (the launcher saw that a block's rows fit)
+          if constexpr (WHOLE) {  // c = ROWS
+            const int first = rev ? ROWS - RI - i * RI : i * RI;
+            copy16(base + first * st, (uint32_t)((rev ? RI - 1 - row0 : row0) * (int)st + col) * (uint32_t)sizeof(T),
+                   lds + i * 1024);
+          } else {
+            const int u = min(row, c - 1);
+            copy16(base, (uint32_t)((rev ? c - 1 - u : u) * (int)st + col) * (uint32_t)sizeof(T), lds + i * 1024);
+          }
+        }
+      }
+    }
+  }
+
+  // the rows from LDS to memory, numbered as in fetch
+  template <int MODE>
+  __device__ static __forceinline__ void put(const char* lds, T* base, int64_t st, int D, int c, bool rev, int lane) {
+    const int row0 = lane / CH, pc = lane % CH;
+#pragma unroll
+    for (int i = 0; i < NI; i++) {
+      const int row = i * RI + row0, col = (pc ^ turn(row)) * PER;
+      if (RI > ROWS && row >= ROWS) continue;
+      const Pack<T, PER> v = *(const Pack<T, PER>*)(lds + (i * 64 + lane) * 16);
+      if (row < c && (MODE == FULL || col < D)) {
+        const int64_t u = rev ? c - 1 - row : row;
+        if constexpr (MODE == SCALAR) {
+#pragma unroll
+          for (int k = 0; k < PER; k++)
+            if (col + k < D) base[u * st + col + k] = v.e[k];
+        } else {
+          *(Pack<T, PER>*)((char*)base + (uint32_t)((int)u * (int)st + col) * (uint32_t)sizeof(T)) = v;
+        }
+      }
+    }
+  }
+};
+
+// the same value, but not known to be: keeps what a rare branch computes from it inside that branch
+__device__ __forceinline__ int here(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
+__device__ __forceinline__ f32x4 mma(float a, float b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
+}
+
 template <typename T, int NE, int MODE>
 __device__ __forceinline__ void store_cols(T* row, int col, int D, const float* x) {
   if constexpr (MODE == SCALAR) {
@@ -195,37 +285,90 @@ __device__ __forceinline__ void store_cols(T* row, int col, int D, const float* 
   }
 }
 
-__device__ __forceinline__ f32x4 mma(float a, float b, f32x4 c) {
-  return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
-}
-
 // One wave; lane = 16 g + r.  Operands of a 16x16x4 product: A row r, B column r, depth g; result: column r, rows
 // 4 g + i.  Depths and rows may be numbered at will as long as both operands agree, and the numbering below makes
 // every result register the operand register of the product that needs it, so nothing moves between lanes:
-//   tokens       depth step j of lane group g is token 4 g + j  (block of C = 16)
+//   rows         a block of C = 16 tokens in processing order; depth step j of lane group g is row 4 g + j
 //   key columns  4 KT g + e, e = KT i + a: row 4 g + i of state tile a
 //   value cols   VT r + f (operand tile f), 4 VT g + VT i + f (result)
 // S[a][f] = state tile (k columns a, v columns f); P[i] = weight x (k_s . q_t) for s = 4 g + i, t = r;
 // O[f] = out^T: value columns down the rows, tokens along the columns.
+// Blocks are copied to LDS by the load unit, NB of them ahead (no registers; the wait is for the oldest alone), in
+// processing order, so that a reversed pass is causal too: its rows run from the last token to the first.
+template <typename T, int KT, int VT>
+struct Ring {
+  using K = Tile<T, KT, 16>;
+  using V = Tile<T, VT, 16>;
+  static constexpr int BYTES = 2 * K::BYTES + V::BYTES + 256;  // queries, keys, values, episode starts
+  static constexpr int NB = BYTES * 4 <= 20480 ? 4 : BYTES * 3 <= 20480 ? 3 : BYTES * 2 <= 20480 ? 2 : 1;
+};
+template <int N>
+__device__ __forceinline__ void wait_loads() {  // all but the N newest memory operations are done
+  static_assert(N >= 0 && N < 64);
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
+}
+
 template <typename T, int KT, int VT, int MODE>
 __global__ __launch_bounds__(64 * SCAN_WAVES) void k_scan(ScanArgs A) {
   constexpr int C = 16, TPL = 4;
+  using R = Ring<T, KT, VT>;
+  using K = typename R::K;
+  using V = typename R::V;
+  constexpr int NB = R::NB;
+  __shared__ alignas(16) char smem[SCAN_WAVES][NB * R::BYTES];
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+  char* const ring = smem[__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)];
   Unit U;
   if (!U.decode(A)) return;
   const Pass p = A.pass[U.pass];
-  const int64_t n = U.n, seg0 = U.seg0, seg1 = U.seg1, L = U.L;
-  const int h = U.h, seg = U.seg, slice = U.slice;
+  const int64_t n = U.n, L = U.L;
+  const int h = U.h, seg = U.seg;
   const bool rev = p.rev;
-  const int Dk = p.Dk, Dv = p.Dv, v0 = slice * 16 * VT;
-  const T* qb = (const T*)p.q.p + n * p.q.sn + h * p.q.sh + seg0 * p.q.st;
-  const T* kb = (const T*)p.k.p + n * p.k.sn + h * p.k.sh + seg0 * p.k.st;
-  const T* vb = (const T*)p.v.p + n * p.v.sn + h * p.v.sh + seg0 * p.v.st + v0;
-  T* ob = (T*)p.o.p + n * p.o.sn + h * p.o.sh + seg0 * p.o.st + v0;
+  const int Dk = p.Dk, Dv = p.Dv, v0 = U.slice * 16 * VT;
+  const T* qb = (const T*)p.q.p + n * p.q.sn + h * p.q.sh + U.seg0 * p.q.st;
+  const T* kb = (const T*)p.k.p + n * p.k.sn + h * p.k.sh + U.seg0 * p.k.st;
+  const T* vb = (const T*)p.v.p + n * p.v.sn + h * p.v.sh + U.seg0 * p.v.st + v0;
+  T* ob = (T*)p.o.p + n * p.o.sn + h * p.o.sh + U.seg0 * p.o.st + v0;
   const bool want_out = p.o.p != nullptr;
-  const uint8_t* xb = A.starts ? A.starts + n * A.starts_sn + seg0 * A.starts_st : nullptr;
-  const float ld = A.log_decay[h];
-  auto power = [&](int m) { return m == 0 ? 1.0f : expf(ld * (float)m); };
+  const uint8_t* xb = A.starts ? A.starts + n * A.starts_sn + U.seg0 * A.starts_st : nullptr;
+  float ld = A.log_decay[h];
+  ld = ld < -1e30f ? -1e30f : ld;  // g^0 = 1 for g = 0 too
+  auto power = [&](int m) { return expf(ld * (float)m); };
+
+  // rows t0 .. t0 + c - 1 of the segment to a place of the ring
+  auto fetch = [&](char* to, int64_t t0, int c) {
+    auto go = [&](auto whole) {
+      constexpr bool W = decltype(whole)::value;
+      V::template fetch<MODE, W>(to + 2 * K::BYTES, vb + t0 * p.v.st, p.v.st, Dv - v0, c, rev, lane);
+      K::template fetch<MODE, W>(to + K::BYTES, kb + t0 * p.k.st, p.k.st, Dk, c, rev, lane);
+      if (want_out) K::template fetch<MODE, W>(to, qb + t0 * p.q.st, p.q.st, Dk, c, rev, lane);
+    };
+    if (c == C)
+      go(std::true_type());
+    else
+      go(std::false_type());
+    if (xb) {
+      const int u = min(lane, c - 1);
+      copy1(xb + t0 * A.starts_st, (uint32_t)((rev ? c - 1 - u : u) * (int)A.starts_st), to + 2 * K::BYTES + V::BYTES);
+    }
+  };
+  if constexpr (MODE == GUARD) {
+    for (int i = lane * 16; i < NB * R::BYTES; i += 1024) *(u32x4*)(ring + i) = u32x4{0, 0, 0, 0};
+    wait_loads<0>();
+  }
+  // the first blocks
+  int64_t asked = 0;  // tokens whose copy has been asked for
+  int ahead = 0, slot = 0;
+  auto fill = [&](int64_t from, int blocks, int size) {
+    asked = from;
+    slot = 0;
+    for (ahead = 0; ahead < blocks && asked < L; ahead++) {
+      const int c = (int)min((int64_t)size, L - asked);
+      fetch(ring + ahead * R::BYTES, rev ? L - asked - c : asked, c);
+      asked += c;
+    }
+  };
+  fill(0, NB, C);
 
   f32x4 S[KT][VT];
 #pragma unroll
@@ -233,145 +376,194 @@ __global__ __launch_bounds__(64 * SCAN_WAVES) void k_scan(ScanArgs A) {
 #pragma unroll
     for (int f = 0; f < VT; f++) S[a][f] = f32x4{0.f, 0.f, 0.f, 0.f};
   auto column = [&](int f) { return v0 + VT * r + f; };
-  if (p.in.p) load_state<MODE, true>(S, p.in, p.in.p + n * p.in.sn + h * p.in.sh + seg * p.in.sg, Dk, Dv, g, column);
+  if (p.in.p)
+    load_state<MODE, true>(S, p.in, p.in.p + n * p.in.sn + h * p.in.sh + seg * p.in.sg, Dk, Dv, g, column);
 
-  // weights of a whole block; a reversed pass carries g x the state of the token behind it, so that its final
-  // state is the gradient of the initial one and its first weight is 1
-  float wp[4], wi, wu[TPL], em1 = 0.f;
+  // Weights.  A reversed pass carries g x the state of the row before: its first weight is 1, and its final state is
+  // the gradient of the initial one.
+  const int e = rev ? 0 : 1;
+  float wp[4], wi = power(r + e), wu[TPL], em1 = 0.f;
   int cur = 0;
 #pragma unroll
-  for (int i = 0; i < 4; i++) {
-    const int d = rev ? 4 * g + i - r : r - 4 * g - i;
-    wp[i] = d >= 0 ? power(d) : 0.f;
-  }
-  bool fresh = false;    // an episode start among the segment's live tokens
-  int64_t done = 0;      // tokens processed
-  int single = 0;        // blocks of one token still to go (see below)
+  for (int i = 0; i < 4; i++) wp[i] = r >= 4 * g + i ? power(r - 4 * g - i) : 0.f;
+  bool fresh = false;  // an episode start among the live tokens
+  int64_t done = 0;
+  int single = 0;  // blocks of one token still to go
+  int steady = 0;  // blocks since the last fill
+  // memory operations of a block: copies (and the starts'), stores where their number is certain
+  constexpr int ND1 = V::NI + K::NI, ND2 = ND1 + K::NI;
+  constexpr int NST = MODE == FULL ? 4 * VT / vec_elems<T>(4 * VT) : 0;
   while (done < L) {
     const int c = single ? 1 : (int)min((int64_t)C, L - done);
     const int64_t t0 = rev ? L - done - c : done;
-    if (c != cur) {
-      cur = c;
-      wi = power(rev ? max(c - 1 - r, 0) : r + 1);
-#pragma unroll
-      for (int j = 0; j < TPL; j++) {
-        const int s = TPL * g + j;
-        wu[j] = s < c ? power(rev ? s + 1 : c - 1 - s) : 0.f;
-      }
-      em1 = expm1f(ld * (float)c);
+    if (ahead == 0) {
+      wait_loads<0>();
+      fill(done, single ? 1 : NB, single ? 1 : C);
+      steady = 0;
     }
-    uint32_t M = 0;  // bit s: an episode starts at token s of the block
-    if (xb) M = (uint32_t)__ballot(lane < c && xb[(t0 + (lane < c ? lane : 0)) * A.starts_st] != 0);
-    fresh |= M != 0;
+    // Newer than this block's copies are those of the NB - 1 blocks behind it and, NB blocks after a fill, the stores
+    // of the NB - 1 blocks before it.
+    if (MODE == SCALAR || ahead < NB || !want_out) {
+      if (MODE != SCALAR && ahead == NB)
+        wait_loads<(NB - 1) * ND1>();
+      else
+        wait_loads<0>();
+    } else if (steady < NB) {
+      wait_loads<(NB - 1) * ND2>();
+    } else {
+      wait_loads<(NB - 1) * (ND2 + NST)>();
+    }
+    const char* const lq = ring + slot * R::BYTES;
+    const char* const lk = lq + K::BYTES;
+    const char* const lv = lk + K::BYTES;
+    uint32_t M = 0;  // bit u: an episode starts at row u
+    if (xb) M = (uint32_t)__ballot(lane < c && *(const uint8_t*)(lv + V::BYTES + 4 * lane) != 0);
+    // A start at row u of a forward pass cuts every span that contains row u but not from it on; in a reversed pass
+    // the cut lies behind row u, that is at row u + 1.
+    const uint32_t cut = rev ? M << 1 : M;
 
-    // rows behind the block are read from its last token and dropped by zeros
-    float V[TPL][VT], K2[TPL][KT];
+    f32x4 P{0.f, 0.f, 0.f, 0.f};
+    f32x4 O[VT];
+#pragma unroll
+    for (int f = 0; f < VT; f++) O[f] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (want_out) {
+      // columns 4 KT g .. of row r, in the accesses of 16 bytes (or fewer) that hold them
+      constexpr int W = vec_elems<T>(4 * KT);
+#pragma unroll
+      for (int x = 0; x < 4 * KT; x += W) {
+        if (x == 16) asm volatile("" ::: "memory");  // bounds the operands in registers at a time
+        const int col = 4 * KT * g + x, byte = (col % K::PER) * (int)sizeof(T), o = K::at(r, col / K::PER) + byte;
+        float Q[W], K1[W];
+        load_vec<T, W>((const T*)(lq + o), Q);
+        load_vec<T, W>((const T*)(lk + o), K1);
+#pragma unroll
+        for (int y = 0; y < W; y++) {
+          P = mma(K1[y], Q[y], P);
+#pragma unroll
+          for (int f = 0; f < VT; f++) O[f] = mma(S[(x + y) % KT][f][(x + y) / KT], Q[y], O[f]);
+        }
+      }
+    }
+    float Vr[TPL][VT], K2[TPL][KT];
     float bad = 0.f;
 #pragma unroll
     for (int j = 0; j < TPL; j++) {
-      const int s = TPL * g + j;
-      const int64_t row = t0 + min(s, c - 1);
-      load_cols<T, VT, MODE>(vb + row * p.v.st, VT * r, Dv - v0, V[j]);
-      load_cols<T, KT, MODE>(kb + row * p.k.st, KT * r, Dk, K2[j]);
+      constexpr int WV = vec_elems<T>(VT), WK = vec_elems<T>(KT);
 #pragma unroll
-      for (int f = 0; f < VT; f++) {
-        bad += V[j][f];
-        if (s >= c) V[j][f] = 0.f;
-      }
+      for (int x = 0; x < VT; x += WV)
+        load_vec<T, WV>((const T*)(lv + V::at(4 * g + j, (VT * r + x) / V::PER) + (VT * r + x) % V::PER * (int)sizeof(T)), Vr[j] + x);
+#pragma unroll
+      for (int x = 0; x < KT; x += WK)
+        load_vec<T, WK>((const T*)(lk + K::at(4 * g + j, (KT * r + x) / K::PER) + (KT * r + x) % K::PER * (int)sizeof(T)), K2[j] + x);
     }
-    // A masked product is a product with 0, which keeps a value away only while that value is finite.  A block with
-    // an infinity or a NaN among its values is therefore run token by token: nothing is masked then.
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // every read of the block is done: its room is free
+    if (!single && asked < L) {
+      const int c2 = (int)min((int64_t)C, L - asked);
+      fetch(ring + slot * R::BYTES, rev ? L - asked - c2 : asked, c2);
+      asked += c2;
+    } else {
+      ahead--;
+    }
+    slot = slot + 1 == NB ? 0 : slot + 1;
+    steady++;
+
+#pragma unroll
+    for (int j = 0; j < TPL; j++)
+#pragma unroll
+      for (int f = 0; f < VT; f++) bad += Vr[j][f];
+    // A masked product is a product with 0, which keeps a value away only while that value is finite.  A block with an
+    // infinity or a NaN among its values is therefore run token by token: nothing is masked then.
     if (c > 1 && __any(!(fabsf(bad) < __builtin_huge_valf()))) {
       single = c;
+      ahead = 0;
       continue;
     }
-
+    fresh |= M != 0;
+    if (c != cur) {
+      cur = c;
+      const int g4 = here(4 * g);
+#pragma unroll
+      for (int j = 0; j < TPL; j++) wu[j] = power(max(c - e - (g4 + j), 0));
+      em1 = expm1f(ld * (float)c);
+    }
+    if (M != 0 || c < C) {
+      const int g4 = here(4 * g);
+#pragma unroll
+      for (int j = 0; j < TPL; j++) {
+        const bool live = g4 + j < c, open = (cut >> (g4 + j)) >> 1 == 0;
+#pragma unroll
+        for (int f = 0; f < VT; f++) Vr[j][f] = live ? Vr[j][f] : 0.f;
+#pragma unroll
+        for (int a = 0; a < KT; a++) K2[j][a] = live && open ? K2[j][a] : 0.f;
+      }
+    }
     if (want_out) {
-      float Q[4 * KT], K1[4 * KT];
-      load_cols<T, 4 * KT, MODE>(qb + (t0 + min(r, c - 1)) * p.q.st, 4 * KT * g, Dk, Q);
-      load_cols<T, 4 * KT, MODE>(kb + (t0 + min(r, c - 1)) * p.k.st, 4 * KT * g, Dk, K1);
-      if constexpr (MODE != FULL)
 #pragma unroll
-        for (int e = 0; e < 4 * KT; e++)
-          if (4 * KT * g + e >= Dk) Q[e] = 0.f;
-      f32x4 P{0.f, 0.f, 0.f, 0.f};
-      f32x4 O[VT];
+      for (int f = 0; f < VT; f++) O[f] *= wi;
 #pragma unroll
-      for (int f = 0; f < VT; f++) O[f] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int i = 0; i < 4; i++) P[i] = r >= 4 * g + i ? P[i] * wp[i] : 0.f;  // select, never multiply by 0
+      if (M != 0) {
+        const int g4 = here(4 * g), rr = here(r);
+        if (cut & ((2u << rr) - 1))
 #pragma unroll
-      for (int i = 0; i < 4; i++)
+          for (int f = 0; f < VT; f++) O[f] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int a = 0; a < KT; a++) {
-          P = mma(K1[KT * i + a], Q[KT * i + a], P);
-#pragma unroll
-          for (int f = 0; f < VT; f++) O[f] = mma(S[a][f][i], Q[KT * i + a], O[f]);
-        }
-      // weights and masks: select, never multiply by 0
-      const bool blocked = M != 0 && (rev ? (M >> r) >> 1 : M & ((2u << r) - 1)) != 0;
-#pragma unroll
-      for (int f = 0; f < VT; f++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) O[f][i] = blocked ? 0.f : O[f][i] * wi;
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        const int s = 4 * g + i;
-        bool keep = rev ? s >= r && s < c : s <= r;
-        if (M != 0) keep = keep && ((M >> min(s, r)) >> 1 & ((1u << abs(s - r)) - 1)) == 0;
-        P[i] = keep ? P[i] * wp[i] : 0.f;
+        for (int i = 0; i < 4; i++)
+          if (g4 + i < rr && ((cut >> (g4 + i)) >> 1 & ((1u << (rr - g4 - i)) - 1)) != 0) P[i] = 0.f;
       }
 #pragma unroll
       for (int j = 0; j < TPL; j++)
 #pragma unroll
-        for (int f = 0; f < VT; f++) O[f] = mma(V[j][f], P[j], O[f]);
+        for (int f = 0; f < VT; f++) O[f] = mma(Vr[j][f], P[j], O[f]);
       if (r < c) {
         float x[4 * VT];
 #pragma unroll
         for (int i = 0; i < 4; i++)
 #pragma unroll
           for (int f = 0; f < VT; f++) x[VT * i + f] = O[f][i];
-        store_cols<T, 4 * VT, MODE>(ob + (t0 + r) * p.o.st, 4 * VT * g, Dv - v0, x);
+        store_cols<T, 4 * VT, MODE>(ob + (t0 + (rev ? c - 1 - r : r)) * p.o.st, 4 * VT * g, Dv - v0, x);
       }
     }
 
     // the state: g^c S as S + S (g^c - 1), whose rounding does not add up over the blocks of a long memory
+    if (M != 0) {
+#pragma unroll
+      for (int a = 0; a < KT; a++)
+#pragma unroll
+        for (int f = 0; f < VT; f++) S[a][f] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
 #pragma unroll
     for (int a = 0; a < KT; a++)
 #pragma unroll
       for (int f = 0; f < VT; f++)
 #pragma unroll
-        for (int i = 0; i < 4; i++) S[a][f][i] = M != 0 ? 0.f : fmaf(S[a][f][i], em1, S[a][f][i]);
+        for (int i = 0; i < 4; i++) S[a][f][i] = fmaf(S[a][f][i], em1, S[a][f][i]);
 #pragma unroll
-    for (int j = 0; j < TPL; j++) {
-      const int s = TPL * g + j;
-      bool keep = s < c;
-      if (M != 0) keep = keep && (rev ? M & ((2u << s) - 1) : (M >> s) >> 1) == 0;
+    for (int j = 0; j < TPL; j++)
 #pragma unroll
       for (int a = 0; a < KT; a++) {
-        const float kw = keep ? K2[j][a] * wu[j] : 0.f;
+        const float kw = K2[j][a] * wu[j];
 #pragma unroll
-        for (int f = 0; f < VT; f++) S[a][f] = mma(kw, V[j][f], S[a][f]);
+        for (int f = 0; f < VT; f++) S[a][f] = mma(kw, Vr[j][f], S[a][f]);
       }
-    }
     done += c;
     if (single) single--;
   }
 
   if (p.out.p && (seg == A.n_seg - 1 || p.out.sg))
     store_state<MODE, true>(S, p.out, p.out.p + n * p.out.sn + h * p.out.sh + seg * p.out.sg, Dk, Dv, g, column);
-  if (A.factor && slice == 0 && lane == 0)
+  if (A.factor && U.slice == 0 && lane == 0)
     A.factor[((U.pass * A.N + n) * A.H + h) * A.n_seg + seg] = fresh ? 0.f : (L == 0 ? 1.f : expf(ld * (float)L));
   if (want_out) {  // rows behind the sequence's end
     const float z[4 * VT] = {};
-    for (int64_t t = L + r; t < seg1 - seg0; t += 16)
+    for (int64_t t = L + r; t < U.seg1 - U.seg0; t += 16)
       store_cols<T, 4 * VT, MODE>(ob + t * p.o.st, 4 * VT * g, Dv - v0, z);
   }
 }
 
-
 // ------------------------------------------------------------------ bfloat16
-// The same scan on the 16x16x32 product of bfloat16, in blocks of C = 32 tokens.  A block's rows are copied to LDS by
-// the load unit while the block before is computed (no registers, no waiting but for the copy itself), in processing
-// order, so that a reversed pass is causal too: its rows run from the last token to the first.
+// The same scan on the 16x16x32 product of bfloat16, in blocks of C = 32 tokens, the next block's rows copied to LDS
+// while a block is computed.
 //   rows         key tile z: row 16 z + r; query tile z: row 16 z + r; as depth j = 4 z + i of lane group g: row
 //                16 z + 4 g + i -- the result registers of the score product are the operand of the value product
 //   key columns  depth 8 s + j of lane group g: 4 KT g + 8 s + j; state tile a: 4 KT g + 4 a + i down its rows
@@ -386,115 +578,42 @@ __device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
-// 32 rows of 16 NT columns in LDS, as 16-byte chunks; chunk c of a row is stored at c ^ turn(row), so that the 16 lanes
-// that are served together meet in no bank: 16 rows of one chunk (across), or 4 rows of 4 half chunks (down)
+// Operands from the tiles.  Depth step s of rows 16 z + r: columns 4 NT g + 8 s ..
+template <int NT>
+__device__ __forceinline__ u32x4 across(const char* lds, int z, int s, int r, int g) {
+  using X = Tile<bf16, NT, 32>;
+  if constexpr (NT == 1) {
+    const u32x2 v = *(const u32x2*)(lds + X::at(16 * z + r, g >> 1) + 8 * (g & 1));
+    return u32x4{v[0], v[1], 0, 0};
+  } else {
+    return *(const u32x4*)(lds + X::at(16 * z + r, NT * g / 2 + s));
+  }
+}
+// tile t with the rows as depth
 template <int NT, bool VALUES>
-struct Tile {
-  static constexpr int CH = 2 * NT, BYTES = 32 * 16 * CH, RI = 64 / CH, NI = 32 / RI;  // RI rows per copy instruction
-  __device__ static __forceinline__ int turn(int row) {
-    if (VALUES && NT == 4) return (row >> 1 & 1) * 4;
-    return (row / (16 / CH)) & (CH - 1);
-  }
-  __device__ static __forceinline__ int at(int row, int chunk) { return (row * CH + (chunk ^ turn(row))) * 16; }
-
-  // copies rows 0..31 of a block of c rows; row u is token u, or c - 1 - u when reversed; rows behind the block repeat
-  // its last one.  Chunks outside D are left as they are (zeros).  base: the block's first token.
-  template <int MODE, bool WHOLE>
-  __device__ static __forceinline__ void fetch(char* lds, const bf16* base, int64_t st, int D, int c, bool rev, int lane) {
-    const int row0 = lane / CH, pc = lane % CH;
-    if constexpr (MODE == SCALAR) {
-#pragma unroll 1
-      for (int i = 0; i < NI; i++) {
-        const int row = i * RI + row0, col = (pc ^ turn(row)) * 8, u = min(row, c - 1);
-        const bf16* x = base + (int64_t)(rev ? c - 1 - u : u) * st;
-        u32x4 v;
+__device__ __forceinline__ u32x4 down(const char* lds, int t, int r, int g) {
+  using X = Tile<bf16, NT, 32, VALUES>;
+  u32x4 v;
 #pragma unroll
-        for (int m = 0; m < 4; m++) {
-          const uint32_t lo = col + 2 * m < D ? x[col + 2 * m].u : 0, hi = col + 2 * m + 1 < D ? x[col + 2 * m + 1].u : 0;
-          v[m] = lo | hi << 16;
-        }
-        *(u32x4*)(lds + (i * 64 + lane) * 16) = v;
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < NI; i++) {
-        const int row = i * RI + row0, col = (pc ^ turn(row)) * 8;
-        if (MODE == FULL || col < D) {
-          const char* from;
-          if constexpr (WHOLE) {  // c = 32: uniform base + 32-bit lane offset (the launcher saw that 32 rows fit)
-            const int first = rev ? 32 - RI - i * RI : i * RI;
-            from = (const char*)(base + first * st) + (uint32_t)((rev ? RI - 1 - row0 : row0) * (int)st + col) * 2u;
-          } else {
-            const int u = min(row, c - 1);
-            from = (const char*)base + (uint32_t)((rev ? c - 1 - u : u) * (int)st + col) * 2u;
-          }
-          __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
-                                           (__attribute__((address_space(3))) void*)(lds + i * 1024), 16, 0, 0);
-        }
-      }
-    }
+  for (int z = 0; z < 2; z++) {
+    const int byte = (VALUES && NT == 4 ? 16 * (r & 3) + 64 * (t >> 1) + 8 * (t & 1) : 8 * NT * (r & 3) + 8 * t);
+    const int row = 16 * z + 4 * g + (r >> 2);
+    const auto x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (__attribute__((address_space(3))) s16x4*)(lds + X::at(row, byte >> 4) + (byte & 8)));
+    const u32x2 y = __builtin_bit_cast(u32x2, x);
+    v[2 * z] = y[0];
+    v[2 * z + 1] = y[1];
   }
-
-  // the rows from LDS to memory, numbered as in fetch
-  template <int MODE>
-  __device__ static __forceinline__ void put(const char* lds, bf16* base, int64_t st, int D, int c, bool rev, int lane) {
-    const int row0 = lane / CH, pc = lane % CH;
-#pragma unroll
-    for (int i = 0; i < NI; i++) {
-      const int row = i * RI + row0, col = (pc ^ turn(row)) * 8;
-      const u32x4 v = *(const u32x4*)(lds + (i * 64 + lane) * 16);
-      if (row < c && (MODE == FULL || col < D)) {
-        const int64_t u = rev ? c - 1 - row : row;
-        if constexpr (MODE == SCALAR) {
-#pragma unroll
-          for (int k = 0; k < 8; k++)
-            if (col + k < D) base[u * st + col + k].u = (uint16_t)(v[k / 2] >> 16 * (k & 1));
-        } else {
-          *(u32x4*)((char*)base + (uint32_t)((int)u * (int)st + col) * 2u) = v;
-        }
-      }
-    }
-  }
-
-  // depth step s of rows 16 z + r: columns 4 NT g + 8 s ..
-  __device__ static __forceinline__ u32x4 across(const char* lds, int z, int s, int r, int g) {
-    if constexpr (NT == 1) {
-      const u32x2 v = *(const u32x2*)(lds + at(16 * z + r, g >> 1) + 8 * (g & 1));
-      return u32x4{v[0], v[1], 0, 0};
-    } else {
-      return *(const u32x4*)(lds + at(16 * z + r, NT * g / 2 + s));
-    }
-  }
-  // tile t with the rows as depth
-  __device__ static __forceinline__ u32x4 down(const char* lds, int t, int r, int g) {
-    u32x4 v;
-#pragma unroll
-    for (int z = 0; z < 2; z++) {
-      const int byte = (VALUES && NT == 4 ? 16 * (r & 3) + 64 * (t >> 1) + 8 * (t & 1) : 8 * NT * (r & 3) + 8 * t);
-      const int row = 16 * z + 4 * g + (r >> 2);
-      const auto x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-          (__attribute__((address_space(3))) s16x4*)(lds + at(row, byte >> 4) + (byte & 8)));
-      const u32x2 y = __builtin_bit_cast(u32x2, x);
-      v[2 * z] = y[0];
-      v[2 * z + 1] = y[1];
-    }
-    return v;
-  }
-};
-
-// the same value, but not known to be: keeps what a rare branch computes from it inside that branch
-__device__ __forceinline__ int here(int x) {
-  asm volatile("" : "+v"(x));
-  return x;
+  return v;
 }
 
 template <int KT, int VT, int MODE>
 __global__ __launch_bounds__(64 * SCAN_WAVES, 2) void k_scan16(ScanArgs A) {
   constexpr int C = 32, NS = KT < 2 ? 1 : KT / 2;
-  using K = Tile<KT, false>;
-  using V = Tile<VT, true>;
+  using K = Tile<bf16, KT, C>;
+  using V = Tile<bf16, VT, C, true>;
   constexpr int VC = VT == 1 ? 4 : 8;
-  using Out = Tile<VT, false>;
+  using Out = Tile<bf16, VT, C>;
   __shared__ alignas(16) char smem[SCAN_WAVES][2 * K::BYTES + V::BYTES + Out::BYTES];
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
   char* const lq = smem[__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)];
@@ -600,8 +719,8 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, 2) void k_scan16(ScanArgs A) {
 #pragma unroll
       for (int s = 0; s < NS; s++) {
         if (s == 2) asm volatile("" ::: "memory");  // bounds the operands in registers at a time
-        const u32x4 kf[2] = {K::across(lk, 0, s, r, g), K::across(lk, 1, s, r, g)};
-        const u32x4 qf[2] = {K::across(lq, 0, s, r, g), K::across(lq, 1, s, r, g)};
+        const u32x4 kf[2] = {across<KT>(lk, 0, s, r, g), across<KT>(lk, 1, s, r, g)};
+        const u32x4 qf[2] = {across<KT>(lq, 0, s, r, g), across<KT>(lq, 1, s, r, g)};
         P[0] = mma(kf[0], qf[0], P[0]);
         P[1] = mma(kf[0], qf[1], P[1]);
         P[2] = mma(kf[1], qf[1], P[2]);
@@ -624,9 +743,9 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, 2) void k_scan16(ScanArgs A) {
     }
     u32x4 vf[VT], k2[KT];
 #pragma unroll
-    for (int f = 0; f < VT; f++) vf[f] = V::down(lv, f, r, g);
+    for (int f = 0; f < VT; f++) vf[f] = down<VT, true>(lv, f, r, g);
 #pragma unroll
-    for (int a = 0; a < KT; a++) k2[a] = K::down(lk, a, r, g);
+    for (int a = 0; a < KT; a++) k2[a] = down<KT, false>(lk, a, r, g);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // every read of the block is done: its room is free
     loaded = !single && done + c < L;
     if (loaded) {
@@ -1032,6 +1151,7 @@ int check(const fw_linattn* a, const char* who) {
   if (a->dtype < FW_DT_F32 || a->dtype > FW_DT_F16) return bad("dtype must be float32, bfloat16 or float16");
   if (a->T > 0 && a->N > 0 && (!a->q.p || !a->k.p || !a->v.p)) return bad("NULL q, k or v");
   if (!a->log_decay) return bad("NULL log_decay");
+  if (a->starts && (a->starts_st < 0 || a->starts_st >= (int64_t)1 << 26)) return bad("starts_st must be 0..2^26 - 1");
   return FW_OK;
 }
 bool room(const fw_linattn* a, bool backward) {
