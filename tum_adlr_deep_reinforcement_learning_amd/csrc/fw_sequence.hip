@@ -271,20 +271,6 @@ __device__ __forceinline__ f32x4 mma(float a, float b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
 }
 
-template <typename T, int NE, int MODE>
-__device__ __forceinline__ void store_cols(T* row, int col, int D, const float* x) {
-  if constexpr (MODE == SCALAR) {
-#pragma unroll
-    for (int i = 0; i < NE; i++)
-      if (col + i < D) row[col + i] = from_f32<T>(x[i]);
-  } else {
-    constexpr int P = vec_elems<T>(NE);
-#pragma unroll
-    for (int i = 0; i < NE; i += P)
-      if (MODE == FULL || col + i < D) store_vec<T, P>(row + col + i, x + i);
-  }
-}
-
 // One wave; lane = 16 g + r.  Operands of a 16x16x4 product: A row r, B column r, depth g; result: column r, rows
 // 4 g + i.  Depths and rows may be numbered at will as long as both operands agree, and the numbering below makes
 // every result register the operand register of the product that needs it, so nothing moves between lanes:
@@ -300,7 +286,8 @@ struct Ring {
   using K = Tile<T, KT, 16>;
   using V = Tile<T, VT, 16>;
   static constexpr int BYTES = 2 * K::BYTES + V::BYTES + 256;  // queries, keys, values, episode starts
-  static constexpr int NB = BYTES * 4 <= 20480 ? 4 : BYTES * 3 <= 20480 ? 3 : BYTES * 2 <= 20480 ? 2 : 1;
+  static constexpr int ROOM = 20480 - V::BYTES;                // a wave's share of LDS, less the outputs
+  static constexpr int NB = BYTES * 4 <= ROOM ? 4 : BYTES * 3 <= ROOM ? 3 : BYTES * 2 <= ROOM ? 2 : 1;
 };
 template <int N>
 __device__ __forceinline__ void wait_loads() {  // all but the N newest memory operations are done
@@ -315,9 +302,10 @@ __global__ __launch_bounds__(64 * SCAN_WAVES) void k_scan(ScanArgs A) {
   using K = typename R::K;
   using V = typename R::V;
   constexpr int NB = R::NB;
-  __shared__ alignas(16) char smem[SCAN_WAVES][NB * R::BYTES];
+  __shared__ alignas(16) char smem[SCAN_WAVES][NB * R::BYTES + V::BYTES];
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
   char* const ring = smem[__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)];
+  char* const lo_ = ring + NB * R::BYTES;  // the block's outputs
   Unit U;
   if (!U.decode(A)) return;
   const Pass p = A.pass[U.pass];
@@ -347,10 +335,8 @@ __global__ __launch_bounds__(64 * SCAN_WAVES) void k_scan(ScanArgs A) {
       go(std::true_type());
     else
       go(std::false_type());
-    if (xb) {
-      const int u = min(lane, c - 1);
-      copy1(xb + t0 * A.starts_st, (uint32_t)((rev ? c - 1 - u : u) * (int)A.starts_st), to + 2 * K::BYTES + V::BYTES);
-    }
+    if (xb && lane < c)
+      copy1(xb + t0 * A.starts_st, (uint32_t)((rev ? c - 1 - lane : lane) * (int)A.starts_st), to + 2 * K::BYTES + V::BYTES);
   };
   if constexpr (MODE == GUARD) {
     for (int i = lane * 16; i < NB * R::BYTES; i += 1024) *(u32x4*)(ring + i) = u32x4{0, 0, 0, 0};
@@ -392,7 +378,7 @@ __global__ __launch_bounds__(64 * SCAN_WAVES) void k_scan(ScanArgs A) {
   int steady = 0;  // blocks since the last fill
   // memory operations of a block: copies (and the starts'), stores where their number is certain
   constexpr int ND1 = V::NI + K::NI, ND2 = ND1 + K::NI;
-  constexpr int NST = MODE == FULL ? 4 * VT / vec_elems<T>(4 * VT) : 0;
+  constexpr int NST = MODE == FULL ? V::NI : 0;
   while (done < L) {
     const int c = single ? 1 : (int)min((int64_t)C, L - done);
     const int64_t t0 = rev ? L - done - c : done;
@@ -515,14 +501,20 @@ __global__ __launch_bounds__(64 * SCAN_WAVES) void k_scan(ScanArgs A) {
       for (int j = 0; j < TPL; j++)
 #pragma unroll
         for (int f = 0; f < VT; f++) O[f] = mma(Vr[j][f], P[j], O[f]);
-      if (r < c) {
-        float x[4 * VT];
+      // through LDS, so that neighbouring lanes store neighbouring columns
+      float x[4 * VT];
 #pragma unroll
-        for (int i = 0; i < 4; i++)
+      for (int i = 0; i < 4; i++)
 #pragma unroll
-          for (int f = 0; f < VT; f++) x[VT * i + f] = O[f][i];
-        store_cols<T, 4 * VT, MODE>(ob + (t0 + (rev ? c - 1 - r : r)) * p.o.st, 4 * VT * g, Dv - v0, x);
+        for (int f = 0; f < VT; f++) x[VT * i + f] = O[f][i];
+      constexpr int W = vec_elems<T>(4 * VT);
+#pragma unroll
+      for (int k = 0; k < 4 * VT; k += W) {
+        const int col = 4 * VT * g + k;
+        store_vec<T, W>((T*)(lo_ + V::at(r, col / V::PER) + col % V::PER * (int)sizeof(T)), x + k);
       }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      V::template put<MODE>(lo_, ob + t0 * p.o.st, p.o.st, Dv - v0, c, rev, lane);
     }
 
     // the state: g^c S as S + S (g^c - 1), whose rounding does not add up over the blocks of a long memory
@@ -555,9 +547,10 @@ __global__ __launch_bounds__(64 * SCAN_WAVES) void k_scan(ScanArgs A) {
   if (A.factor && U.slice == 0 && lane == 0)
     A.factor[((U.pass * A.N + n) * A.H + h) * A.n_seg + seg] = fresh ? 0.f : (L == 0 ? 1.f : expf(ld * (float)L));
   if (want_out) {  // rows behind the sequence's end
-    const float z[4 * VT] = {};
-    for (int64_t t = L + r; t < U.seg1 - U.seg0; t += 16)
-      store_cols<T, 4 * VT, MODE>(ob + t * p.o.st, 4 * VT * g, Dv - v0, z);
+    for (int i = lane * 16; i < V::BYTES; i += 1024) *(u32x4*)(lo_ + i) = u32x4{0, 0, 0, 0};
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    for (int64_t t = L; t < U.seg1 - U.seg0; t += C)
+      V::template put<MODE>(lo_, ob + t * p.o.st, p.o.st, Dv - v0, (int)min((int64_t)C, U.seg1 - U.seg0 - t), false, lane);
   }
 }
 
@@ -899,6 +892,7 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, 2) void k_scan16(ScanArgs A) {
   if (A.factor && U.slice == 0 && lane == 0)
     A.factor[((U.pass * A.N + n) * A.H + h) * A.n_seg + seg] = fresh ? 0.f : (L == 0 ? 1.f : expf(ld * (float)L));
   if (want_out) {  // rows behind the sequence's end
+#pragma unroll
     for (int i = 0; i < Out::NI; i++) *(u32x4*)(lo_ + (i * 64 + lane) * 16) = u32x4{0, 0, 0, 0};
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     for (int64_t t = L; t < U.seg1 - U.seg0; t += C)
