@@ -285,8 +285,8 @@ template <typename T, int KT, int VT>
 struct Ring {
   using K = Tile<T, KT, 16>;
   using V = Tile<T, VT, 16>;
-  static constexpr int BYTES = 2 * K::BYTES + V::BYTES + 256;  // queries, keys, values, episode starts
-  static constexpr int ROOM = 20480 - V::BYTES;                // a wave's share of LDS, less the outputs
+  static constexpr int BYTES = 2 * K::BYTES + V::BYTES + 64;  // queries, keys, values, episode starts
+  static constexpr int ROOM = 20480;                           // a wave's share of LDS: eight waves on a CU
   static constexpr int NB = BYTES * 4 <= ROOM ? 4 : BYTES * 3 <= ROOM ? 3 : BYTES * 2 <= ROOM ? 2 : 1;
 };
 template <int N>
@@ -296,16 +296,15 @@ __device__ __forceinline__ void wait_loads() {  // all but the N newest memory o
 }
 
 template <typename T, int KT, int VT, int MODE>
-__global__ __launch_bounds__(64 * SCAN_WAVES) void k_scan(ScanArgs A) {
+__global__ __launch_bounds__(64 * SCAN_WAVES, KT * VT <= 16 ? 2 : 1) void k_scan(ScanArgs A) {
   constexpr int C = 16, TPL = 4;
   using R = Ring<T, KT, VT>;
   using K = typename R::K;
   using V = typename R::V;
   constexpr int NB = R::NB;
-  __shared__ alignas(16) char smem[SCAN_WAVES][NB * R::BYTES + V::BYTES];
+  __shared__ alignas(16) char smem[SCAN_WAVES][NB * R::BYTES];
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
   char* const ring = smem[__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)];
-  char* const lo_ = ring + NB * R::BYTES;  // the block's outputs
   Unit U;
   if (!U.decode(A)) return;
   const Pass p = A.pass[U.pass];
@@ -323,11 +322,10 @@ __global__ __launch_bounds__(64 * SCAN_WAVES) void k_scan(ScanArgs A) {
   ld = ld < -1e30f ? -1e30f : ld;  // g^0 = 1 for g = 0 too
   auto power = [&](int m) { return expf(ld * (float)m); };
 
-  // rows t0 .. t0 + c - 1 of the segment to a place of the ring
-  auto fetch = [&](char* to, int64_t t0, int c) {
+  // rows t0 .. t0 + c - 1 of the segment to a place of the ring: queries, keys and starts, then values
+  auto fetch_k = [&](char* to, int64_t t0, int c) {
     auto go = [&](auto whole) {
       constexpr bool W = decltype(whole)::value;
-      V::template fetch<MODE, W>(to + 2 * K::BYTES, vb + t0 * p.v.st, p.v.st, Dv - v0, c, rev, lane);
       K::template fetch<MODE, W>(to + K::BYTES, kb + t0 * p.k.st, p.k.st, Dk, c, rev, lane);
       if (want_out) K::template fetch<MODE, W>(to, qb + t0 * p.q.st, p.q.st, Dk, c, rev, lane);
     };
@@ -337,6 +335,12 @@ __global__ __launch_bounds__(64 * SCAN_WAVES) void k_scan(ScanArgs A) {
       go(std::false_type());
     if (xb && lane < c)
       copy1(xb + t0 * A.starts_st, (uint32_t)((rev ? c - 1 - lane : lane) * (int)A.starts_st), to + 2 * K::BYTES + V::BYTES);
+  };
+  auto fetch_v = [&](char* to, int64_t t0, int c) {
+    if (c == C)
+      V::template fetch<MODE, true>(to + 2 * K::BYTES, vb + t0 * p.v.st, p.v.st, Dv - v0, c, rev, lane);
+    else
+      V::template fetch<MODE, false>(to + 2 * K::BYTES, vb + t0 * p.v.st, p.v.st, Dv - v0, c, rev, lane);
   };
   if constexpr (MODE == GUARD) {
     for (int i = lane * 16; i < NB * R::BYTES; i += 1024) *(u32x4*)(ring + i) = u32x4{0, 0, 0, 0};
@@ -350,7 +354,8 @@ __global__ __launch_bounds__(64 * SCAN_WAVES) void k_scan(ScanArgs A) {
     slot = 0;
     for (ahead = 0; ahead < blocks && asked < L; ahead++) {
       const int c = (int)min((int64_t)size, L - asked);
-      fetch(ring + ahead * R::BYTES, rev ? L - asked - c : asked, c);
+      fetch_k(ring + ahead * R::BYTES, rev ? L - asked - c : asked, c);
+      fetch_v(ring + ahead * R::BYTES, rev ? L - asked - c : asked, c);
       asked += c;
     }
   };
@@ -399,9 +404,9 @@ __global__ __launch_bounds__(64 * SCAN_WAVES) void k_scan(ScanArgs A) {
     } else {
       wait_loads<(NB - 1) * (ND2 + NST)>();
     }
-    const char* const lq = ring + slot * R::BYTES;
-    const char* const lk = lq + K::BYTES;
-    const char* const lv = lk + K::BYTES;
+    char* const lq = ring + slot * R::BYTES;
+    char* const lk = lq + K::BYTES;
+    char* const lv = lk + K::BYTES;
     uint32_t M = 0;  // bit u: an episode starts at row u
     if (xb) M = (uint32_t)__ballot(lane < c && *(const uint8_t*)(lv + V::BYTES + 4 * lane) != 0);
     // A start at row u of a forward pass cuts every span that contains row u but not from it on; in a reversed pass
@@ -443,9 +448,11 @@ __global__ __launch_bounds__(64 * SCAN_WAVES) void k_scan(ScanArgs A) {
         load_vec<T, WK>((const T*)(lk + K::at(4 * g + j, (KT * r + x) / K::PER) + (KT * r + x) % K::PER * (int)sizeof(T)), K2[j] + x);
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // every read of the block is done: its room is free
-    if (!single && asked < L) {
-      const int c2 = (int)min((int64_t)C, L - asked);
-      fetch(ring + slot * R::BYTES, rev ? L - asked - c2 : asked, c2);
+    const bool more = !single && asked < L;  // a block to copy there; its values after the outputs have used their room
+    const int c2 = (int)min((int64_t)C, L - asked);
+    const int64_t t2 = rev ? L - asked - c2 : asked;
+    if (more) {
+      fetch_k(lq, t2, c2);
       asked += c2;
     } else {
       ahead--;
@@ -511,11 +518,14 @@ __global__ __launch_bounds__(64 * SCAN_WAVES) void k_scan(ScanArgs A) {
 #pragma unroll
       for (int k = 0; k < 4 * VT; k += W) {
         const int col = 4 * VT * g + k;
-        store_vec<T, W>((T*)(lo_ + V::at(r, col / V::PER) + col % V::PER * (int)sizeof(T)), x + k);
+        if (MODE != GUARD || col < Dv - v0)  // (the chunks outside stay zeros)
+          store_vec<T, W>((T*)(lv + V::at(r, col / V::PER) + col % V::PER * (int)sizeof(T)), x + k);
       }
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      V::template put<MODE>(lo_, ob + t0 * p.o.st, p.o.st, Dv - v0, c, rev, lane);
+      V::template put<MODE>(lv, ob + t0 * p.o.st, p.o.st, Dv - v0, c, rev, lane);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
+    if (more) fetch_v(lq, t2, c2);
 
     // the state: g^c S as S + S (g^c - 1), whose rounding does not add up over the blocks of a long memory
     if (M != 0) {
@@ -547,10 +557,10 @@ __global__ __launch_bounds__(64 * SCAN_WAVES) void k_scan(ScanArgs A) {
   if (A.factor && U.slice == 0 && lane == 0)
     A.factor[((U.pass * A.N + n) * A.H + h) * A.n_seg + seg] = fresh ? 0.f : (L == 0 ? 1.f : expf(ld * (float)L));
   if (want_out) {  // rows behind the sequence's end
-    for (int i = lane * 16; i < V::BYTES; i += 1024) *(u32x4*)(lo_ + i) = u32x4{0, 0, 0, 0};
+    for (int i = lane * 16; i < V::BYTES; i += 1024) *(u32x4*)(ring + i) = u32x4{0, 0, 0, 0};
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     for (int64_t t = L; t < U.seg1 - U.seg0; t += C)
-      V::template put<MODE>(lo_, ob + t * p.o.st, p.o.st, Dv - v0, (int)min((int64_t)C, U.seg1 - U.seg0 - t), false, lane);
+      V::template put<MODE>(ring, ob + t * p.o.st, p.o.st, Dv - v0, (int)min((int64_t)C, U.seg1 - U.seg0 - t), false, lane);
   }
 }
 
