@@ -1,10 +1,11 @@
 // fw_groupnorm.hip -- group norm with an activation over channels-last rows (include/fwrollout.h).
 //
-// A unit is one sample's group: L rows of cg = C / G adjacent channels, read as vectors of VW channels.  Three sizes:
+// A unit is one sample's group: L rows of cg = C / G adjacent channels, read as vectors of VW channels.  The kernels, by a unit's size:
 //   k_gn_wave   a unit fits 64 lanes x 4 vectors: 2^k lanes per unit, several units per wave; for one row per sample
 //               (a policy's features) this is a plain stream over the tensor
 //   k_gn_block  a unit fits a block's registers: read once, written once
-//   k_gn_*big   larger: statistics per part of the rows, joined by the blocks that apply them
+//   k_gn_bundle several neighbouring units do, where one has too few channels for 16-byte accesses
+//   k_gn_stream_*  larger: two passes over the tensor
 // All statistics are sums of deviations from a mean, so a large mean does not cancel.  Memory bound: x in, y out (and
 // dy in, dx out); the gradients of weight and bias are column sums of per-unit partial sums, in a fixed order.
 #include <algorithm>
@@ -28,7 +29,7 @@ struct GnArgs {
   float* stats;  // [N][G][2] or NULL
   float* dw;     // partial sums [R][C], or NULL
   float* db;
-  float* sums;   // big: [N][G][split][3]
+  float* sums;   // streams: [N][split][G][3]
 };
 
 __device__ __forceinline__ float param(const void* p, int dt, int c, float none) {
@@ -38,31 +39,66 @@ __device__ __forceinline__ float param(const void* p, int dt, int c, float none)
   return to_f32(((const f16*)p)[c]);
 }
 
-constexpr float RSQRT2 = 0.70710678118654752f, RSQRT2PI = 0.39894228040143268f;
+// Activations from the hardware's exp2 and reciprocal (an ulp each), with no division and no branch.
+__device__ __forceinline__ float exp_fast(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504f); }
+__device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.f + exp_fast(-z)); }
+__device__ __forceinline__ float tanh_fast(float z) {
+  // near 0 the difference below loses what it has; there the series to z^9 (next term 9e-9 of z at 1/4)
+  const float t = z * z;
+  const float p = fmaf(t, fmaf(t, fmaf(t, fmaf(t, 62.f / 2835.f, -17.f / 315.f), 2.f / 15.f), -1.f / 3.f), 1.f) * z;
+  const float q = fmaf(-2.f, __builtin_amdgcn_rcpf(1.f + exp_fast(2.f * z)), 1.f);
+  return fabsf(z) < 0.25f ? p : q;
+}
+// Phi(z), and e = exp(-z^2 / 2) beside it.  16-bit types: Abramowitz and Stegun 7.1.26 for erfc (absolute error 1.5e-7
+// of it, against 5e-4 of the types' own step); float32: the library's erfc.
+template <typename T>
+__device__ __forceinline__ float normal_cdf(float z, float& e) {
+  e = exp_fast(-0.5f * z * z);
+  if constexpr (sizeof(T) == 4) {
+    return 0.5f * erfcf(-z * 0.70710678f);
+  } else {
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f * 0.70710678f, fabsf(z), 1.f));
+    const float q = t * e *
+                    fmaf(t, fmaf(t, fmaf(t, fmaf(t, 0.5307027145f, -0.7265760135f), 0.7107068705f), -0.142248368f), 0.127414796f);
+    return z >= 0.f ? 1.f - q : (z < 0.f ? q : z);
+  }
+}
 
+template <typename T>
 __device__ __forceinline__ float act_value(float z, int act) {
+  float e;
   switch (act) {
     case FW_ACT_RELU: return z > 0.f ? z : (z != z ? z : 0.f);
-    case FW_ACT_SILU: return z / (1.f + expf(-z));
-    case FW_ACT_GELU: return 0.5f * z * erfcf(-z * RSQRT2);
-    case FW_ACT_TANH: return tanhf(z);
+    case FW_ACT_SILU: return z * sigmoid(z);
+    case FW_ACT_GELU: return z * normal_cdf<T>(z, e);
+    case FW_ACT_TANH: return tanh_fast(z);
   }
   return z;
 }
+template <typename T>
 __device__ __forceinline__ float act_slope(float z, int act) {
   switch (act) {
     case FW_ACT_RELU: return z > 0.f ? 1.f : 0.f;
     case FW_ACT_SILU: {
-      const float s = 1.f / (1.f + expf(-z));
-      return s * (1.f + z * (1.f - s));
+      const float s = sigmoid(z);
+      return s * fmaf(z, 1.f - s, 1.f);
     }
-    case FW_ACT_GELU: return 0.5f * erfcf(-z * RSQRT2) + z * RSQRT2PI * expf(-0.5f * z * z);
+    case FW_ACT_GELU: {
+      float e;
+      const float c = normal_cdf<T>(z, e);
+      return fmaf(z * 0.39894228f, e, c);
+    }
     case FW_ACT_TANH: {
-      const float t = tanhf(z);
-      return 1.f - t * t;
+      const float t = tanh_fast(z);
+      return fmaf(-t, t, 1.f);
     }
   }
   return 1.f;
+}
+// 1 / sqrt(x): the hardware's estimate and one step of Newton's
+__device__ __forceinline__ float inv_sqrt(float x) {
+  const float r = __builtin_amdgcn_rsqf(x);
+  return x < 1e-30f ? 1.f / sqrtf(x) : r * fmaf(-0.5f * x * r, r, 1.5f);
 }
 
 // ------------------------------------------------------------------ units of a few lanes
@@ -120,7 +156,7 @@ __global__ __launch_bounds__(256) void k_gn_wave(GnArgs A) {
         x[i][k] -= mean;
         s += ok[i] ? x[i][k] * x[i][k] : 0.f;
       }
-    const float r = 1.f / sqrtf(total_of(s) * inv + A.eps);
+    const float r = inv_sqrt(total_of(s) * inv + A.eps);
     if constexpr (!BWD) {
       if (A.stats && live && sub == 0) {
         A.stats[2 * (n * A.G + g)] = mean;
@@ -129,7 +165,7 @@ __global__ __launch_bounds__(256) void k_gn_wave(GnArgs A) {
 #pragma unroll
       for (int i = 0; i < VPL; i++) {
 #pragma unroll
-        for (int k = 0; k < VW; k++) x[i][k] = act_value(fmaf(x[i][k] * r, w[i][k], b[i][k]), A.act);
+        for (int k = 0; k < VW; k++) x[i][k] = act_value<T>(fmaf(x[i][k] * r, w[i][k], b[i][k]), A.act);
         if (ok[i] && live) store_vec<T, VW>((T*)A.y.p + n * A.y.sn + row[i] * A.y.sl + g * A.cg + col[i], x[i]);
       }
     } else {
@@ -139,7 +175,7 @@ __global__ __launch_bounds__(256) void k_gn_wave(GnArgs A) {
 #pragma unroll
         for (int k = 0; k < VW; k++) {
           x[i][k] *= r;
-          const float dz = ok[i] && live ? dy[i][k] * act_slope(fmaf(x[i][k], w[i][k], b[i][k]), A.act) : 0.f;
+          const float dz = ok[i] && live ? dy[i][k] * act_slope<T>(fmaf(x[i][k], w[i][k], b[i][k]), A.act) : 0.f;
           db[i][k] += dz;
           dw[i][k] += ok[i] && live ? dz * x[i][k] : 0.f;
           dy[i][k] = dz * w[i][k];
@@ -232,8 +268,13 @@ __device__ __forceinline__ int64_t xcd_unit(int64_t b, int64_t total) {
 }
 
 // ------------------------------------------------------------------ units held by one block
+// A thread holds up to `hold` vectors; with 8 channels a vector the backward kernel needs 6 x (4 + 4 + 8) registers and
+// as much for the channels' constants and sums, which 768 threads have and 1024 do not.
+constexpr int max_threads(bool bwd, int vw) { return bwd && vw == 8 ? 768 : 1024; }
+constexpr int max_hold(bool bwd, int vw) { return vw == 8 ? (bwd ? 6 : 8) : bwd ? 8 : 16; }
+
 template <typename T, int VW, int VPT, bool BWD>
-__global__ __launch_bounds__(1024) void k_gn_block(GnArgs A) {
+__global__ __launch_bounds__(max_threads(BWD, VW)) void k_gn_block(GnArgs A) {
   __shared__ float red[16][2];
   extern __shared__ float cols[];  // VW * 1024 floats in the backward kernel
   const int64_t u = xcd_unit(blockIdx.x, A.N * A.G);
@@ -275,7 +316,7 @@ __global__ __launch_bounds__(1024) void k_gn_block(GnArgs A) {
           v[0] = fmaf(d, d, v[0]);
         }
     block_sum<2>(v, red);
-    r = 1.f / sqrtf(v[0] * inv + A.eps);
+    r = inv_sqrt(v[0] * inv + A.eps);
     if (A.stats && t == 0) {
       A.stats[2 * u] = mean;
       A.stats[2 * u + 1] = r;
@@ -293,7 +334,7 @@ __global__ __launch_bounds__(1024) void k_gn_block(GnArgs A) {
       if (have(i)) {
         float y[VW];
 #pragma unroll
-        for (int k = 0; k < VW; k++) y[k] = act_value(fmaf((to_f32(xv[i].e[k]) - mean) * r, w[k], b[k]), A.act);
+        for (int k = 0; k < VW; k++) y[k] = act_value<T>(fmaf((to_f32(xv[i].e[k]) - mean) * r, w[k], b[k]), A.act);
         store_vec<T, VW>((T*)A.y.p + n * A.y.sn + (r0 + (int64_t)rp * i) * A.y.sl + c, y);
       }
   } else {
@@ -307,7 +348,7 @@ __global__ __launch_bounds__(1024) void k_gn_block(GnArgs A) {
 #pragma unroll
         for (int k = 0; k < VW; k++) {
           const float xh = (to_f32(xv[i].e[k]) - mean) * r;
-          const float dz = to_f32(dv[i].e[k]) * act_slope(fmaf(xh, w[k], b[k]), A.act);
+          const float dz = to_f32(dv[i].e[k]) * act_slope<T>(fmaf(xh, w[k], b[k]), A.act);
           db[k] += dz;
           dw[k] = fmaf(dz, xh, dw[k]);
           d[i][k] = dz * w[k];
@@ -339,234 +380,445 @@ __global__ __launch_bounds__(1024) void k_gn_block(GnArgs A) {
   }
 }
 
-// ------------------------------------------------------------------ units of any size
+// ------------------------------------------------------------------ several units held by one block
+// Where a group's channels do not fill 16-byte vectors, a block takes `bundle` neighbouring groups that together do.  A
+// vector's channels may then belong to different groups, so sums are kept per channel and joined per group at the end;
+// the backward pass needs the sums per channel anyway.
+template <typename T, int VPT, bool BWD>
+__global__ __launch_bounds__(max_threads(BWD, 16 / sizeof(T))) void k_gn_bundle(GnArgs A, int bundle) {
+  constexpr int VW = 16 / sizeof(T);
+  extern __shared__ float lds[];  // VW * 1024 for the column sums
+  __shared__ float chan[2][1024], group[2][64];
+  const int64_t u = xcd_unit(blockIdx.x, A.N * A.G / bundle);
+  const int64_t n = u / (A.G / bundle);
+  const int g0 = (int)(u % (A.G / bundle)) * bundle, t = threadIdx.x, width = bundle * A.cg;
+  const int cols = width / VW, rp = (int)blockDim.x / cols;
+  const bool on = t < rp * cols;
+  const int r0 = t / cols, col = (on ? t - r0 * cols : 0) * VW, c = g0 * A.cg + col;
+  const float inv = 1.f / ((float)A.L * (float)A.cg);
+  auto have = [&](int i) { return on && r0 + (int64_t)rp * i < A.L; };
+  Pack<T, VW> xv[VPT], dv[VPT];
+#pragma unroll
+  for (int i = 0; i < VPT; i++)
+    if (have(i)) {
+      const int64_t row = r0 + (int64_t)rp * i;
+      xv[i] = *(const Pack<T, VW>*)((const T*)A.x.p + n * A.x.sn + row * A.x.sl + c);
+      if constexpr (BWD) dv[i] = *(const Pack<T, VW>*)((const T*)A.dy.p + n * A.dy.sn + row * A.dy.sl + c);
+    }
+  int gi[VW];
+#pragma unroll
+  for (int k = 0; k < VW; k++) gi[k] = (col + k) / A.cg;
+  // per group, on every thread: the sum over the group's channels of v's sums over the rows, times scale[channel]
+  auto group_sums = [&](float* v, int which, const float* scale) {
+    column_sum<VW>(v, t, rp, cols, on, lds);
+    if (t < cols)
+#pragma unroll
+      for (int k = 0; k < VW; k++) chan[which][col + k] = scale ? v[k] * scale[k] : v[k];
+    __syncthreads();
+    if (t < bundle) {
+      float s = 0.f;
+      for (int k = 0; k < A.cg; k++) s += chan[which][t * A.cg + k];
+      group[which][t] = s;
+    }
+    __syncthreads();
+  };
+  float v[VW], mean[VW], r[VW], w[VW], b[VW];
+  if (BWD && A.stats) {
+#pragma unroll
+    for (int k = 0; k < VW; k++) {
+      mean[k] = A.stats[2 * (n * A.G + g0 + gi[k])];
+      r[k] = A.stats[2 * (n * A.G + g0 + gi[k]) + 1];
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < VW; k++) v[k] = 0.f;
+#pragma unroll
+    for (int i = 0; i < VPT; i++)
+      if (have(i))
+#pragma unroll
+        for (int k = 0; k < VW; k++) v[k] += to_f32(xv[i].e[k]);
+    group_sums(v, 0, nullptr);
+#pragma unroll
+    for (int k = 0; k < VW; k++) {
+      mean[k] = group[0][gi[k]] * inv;
+      v[k] = 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < VPT; i++)
+      if (have(i))
+#pragma unroll
+        for (int k = 0; k < VW; k++) {
+          const float d = to_f32(xv[i].e[k]) - mean[k];
+          v[k] = fmaf(d, d, v[k]);
+        }
+    group_sums(v, 1, nullptr);
+#pragma unroll
+    for (int k = 0; k < VW; k++) r[k] = inv_sqrt(group[1][gi[k]] * inv + A.eps);
+    if (A.stats && t < bundle) {
+      A.stats[2 * (n * A.G + g0 + t)] = group[0][t] * inv;
+      A.stats[2 * (n * A.G + g0 + t) + 1] = inv_sqrt(group[1][t] * inv + A.eps);
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < VW; k++) {
+    w[k] = param(A.w, A.wdt, c + k, 1.f);
+    b[k] = param(A.b, A.wdt, c + k, 0.f);
+  }
+  if constexpr (!BWD) {
+#pragma unroll
+    for (int i = 0; i < VPT; i++)
+      if (have(i)) {
+        float y[VW];
+#pragma unroll
+        for (int k = 0; k < VW; k++) y[k] = act_value<T>(fmaf((to_f32(xv[i].e[k]) - mean[k]) * r[k], w[k], b[k]), A.act);
+        store_vec<T, VW>((T*)A.y.p + n * A.y.sn + (r0 + (int64_t)rp * i) * A.y.sl + c, y);
+      }
+  } else {
+    float dw[VW], db[VW], d[VPT][VW];
+#pragma unroll
+    for (int k = 0; k < VW; k++) dw[k] = db[k] = 0.f;
+#pragma unroll
+    for (int i = 0; i < VPT; i++)
+      if (have(i))
+#pragma unroll
+        for (int k = 0; k < VW; k++) {
+          const float xh = (to_f32(xv[i].e[k]) - mean[k]) * r[k];
+          d[i][k] = to_f32(dv[i].e[k]) * act_slope<T>(fmaf(xh, w[k], b[k]), A.act);
+          db[k] += d[i][k];
+          dw[k] = fmaf(d[i][k], xh, dw[k]);
+        }
+    group_sums(db, 0, w);  // sum dxh = sum w db, sum dxh xh = sum w dw
+    group_sums(dw, 1, w);
+    if (t < cols)
+#pragma unroll
+      for (int k = 0; k < VW; k++) {
+        if (A.dw) A.dw[n * A.G * A.cg + c + k] = dw[k];
+        if (A.db) A.db[n * A.G * A.cg + c + k] = db[k];
+      }
+#pragma unroll
+    for (int i = 0; i < VPT; i++)
+      if (have(i)) {
+        float y[VW];
+#pragma unroll
+        for (int k = 0; k < VW; k++) {
+          const float xh = (to_f32(xv[i].e[k]) - mean[k]) * r[k];
+          y[k] = r[k] * (d[i][k] * w[k] - group[0][gi[k]] * inv - xh * (group[1][gi[k]] * inv));
+        }
+        store_vec<T, VW>((T*)A.dx.p + n * A.dx.sn + (r0 + (int64_t)rp * i) * A.dx.sl + c, y);
+      }
+  }
+}
+
+// ------------------------------------------------------------------ streams over whole rows
+// Two passes over the tensor, each a plain stream: a block takes some rows of a sample and all its channels (256 vectors
+// at a time, so that a thread keeps its channels), and leaves sums per group (and, backward, per channel); these are
+// joined, and the second pass applies them.
+
 // (count, mean, sum of squared deviations) of two sets joined
 __device__ __forceinline__ void join(float& n, float& m, float& q, float n2, float m2, float q2) {
   if (n2 == 0.f) return;
-  const float t = n + n2, d = m2 - m;
-  m = fmaf(d, n2 / t, m);
-  q += q2 + d * d * (n * n2 / t);
+  const float t = n + n2, d = m2 - m, f = n2 * __builtin_amdgcn_rcpf(t);
+  m = fmaf(d, f, m);
+  q += q2 + d * d * (n * f);
   n = t;
 }
-// the same over a block, in a fixed order; the result on every thread
-__device__ __forceinline__ void block_join(float& n, float& m, float& q, float (*lds)[3]) {
-#pragma unroll
-  for (int s = 1; s < 64; s <<= 1) {
-    const float n2 = __shfl_xor(n, s), m2 = __shfl_xor(m, s), q2 = __shfl_xor(q, s);
-    // the lower lane's set first on both sides, so that both get the same bits
-    if (threadIdx.x & s) {
-      float a = n2, b = m2, c = q2;
-      join(a, b, c, n, m, q);
-      n = a;
-      m = b;
-      q = c;
-    } else {
-      join(n, m, q, n2, m2, q2);
-    }
-  }
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) {
-    lds[threadIdx.x >> 6][0] = n;
-    lds[threadIdx.x >> 6][1] = m;
-    lds[threadIdx.x >> 6][2] = q;
-  }
-  __syncthreads();
-  n = m = q = 0.f;
-  for (int w = 0; w < (int)blockDim.x / 64; w++) join(n, m, q, lds[w][0], lds[w][1], lds[w][2]);
-}
 
-// The part's rows [l0, l1), and for each column chunk f(row, column, i) with the column fixed for a thread.
 struct Part {
-  int64_t n, u, l0, l1;
-  int g, s;
+  int64_t n, l0, l1;
+  int s;
 };
 __device__ __forceinline__ Part part_of(const GnArgs& A) {
   Part p;
-  const int64_t b = xcd_unit(blockIdx.x, A.N * A.G * A.split);
-  // parts of neighbouring groups are neighbours: (n, s, g)
-  p.g = (int)(b % A.G);
-  p.s = (int)(b / A.G % A.split);
-  p.n = b / A.G / A.split;
-  p.u = p.n * A.G + p.g;
+  p.n = blockIdx.x / A.split;
+  p.s = blockIdx.x % A.split;
   const int64_t per = (A.L + A.split - 1) / A.split;
   p.l0 = min(A.L, p.s * per);
   p.l1 = min(A.L, p.l0 + per);
   return p;
 }
+// this thread's place in a chunk of columns that begins with vector c0
+struct Place {
+  int cols, rp, r0, v;  // columns of the chunk, rows at a time, first row, vector
+  bool on;
+};
+__device__ __forceinline__ Place place_of(int vectors, int c0) {
+  Place p;
+  p.cols = min(256, vectors - c0);
+  p.rp = 256 / p.cols;
+  p.r0 = (int)threadIdx.x / p.cols;
+  p.on = p.r0 < p.rp;
+  p.v = c0 + (int)threadIdx.x % p.cols;
+  return p;
+}
 
 template <typename T, int VW>
-__global__ __launch_bounds__(256) void k_gn_big_stats(GnArgs A) {
-  __shared__ float lds[4][3];
+__global__ __launch_bounds__(256) void k_gn_stream_stats(GnArgs A) {
+  __shared__ float lds[3][VW][256];
   const Part p = part_of(A);
-  const int cgv = A.cg / VW, t = threadIdx.x;
-  float n = 0.f, m = 0.f, q = 0.f;
-  const int step = min(cgv, 256), rp = 256 / step;
-  for (int c0 = 0; c0 < cgv; c0 += step) {
-    const int cv = c0 + t % step;
-    if (t >= rp * step || cv >= cgv) continue;
-    const T* x = (const T*)A.x.p + p.n * A.x.sn + p.g * A.cg + cv * VW;
-    constexpr int B = 4;  // rows at a time: exact deviations within, joined outside
-    for (int64_t l = p.l0 + t / step; l < p.l1; l += (int64_t)rp * B) {
-      float v[B][VW], s = 0.f, d2 = 0.f, cnt = 0.f;
+  const int C = A.G * A.cg, t = threadIdx.x;
+  float* out = A.sums + (p.n * A.split + p.s) * A.G * 3;
+  for (int c0 = 0; c0 < C / VW; c0 += 256) {
+    const Place at = place_of(C / VW, c0);
+    // per channel and thread: running mean and squared deviations
+    float n = 0.f, m[VW], q[VW];
 #pragma unroll
-      for (int i = 0; i < B; i++) {
-        const int64_t row = l + (int64_t)rp * i;
-        load_vec<T, VW>(x + min(row, p.l1 - 1) * A.x.sl, v[i]);
-        if (row < p.l1) {
-          cnt += VW;
+    for (int k = 0; k < VW; k++) m[k] = q[k] = 0.f;
+    const T* x = (const T*)A.x.p + p.n * A.x.sn + at.v * VW;
+    if (at.on) {
+      constexpr int B = 4;  // rows in flight
+      for (int64_t l = p.l0 + at.r0; l < p.l1; l += (int64_t)at.rp * B) {
+        float v[B][VW];
 #pragma unroll
-          for (int k = 0; k < VW; k++) s += v[i][k];
-        }
+        for (int i = 0; i < B; i++) load_vec<T, VW>(x + min(l + (int64_t)at.rp * i, p.l1 - 1) * A.x.sl, v[i]);
+#pragma unroll
+        for (int i = 0; i < B; i++)
+          if (l + (int64_t)at.rp * i < p.l1) {
+            n += 1.f;
+            const float f = __builtin_amdgcn_rcpf(n);
+#pragma unroll
+            for (int k = 0; k < VW; k++) {
+              const float d = v[i][k] - m[k];
+              m[k] = fmaf(d, f, m[k]);
+              q[k] = fmaf(d, v[i][k] - m[k], q[k]);
+            }
+          }
       }
-      const float mm = s / cnt;
+    }
+    // over the threads of a column, in a fixed order
+    __syncthreads();
 #pragma unroll
-      for (int i = 0; i < B; i++)
-        if (l + (int64_t)rp * i < p.l1)
+    for (int k = 0; k < VW; k++) {
+      lds[0][k][t] = n;
+      lds[1][k][t] = m[k];
+      lds[2][k][t] = q[k];
+    }
+    __syncthreads();
+    for (int rows = at.rp; rows > 1; rows = (rows + 1) >> 1) {
+      const int other = t + ((rows + 1) >> 1) * at.cols;
+      if (at.on && t < (rows >> 1) * at.cols)
 #pragma unroll
-          for (int k = 0; k < VW; k++) d2 = fmaf(v[i][k] - mm, v[i][k] - mm, d2);
-      join(n, m, q, cnt, mm, d2);
+        for (int k = 0; k < VW; k++)
+          join(lds[0][k][t], lds[1][k][t], lds[2][k][t], lds[0][k][other], lds[1][k][other], lds[2][k][other]);
+      __syncthreads();
+    }
+    // over the channels of a group; a group that began in the chunk before goes on
+    const int g0 = c0 * VW / A.cg, g1 = ((c0 + at.cols) * VW - 1) / A.cg;
+    for (int g = g0 + t; g <= g1; g += 256) {
+      float n = 0.f, m = 0.f, q = 0.f;
+      if (g * A.cg < c0 * VW) {
+        n = out[3 * g];
+        m = out[3 * g + 1];
+        q = out[3 * g + 2];
+      }
+      const int first = max(g * A.cg, c0 * VW), last = min((g + 1) * A.cg, (c0 + at.cols) * VW);
+      for (int c = first; c < last; c++) {
+        const int v = c / VW - c0, k = c % VW;
+        join(n, m, q, lds[0][k][v], lds[1][k][v], lds[2][k][v]);
+      }
+      out[3 * g] = n;
+      out[3 * g + 1] = m;
+      out[3 * g + 2] = q;
+    }
+    __syncthreads();
+  }
+}
+
+// The parts of a sample's group joined, one wave each, in a fixed order: its mean and 1 / sqrt(var + eps), or (BWD) the
+// means of dxh and of dxh xh.
+template <bool BWD>
+__global__ __launch_bounds__(256) void k_gn_stream_join(GnArgs A, float* out) {
+  const int64_t u = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  if (u >= A.N * A.G) return;
+  float n = 0.f, m = 0.f, q = 0.f;
+  for (int s = lane; s < A.split; s += 64) {
+    const float* o = A.sums + ((u / A.G * A.split + s) * A.G + u % A.G) * 3;
+    if constexpr (BWD) {
+      m += o[0];
+      q += o[1];
+    } else {
+      join(n, m, q, o[0], o[1], o[2]);
     }
   }
-  block_join(n, m, q, lds);
-  if (t == 0) {
-    float* o = A.sums + (p.u * A.split + p.s) * 3;
-    o[0] = n;
-    o[1] = m;
-    o[2] = q;
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) {
+    const float n2 = __shfl_down(n, d), m2 = __shfl_down(m, d), q2 = __shfl_down(q, d);
+    if constexpr (BWD) {
+      m += m2;
+      q += q2;
+    } else {
+      join(n, m, q, n2, m2, q2);
+    }
+  }
+  if (lane == 0) {
+    const float inv = 1.f / ((float)A.L * (float)A.cg);
+    out[2 * u] = BWD ? m * inv : m;
+    out[2 * u + 1] = BWD ? q * inv : inv_sqrt(q * inv + A.eps);
   }
 }
 
 template <typename T, int VW>
-__global__ __launch_bounds__(256) void k_gn_big_apply(GnArgs A) {
+__global__ __launch_bounds__(256) void k_gn_stream_apply(GnArgs A) {
   const Part p = part_of(A);
-  float n = 0.f, m = 0.f, q = 0.f;
-  for (int s = 0; s < A.split; s++) {
-    const float* o = A.sums + (p.u * A.split + s) * 3;
-    join(n, m, q, o[0], o[1], o[2]);
-  }
-  const float r = 1.f / sqrtf(q / n + A.eps);
-  const int cgv = A.cg / VW, t = threadIdx.x;
-  if (A.stats && p.s == 0 && t == 0) {
-    A.stats[2 * p.u] = m;
-    A.stats[2 * p.u + 1] = r;
-  }
-  const int step = min(cgv, 256), rp = 256 / step;
-  for (int c0 = 0; c0 < cgv; c0 += step) {
-    const int cv = c0 + t % step;
-    if (t >= rp * step || cv >= cgv) continue;
-    const int c = p.g * A.cg + cv * VW;
-    float w[VW], b[VW];
+  const int C = A.G * A.cg;
+  for (int c0 = 0; c0 < C / VW; c0 += 256) {
+    const Place at = place_of(C / VW, c0);
+    if (!at.on) continue;
+    const int c = at.v * VW;
+    float m[VW], w[VW], b[VW];
 #pragma unroll
     for (int k = 0; k < VW; k++) {
-      w[k] = param(A.w, A.wdt, c + k, 1.f);
+      const int64_t g = p.n * A.G + (c + k) / A.cg;
+      m[k] = A.stats[2 * g];
+      w[k] = A.stats[2 * g + 1] * param(A.w, A.wdt, c + k, 1.f);
       b[k] = param(A.b, A.wdt, c + k, 0.f);
     }
-    for (int64_t l = p.l0 + t / step; l < p.l1; l += rp) {
-      float x[VW];
-      load_vec<T, VW>((const T*)A.x.p + p.n * A.x.sn + l * A.x.sl + c, x);
+    const T* x = (const T*)A.x.p + p.n * A.x.sn + c;
+    T* y = (T*)A.y.p + p.n * A.y.sn + c;
+    constexpr int B = 4;
+    for (int64_t l = p.l0 + at.r0; l < p.l1; l += (int64_t)at.rp * B) {
+      float v[B][VW];
 #pragma unroll
-      for (int k = 0; k < VW; k++) x[k] = act_value(fmaf((x[k] - m) * r, w[k], b[k]), A.act);
-      store_vec<T, VW>((T*)A.y.p + p.n * A.y.sn + l * A.y.sl + c, x);
+      for (int i = 0; i < B; i++) load_vec<T, VW>(x + min(l + (int64_t)at.rp * i, p.l1 - 1) * A.x.sl, v[i]);
+#pragma unroll
+      for (int i = 0; i < B; i++)
+        if (l + (int64_t)at.rp * i < p.l1) {
+#pragma unroll
+          for (int k = 0; k < VW; k++) v[i][k] = act_value<T>(fmaf(v[i][k] - m[k], w[k], b[k]), A.act);
+          store_vec<T, VW>(y + (l + (int64_t)at.rp * i) * A.y.sl, v[i]);
+        }
     }
   }
 }
 
-// backward: the two sums of a unit and the partial sums of the parameter gradients
+// backward: the sums of dz and dz xh per channel of a part, and of w dz and w dz xh per group
 template <typename T, int VW>
-__global__ __launch_bounds__(256) void k_gn_big_sums(GnArgs A) {
-  __shared__ float red[16][2];
-  extern __shared__ float cols[];
+__global__ __launch_bounds__(256) void k_gn_stream_sums(GnArgs A) {
+  __shared__ float lds[2][VW][256];
   const Part p = part_of(A);
-  const int cgv = A.cg / VW, t = threadIdx.x;
-  const float m = A.stats[2 * p.u], r = A.stats[2 * p.u + 1];
-  float v[2] = {0.f, 0.f};
-  const int step = min(cgv, 256), rp = 256 / step;
-  for (int c0 = 0; c0 < cgv; c0 += step) {
-    const int cv = c0 + t % step;
-    const bool on = t < rp * step && cv < cgv;
-    const int c = p.g * A.cg + (on ? cv : 0) * VW;
-    float w[VW], b[VW], dw[VW], db[VW];
+  const int C = A.G * A.cg, t = threadIdx.x;
+  float* out = A.sums + (p.n * A.split + p.s) * A.G * 3;
+  for (int c0 = 0; c0 < C / VW; c0 += 256) {
+    const Place at = place_of(C / VW, c0);
+    const int c = at.v * VW;
+    float m[VW], r[VW], w[VW], b[VW], dw[VW], db[VW];
 #pragma unroll
     for (int k = 0; k < VW; k++) {
+      const int64_t g = p.n * A.G + (c + k) / A.cg;
+      m[k] = A.stats[2 * g];
+      r[k] = A.stats[2 * g + 1];
       w[k] = param(A.w, A.wdt, c + k, 1.f);
       b[k] = param(A.b, A.wdt, c + k, 0.f);
       dw[k] = db[k] = 0.f;
     }
-    if (on)
-      for (int64_t l = p.l0 + t / step; l < p.l1; l += rp) {
-        float x[VW], dy[VW];
-        load_vec<T, VW>((const T*)A.x.p + p.n * A.x.sn + l * A.x.sl + c, x);
-        load_vec<T, VW>((const T*)A.dy.p + p.n * A.dy.sn + l * A.dy.sl + c, dy);
+    const T* x = (const T*)A.x.p + p.n * A.x.sn + c;
+    const T* dy = (const T*)A.dy.p + p.n * A.dy.sn + c;
+    if (at.on) {
+      constexpr int B = 2;
+      for (int64_t l = p.l0 + at.r0; l < p.l1; l += (int64_t)at.rp * B) {
+        float v[B][VW], d[B][VW];
 #pragma unroll
-        for (int k = 0; k < VW; k++) {
-          const float xh = (x[k] - m) * r, dz = dy[k] * act_slope(fmaf(xh, w[k], b[k]), A.act);
-          db[k] += dz;
-          dw[k] = fmaf(dz, xh, dw[k]);
+        for (int i = 0; i < B; i++) {
+          const int64_t row = min(l + (int64_t)at.rp * i, p.l1 - 1);
+          load_vec<T, VW>(x + row * A.x.sl, v[i]);
+          load_vec<T, VW>(dy + row * A.dy.sl, d[i]);
         }
+#pragma unroll
+        for (int i = 0; i < B; i++)
+          if (l + (int64_t)at.rp * i < p.l1)
+#pragma unroll
+            for (int k = 0; k < VW; k++) {
+              const float xh = (v[i][k] - m[k]) * r[k], dz = d[i][k] * act_slope<T>(fmaf(xh, w[k], b[k]), A.act);
+              db[k] += dz;
+              dw[k] = fmaf(dz, xh, dw[k]);
+            }
       }
-    // the unit's sums, from the columns' sums: sum dxh = sum w db, sum dxh xh = sum w dw
+    }
+    __syncthreads();
 #pragma unroll
     for (int k = 0; k < VW; k++) {
-      v[0] = fmaf(w[k], db[k], v[0]);
-      v[1] = fmaf(w[k], dw[k], v[1]);
+      lds[0][k][t] = db[k];
+      lds[1][k][t] = dw[k];
     }
-    const int64_t o = ((p.n * A.split + p.s) * A.G + p.g) * A.cg + cv * VW;
-    if (A.dw) {
-      column_sum<VW>(dw, t, rp, step, t < rp * step, cols);
-      if (t < step && cv < cgv)
+    __syncthreads();
+    for (int rows = at.rp; rows > 1; rows = (rows + 1) >> 1) {
+      const int other = t + ((rows + 1) >> 1) * at.cols;
+      if (at.on && t < (rows >> 1) * at.cols)
 #pragma unroll
-        for (int k = 0; k < VW; k++) A.dw[o + k] = dw[k];
+        for (int k = 0; k < VW; k++) {
+          lds[0][k][t] += lds[0][k][other];
+          lds[1][k][t] += lds[1][k][other];
+        }
+      __syncthreads();
     }
-    if (A.db) {
-      column_sum<VW>(db, t, rp, step, t < rp * step, cols);
-      if (t < step && cv < cgv)
+    if (t < at.cols)
 #pragma unroll
-        for (int k = 0; k < VW; k++) A.db[o + k] = db[k];
+      for (int k = 0; k < VW; k++) {
+        const int64_t o = (p.n * A.split + p.s) * C + c + k;
+        if (A.db) A.db[o] = lds[0][k][t];
+        if (A.dw) A.dw[o] = lds[1][k][t];
+        lds[0][k][t] *= w[k];
+        lds[1][k][t] *= w[k];
+      }
+    __syncthreads();
+    const int g0 = c0 * VW / A.cg, g1 = ((c0 + at.cols) * VW - 1) / A.cg;
+    for (int g = g0 + t; g <= g1; g += 256) {
+      const bool begun = g * A.cg < c0 * VW;
+      float s1 = begun ? out[3 * g] : 0.f, s2 = begun ? out[3 * g + 1] : 0.f;
+      const int first = max(g * A.cg, c0 * VW), last = min((g + 1) * A.cg, (c0 + at.cols) * VW);
+      for (int ch = first; ch < last; ch++) {
+        s1 += lds[0][ch % VW][ch / VW - c0];
+        s2 += lds[1][ch % VW][ch / VW - c0];
+      }
+      out[3 * g] = s1;
+      out[3 * g + 1] = s2;
     }
-  }
-  block_sum<2>(v, red);
-  if (t == 0) {
-    float* o = A.sums + (p.u * A.split + p.s) * 3;
-    o[0] = v[0];
-    o[1] = v[1];
+    __syncthreads();
   }
 }
 
 template <typename T, int VW>
-__global__ __launch_bounds__(256) void k_gn_big_dx(GnArgs A) {
+__global__ __launch_bounds__(256) void k_gn_stream_dx(GnArgs A, const float* means) {
   const Part p = part_of(A);
-  const float m = A.stats[2 * p.u], r = A.stats[2 * p.u + 1];
-  float s1 = 0.f, s2 = 0.f;
-  for (int s = 0; s < A.split; s++) {
-    const float* o = A.sums + (p.u * A.split + s) * 3;
-    s1 += o[0];
-    s2 += o[1];
-  }
-  const float inv = 1.f / ((float)A.L * (float)A.cg);
-  s1 *= inv;
-  s2 *= inv;
-  const int cgv = A.cg / VW, t = threadIdx.x;
-  const int step = min(cgv, 256), rp = 256 / step;
-  for (int c0 = 0; c0 < cgv; c0 += step) {
-    const int cv = c0 + t % step;
-    if (t >= rp * step || cv >= cgv) continue;
-    const int c = p.g * A.cg + cv * VW;
-    float w[VW], b[VW];
+  const int C = A.G * A.cg;
+  for (int c0 = 0; c0 < C / VW; c0 += 256) {
+    const Place at = place_of(C / VW, c0);
+    if (!at.on) continue;
+    const int c = at.v * VW;
+    float m[VW], r[VW], w[VW], b[VW], s1[VW], s2[VW];
 #pragma unroll
     for (int k = 0; k < VW; k++) {
+      const int64_t g = p.n * A.G + (c + k) / A.cg;
+      m[k] = A.stats[2 * g];
+      r[k] = A.stats[2 * g + 1];
+      s1[k] = means[2 * g];
+      s2[k] = means[2 * g + 1];
       w[k] = param(A.w, A.wdt, c + k, 1.f);
       b[k] = param(A.b, A.wdt, c + k, 0.f);
     }
-    for (int64_t l = p.l0 + t / step; l < p.l1; l += rp) {
-      float x[VW], dy[VW];
-      load_vec<T, VW>((const T*)A.x.p + p.n * A.x.sn + l * A.x.sl + c, x);
-      load_vec<T, VW>((const T*)A.dy.p + p.n * A.dy.sn + l * A.dy.sl + c, dy);
+    const T* x = (const T*)A.x.p + p.n * A.x.sn + c;
+    const T* dy = (const T*)A.dy.p + p.n * A.dy.sn + c;
+    T* dx = (T*)A.dx.p + p.n * A.dx.sn + c;
+    constexpr int B = 2;
+    for (int64_t l = p.l0 + at.r0; l < p.l1; l += (int64_t)at.rp * B) {
+      float v[B][VW], d[B][VW];
 #pragma unroll
-      for (int k = 0; k < VW; k++) {
-        const float xh = (x[k] - m) * r;
-        x[k] = r * (dy[k] * act_slope(fmaf(xh, w[k], b[k]), A.act) * w[k] - s1 - xh * s2);
+      for (int i = 0; i < B; i++) {
+        const int64_t row = min(l + (int64_t)at.rp * i, p.l1 - 1);
+        load_vec<T, VW>(x + row * A.x.sl, v[i]);
+        load_vec<T, VW>(dy + row * A.dy.sl, d[i]);
       }
-      store_vec<T, VW>((T*)A.dx.p + p.n * A.dx.sn + l * A.dx.sl + c, x);
+#pragma unroll
+      for (int i = 0; i < B; i++)
+        if (l + (int64_t)at.rp * i < p.l1) {
+#pragma unroll
+          for (int k = 0; k < VW; k++) {
+            const float xh = (v[i][k] - m[k]) * r[k];
+            const float dxh = d[i][k] * act_slope<T>(fmaf(xh, w[k], b[k]), A.act) * w[k];
+            v[i][k] = r[k] * (dxh - s1[k] - xh * s2[k]);
+          }
+          store_vec<T, VW>(dx + (l + (int64_t)at.rp * i) * A.dx.sl, v[i]);
+        }
     }
   }
 }
@@ -599,14 +851,15 @@ __global__ __launch_bounds__(1024) void k_gn_params(const float* dw, const float
 }
 
 // ------------------------------------------------------------------ host side
-enum { WAVE, BLOCK, BIG };
+enum { WAVE, BLOCK, BUNDLE, STREAM };
 struct Plan {
-  int kind, vw, per, lanes_log2, threads, split;
+  int kind, vw, per, lanes_log2, threads, split, bundle;
   int64_t grid, R;  // R: rows of partial sums
 };
 
-int vector_width(const fw_group_norm* a, bool backward) {
-  const int e = a->dtype == FW_DT_F32 ? 4 : 2, cg = a->C / a->G;
+// the widest vector that fits runs of `cg` channels and every tensor's alignment
+int vector_width(const fw_group_norm* a, bool backward, int64_t cg) {
+  const int e = a->dtype == FW_DT_F32 ? 4 : 2;
   int vw = 16 / e;
   auto fits = [&](const fw_rows& r) {
     return (uintptr_t)r.p % (vw * e) == 0 && (r.sn % vw == 0 || a->N < 2) && (r.sl % vw == 0 || a->L < 2);
@@ -623,7 +876,7 @@ bool needs_stats(const fw_group_norm* a) { return a->L * (a->C / a->G) > 1024; }
 Plan plan(const fw_group_norm* a, bool backward) {
   Plan p{};
   const int64_t cg = a->C / a->G, units = a->N * a->G;
-  p.vw = vector_width(a, backward);
+  p.vw = vector_width(a, backward, cg);
   const int64_t cgv = cg / p.vw, vecs = a->L * cgv;
   if (vecs <= 64 * 4) {
     p.kind = WAVE;
@@ -637,27 +890,47 @@ Plan plan(const fw_group_norm* a, bool backward) {
     p.R = slots_per_block % a->G == 0 ? p.grid : p.grid * slots_per_block / a->G;
     return p;
   }
-  const int hold = backward || p.vw == 8 ? 8 : 16;  // vectors a thread holds: 64 floats of 128 registers
-  if (cgv <= 1024 && (a->L + 1024 / cgv - 1) / (1024 / cgv) <= hold) {
+  // the fewest threads that hold `cols` columns of vectors, with at most `hold` each; 0 if none do
+  auto block_of = [&](int64_t cols, int vw, int hold) {
+    for (int threads : {256, 512, 768, 1024})
+      if (threads <= max_threads(backward, vw) && cols <= threads && (a->L + threads / cols - 1) / (threads / cols) <= hold) {
+        p.threads = threads;
+        const int64_t per = (a->L + threads / cols - 1) / (threads / cols);
+        p.per = 2 * per <= hold ? hold / 2 : hold;
+        return true;
+      }
+    return false;
+  };
+  // a block for the fewest neighbouring groups that fill 16-byte vectors, where one group does not
+  const int full = a->dtype == FW_DT_F32 ? 4 : 8;
+  if (p.vw < full)
+    for (int64_t q = 2; q <= 32 && q * cg <= 1024; q++)
+      if (a->G % q == 0 && q * cg % full == 0) {
+        if (vector_width(a, backward, q * cg) < full || !block_of(q * cg / full, full, backward && full == 8 ? 6 : 8)) break;
+        p.kind = BUNDLE;
+        p.bundle = (int)q;
+        p.grid = units / q;
+        p.R = a->N;
+        return p;
+      }
+  if (block_of(cgv, p.vw, max_hold(backward, p.vw))) {
     p.kind = BLOCK;
-    p.threads = 256;  // the fewest threads whose registers hold the unit with at most `hold` vectors each
-    while (p.threads < 1024 && (cgv > p.threads || (a->L + p.threads / cgv - 1) / (p.threads / cgv) > hold)) p.threads *= 2;
-    const int64_t per = (a->L + p.threads / cgv - 1) / (p.threads / cgv);
-    p.per = per <= 4 ? 4 : per <= 8 ? 8 : 16;
     p.grid = units;
     p.R = a->N;
     return p;
   }
-  p.kind = BIG;
-  const int64_t want = std::max<int64_t>(1, 2048 / units);  // blocks per unit
-  p.split = (int)std::max<int64_t>(1, std::min<int64_t>({want, (vecs + 1023) / 1024, a->L, 256}));
-  p.grid = units * p.split;
+  p.kind = STREAM;
+  p.vw = vector_width(a, backward, a->C);
+  // about 1024 blocks of at least 16 KB each
+  const int64_t bytes = a->L * a->C * (a->dtype == FW_DT_F32 ? 4 : 2);
+  p.split = (int)std::max<int64_t>(1, std::min<int64_t>({(1024 + a->N - 1) / a->N, bytes / 16384, a->L, 256}));
+  p.grid = a->N * p.split;
   p.R = a->N * p.split;
   return p;
 }
 size_t part_floats(const fw_group_norm* a, const Plan& p) { return (size_t)p.R * a->C; }
 size_t sum_floats(const fw_group_norm* a, const Plan& p) {
-  return p.kind == BIG ? (size_t)a->N * a->G * p.split * 3 : 0;
+  return p.kind == STREAM ? (size_t)a->N * a->G * (p.split * 3 + 2) : 0;
 }
 
 template <typename T, int VW, bool BWD>
@@ -673,20 +946,36 @@ int launch(const GnArgs& A, const Plan& p, hipStream_t s) {
       hipLaunchKernelGGL((k_gn_wave<T, VW, 4, BWD>), grid, dim3(256), lds, s, A);
   } else if (p.kind == BLOCK) {
     const size_t lds = BWD ? VW * 1024 * sizeof(float) : 0;
-    if (p.per == 4)
-      hipLaunchKernelGGL((k_gn_block<T, VW, 4, BWD>), grid, dim3(p.threads), lds, s, A);
-    else if (p.per == 8)
-      hipLaunchKernelGGL((k_gn_block<T, VW, 8, BWD>), grid, dim3(p.threads), lds, s, A);
-    else if constexpr (!BWD && VW < 8)
-      hipLaunchKernelGGL((k_gn_block<T, VW, 16, BWD>), grid, dim3(p.threads), lds, s, A);
-  } else if constexpr (!BWD) {
-    hipLaunchKernelGGL((k_gn_big_stats<T, VW>), grid, dim3(256), 0, s, A);
-    FW_HIP(hipGetLastError());
-    hipLaunchKernelGGL((k_gn_big_apply<T, VW>), grid, dim3(256), 0, s, A);
+    constexpr int HOLD = max_hold(BWD, VW);
+    if (p.per < HOLD)
+      hipLaunchKernelGGL((k_gn_block<T, VW, HOLD / 2, BWD>), grid, dim3(p.threads), lds, s, A);
+    else
+      hipLaunchKernelGGL((k_gn_block<T, VW, HOLD, BWD>), grid, dim3(p.threads), lds, s, A);
+  } else if (p.kind == BUNDLE) {
+    const size_t lds = 16 / sizeof(T) * 1024 * sizeof(float);
+    constexpr int HOLD = BWD && sizeof(T) == 2 ? 6 : 8;
+    if (p.per < HOLD)
+      hipLaunchKernelGGL((k_gn_bundle<T, HOLD / 2, BWD>), grid, dim3(p.threads), lds, s, A, p.bundle);
+    else
+      hipLaunchKernelGGL((k_gn_bundle<T, HOLD, BWD>), grid, dim3(p.threads), lds, s, A, p.bundle);
   } else {
-    hipLaunchKernelGGL((k_gn_big_sums<T, VW>), grid, dim3(256), VW * 1024 * sizeof(float), s, A);
-    FW_HIP(hipGetLastError());
-    hipLaunchKernelGGL((k_gn_big_dx<T, VW>), grid, dim3(256), 0, s, A);
+    const dim3 joins((unsigned)((A.N * A.G + 3) / 4));
+    float* pairs = A.sums + A.N * A.G * A.split * 3;  // [N][G][2]
+    if constexpr (!BWD) {
+      GnArgs B = A;
+      if (!B.stats) B.stats = pairs;
+      hipLaunchKernelGGL((k_gn_stream_stats<T, VW>), grid, dim3(256), 0, s, A);
+      FW_HIP(hipGetLastError());
+      hipLaunchKernelGGL((k_gn_stream_join<false>), joins, dim3(256), 0, s, A, B.stats);
+      FW_HIP(hipGetLastError());
+      hipLaunchKernelGGL((k_gn_stream_apply<T, VW>), grid, dim3(256), 0, s, B);
+    } else {
+      hipLaunchKernelGGL((k_gn_stream_sums<T, VW>), grid, dim3(256), 0, s, A);
+      FW_HIP(hipGetLastError());
+      hipLaunchKernelGGL((k_gn_stream_join<true>), joins, dim3(256), 0, s, A, pairs);
+      FW_HIP(hipGetLastError());
+      hipLaunchKernelGGL((k_gn_stream_dx<T, VW>), grid, dim3(256), 0, s, A, (const float*)pairs);
+    }
   }
   FW_HIP(hipGetLastError());
   return FW_OK;
@@ -768,7 +1057,7 @@ int fw_group_norm_backward(const fw_group_norm* a, void* stream) {
   if (a->N == 0 || a->L == 0) return fw::set_error(FW_E_INVALID, "fw_group_norm_backward: empty");
   if (!a->x.p || !a->dy.p || !a->dx.p) return fw::set_error(FW_E_INVALID, "fw_group_norm_backward: NULL x, dy or dx");
   const Plan p = plan(a, true);
-  if (p.kind == BIG && !a->stats) return fw::set_error(FW_E_INVALID, "fw_group_norm_backward: stats needed");
+  if (p.kind == STREAM && !a->stats) return fw::set_error(FW_E_INVALID, "fw_group_norm_backward: stats needed");
   const size_t need = fw_group_norm_workspace_bytes(a, 1);
   if (need && (!a->workspace || a->workspace_bytes < need))
     return fw::set_error(FW_E_INVALID, "fw_group_norm_backward: workspace too small");
