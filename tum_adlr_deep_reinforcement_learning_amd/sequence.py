@@ -26,8 +26,17 @@ def _ptr(t):
     return t.data_ptr() if t is not None else None
 
 
-def _stream(device):
-    return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+def _launch(name, args, device):
+    """lib.<name>(&args, current stream) with `device` current; a few microseconds matter here, so the common case (it
+    is already) takes no context manager."""
+    fn = getattr(_native.load(), name)
+    if torch.cuda.current_device() == device.index:
+        rc = fn(ctypes.byref(args), torch.cuda.current_stream(device).cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(ctypes.byref(args), torch.cuda.current_stream(device).cuda_stream)
+    if rc:
+        _native.check(rc, name)
 
 
 def _operand(s, t, step=False):
@@ -103,23 +112,21 @@ def _linattn_args(q, k, v, log_decay, starts, lengths):
     return a
 
 
-def _workspace(lib, a, device, backward):
-    n = lib.fw_linattn_workspace_bytes(a.T, a.N, a.H, a.Dk, a.Dv, a.dtype, backward)
+def _workspace(a, device, backward):
+    n = _native.load().fw_linattn_workspace_bytes(a.T, a.N, a.H, a.Dk, a.Dv, a.dtype, backward)
     ws = torch.empty(n, dtype=torch.uint8, device=device) if n else None
     a.workspace, a.workspace_bytes = _ptr(ws), n
     return ws  # referenced until the launches are queued; the allocator reuses it in stream order
 
 
 def _linattn_forward(q, k, v, log_decay, state, starts, lengths):
-    lib = _native.load()
     a = _linattn_args(q, k, v, log_decay, starts, lengths)
     out = torch.empty(v.shape, dtype=v.dtype, device=v.device)
     final = torch.empty((a.N, a.H, a.Dk, a.Dv), dtype=torch.float32, device=v.device)
     _operand(a.out, out)
     a.state_in, a.state_out = _ptr(state), final.data_ptr()
-    with torch.cuda.device(q.device):
-        ws = _workspace(lib, a, q.device, 0)  # noqa: F841
-        _native.check(lib.fw_linattn_forward(ctypes.byref(a), _stream(q.device)), "fw_linattn_forward")
+    ws = _workspace(a, q.device, 0)  # noqa: F841
+    _launch("fw_linattn_forward", a, q.device)
     return out, final
 
 
@@ -135,7 +142,6 @@ class _LinearAttention(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dout, dfinal):
         q, k, v, log_decay, state, starts, lengths = ctx.saved_tensors
-        lib = _native.load()
         a = _linattn_args(q, k, v, log_decay, starts, lengths)
         dout = _dense(dout) if dout is not None else torch.zeros(v.shape, dtype=v.dtype, device=v.device)
         dfinal = dfinal.contiguous() if dfinal is not None else None
@@ -144,9 +150,8 @@ class _LinearAttention(torch.autograd.Function):
             _operand(s, t)
         dstate = torch.empty_like(state) if state is not None and ctx.needs_input_grad[4] else None
         a.state_in, a.dstate, a.dstate_in = _ptr(state), _ptr(dfinal), _ptr(dstate)
-        with torch.cuda.device(q.device):
-            ws = _workspace(lib, a, q.device, 1)  # noqa: F841
-            _native.check(lib.fw_linattn_backward(ctypes.byref(a), _stream(q.device)), "fw_linattn_backward")
+        ws = _workspace(a, q.device, 1)  # noqa: F841
+        _launch("fw_linattn_backward", a, q.device)
         return dq, dk, dv, None, dstate, None, None
 
 
@@ -221,8 +226,7 @@ def linear_attention_step(q, k, v, log_decay, state, episode_starts=None, state_
     if starts is not None:
         a.starts, a.starts_sn = starts.data_ptr(), starts.stride(0)
     a.state, a.state_out = state.data_ptr(), new.data_ptr()
-    with torch.cuda.device(dev):
-        _native.check(_native.load().fw_linattn_step(ctypes.byref(a), _stream(dev)), "fw_linattn_step")
+    _launch("fw_linattn_step", a, dev)
     return out
 
 
@@ -245,25 +249,23 @@ def _norm_args(x, groups, weight, bias, eps, act):
     return a
 
 
-def _norm_workspace(lib, a, device, backward):
-    n = lib.fw_group_norm_workspace_bytes(ctypes.byref(a), backward)
+def _norm_workspace(a, device, backward):
+    n = _native.load().fw_group_norm_workspace_bytes(ctypes.byref(a), backward)
     ws = torch.empty(n, dtype=torch.uint8, device=device) if n else None
     a.workspace, a.workspace_bytes = _ptr(ws), n
     return ws
 
 
 def _norm_forward(x, groups, weight, bias, eps, act, keep):
-    lib = _native.load()
     a = _norm_args(x, groups, weight, bias, eps, act)
     y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     _rows(a.y, y)
     stats = None
-    if keep and lib.fw_group_norm_stats(ctypes.byref(a)):
+    if keep and _native.load().fw_group_norm_stats(ctypes.byref(a)):
         stats = torch.empty((a.N, groups, 2), dtype=torch.float32, device=x.device)
         a.stats = stats.data_ptr()
-    with torch.cuda.device(x.device):
-        ws = _norm_workspace(lib, a, x.device, 0)  # noqa: F841
-        _native.check(lib.fw_group_norm_forward(ctypes.byref(a), _stream(x.device)), "fw_group_norm_forward")
+    ws = _norm_workspace(a, x.device, 0)  # noqa: F841
+    _launch("fw_group_norm_forward", a, x.device)
     return y, stats
 
 
@@ -280,7 +282,6 @@ class _GroupNormAct(torch.autograd.Function):
     def backward(ctx, dy):
         x, weight, bias, stats = ctx.saved_tensors
         groups, eps, act = ctx.conf
-        lib = _native.load()
         dy = _dense(dy)
         dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
         dw = torch.empty_like(weight) if weight is not None and ctx.needs_input_grad[1] else None
@@ -291,9 +292,8 @@ class _GroupNormAct(torch.autograd.Function):
         _rows(a.dy, dy)
         _rows(a.dx, dx)
         a.dweight, a.dbias, a.stats = _ptr(dw), _ptr(db), _ptr(stats)
-        with torch.cuda.device(x.device):
-            ws = _norm_workspace(lib, a, x.device, 1)  # noqa: F841
-            _native.check(lib.fw_group_norm_backward(ctypes.byref(a), _stream(x.device)), "fw_group_norm_backward")
+        ws = _norm_workspace(a, x.device, 1)  # noqa: F841
+        _launch("fw_group_norm_backward", a, x.device)
         return dx, dw, db, None, None, None
 
 
