@@ -25,7 +25,7 @@ import numpy as np
 import torch
 from torch import nn
 
-from . import _native
+from . import _native, sequence
 from .sharding import all_gather_flat
 
 RolloutBufferSamples = collections.namedtuple(
@@ -268,6 +268,88 @@ class MlpActorCritic(nn.Module):
         return self.value_net(self.vf(obs))
 
 
+class RetentionActorCritic(nn.Module):
+    """Actor-critic with a memory (no counterpart in the reference, whose policies see one observation): per head a
+    key-value state that decays with its own time constant and is cleared at episode starts.
+
+        x = tanh(embed(obs));  q, k, v = split(qkv(x));  m = memory(q, k, v);  f = x + mix(group_norm_act(m))
+        mean = action_net(f), value = value_net(f), state-independent log-std
+
+    In the collect loop (``RolloutCollector``, which holds the environments' memory) it is stepped for one token per
+    environment (``forward``, with ``sequence.linear_attention_step``); an update runs it over whole columns of the
+    rollout, all of them or some (``evaluate_actions``, with ``sequence.linear_attention``), from the memory the
+    collection began with (``RolloutCollector.rollout_memory``) and with the buffer's episode starts
+    (``RolloutBuffer.dones``)."""
+
+    recurrent = True
+    deterministic_rollout = False  # forward() without exploration noise (actions = mean)
+
+    def __init__(self, obs_dim, act_dim, width=64, heads=4, time_constants=(4.0, 1000.0), log_std_init=0.0):
+        super().__init__()
+        if width % heads:
+            raise ValueError("RetentionActorCritic: width %d does not divide into %d heads" % (width, heads))
+        self.heads, self.head_dim = heads, width // heads
+        self.embed, self.qkv, self.mix = nn.Linear(obs_dim, width), nn.Linear(width, 3 * width), nn.Linear(width, width)
+        self.norm_weight, self.norm_bias = nn.Parameter(torch.ones(width)), nn.Parameter(torch.zeros(width))
+        self.action_net, self.value_net = nn.Linear(width, act_dim), nn.Linear(width, 1)
+        self.log_std = nn.Parameter(torch.full((act_dim,), float(log_std_init)))
+        for layer, g in ((self.embed, np.sqrt(2)), (self.qkv, 1.0), (self.mix, 1.0), (self.action_net, 0.01),
+                         (self.value_net, 1.0)):
+            nn.init.orthogonal_(layer.weight, gain=g)
+            nn.init.zeros_(layer.bias)
+        lo, hi = time_constants  # steps, geometric over the heads
+        tau = lo * (hi / lo) ** (torch.arange(heads) / max(1, heads - 1))
+        self.register_buffer("log_decay", (-1.0 / tau).float())
+
+    def new_memory(self, n_envs):
+        """An empty memory, [n_envs][heads][D][D] float32."""
+        return torch.zeros(n_envs, self.heads, self.head_dim, self.head_dim, dtype=torch.float32,
+                           device=self.log_decay.device)
+
+    def _project(self, obs):
+        x = torch.tanh(self.embed(obs))
+        q, k, v = self.qkv(x).unflatten(-1, (3, self.heads, self.head_dim)).unbind(-3)
+        return x, q * self.head_dim ** -0.5, k, v
+
+    def _features(self, x, m):
+        rows = m.reshape(-1, self.heads * self.head_dim)
+        y = sequence.group_norm_act(rows, self.heads, self.norm_weight, self.norm_bias, activation="silu")
+        return x + self.mix(y.view(x.shape))
+
+    def _step(self, obs, memory, episode_starts, memory_out=None):
+        x, q, k, v = self._project(obs)
+        return self._features(x, sequence.linear_attention_step(q, k, v, self.log_decay, memory, episode_starts,
+                                                                memory_out))
+
+    @torch.no_grad()
+    def forward(self, obs, memory, episode_starts=None, deterministic=False):
+        """One collect step: (actions, values, log_prob) like MlpActorCritic.forward; ``memory`` is advanced in place."""
+        f = self._step(obs, memory, episode_starts)
+        mean = self.action_net(f)
+        if deterministic or self.deterministic_rollout:
+            actions = mean
+        else:
+            actions = mean + self.log_std.exp() * torch.randn_like(mean)
+        return actions, self.value_net(f), self._log_prob(actions, mean)
+
+    @torch.no_grad()
+    def predict_values(self, obs, memory, episode_starts=None):
+        """Values of the observations that follow; ``memory`` stays as it is."""
+        return self.value_net(self._step(obs, memory, episode_starts, torch.empty_like(memory)))
+
+    def evaluate_actions(self, obs, actions, episode_starts, memory=None):
+        """Columns of a rollout, [T][N] rows: (values [T][N], log_prob [T][N], entropy []), with gradients."""
+        x, q, k, v = self._project(obs)
+        m, _ = sequence.linear_attention(q, k, v, self.log_decay, memory, episode_starts)
+        f = self._features(x, m)
+        entropy = (0.5 + 0.5 * np.log(2 * np.pi) + self.log_std).sum()
+        return self.value_net(f).squeeze(-1), self._log_prob(actions, self.action_net(f)), entropy
+
+    def _log_prob(self, actions, mean):
+        std = self.log_std.exp()
+        return (-((actions - mean) ** 2) / (2 * std * std) - self.log_std - 0.5 * np.log(2 * np.pi)).sum(-1)
+
+
 class RolloutCollector:
     capture_collective = True  # a sharded fused step captures its RCCL exchange inside the one graph
     steps_per_graph = 16       # the fused step is also captured K times in one graph (one replay per K steps)
@@ -281,7 +363,10 @@ class RolloutCollector:
     ``env`` is a FixedWingVecEnv (or a VecNormalize-style wrapper around one) built with
     ``return_tensors=True``.  Per step: copy the last observation into the buffer slot, run the
     policy on it, clip the actions to the action space, step the env, store reward / episode start /
-    value / log-prob.  No host synchronisation inside the loop."""
+    value / log-prob.  No host synchronisation inside the loop.
+
+    A ``recurrent`` policy (``RetentionActorCritic``) is also given the environments' ``memory``, which it advances, and
+    the episode starts, eager and captured; ``rollout_memory`` is a copy of the memory before the first stored row."""
 
     def __init__(self, env, policy, buffer):
         self.env, self.policy, self.buffer = env, policy, buffer
@@ -291,6 +376,19 @@ class RolloutCollector:
         self.high = torch.as_tensor(space.high, device=dev)
         self.last_obs = None
         self.last_dones = torch.zeros(env.num_envs, dtype=torch.uint8, device=dev)
+        self.memory = self.rollout_memory = None
+
+    def _recurrent(self):
+        return getattr(self.policy, "recurrent", False)
+
+    def _act(self, obs, starts):
+        return self.policy(obs, self.memory, starts) if self._recurrent() else self.policy(obs)
+
+    def _bootstrap(self):
+        """Values of the observations behind the last stored row."""
+        if self._recurrent():
+            return self.policy.predict_values(self.last_obs, self.memory, self.last_dones)
+        return self.policy.predict_values(self.last_obs)
 
     @torch.no_grad()
     def collect(self, n_rollout_steps=None, graph=False):
@@ -306,6 +404,10 @@ class RolloutCollector:
         n = n_rollout_steps or buf.buffer_size
         if self.last_obs is None:
             self.last_obs = env.reset()
+        if self._recurrent():
+            if self.memory is None:
+                self.memory = self.policy.new_memory(buf.n_envs)
+            self.rollout_memory = self.memory.clone()
         if graph and self._graph_ok():
             return self._collect_graphed(n)
         buf.reset()
@@ -318,7 +420,7 @@ class RolloutCollector:
                 actions, clipped, values, log_probs = self.policy.collect_step(
                     obs_slot, self.low, self.high, noise=noise[t] if noise is not None else None)
             else:
-                actions, values, log_probs = self.policy(obs_slot)
+                actions, values, log_probs = self._act(obs_slot, self.last_dones)
                 clipped = torch.max(torch.min(actions, self.high), self.low)
             new_obs, rewards, dones, _ = env.step(clipped)
             buf.actions[t].copy_(actions)
@@ -329,7 +431,7 @@ class RolloutCollector:
             self.last_obs = new_obs
             self.last_dones = dones.to(torch.uint8).clone()
         buf.pos, buf.full = n, n == buf.buffer_size
-        last_values = self.policy.predict_values(self.last_obs)
+        last_values = self._bootstrap()
         buf.compute_returns_and_advantage(last_values, self.last_dones)
         self._eager_done = True
         return buf
@@ -379,7 +481,8 @@ class RolloutCollector:
         env_key = self.env.graph_key() if hasattr(self.env, "graph_key") else None
         pol = self.policy
         pol_key = (id(pol), bool(getattr(pol, "deterministic_rollout", False)),
-                   tuple(p.data_ptr() for p in pol.parameters()) if isinstance(pol, nn.Module) else None)
+                   tuple(p.data_ptr() for p in pol.parameters()) if isinstance(pol, nn.Module) else None,
+                   self.memory.data_ptr() if self._recurrent() else None)
         return (env_key, self._split(), self.buffer.slab.data_ptr(), self.buffer.buffer_size, pol_key,
                 self.capture_collective, self.steps_per_graph, self.defer_final_merge)
 
@@ -402,6 +505,7 @@ class RolloutCollector:
         self.s_clip = torch.empty(N, A, dtype=torch.float32, device=dev)
         self.s_val = torch.empty(N, dtype=torch.float32, device=dev)
         self.s_logp = torch.empty(N, dtype=torch.float32, device=dev)
+        self.s_first = torch.zeros(N, dtype=torch.uint8, device=dev)  # the episode starts a recurrent policy acts on
         self._ctrl = torch.zeros(2, dtype=torch.int32, device=dev)  # {row, n_rows} of fw_rollout_store
         lib = _native.load()
         split = self._split()
@@ -415,7 +519,7 @@ class RolloutCollector:
                                          noise=noise, noise_row=self._ctrl if noise is not None else None)
                 clipped = self.s_clip
             else:
-                actions, values, log_probs = self.policy(self.s_obs)
+                actions, values, log_probs = self._act(self.s_obs, self.s_first)
                 clipped = torch.max(torch.min(actions, self.high), self.low)
                 self.s_act.copy_(actions)
                 self.s_val.copy_(values.reshape(-1))
@@ -436,6 +540,8 @@ class RolloutCollector:
                 self.s_start.copy_(d8)
                 d8 = self.s_start
             self._dsrc = d8  # the episode starts of the next row (and, after the last step, last_dones)
+            if self._recurrent():
+                self.s_first.copy_(d8)
             # the step's rows straight from where they were produced (the captured env outputs keep their
             # addresses on every replay); the episode starts of row t + 1 from the static s_start
             rew = rewards.reshape(N)
@@ -480,6 +586,7 @@ class RolloutCollector:
         self.s_obs.copy_(self.last_obs.reshape(N, D))
         buf.observations[0].copy_(self.s_obs)  # the inputs of step 0; step t stores those of t + 1
         buf.dones[0].copy_(self.last_dones)
+        self.s_first.copy_(self.last_dones)
         self._ctrl[0] = 0
         self._ctrl[1] = n
         if len(self._graphs) == 1:
@@ -495,7 +602,7 @@ class RolloutCollector:
         self.last_obs = self.s_obs.clone().reshape(self.last_obs.shape)
         self.last_dones = self._dsrc.clone()
         buf.pos, buf.full = n, n == buf.buffer_size
-        last_values = self.policy.predict_values(self.last_obs)
+        last_values = self._bootstrap()
         buf.compute_returns_and_advantage(last_values, self.last_dones)
         return buf
 
