@@ -56,7 +56,7 @@ def _close(name, got, ref, bulk, steps):
         tol = tol + 2.0 ** -15 * bulk
     tol = tol + torch.finfo(dt).eps / 2 * (ref.abs() + tol) + torch.finfo(dt).tiny
     err = (got.detach().cpu().double() - ref).abs()
-    bad = err > tol
+    bad = ~(err <= tol)
     assert not bool(bad.any()), "%s: %d of %d off, worst %.3g times its tolerance" % (
         name, int(bad.sum()), bad.numel(), float((err / tol).max()))
 

@@ -935,6 +935,8 @@ size_t sum_floats(const fw_group_norm* a, const Plan& p) {
 
 template <typename T, int VW, bool BWD>
 int launch(const GnArgs& A, const Plan& p, hipStream_t s) {
+  if (p.grid > UINT32_MAX / (p.kind == BLOCK || p.kind == BUNDLE ? p.threads : 256))  // threads of a launch
+    return fw::set_error(FW_E_INVALID, "group norm: too many groups for one call");
   const dim3 grid((unsigned)p.grid);
   if (p.kind == WAVE) {
     const size_t lds = BWD ? (size_t)4 * (64 >> p.lanes_log2) * A.L * A.cg * sizeof(float) : 0;  // at most 32 KB
@@ -1003,7 +1005,7 @@ int check(const fw_group_norm* a, const char* who) {
   if (a->wdtype != FW_DT_F32 && a->wdtype != a->dtype) return bad("wdtype must be float32 or dtype");
   if (a->act < FW_ACT_NONE || a->act > FW_ACT_TANH) return bad("unknown activation");
   if (!(a->eps >= 0.0)) return bad("eps must be >= 0");
-  if (a->N > 0 && a->N * (int64_t)a->G > INT32_MAX) return bad("too many groups for one call");
+  if (a->N > INT32_MAX / a->G) return bad("too many groups for one call");
   return FW_OK;
 }
 GnArgs base(const fw_group_norm* a, const Plan& p) {

@@ -533,6 +533,12 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, KT * VT <= 16 ? 2 : 1) void k_scan
       for (int a = 0; a < KT; a++)
 #pragma unroll
         for (int f = 0; f < VT; f++) S[a][f] = f32x4{0.f, 0.f, 0.f, 0.f};
+      // a block of one token that a reversed pass cuts off behind itself: its value, perhaps an infinity, adds nothing
+      if (rev && c == 1)
+#pragma unroll
+        for (int j = 0; j < TPL; j++)
+#pragma unroll
+          for (int f = 0; f < VT; f++) Vr[j][f] = 0.f;
     }
 #pragma unroll
     for (int a = 0; a < KT; a++)
@@ -855,6 +861,10 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, 2) void k_scan16(ScanArgs A) {
       for (int a = 0; a < KT; a++)
 #pragma unroll
         for (int f = 0; f < VT; f++) S[a][f] = f32x4{0.f, 0.f, 0.f, 0.f};
+      // a block of one token that a reversed pass cuts off behind itself: its value, perhaps an infinity, adds nothing
+      if (rev && c == 1)
+#pragma unroll
+        for (int f = 0; f < VT; f++) vf[f] = u32x4{0, 0, 0, 0};
     }
 #pragma unroll
     for (int a = 0; a < KT; a++)
@@ -1105,8 +1115,8 @@ int tiles(int d) { return d <= 16 ? 1 : d <= 32 ? 2 : d <= 64 ? 4 : 8; }
 // value tiles of one wave: the state is KT x VT tiles of registers
 int slice_tiles(int dtype, int Dk, int Dv) { return std::min(tiles(Dv), dtype == FW_DT_BF16 && tiles(Dk) == 8 ? 2 : 4); }
 int slices(int dtype, int Dk, int Dv) {
-  const int vt = slice_tiles(dtype, Dk, Dv);
-  return (tiles(Dv) + vt - 1) / vt;
+  const int cols = 16 * slice_tiles(dtype, Dk, Dv);
+  return (Dv + cols - 1) / cols;
 }
 
 // Time segments: with fewer than SEG_WAVES waves the card is not full, so the time axis is cut, at the price of
@@ -1143,7 +1153,7 @@ template <typename T, int KT, int VT>
 int launch_mode(const ScanArgs& A, int mode, hipStream_t s) {
   const int64_t units = A.n_pass * (int64_t)A.n_slice * A.H * A.N;
   const int64_t blocks = (units + SCAN_WAVES - 1) / SCAN_WAVES;
-  if (blocks > INT32_MAX / SCAN_WAVES)
+  if (blocks > UINT32_MAX / (64 * SCAN_WAVES))  // threads of a launch
     return fw::set_error(FW_E_INVALID, "linear attention: too many sequences for one call");
   const dim3 grid((unsigned)blocks, A.run_seg), block(64 * SCAN_WAVES);
   auto kernel = [&](auto m) {
@@ -1185,16 +1195,15 @@ int launch_scan(ScanArgs A, int kt, int vt, hipStream_t s) {
   return fw::set_error(FW_E_INVALID, "linear attention: head sizes 1..128");
 }
 
-// Passes of equal tile counts go in one launch.
+// Passes of equal tiles and slices go in one launch.
 int launch_passes(int dtype, ScanArgs A, const Pass* pass, int n_pass, hipStream_t s) {
   for (int i = 0; i < n_pass; i += A.n_pass) {
     const int kt = tiles(pass[i].Dk), vt = slice_tiles(dtype, pass[i].Dk, pass[i].Dv);
     A.n_slice = slices(dtype, pass[i].Dk, pass[i].Dv);
     A.n_pass = 0;
-    while (i + A.n_pass < n_pass && tiles(pass[i + A.n_pass].Dk) == kt && tiles(pass[i + A.n_pass].Dv) == tiles(pass[i].Dv)) {
-      A.pass[A.n_pass] = pass[i + A.n_pass];
-      A.n_pass++;
-    }
+    for (int j = i; j < n_pass && tiles(pass[j].Dk) == kt && slice_tiles(dtype, pass[j].Dk, pass[j].Dv) == vt &&
+                    slices(dtype, pass[j].Dk, pass[j].Dv) == A.n_slice; j++)
+      A.pass[A.n_pass++] = pass[j];
     const int rc = dtype == FW_DT_F32    ? launch_scan<float>(A, kt, vt, s)
                    : dtype == FW_DT_BF16 ? launch_scan<bf16>(A, kt, vt, s)
                                          : launch_scan<f16>(A, kt, vt, s);
@@ -1235,12 +1244,17 @@ int check(const fw_linattn* a, const char* who) {
   if (a->dtype < FW_DT_F32 || a->dtype > FW_DT_F16) return bad("dtype must be float32, bfloat16 or float16");
   if (a->T > 0 && a->N > 0 && (!a->q.p || !a->k.p || !a->v.p)) return bad("NULL q, k or v");
   if (!a->log_decay) return bad("NULL log_decay");
+  if (a->N > INT32_MAX / a->H) return bad("too many sequences for one call");
   if (a->starts && (a->starts_st < 0 || a->starts_st >= (int64_t)1 << 26)) return bad("starts_st must be 0..2^26 - 1");
   return FW_OK;
 }
 bool room(const fw_linattn* a, bool backward) {
   const size_t need = fw_linattn_workspace_bytes(a->T, a->N, a->H, a->Dk, a->Dv, a->dtype, backward);
-  return need == 0 || (a->workspace && a->workspace_bytes >= need);
+  return need == 0 || (a->workspace && a->workspace_bytes >= need && (uintptr_t)a->workspace % 16 == 0);
+}
+// the strides of single tokens, sequences and heads mean nothing and are not to cost an operand its alignment
+Operand in(const fw_linattn* a, const fw_seq_tensor& t) {
+  return {t.p, a->T > 1 ? t.st : 0, a->N > 1 ? t.sn : 0, a->H > 1 ? t.sh : 0};
 }
 Operand in(const fw_seq_tensor& t) { return {t.p, t.st, t.sn, t.sh}; }
 ScanArgs base(const fw_linattn* a, const Plan& pl) {
@@ -1285,11 +1299,11 @@ int fw_linattn_forward(const fw_linattn* a, void* stream) {
   if (a->N == 0) return FW_OK;
   if (a->T > 0 && !a->out.p) return fw::set_error(FW_E_INVALID, "fw_linattn_forward: NULL out");
   const Plan pl = plan(a->dtype, a->T, a->N, a->H, a->Dk, a->Dv);
-  if (!room(a, false)) return fw::set_error(FW_E_INVALID, "fw_linattn_forward: workspace too small");
+  if (!room(a, false)) return fw::set_error(FW_E_INVALID, "fw_linattn_forward: workspace too small or not 16-byte aligned");
   hipStream_t s = (hipStream_t)stream;
   float* ws = (float*)a->workspace;
   const ScanArgs A = base(a, pl);
-  Pass p{in(a->q), in(a->k), in(a->v), in(a->out), straight(a, a->state_in), straight(a, a->state_out), 0, a->Dk, a->Dv};
+  Pass p{in(a, a->q), in(a, a->k), in(a, a->v), in(a, a->out), straight(a, a->state_in), straight(a, a->state_out), 0, a->Dk, a->Dv};
   if (pl.n_seg > 1) {
     const State seg = segments(a, ws, 0, pl.n_seg);
     const Pass add{p.q, p.k, p.v, Operand{}, State{}, seg, 0, a->Dk, a->Dv};
@@ -1305,7 +1319,7 @@ int fw_linattn_backward(const fw_linattn* a, void* stream) {
   if (a->T > 0 && (!a->dout.p || !a->dq.p || !a->dk.p || !a->dv.p))
     return fw::set_error(FW_E_INVALID, "fw_linattn_backward: NULL dout, dq, dk or dv");
   const Plan pl = plan(a->dtype, a->T, a->N, a->H, a->Dk, a->Dv);
-  if (!room(a, true)) return fw::set_error(FW_E_INVALID, "fw_linattn_backward: workspace too small");
+  if (!room(a, true)) return fw::set_error(FW_E_INVALID, "fw_linattn_backward: workspace too small or not 16-byte aligned");
   hipStream_t s = (hipStream_t)stream;
   float* ws = (float*)a->workspace;
   const ScanArgs A = base(a, pl);
@@ -1314,14 +1328,14 @@ int fw_linattn_backward(const fw_linattn* a, void* stream) {
     const State in_[2] = {S, R};
     S = segments(a, ws, 0, pl.n_seg);
     R = segments(a, ws, 1, pl.n_seg);
-    const Pass add[2] = {{in(a->q), in(a->k), in(a->v), Operand{}, State{}, S, 0, a->Dk, a->Dv},
-                         {in(a->k), in(a->q), in(a->dout), Operand{}, State{}, R, 1, a->Dk, a->Dv}};
+    const Pass add[2] = {{in(a, a->q), in(a, a->k), in(a, a->v), Operand{}, State{}, S, 0, a->Dk, a->Dv},
+                         {in(a, a->k), in(a, a->q), in(a, a->dout), Operand{}, State{}, R, 1, a->Dk, a->Dv}};
     if (int rc = segment_states(a->dtype, A, add, in_, 2, ws, s)) return rc;
   }
   const Pass main[3] = {
-      {in(a->dout), in(a->v), in(a->k), in(a->dq), turned(S), State{}, 0, a->Dv, a->Dk},
-      {in(a->v), in(a->dout), in(a->q), in(a->dk), turned(R), State{}, 1, a->Dv, a->Dk},
-      {in(a->k), in(a->q), in(a->dout), in(a->dv), R, straight(a, a->dstate_in), 1, a->Dk, a->Dv}};
+      {in(a, a->dout), in(a, a->v), in(a, a->k), in(a, a->dq), turned(S), State{}, 0, a->Dv, a->Dk},
+      {in(a, a->v), in(a, a->dout), in(a, a->q), in(a, a->dk), turned(R), State{}, 1, a->Dv, a->Dk},
+      {in(a, a->k), in(a, a->q), in(a, a->dout), in(a, a->dv), R, straight(a, a->dstate_in), 1, a->Dk, a->Dv}};
   return launch_passes(a->dtype, A, main, 3, s);
 }
 
@@ -1339,7 +1353,7 @@ int fw_linattn_step(const fw_linattn_token* a, void* stream_) {
   int lv = 0;
   while ((4 << lv) < a->Dv) lv++;
   const int64_t units = a->N * a->H;
-  if (units > INT32_MAX) return bad("too many sequences for one call");
+  if (a->N > INT32_MAX / a->H) return bad("too many sequences for one call");
   auto fours = [&](const fw_seq_tensor& t) {
     return (uintptr_t)t.p % (a->dtype == FW_DT_F32 ? 16 : 8) == 0 && t.sn % 4 == 0 && t.sh % 4 == 0;
   };
@@ -1350,7 +1364,9 @@ int fw_linattn_step(const fw_linattn_token* a, void* stream_) {
   const bool split = accesses >= 8 && units <= 2048;
   const bool stream = vec && !split && units * a->Dk * a->Dv * 4 >= (int64_t)192 << 20;
   const int B = accesses == 1 ? 4 : accesses == 2 ? 2 : 1;
-  const dim3 grid((unsigned)(split ? units : (units + 4 * B - 1) / (4 * B))), block(256);
+  const int64_t blocks = split ? units : (units + 4 * B - 1) / (4 * B);
+  if (blocks > UINT32_MAX / 256) return bad("too many sequences for one call");  // threads of a launch
+  const dim3 grid((unsigned)blocks), block(256);
   hipStream_t s = (hipStream_t)stream_;
 #define FW_TOKEN_K(T, B_, SP)                                                          \
   if (!vec)                                                                            \
