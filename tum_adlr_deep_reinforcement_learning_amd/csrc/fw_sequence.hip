@@ -978,14 +978,20 @@ struct TokenArgs {
   int32_t H, Dk, Dv;
 };
 
-// Bound by the state, read once and written once.  A wave takes B pairs (n, h); 2^lv lanes cover a state row in vectors of
-// 4, 64 >> lv rows an access, and four accesses are in flight before the first is used (65536 x 4 x 16 x 16: one access
-// is a whole state, so B = 4).  The state of a row that starts afresh is read all the same: waiting for its flag first
-// would cost every row a memory round trip.
+// Bound by the state, read once and written once.  A wave takes B pairs (n, h); nv lanes cover a state row in vectors of
+// 4, 64 / nv rows an access, and four accesses are in flight before the first is used (65536 x 4 x 16 x 16: one access
+// is a whole state, so B = 4).  Where 4 does not divide a row its last vector begins earlier and shares columns with the
+// one before: both lanes compute and store the same values there.  Rows then begin at any multiple of 4 bytes, which
+// the load unit takes (2165 x 12 of 116 x 41: 4670 GB/s; by elements 2770).
+// The state of a row that starts afresh is read all the same: waiting for its flag first would cost every row a memory
+// round trip.
+// VEC: v and out are read and written in vectors too.
 // SPLIT: a block's four waves share one pair's rows, where there are too few pairs to fill the card.
-// STREAM: the states are larger than the last-level cache, so they pass it by.
+// STREAM: the states are larger than the last-level cache and pass it by.  Rows of whole vectors only: without the cache
+// the parts of a memory line that two accesses write do not meet (116 x 41: 4050 GB/s with it).
+typedef f32x4 __attribute__((aligned(4))) f32x4_any;  // at any element
 template <typename T, bool VEC, int B, bool SPLIT, bool STREAM>
-__global__ __launch_bounds__(256) void k_token(TokenArgs A, int lv) {
+__global__ __launch_bounds__(256) void k_token(TokenArgs A, int nv, int rows, int magic) {
   static_assert(!SPLIT || B == 1);
   constexpr int R = 4 / B;
   __shared__ float part[SPLIT ? 4 : 1][SPLIT ? MAXDIM : 1];
@@ -994,8 +1000,9 @@ __global__ __launch_bounds__(256) void k_token(TokenArgs A, int lv) {
   const uint32_t units = (uint32_t)(A.N * A.H);
   const uint32_t u0 = SPLIT ? blockIdx.x : (blockIdx.x * 4 + wave) * B;
   if (u0 >= units) return;
-  const int rows = 64 >> lv, c = (lane & ((1 << lv) - 1)) * 4, rr = lane >> lv;
-  const bool on = c < A.Dv;
+  const int rr = lane * magic >> 16;  // lane / nv
+  const int c = VEC ? (lane - rr * nv) * 4 : min((lane - rr * nv) * 4, A.Dv - 4);
+  const bool on = rr < rows;
   const int E = A.Dk * A.Dv;
   const T *q[B], *k[B], *v[B];
   T* o[B];
@@ -1026,22 +1033,15 @@ __global__ __launch_bounds__(256) void k_token(TokenArgs A, int lv) {
 #pragma unroll
     for (int x = 0; x < 4; x++) acc[b][x] = 0.f;
   for (int d0 = first; d0 < A.Dk; d0 += step) {
-    float s[B][R][4], kd[B][R], qd[B][R];
+    f32x4 s[B][R];
+    float kd[B][R], qd[B][R];
 #pragma unroll
     for (int b = 0; b < B; b++)
 #pragma unroll
       for (int i = 0; i < R; i++) {
         const int d = min(d0 + i * rows, A.Dk - 1);
-        const float* p = in0 + min(b, live - 1) * E + d * A.Dv;
-        if constexpr (VEC) {
-          const f32x4* from = (const f32x4*)(p + (on ? c : 0));
-          const f32x4 y = STREAM ? __builtin_nontemporal_load(from) : *from;
-#pragma unroll
-          for (int x = 0; x < 4; x++) s[b][i][x] = y[x];
-        } else {
-#pragma unroll
-          for (int x = 0; x < 4; x++) s[b][i][x] = p[c + x < A.Dv ? c + x : 0];
-        }
+        const f32x4_any* from = (const f32x4_any*)(in0 + min(b, live - 1) * E + d * A.Dv + c);
+        s[b][i] = STREAM ? __builtin_nontemporal_load(from) : *from;
         kd[b][i] = to_f32(k[b][d]);
         qd[b][i] = to_f32(q[b][d]);
       }
@@ -1049,10 +1049,10 @@ __global__ __launch_bounds__(256) void k_token(TokenArgs A, int lv) {
 #pragma unroll
       for (int b = 0; b < B; b++) {
         if constexpr (VEC) {
-          load_vec<T, 4>(v[b] + (on ? c : 0), vv[b]);
+          load_vec<T, 4>(v[b] + c, vv[b]);
         } else {
 #pragma unroll
-          for (int x = 0; x < 4; x++) vv[b][x] = to_f32(v[b][c + x < A.Dv ? c + x : 0]);
+          for (int x = 0; x < 4; x++) vv[b][x] = to_f32(v[b][c + x]);
         }
         em1[b] = expm1f(em1[b]);
       }
@@ -1062,51 +1062,78 @@ __global__ __launch_bounds__(256) void k_token(TokenArgs A, int lv) {
       for (int i = 0; i < R; i++) {
         const int d = d0 + i * rows;
         if (d < A.Dk && on && b < live) {
-          float* so = out0 + b * E + d * A.Dv + c;
 #pragma unroll
           for (int x = 0; x < 4; x++) {
             const float old = start[b] ? 0.f : fmaf(s[b][i][x], em1[b], s[b][i][x]);
             s[b][i][x] = fmaf(kd[b][i], vv[b][x], old);
             acc[b][x] = fmaf(qd[b][i], s[b][i][x], acc[b][x]);
           }
-          if constexpr (VEC) {
-            const f32x4 y{s[b][i][0], s[b][i][1], s[b][i][2], s[b][i][3]};
-            if (STREAM)
-              __builtin_nontemporal_store(y, (f32x4*)so);
-            else
-              *(f32x4*)so = y;
-          } else {
-#pragma unroll
-            for (int x = 0; x < 4; x++)
-              if (c + x < A.Dv) so[x] = s[b][i][x];
-          }
+          f32x4_any* so = (f32x4_any*)(out0 + b * E + d * A.Dv + c);
+          if (STREAM)
+            __builtin_nontemporal_store(s[b][i], so);
+          else
+            *so = s[b][i];
         }
       }
   }
 #pragma unroll
   for (int b = 0; b < B; b++) {
-    for (int m = 1 << lv; m < 64; m <<= 1)
+    // the rows' shares, in a fixed order, to row 0
+    for (int r = rows; r > 1; r = (r + 1) >> 1) {
+      const int half = (r + 1) >> 1;
 #pragma unroll
-      for (int x = 0; x < 4; x++) acc[b][x] += __shfl_xor(acc[b][x], m);
+      for (int x = 0; x < 4; x++) {
+        const float y = __shfl(acc[b][x], lane + half * nv);
+        acc[b][x] += rr < r - half ? y : 0.f;
+      }
+    }
     if constexpr (SPLIT) {  // the waves' shares, in their order
-      if (rr == 0 && on)
+      if (rr == 0)
 #pragma unroll
         for (int x = 0; x < 4; x++) part[wave][c + x] = acc[b][x];
       __syncthreads();
       if (wave != 0) return;
-      if (on)
+      if (rr == 0)
 #pragma unroll
         for (int x = 0; x < 4; x++) acc[b][x] = ((part[0][c + x] + part[1][c + x]) + part[2][c + x]) + part[3][c + x];
     }
-    if (rr == 0 && b < live && on) {
+    if (rr == 0 && b < live) {
       if constexpr (VEC) {
         store_vec<T, 4>(o[b] + c, acc[b]);
       } else {
 #pragma unroll
-        for (int x = 0; x < 4; x++)
-          if (c + x < A.Dv) o[b][c + x] = from_f32<T>(acc[b][x]);
+        for (int x = 0; x < 4; x++) o[b][c + x] = from_f32<T>(acc[b][x]);
       }
     }
+  }
+}
+
+// Rows of fewer than 4 columns: a wave per pair, a lane per key.
+template <typename T>
+__global__ __launch_bounds__(256) void k_token_narrow(TokenArgs A) {
+  const uint32_t units = (uint32_t)(A.N * A.H), u = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (u >= units) return;
+  const int lane = threadIdx.x & 63;
+  const uint32_t n = u / (uint32_t)A.H, h = u - n * (uint32_t)A.H;
+  const T* q = (const T*)A.q.p + n * A.q.sn + h * A.q.sh;
+  const T* k = (const T*)A.k.p + n * A.k.sn + h * A.k.sh;
+  const T* v = (const T*)A.v.p + n * A.v.sn + h * A.v.sh;
+  T* o = (T*)A.o.p + n * A.o.sn + h * A.o.sh;
+  const bool start = A.starts && A.starts[n * A.starts_sn] != 0;
+  const float em1 = expm1f(A.log_decay[h]);
+  const int64_t at = (int64_t)u * A.Dk * A.Dv;
+  for (int c = 0; c < A.Dv; c++) {
+    const float vc = to_f32(v[c]);
+    float acc = 0.f;
+    for (int d = lane; d < A.Dk; d += 64) {
+      const float s = A.in[at + d * A.Dv + c];
+      const float y = fmaf(to_f32(k[d]), vc, start ? 0.f : fmaf(s, em1, s));
+      A.out[at + d * A.Dv + c] = y;
+      acc = fmaf(to_f32(q[d]), y, acc);
+    }
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) acc += __shfl_xor(acc, m);
+    if (lane == 0) o[c] = from_f32<T>(acc);
   }
 }
 
@@ -1350,33 +1377,38 @@ int fw_linattn_step(const fw_linattn_token* a, void* stream_) {
   if ((uintptr_t)a->state % 16 || (uintptr_t)a->state_out % 16) return bad("states must be 16-byte aligned");
   TokenArgs A{in(a->q), in(a->k), in(a->v), in(a->out), a->log_decay, a->starts, a->starts_sn, a->N,
               a->state, a->state_out, a->H, a->Dk, a->Dv};
-  int lv = 0;
-  while ((4 << lv) < a->Dv) lv++;
-  const int64_t units = a->N * a->H;
   if (a->N > INT32_MAX / a->H) return bad("too many sequences for one call");
+  const int64_t units = a->N * a->H;
+  const int nv = (a->Dv + 3) / 4, rows = 64 / nv;
   auto fours = [&](const fw_seq_tensor& t) {
     return (uintptr_t)t.p % (a->dtype == FW_DT_F32 ? 16 : 8) == 0 && t.sn % 4 == 0 && t.sh % 4 == 0;
   };
   const bool vec = a->Dv % 4 == 0 && fours(a->v) && fours(a->out);
   // Measured in float32: split against not, 128 pairs of 128 x 128: 6.8 against 14.9 us, 1024 pairs: 23 against 28;
   // stream against not, 537 MB of states: 5290 against 4700 GB/s, 134 MB: 4970 against 6050 (it is 256 MB of cache).
-  const int accesses = (a->Dk + (64 >> lv) - 1) / (64 >> lv);  // of one state
-  const bool split = accesses >= 8 && units <= 2048;
-  const bool stream = vec && !split && units * a->Dk * a->Dv * 4 >= (int64_t)192 << 20;
-  const int B = accesses == 1 ? 4 : accesses == 2 ? 2 : 1;
+  const int accesses = (a->Dk + rows - 1) / rows;  // of one state
+  const bool narrow = a->Dv < 4, split = !narrow && accesses >= 8 && units <= 2048;
+  const bool stream = !split && a->Dv % 4 == 0 && units * a->Dk * a->Dv * 4 >= (int64_t)192 << 20;
+  const int B = narrow ? 1 : accesses == 1 ? 4 : accesses == 2 ? 2 : 1;
   const int64_t blocks = split ? units : (units + 4 * B - 1) / (4 * B);
   if (blocks > UINT32_MAX / 256) return bad("too many sequences for one call");  // threads of a launch
   const dim3 grid((unsigned)blocks), block(256);
   hipStream_t s = (hipStream_t)stream_;
-#define FW_TOKEN_K(T, B_, SP)                                                          \
-  if (!vec)                                                                            \
-    hipLaunchKernelGGL((k_token<T, false, B_, SP, false>), grid, block, 0, s, A, lv);  \
-  else if (stream)                                                                     \
-    hipLaunchKernelGGL((k_token<T, true, B_, SP, !SP>), grid, block, 0, s, A, lv);     \
+#define FW_TOKEN_V(T, V, B_, SP)                                                       \
+  if (stream)                                                                          \
+    hipLaunchKernelGGL((k_token<T, V, B_, SP, !SP>), grid, block, 0, s, A, nv, rows, 65536 / nv + 1); \
   else                                                                                 \
-    hipLaunchKernelGGL((k_token<T, true, B_, SP, false>), grid, block, 0, s, A, lv)
+    hipLaunchKernelGGL((k_token<T, V, B_, SP, false>), grid, block, 0, s, A, nv, rows, 65536 / nv + 1)
+#define FW_TOKEN_K(T, B_, SP)                                                          \
+  if (vec) {                                                                           \
+    FW_TOKEN_V(T, true, B_, SP);                                                       \
+  } else {                                                                             \
+    FW_TOKEN_V(T, false, B_, SP);                                                      \
+  }
 #define FW_TOKEN(T)                                                                    \
-  if (split) {                                                                         \
+  if (narrow) {                                                                        \
+    hipLaunchKernelGGL((k_token_narrow<T>), grid, block, 0, s, A);                     \
+  } else if (split) {                                                                  \
     FW_TOKEN_K(T, 1, true);                                                            \
   } else if (B == 4) {                                                                 \
     FW_TOKEN_K(T, 4, false);                                                           \
@@ -1394,6 +1426,7 @@ int fw_linattn_step(const fw_linattn_token* a, void* stream_) {
   }
 #undef FW_TOKEN
 #undef FW_TOKEN_K
+#undef FW_TOKEN_V
   FW_HIP(hipGetLastError());
   return FW_OK;
 }

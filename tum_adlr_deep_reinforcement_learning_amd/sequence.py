@@ -12,6 +12,8 @@ gradients of parameters are float32.  There is no CPU path: CPU tensors are refu
 The reference's policies are memoryless; these have no counterpart there.
 """
 import ctypes
+import functools
+import struct
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -22,31 +24,58 @@ _DT = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # include/fwrollo
 MAX_HEAD = 128
 
 
+def _packer(cls):
+    """A ctypes structure's fields as one struct.pack: a fifth of the time of setting them one by one, and a small call
+    is bound by the host."""
+    code = {ctypes.c_int64: "q", ctypes.c_int32: "i", ctypes.c_double: "d", ctypes.c_size_t: "N", ctypes.c_void_p: "P"}
+
+    def flat(c):
+        return "".join(code[t] if t in code else flat(t) for _, t in c._fields_)
+    p = struct.Struct("@" + flat(cls))
+    assert p.size == ctypes.sizeof(cls)
+    return p.pack
+
+
+_pack_linattn, _pack_token, _pack_norm = (_packer(c) for c in (_native.FwLinattn, _native.FwLinattnToken,
+                                                               _native.FwGroupNorm))
+_NO_ROWS = (0, 0, 0, 0)
+
+
 def _ptr(t):
-    return t.data_ptr() if t is not None else None
+    return t.data_ptr() if t is not None else 0
 
 
 def _launch(name, args, device):
-    """lib.<name>(&args, current stream) with `device` current; a few microseconds matter here, so the common case (it
-    is already) takes no context manager."""
-    fn = getattr(_native.load(), name)
-    if torch.cuda.current_device() == device.index:
-        rc = fn(ctypes.byref(args), torch.cuda.current_stream(device).cuda_stream)
+    """lib.<name>(args, current stream) with `device` current, which it mostly is."""
+    fn, i = getattr(_native.load(), name), device.index
+    if torch._C._cuda_getDevice() == i:
+        rc = fn(args, torch._C._cuda_getCurrentRawStream(i))
     else:
         with torch.cuda.device(device):
-            rc = fn(ctypes.byref(args), torch.cuda.current_stream(device).cuda_stream)
+            rc = fn(args, torch._C._cuda_getCurrentRawStream(i))
     if rc:
         _native.check(rc, name)
 
 
-def _operand(s, t, step=False):
-    """Fills an fw_seq_tensor from a [T][N][H][D] (or [N][H][D]) tensor with unit stride in D."""
+def _once(backward):
+    """once_differentiable, whose context is needed only where a graph of the gradients is asked for."""
+    guarded = once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return run
+
+
+def _rows4(t):
+    """The fields of an fw_seq_tensor for a [T][N][H][D] tensor with unit stride in D."""
     st = t.stride()
-    s.p = t.data_ptr()
-    if step:
-        s.st, s.sn, s.sh = 0, st[0], st[1]
-    else:
-        s.st, s.sn, s.sh = st[0], st[1], st[2]
+    return t.data_ptr(), st[0], st[1], st[2]
+
+
+def _rows3(t):
+    """The same for one token, [N][H][D]."""
+    st = t.stride()
+    return t.data_ptr(), 0, st[0], st[1]
 
 
 def _dense(t):
@@ -55,7 +84,15 @@ def _dense(t):
 
 
 def _heads(who, q, k, v, dims):
-    lay = "[T, N, H, D]" if dims == 4 else "[N, H, D]"
+    try:
+        dt, dev, sq, sv = q.dtype, q.get_device(), q.shape, v.shape
+        if dev >= 0 and k.get_device() == dev == v.get_device() and dt in _DT and k.dtype is dt and v.dtype is dt and \
+                len(sq) == dims and k.shape == sq and sv[:-1] == sq[:-1] and 1 <= sq[-1] <= MAX_HEAD and \
+                1 <= sv[-1] <= MAX_HEAD and sq[-2] >= 1:
+            return
+    except (AttributeError, IndexError, TypeError):
+        pass
+    lay = "[T, N, H, D]" if dims == 4 else "[N, H, D]"  # what is wrong
     for name, t in (("q", q), ("k", k), ("v", v)):
         if not isinstance(t, torch.Tensor) or t.dim() != dims:
             raise ValueError("%s: %s must be a %s tensor" % (who, name, lay))
@@ -97,36 +134,38 @@ def _state(who, x, shape, device, name):
     return x
 
 
-def _linattn_args(q, k, v, log_decay, starts, lengths):
-    a = _native.FwLinattn()
-    a.T, a.N, a.H, a.Dk = q.shape
-    a.Dv, a.dtype = v.shape[3], _DT[q.dtype]
-    _operand(a.q, q)
-    _operand(a.k, k)
-    _operand(a.v, v)
-    a.log_decay = log_decay.data_ptr()
-    if starts is not None:
-        a.starts = starts.data_ptr()
-        a.starts_st, a.starts_sn = starts.stride()
-    a.lengths = _ptr(lengths)
-    return a
+@functools.lru_cache(maxsize=256)
+def _linattn_bytes(T, N, H, Dk, Dv, dtype, backward):  # of the sizes alone
+    return _native.load().fw_linattn_workspace_bytes(T, N, H, Dk, Dv, dtype, backward)
 
 
-def _workspace(a, device, backward):
-    n = _native.load().fw_linattn_workspace_bytes(a.T, a.N, a.H, a.Dk, a.Dv, a.dtype, backward)
-    ws = torch.empty(n, dtype=torch.uint8, device=device) if n else None
-    a.workspace, a.workspace_bytes = _ptr(ws), n
-    return ws  # referenced until the launches are queued; the allocator reuses it in stream order
+def _linattn_head(q, v):
+    T, N, H, Dk = q.shape
+    return T, N, H, Dk, v.shape[3], _DT[q.dtype]
+
+
+def _linattn_masks(log_decay, starts, lengths):
+    if starts is None:
+        return log_decay.data_ptr(), 0, 0, 0, _ptr(lengths)
+    st = starts.stride()
+    return log_decay.data_ptr(), starts.data_ptr(), st[0], st[1], _ptr(lengths)
+
+
+def _workspace(n, device):
+    # referenced until the launches are queued; the allocator reuses it in stream order
+    return torch.empty(n, dtype=torch.uint8, device=device) if n else None
 
 
 def _linattn_forward(q, k, v, log_decay, state, starts, lengths):
-    a = _linattn_args(q, k, v, log_decay, starts, lengths)
-    out = torch.empty(v.shape, dtype=v.dtype, device=v.device)
-    final = torch.empty((a.N, a.H, a.Dk, a.Dv), dtype=torch.float32, device=v.device)
-    _operand(a.out, out)
-    a.state_in, a.state_out = _ptr(state), final.data_ptr()
-    ws = _workspace(a, q.device, 0)  # noqa: F841
-    _launch("fw_linattn_forward", a, q.device)
+    head = T, N, H, Dk, Dv, code = _linattn_head(q, v)
+    out = v.new_empty((T, N, H, Dv))
+    final = log_decay.new_empty((N, H, Dk, Dv))
+    n = _linattn_bytes(T, N, H, Dk, Dv, code, 0)
+    ws = _workspace(n, q.device)
+    _launch("fw_linattn_forward",
+            _pack_linattn(*head, *_rows4(q), *_rows4(k), *_rows4(v), *_rows4(out),
+                          *_linattn_masks(log_decay, starts, lengths), _ptr(state), final.data_ptr(),
+                          *_NO_ROWS, *_NO_ROWS, *_NO_ROWS, *_NO_ROWS, 0, 0, _ptr(ws), n), q.device)
     return out, final
 
 
@@ -139,19 +178,21 @@ class _LinearAttention(torch.autograd.Function):
         return out, final
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dout, dfinal):
         q, k, v, log_decay, state, starts, lengths = ctx.saved_tensors
-        a = _linattn_args(q, k, v, log_decay, starts, lengths)
-        dout = _dense(dout) if dout is not None else torch.zeros(v.shape, dtype=v.dtype, device=v.device)
+        head = T, N, H, Dk, Dv, code = _linattn_head(q, v)
+        dout = _dense(dout) if dout is not None else v.new_zeros((T, N, H, Dv))
         dfinal = dfinal.contiguous() if dfinal is not None else None
-        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-        for s, t in ((a.dout, dout), (a.dq, dq), (a.dk, dk), (a.dv, dv)):
-            _operand(s, t)
+        dq, dk, dv = q.new_empty((T, N, H, Dk)), k.new_empty((T, N, H, Dk)), v.new_empty((T, N, H, Dv))
         dstate = torch.empty_like(state) if state is not None and ctx.needs_input_grad[4] else None
-        a.state_in, a.dstate, a.dstate_in = _ptr(state), _ptr(dfinal), _ptr(dstate)
-        ws = _workspace(a, q.device, 1)  # noqa: F841
-        _launch("fw_linattn_backward", a, q.device)
+        n = _linattn_bytes(T, N, H, Dk, Dv, code, 1)
+        ws = _workspace(n, q.device)
+        _launch("fw_linattn_backward",
+                _pack_linattn(*head, *_rows4(q), *_rows4(k), *_rows4(v), *_NO_ROWS,
+                              *_linattn_masks(log_decay, starts, lengths), _ptr(state), 0,
+                              *_rows4(dout), *_rows4(dq), *_rows4(dk), *_rows4(dv), _ptr(dfinal), _ptr(dstate),
+                              _ptr(ws), n), q.device)
         return dq, dk, dv, None, dstate, None, None
 
 
@@ -209,24 +250,19 @@ def linear_attention_step(q, k, v, log_decay, state, episode_starts=None, state_
     starts = _starts(who, episode_starts, (N,), dev)
     shape = (N, H, Dk, v.shape[2])
     new = state if state_out is None else state_out
-    for name, t in (("state", state), ("state_out", new)):
+    for name, t in (("state", state), ("state_out", new))[:1 if new is state else 2]:
         _state(who, t, shape, dev, name)
         if not t.is_contiguous() or t.data_ptr() % 16:
             raise ValueError("%s: %s must be contiguous and 16-byte aligned" % (who, name))
-    b = new.numel() * 4
-    if new.data_ptr() != state.data_ptr() and abs(new.data_ptr() - state.data_ptr()) < b:
+    if new is not state and new.data_ptr() != state.data_ptr() and \
+            abs(new.data_ptr() - state.data_ptr()) < new.numel() * 4:
         raise ValueError("%s: state_out overlaps state" % who)
     q, k, v = _dense(q), _dense(k), _dense(v)
-    out = torch.empty(v.shape, dtype=v.dtype, device=dev)
-    a = _native.FwLinattnToken()
-    a.N, a.H, a.Dk, a.Dv, a.dtype = N, H, Dk, v.shape[2], _DT[q.dtype]
-    for s, t in ((a.q, q), (a.k, k), (a.v, v), (a.out, out)):
-        _operand(s, t, step=True)
-    a.log_decay = log_decay.data_ptr()
-    if starts is not None:
-        a.starts, a.starts_sn = starts.data_ptr(), starts.stride(0)
-    a.state, a.state_out = state.data_ptr(), new.data_ptr()
-    _launch("fw_linattn_step", a, dev)
+    out = v.new_empty((N, H, shape[3]))
+    _launch("fw_linattn_step",
+            _pack_token(N, H, Dk, shape[3], _DT[q.dtype], *_rows3(q), *_rows3(k), *_rows3(v), *_rows3(out),
+                        log_decay.data_ptr(), _ptr(starts), starts.stride(0) if starts is not None else 0,
+                        state.data_ptr(), new.data_ptr()), dev)
     return out
 
 
@@ -234,38 +270,29 @@ def linear_attention_step(q, k, v, log_decay, state, episode_starts=None, state_
 _ACT = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "tanh": 4}  # include/fwrollout.h FW_ACT_*
 
 
-def _rows(s, t):
-    s.p, s.sn, s.sl = t.data_ptr(), t.stride(0), t.stride(1)
+@functools.lru_cache(maxsize=256)
+def _norm_stats(N, L, C, groups):  # of the sizes alone
+    return _native.load().fw_group_norm_stats(_pack_norm(N, L, C, groups, 0, 0, 0, 0, 0.0, *(0,) * 19))
 
 
-def _norm_args(x, groups, weight, bias, eps, act):
-    a = _native.FwGroupNorm()
-    a.N, a.L, a.C = x.shape
-    a.G, a.dtype, a.act, a.eps = groups, _DT[x.dtype], act, eps
-    p = weight if weight is not None else bias
-    a.wdtype = _DT[p.dtype] if p is not None else 0
-    a.weight, a.bias = _ptr(weight), _ptr(bias)
-    _rows(a.x, x)
-    return a
-
-
-def _norm_workspace(a, device, backward):
-    n = _native.load().fw_group_norm_workspace_bytes(ctypes.byref(a), backward)
-    ws = torch.empty(n, dtype=torch.uint8, device=device) if n else None
-    a.workspace, a.workspace_bytes = _ptr(ws), n
-    return ws
+def _rows(t):
+    st = t.stride()
+    return t.data_ptr(), st[0], st[1]
 
 
 def _norm_forward(x, groups, weight, bias, eps, act, keep):
-    a = _norm_args(x, groups, weight, bias, eps, act)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    _rows(a.y, y)
-    stats = None
-    if keep and _native.load().fw_group_norm_stats(ctypes.byref(a)):
-        stats = torch.empty((a.N, groups, 2), dtype=torch.float32, device=x.device)
-        a.stats = stats.data_ptr()
-    ws = _norm_workspace(a, x.device, 0)  # noqa: F841
-    _launch("fw_group_norm_forward", a, x.device)
+    N, L, C = x.shape
+    y = x.new_empty((N, L, C))
+    stats = ws = None
+    n = 0
+    p = weight if weight is not None else bias
+    head = (N, L, C, groups, _DT[x.dtype], _DT[p.dtype] if p is not None else 0, act, 0, eps, *_rows(x), *_rows(y),
+            0, 0, 0, 0, 0, 0, _ptr(weight), _ptr(bias), 0, 0)
+    if _norm_stats(N, L, C, groups):  # (units that need neither fit a block)
+        n = _native.load().fw_group_norm_workspace_bytes(_pack_norm(*head, 0, 0, 0), 0)
+        ws = _workspace(n, x.device)
+        stats = torch.empty((N, groups, 2), dtype=torch.float32, device=x.device) if keep else None
+    _launch("fw_group_norm_forward", _pack_norm(*head, _ptr(stats), _ptr(ws), n), x.device)
     return y, stats
 
 
@@ -278,22 +305,23 @@ class _GroupNormAct(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dy):
         x, weight, bias, stats = ctx.saved_tensors
         groups, eps, act = ctx.conf
         dy = _dense(dy)
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        N, L, C = x.shape
+        dx = x.new_empty((N, L, C))
         dw = torch.empty_like(weight) if weight is not None and ctx.needs_input_grad[1] else None
         db = torch.empty_like(bias) if bias is not None and ctx.needs_input_grad[2] else None
         if x.numel() == 0:
             return (dx,) + tuple(t.zero_() if t is not None else None for t in (dw, db)) + (None, None, None)
-        a = _norm_args(x, groups, weight, bias, eps, act)
-        _rows(a.dy, dy)
-        _rows(a.dx, dx)
-        a.dweight, a.dbias, a.stats = _ptr(dw), _ptr(db), _ptr(stats)
-        ws = _norm_workspace(a, x.device, 1)  # noqa: F841
-        _launch("fw_group_norm_backward", a, x.device)
+        p = weight if weight is not None else bias
+        head = (N, L, C, groups, _DT[x.dtype], _DT[p.dtype] if p is not None else 0, act, 0, eps, *_rows(x), 0, 0, 0,
+                *_rows(dy), *_rows(dx), _ptr(weight), _ptr(bias), _ptr(dw), _ptr(db), _ptr(stats))
+        n = _native.load().fw_group_norm_workspace_bytes(_pack_norm(*head, 0, 0), 1)
+        ws = _workspace(n, x.device)
+        _launch("fw_group_norm_backward", _pack_norm(*head, _ptr(ws), n), x.device)
         return dx, dw, db, None, None, None
 
 
@@ -307,7 +335,7 @@ def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, activation="
     read in place.  Differentiable in x, weight and bias; deterministic."""
     if not isinstance(x, torch.Tensor) or x.dim() < 2:
         raise ValueError("group_norm_act: x must be an [N, ..., C] tensor")
-    if x.device.type != "cuda":
+    if not x.is_cuda:
         raise ValueError("group_norm_act: x must be on the GPU (no CPU path exists)")
     if x.dtype not in _DT:
         raise ValueError("group_norm_act: x must be float32, bfloat16 or float16")
@@ -325,10 +353,12 @@ def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, activation="
     if weight is not None and bias is not None and weight.dtype != bias.dtype:
         raise ValueError("group_norm_act: weight and bias must share a dtype")
     shape = x.shape
-    rows = 1
-    for d in shape[1:-1]:
-        rows *= d
-    x = _dense(x.reshape(shape[0], rows, C))
+    if len(shape) != 3:
+        rows = 1
+        for d in shape[1:-1]:
+            rows *= d
+        x = x.reshape(shape[0], rows, C)
+    x = _dense(x)
     weight = weight.contiguous() if weight is not None else None
     bias = bias.contiguous() if bias is not None else None
     if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or
@@ -336,4 +366,4 @@ def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, activation="
         y = _GroupNormAct.apply(x, weight, bias, groups, float(eps), _ACT[activation])
     else:
         y = _norm_forward(x, groups, weight, bias, float(eps), _ACT[activation], False)[0]
-    return y.view(shape)
+    return y if len(shape) == 3 else y.view(shape)
