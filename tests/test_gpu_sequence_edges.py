@@ -59,11 +59,12 @@ def test_strides_of_single_rows_mean_nothing(dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("strides", ["tokens", "tokens far apart", "sequences"])
+@pytest.mark.parametrize("strides", ["tokens", "tokens far apart", "tokens at the limit", "tokens beyond it", "sequences"])
 def test_offsets_beyond_32_bits(strides, dtype):
-    """Views whose rows lie gigabytes apart (tokens up to 2^24 elements apart, and further, in one allocation)."""
+    """Views whose rows lie gigabytes apart (a block's rows are addressed by 32-bit offsets up to 2^26 elements apart)."""
     T, N, H, D = 70, 2, 2, 32
-    st, sn = {"tokens": (2 ** 24 - 64, H * D), "tokens far apart": (2 ** 25 + 64, H * D), "sequences": (H * D, 2 ** 31)}[strides]
+    st, sn = {"tokens": (2 ** 24 - 64, H * D), "tokens far apart": (2 ** 25 + 64, H * D), "sequences": (H * D, 2 ** 31),
+              "tokens at the limit": (2 ** 26, H * D), "tokens beyond it": (2 ** 26 + 64, H * D)}[strides]
     n = (T - 1) * st + (N - 1) * sn + H * D
 
     def view(x):
@@ -170,3 +171,28 @@ def test_two_streams_at_once():
         torch.cuda.synchronize()
         for g, w in zip(got, want):
             assert all(torch.equal(p, r) for p, r in zip(g, w))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("Dk,Dv", [(1, 2), (3, 9), (4, 4), (5, 8), (7, 17), (9, 31), (17, 65), (66, 127), (127, 64), (101, 97)])
+def test_rows_of_any_length_and_address(Dk, Dv, dtype):
+    """Rows that are no whole vectors, packed and behind one odd element."""
+    _check(_case(75, 2, 2, Dk, Dv, dtype, seed=Dk, starts=0.05, lengths=[75, 38]))
+
+    def odd(x):
+        y = torch.full((x.numel() + 1,), float("nan"), dtype=x.dtype, device=DEV)
+        y[1:] = x.reshape(-1)
+        return y[1:].view(x.shape)
+    _check(_case(34, 3, 1, Dk, Dv, dtype, seed=Dv), view=odd)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("N,H,Dk,Dv", [(3, 2, 9, 1), (2, 2, 70, 2), (5, 1, 128, 3), (3, 2, 8, 5), (2, 3, 20, 17), (70, 2, 64, 35),
+                                       (2, 2, 128, 69), (40, 4, 100, 101), (3000, 1, 10, 127), (700, 3, 33, 33)])
+def test_step_rows_of_any_length(N, H, Dk, Dv, dtype):
+    c = _case(1, N, H, Dk, Dv, dtype, seed=Dv, starts=0.2)
+    s, d = _seq(), _dev(c)
+    ref, bulk = _oracle(c, False)
+    out = s.linear_attention_step(d["q"][0], d["k"][0], d["v"][0], d["log_decay"], d["state"], d["starts"][0])
+    _close("out", out, ref[0][0], bulk[0][0], Dk + 16)
+    _close("state", d["state"], ref[1], bulk[1], 16)

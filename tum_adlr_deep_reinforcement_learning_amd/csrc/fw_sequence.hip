@@ -76,7 +76,8 @@ struct Unit {
 };
 
 
-enum { FULL, GUARD, SCALAR };  // D fills the tiles; whole vectors in or out; element by element
+// D fills the tiles; whole vectors in or out; rows of any length at any address, through registers
+enum { FULL, GUARD, ANY };
 
 // Element j of the result on lane x of four is element x of lane j's argument.
 template <int CTRL>
@@ -192,6 +193,15 @@ __device__ __forceinline__ void copy1(const void* base, uint32_t off, char* lds)
                : "memory");
 }
 
+// the same value, but not known to be: keeps what a rare branch computes from it inside that branch
+__device__ __forceinline__ int here(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
+typedef u32x4 __attribute__((aligned(4))) u32x4_any4;
+typedef u32x4 __attribute__((aligned(2))) u32x4_any2;
+
 // ROWS rows of 16 NT columns in LDS, as 16-byte chunks; chunk c of a row is stored at c ^ turn(row), so that the 16
 // lanes that are served together meet in no bank: 16 rows of one chunk, or (TRANSPOSED) 4 rows of 4 half chunks
 template <typename T, int NT, int ROWS, bool TRANSPOSED = false>
@@ -209,31 +219,68 @@ struct Tile {
   template <int MODE, bool WHOLE>
   __device__ static __forceinline__ void fetch(char* lds, const T* base, int64_t st, int D, int c, bool rev, int lane) {
     const int row0 = lane / CH, pc = lane % CH;
-    if constexpr (MODE == SCALAR) {
-#pragma unroll 1
-      for (int i = 0; i < NI; i++) {
-        const int row = i * RI + row0, col = (pc ^ turn(row)) * PER, u = min(row, c - 1);
-        const T* x = base + (int64_t)(rev ? c - 1 - u : u) * st;
-        Pack<T, PER> v;
 #pragma unroll
-        for (int m = 0; m < PER; m++) v.e[m] = col + m < D ? x[col + m] : T{};
-        if (row < ROWS) *(Pack<T, PER>*)(lds + (i * 64 + lane) * 16) = v;
+    for (int i = 0; i < NI; i++) {
+      const int row = i * RI + row0, col = (pc ^ turn(row)) * PER;
+      if ((RI <= ROWS || row < ROWS) && (MODE == FULL || col < D)) {
+        // uniform base + 32-bit lane offset (the launcher saw that a block's rows fit)
+        if constexpr (WHOLE) {  // c = ROWS
+          const int first = rev ? ROWS - RI - i * RI : i * RI;
+          copy16(base + first * st, ((rev ? RI - 1 - row0 : row0) * (uint32_t)st + col) * (uint32_t)sizeof(T),
+                 lds + i * 1024);
+        } else {
+          const int u = min(row, c - 1);
+          copy16(base, ((rev ? c - 1 - u : u) * (uint32_t)st + col) * (uint32_t)sizeof(T), lds + i * 1024);
+        }
       }
-    } else {
+    }
+  }
+
+  // The same rows at any address and of any length, by way of registers: `hold` asks for them, `commit` writes them with
+  // zeros behind D.  A row's last chunk is read from where it ends with the row and moved down into place, so nothing
+  // outside the row is read.  whole: a row has a chunk at all (base may be some columns into it); else commit reads it by
+  // elements.  Addresses are worked out each time: kept, they would take the registers that hold the rows.
+  using any16 = std::conditional_t<sizeof(T) == 4, u32x4_any4, u32x4_any2>;
+  __device__ static __forceinline__ const T* source(const T* base, int64_t st, int row, int c, bool rev) {
+    const int u = min(row, c - 1);
+    return base + (int64_t)(rev ? c - 1 - u : u) * st;
+  }
+  __device__ static __forceinline__ void hold(u32x4 (&held)[NI], const T* base, int64_t st, int D, bool whole, int c,
+                                              bool rev, int lane) {
+    if (!whole) return;
+    lane = here(lane);
+    const int row0 = lane / CH, pc = lane % CH;
+#pragma unroll
+    for (int i = 0; i < NI; i++) {
+      const int row = i * RI + row0, col = (pc ^ turn(row)) * PER;
+      held[i] = *(const any16*)(source(base, st, row, c, rev) + min(col, D - PER));
+    }
+  }
+  __device__ static __forceinline__ void commit(char* lds, const u32x4 (&held)[NI], const T* base, int64_t st, int D,
+                                                bool whole, int c, bool rev, int lane) {
+    lane = here(lane);
+    const int row0 = lane / CH, pc = lane % CH;
+    if (whole) {
 #pragma unroll
       for (int i = 0; i < NI; i++) {
         const int row = i * RI + row0, col = (pc ^ turn(row)) * PER;
-        if ((RI <= ROWS || row < ROWS) && (MODE == FULL || col < D)) {
-          // uniform base + 32-bit lane offset (the launcher saw that a block's rows fit)
-          if constexpr (WHOLE) {  // c = ROWS
-            const int first = rev ? ROWS - RI - i * RI : i * RI;
-            copy16(base + first * st, (uint32_t)((rev ? RI - 1 - row0 : row0) * (int)st + col) * (uint32_t)sizeof(T),
-                   lds + i * 1024);
-          } else {
-            const int u = min(row, c - 1);
-            copy16(base, (uint32_t)((rev ? c - 1 - u : u) * (int)st + col) * (uint32_t)sizeof(T), lds + i * 1024);
-          }
-        }
+        u32x4 v = held[i];
+        const int by = (col - min(col, D - PER)) * (int)sizeof(T) * 8;  // bits; 128 and more: outside
+        uint64_t lo = (uint64_t)v[1] << 32 | v[0], hi = (uint64_t)v[3] << 32 | v[2];
+        lo = by & 64 ? hi : lo;
+        hi = by & 64 ? 0 : hi;
+        lo = lo >> (by & 63) | (hi << 1) << (63 - (by & 63));
+        hi >>= by & 63;
+        const uint32_t in = by < 128 ? ~0u : 0u;
+        v = u32x4{(uint32_t)lo & in, (uint32_t)(lo >> 32) & in, (uint32_t)hi & in, (uint32_t)(hi >> 32) & in};
+        if (RI <= ROWS || row < ROWS) *(u32x4*)(lds + (i * 64 + lane) * 16) = v;
+      }
+    } else {
+#pragma unroll 1
+      for (int i = 0; i < NI * PER; i++) {
+        const int row = i / PER * RI + row0, col = (pc ^ turn(row)) * PER + i % PER;
+        const T x = col < D ? source(base, st, row, c, rev)[col] : T{};
+        if (RI <= ROWS || row < ROWS) ((T*)(lds + (i / PER * 64 + lane) * 16))[i % PER] = x;
       }
     }
   }
@@ -249,23 +296,22 @@ struct Tile {
       const Pack<T, PER> v = *(const Pack<T, PER>*)(lds + (i * 64 + lane) * 16);
       if (row < c && (MODE == FULL || col < D)) {
         const int64_t u = rev ? c - 1 - row : row;
-        if constexpr (MODE == SCALAR) {
+        if constexpr (MODE == ANY) {
+          T* x = base + u * st + col;
+          if (col + PER <= D) {
+            *(any16*)x = __builtin_bit_cast(u32x4, v);
+          } else {
 #pragma unroll
-          for (int k = 0; k < PER; k++)
-            if (col + k < D) base[u * st + col + k] = v.e[k];
+            for (int k = 0; k < PER; k++)
+              if (col + k < D) x[k] = v.e[k];
+          }
         } else {
-          *(Pack<T, PER>*)((char*)base + (uint32_t)((int)u * (int)st + col) * (uint32_t)sizeof(T)) = v;
+          *(Pack<T, PER>*)((char*)base + ((uint32_t)u * (uint32_t)st + col) * (uint32_t)sizeof(T)) = v;
         }
       }
     }
   }
 };
-
-// the same value, but not known to be: keeps what a rare branch computes from it inside that branch
-__device__ __forceinline__ int here(int x) {
-  asm volatile("" : "+v"(x));
-  return x;
-}
 
 __device__ __forceinline__ f32x4 mma(float a, float b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
@@ -301,7 +347,7 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, KT * VT <= 16 ? 2 : 1) void k_scan
   using R = Ring<T, KT, VT>;
   using K = typename R::K;
   using V = typename R::V;
-  constexpr int NB = R::NB;
+  constexpr int NB = MODE == ANY ? 1 : R::NB;
   __shared__ alignas(16) char smem[SCAN_WAVES][NB * R::BYTES];
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
   char* const ring = smem[__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)];
@@ -359,7 +405,24 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, KT * VT <= 16 ? 2 : 1) void k_scan
       asked += c;
     }
   };
-  fill(0, NB, C);
+  if constexpr (MODE != ANY) fill(0, NB, C);
+  // MODE ANY: one block ahead, in registers
+  u32x4 hq[K::NI], hk[K::NI], hv[V::NI];
+  uint32_t hx = 0;
+  bool held = false;
+  auto hold = [&](int64_t t0, int c) __attribute__((always_inline)) {
+    constexpr int PER = K::PER;
+    K::hold(hk, kb + t0 * p.k.st, p.k.st, Dk, Dk >= PER, c, rev, lane);
+    if (want_out) K::hold(hq, qb + t0 * p.q.st, p.q.st, Dk, Dk >= PER, c, rev, lane);
+    V::hold(hv, vb + t0 * p.v.st, p.v.st, Dv - v0, Dv >= PER, c, rev, lane);
+    const int u = min(lane, c - 1);
+    if (xb) hx = lane < c ? xb[(t0 + (rev ? c - 1 - u : u)) * A.starts_st] : 0;
+    held = true;
+  };
+  if (MODE == ANY && L > 0) {
+    const int c = (int)min((int64_t)C, L);
+    hold(rev ? L - c : 0, c);
+  }
 
   f32x4 S[KT][VT];
 #pragma unroll
@@ -387,28 +450,33 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, KT * VT <= 16 ? 2 : 1) void k_scan
   while (done < L) {
     const int c = single ? 1 : (int)min((int64_t)C, L - done);
     const int64_t t0 = rev ? L - done - c : done;
-    if (ahead == 0) {
-      wait_loads<0>();
-      fill(done, single ? 1 : NB, single ? 1 : C);
-      steady = 0;
-    }
-    // Newer than this block's copies are those of the NB - 1 blocks behind it and, NB blocks after a fill, the stores
-    // of the NB - 1 blocks before it.
-    if (MODE == SCALAR || ahead < NB || !want_out) {
-      if (MODE != SCALAR && ahead == NB)
-        wait_loads<(NB - 1) * ND1>();
-      else
-        wait_loads<0>();
-    } else if (steady < NB) {
-      wait_loads<(NB - 1) * ND2>();
+    if constexpr (MODE == ANY) {
+      if (!held) hold(t0, c);
+      K::commit(ring + K::BYTES, hk, kb + t0 * p.k.st, p.k.st, Dk, Dk >= K::PER, c, rev, lane);
+      if (want_out) K::commit(ring, hq, qb + t0 * p.q.st, p.q.st, Dk, Dk >= K::PER, c, rev, lane);
+      V::commit(ring + 2 * K::BYTES, hv, vb + t0 * p.v.st, p.v.st, Dv - v0, Dv >= K::PER, c, rev, lane);
     } else {
-      wait_loads<(NB - 1) * (ND2 + NST)>();
+      if (ahead == 0) {
+        wait_loads<0>();
+        fill(done, single ? 1 : NB, single ? 1 : C);
+        steady = 0;
+      }
+      // Newer than this block's copies are those of the NB - 1 blocks behind it and, NB blocks after a fill, the stores
+      // of the NB - 1 blocks before it.
+      if (ahead < NB)
+        wait_loads<0>();
+      else if (!want_out)
+        wait_loads<(NB - 1) * ND1>();
+      else if (steady < NB)
+        wait_loads<(NB - 1) * ND2>();
+      else
+        wait_loads<(NB - 1) * (ND2 + NST)>();
     }
     char* const lq = ring + slot * R::BYTES;
     char* const lk = lq + K::BYTES;
     char* const lv = lk + K::BYTES;
     uint32_t M = 0;  // bit u: an episode starts at row u
-    if (xb) M = (uint32_t)__ballot(lane < c && *(const uint8_t*)(lv + V::BYTES + 4 * lane) != 0);
+    if (xb) M = (uint32_t)__ballot(MODE == ANY ? hx != 0 : lane < c && *(const uint8_t*)(lv + V::BYTES + 4 * lane) != 0);
     // A start at row u of a forward pass cuts every span that contains row u but not from it on; in a reversed pass
     // the cut lies behind row u, that is at row u + 1.
     const uint32_t cut = rev ? M << 1 : M;
@@ -448,17 +516,23 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, KT * VT <= 16 ? 2 : 1) void k_scan
         load_vec<T, WK>((const T*)(lk + K::at(4 * g + j, (KT * r + x) / K::PER) + (KT * r + x) % K::PER * (int)sizeof(T)), K2[j] + x);
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // every read of the block is done: its room is free
+    if constexpr (MODE == ANY) asked = done + c;
     const bool more = !single && asked < L;  // a block to copy there; its values after the outputs have used their room
     const int c2 = (int)min((int64_t)C, L - asked);
     const int64_t t2 = rev ? L - asked - c2 : asked;
-    if (more) {
-      fetch_k(lq, t2, c2);
-      asked += c2;
+    if constexpr (MODE == ANY) {
+      held = false;
+      if (more) hold(t2, c2);
     } else {
-      ahead--;
+      if (more) {
+        fetch_k(lq, t2, c2);
+        asked += c2;
+      } else {
+        ahead--;
+      }
+      slot = slot + 1 == NB ? 0 : slot + 1;
+      steady++;
     }
-    slot = slot + 1 == NB ? 0 : slot + 1;
-    steady++;
 
 #pragma unroll
     for (int j = 0; j < TPL; j++)
@@ -469,6 +543,7 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, KT * VT <= 16 ? 2 : 1) void k_scan
     if (c > 1 && __any(!(fabsf(bad) < __builtin_huge_valf()))) {
       single = c;
       ahead = 0;
+      held = false;
       continue;
     }
     fresh |= M != 0;
@@ -525,7 +600,7 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, KT * VT <= 16 ? 2 : 1) void k_scan
       V::template put<MODE>(lv, ob + t0 * p.o.st, p.o.st, Dv - v0, c, rev, lane);
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
-    if (more) fetch_v(lq, t2, c2);
+    if (MODE != ANY && more) fetch_v(lq, t2, c2);
 
     // the state: g^c S as S + S (g^c - 1), whose rounding does not add up over the blocks of a long memory
     if (M != 0) {
@@ -662,10 +737,24 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, 2) void k_scan16(ScanArgs A) {
     for (int i = lane * 16; i < 2 * K::BYTES + V::BYTES; i += 1024) *(u32x4*)(lq + i) = u32x4{0, 0, 0, 0};
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   }
+  // MODE ANY: by way of registers
+  u32x4 hq[K::NI], hk[K::NI], hv[V::NI];
+  auto hold = [&](int64_t t0, int c) __attribute__((always_inline)) {
+    constexpr int PER = K::PER;
+    V::hold(hv, vb + t0 * p.v.st, p.v.st, Dv - v0, Dv >= PER, c, rev, lane);
+    K::hold(hk, kb + t0 * p.k.st, p.k.st, Dk, Dk >= PER, c, rev, lane);
+    if (want_out) K::hold(hq, qb + t0 * p.q.st, p.q.st, Dk, Dk >= PER, c, rev, lane);
+  };
+  auto ask = [&](int64_t t0, int c) __attribute__((always_inline)) {
+    if constexpr (MODE == ANY)
+      hold(t0, c);
+    else
+      fetch(t0, c);
+  };
   bool loaded = L > 0;
   if (loaded) {
     const int c = (int)min((int64_t)C, L);
-    fetch(rev ? L - c : 0, c);
+    ask(rev ? L - c : 0, c);
   }
 
   f32x4 S[KT][VT];
@@ -698,7 +787,12 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, 2) void k_scan16(ScanArgs A) {
     const int64_t t0 = rev ? L - done - c : done;
     if (!loaded) {
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-      fetch(t0, c);
+      ask(t0, c);
+    }
+    if constexpr (MODE == ANY) {
+      V::commit(lv, hv, vb + t0 * p.v.st, p.v.st, Dv - v0, Dv >= K::PER, c, rev, lane);
+      K::commit(lk, hk, kb + t0 * p.k.st, p.k.st, Dk, Dk >= K::PER, c, rev, lane);
+      if (want_out) K::commit(lq, hq, qb + t0 * p.q.st, p.q.st, Dk, Dk >= K::PER, c, rev, lane);
     }
     uint32_t M = 0;  // bit u: an episode starts at row u
     if (xb) {
@@ -759,7 +853,7 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, 2) void k_scan16(ScanArgs A) {
     loaded = !single && done + c < L;
     if (loaded) {
       const int c2 = (int)min((int64_t)C, L - done - c);
-      fetch(rev ? t0 - c2 : t0 + c, c2);
+      ask(rev ? t0 - c2 : t0 + c, c2);
     }
     // Masks.  A start at row u of a forward pass cuts every span that contains row u but not from it on; in a reversed
     // pass the cut lies behind row u, that is at row u + 1.
@@ -1171,9 +1265,9 @@ size_t plan_floats(const Plan& pl, int dirs, int64_t N, int H, int Dk, int Dv) {
 template <typename T>
 bool aligned(const Operand& o, int D) {
   const int per16 = 16 / sizeof(T);
-  // (a block's rows are addressed by 32-bit offsets)
+  // (a block's rows, 16 of 4 or 2 bytes or 32 of 2, are addressed by 32-bit offsets)
   return D % per16 == 0 && (uintptr_t)o.p % 16 == 0 && o.st % per16 == 0 && o.sn % per16 == 0 && o.sh % per16 == 0 &&
-         o.st >= 0 && o.st < (int64_t)1 << 24;
+         o.st >= 0 && o.st <= (int64_t)1 << 26;
 }
 
 template <typename T, int KT, int VT>
@@ -1195,7 +1289,7 @@ int launch_mode(const ScanArgs& A, int mode, hipStream_t s) {
   else if (mode == GUARD)
     hipLaunchKernelGGL(kernel(std::integral_constant<int, GUARD>()), grid, block, 0, s, A);
   else
-    hipLaunchKernelGGL(kernel(std::integral_constant<int, SCALAR>()), grid, block, 0, s, A);
+    hipLaunchKernelGGL(kernel(std::integral_constant<int, ANY>()), grid, block, 0, s, A);
   FW_HIP(hipGetLastError());
   return FW_OK;
 }
@@ -1206,7 +1300,7 @@ int launch_scan(ScanArgs A, int kt, int vt, hipStream_t s) {
   for (int i = 0; i < A.n_pass; i++) {
     const Pass& p = A.pass[i];
     bool vec = aligned<T>(p.q, p.Dk) && aligned<T>(p.k, p.Dk) && aligned<T>(p.v, p.Dv) && aligned<T>(p.o, p.Dv);
-    mode = std::max<int>(mode, !vec ? SCALAR : p.Dk == 16 * kt && p.Dv % (16 * vt) == 0 ? FULL : GUARD);
+    mode = std::max<int>(mode, !vec ? ANY : p.Dk == 16 * kt && p.Dv % (16 * vt) == 0 ? FULL : GUARD);
   }
   switch (kt * 8 + vt) {
 #define FW_CASE(K, V) \
