@@ -1240,18 +1240,21 @@ int slices(int dtype, int Dk, int Dv) {
   return (Dv + cols - 1) / cols;
 }
 
-// Time segments: with fewer than SEG_WAVES waves the card is not full, so the time axis is cut, at the price of
-// reading k and v twice and of a state per segment.
+// Time segments: with few waves the card is not full, so the time axis is cut, at the price of reading k and v twice and
+// of a state per segment.  SEG_WAVES is two waves per SIMD; the backward pass runs three passes at once and wants fewer.
+// Two segments cost more than they bring unless all their waves have a SIMD each (measured, us; 1000 waves of 500 tokens:
+// 1 segment 111 forward and 250 backward, 2 segments 125 and 291; 400 waves of 512, backward: 1 segment 75, 2: 102, 4: 111;
+// 256 waves of 2048: forward 4 segments 109, 8: 104, backward 4 segments 213, 8: 251).
 constexpr int SEG_WAVES = 2048;
 constexpr int SEG_MIN = 128;  // tokens
 struct Plan {
   int64_t seg_len;
   int n_seg;
 };
-Plan plan(int dtype, int64_t T, int64_t N, int H, int Dk, int Dv) {
-  const int64_t waves = N * H * slices(dtype, Dk, Dv);
-  const int64_t segs = std::min<int64_t>(SEG_WAVES / std::max<int64_t>(1, waves), T / SEG_MIN);
-  if (segs < 2) return {std::max<int64_t>(T, 1), 1};
+Plan plan(int dtype, int64_t T, int64_t N, int H, int Dk, int Dv, bool backward) {
+  const int64_t waves = std::max<int64_t>(1, N * H * slices(dtype, Dk, Dv));
+  const int64_t segs = std::min<int64_t>((backward ? SEG_WAVES / 2 : SEG_WAVES) / waves, T / SEG_MIN);
+  if (segs < 2 || (segs == 2 && (backward ? 3 : 1) * 2 * waves > SEG_WAVES / 2)) return {std::max<int64_t>(T, 1), 1};
   const int64_t len = ((T + segs - 1) / segs + 31) / 32 * 32;
   return {len, (int)((T + len - 1) / len)};
 }
@@ -1412,14 +1415,14 @@ extern "C" {
 
 size_t fw_linattn_workspace_bytes(int64_t T, int64_t N, int32_t H, int32_t Dk, int32_t Dv, int32_t dtype, int32_t backward) {
   if (T < 1 || N < 1 || H < 1 || Dk < 1 || Dk > MAXDIM || Dv < 1 || Dv > MAXDIM) return 0;
-  return sizeof(float) * plan_floats(plan(dtype, T, N, H, Dk, Dv), backward ? 2 : 1, N, H, Dk, Dv);
+  return sizeof(float) * plan_floats(plan(dtype, T, N, H, Dk, Dv, backward), backward ? 2 : 1, N, H, Dk, Dv);
 }
 
 int fw_linattn_forward(const fw_linattn* a, void* stream) {
   if (int rc = check(a, "fw_linattn_forward")) return rc;
   if (a->N == 0) return FW_OK;
   if (a->T > 0 && !a->out.p) return fw::set_error(FW_E_INVALID, "fw_linattn_forward: NULL out");
-  const Plan pl = plan(a->dtype, a->T, a->N, a->H, a->Dk, a->Dv);
+  const Plan pl = plan(a->dtype, a->T, a->N, a->H, a->Dk, a->Dv, false);
   if (!room(a, false)) return fw::set_error(FW_E_INVALID, "fw_linattn_forward: workspace too small or not 16-byte aligned");
   hipStream_t s = (hipStream_t)stream;
   float* ws = (float*)a->workspace;
@@ -1439,7 +1442,7 @@ int fw_linattn_backward(const fw_linattn* a, void* stream) {
   if (a->N == 0) return FW_OK;
   if (a->T > 0 && (!a->dout.p || !a->dq.p || !a->dk.p || !a->dv.p))
     return fw::set_error(FW_E_INVALID, "fw_linattn_backward: NULL dout, dq, dk or dv");
-  const Plan pl = plan(a->dtype, a->T, a->N, a->H, a->Dk, a->Dv);
+  const Plan pl = plan(a->dtype, a->T, a->N, a->H, a->Dk, a->Dv, true);
   if (!room(a, true)) return fw::set_error(FW_E_INVALID, "fw_linattn_backward: workspace too small or not 16-byte aligned");
   hipStream_t s = (hipStream_t)stream;
   float* ws = (float*)a->workspace;
