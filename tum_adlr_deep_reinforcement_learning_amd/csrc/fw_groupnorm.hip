@@ -9,6 +9,7 @@
 // All statistics are sums of deviations from a mean, so a large mean does not cancel.  Memory bound: x in, y out (and
 // dy in, dx out); the gradients of weight and bias are column sums of per-unit partial sums, in a fixed order.
 #include <algorithm>
+#include <type_traits>
 
 #include "fw_seq_common.hpp"
 
@@ -49,18 +50,17 @@ __device__ __forceinline__ float tanh_fast(float z) {
   const float q = fmaf(-2.f, __builtin_amdgcn_rcpf(1.f + exp_fast(2.f * z)), 1.f);
   return fabsf(z) < 0.25f ? p : q;
 }
-// Phi(z), and e = exp(-z^2 / 2) beside it.  16-bit types: Abramowitz and Stegun 7.1.26 for erfc (absolute error 1.5e-7
+// Phi(-|z|), and e = exp(-z^2 / 2) beside it.  16-bit types: Abramowitz and Stegun 7.1.26 for erfc (absolute error 1.5e-7
 // of it, against 5e-4 of the types' own step); float32: the library's erfc.
 template <typename T>
-__device__ __forceinline__ float normal_cdf(float z, float& e) {
-  e = exp_fast(-0.5f * z * z);
+__device__ __forceinline__ float normal_tail(float z, float& e) {
+  e = __builtin_amdgcn_exp2f(z * -0.72134752f * z);
   if constexpr (sizeof(T) == 4) {
-    return 0.5f * erfcf(-z * 0.70710678f);
+    return 0.5f * erfcf(fabsf(z) * 0.70710678f);
   } else {
     const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f * 0.70710678f, fabsf(z), 1.f));
-    const float q = t * e *
-                    fmaf(t, fmaf(t, fmaf(t, fmaf(t, 0.5307027145f, -0.7265760135f), 0.7107068705f), -0.142248368f), 0.127414796f);
-    return z >= 0.f ? 1.f - q : (z < 0.f ? q : z);
+    return t * e *
+           fmaf(t, fmaf(t, fmaf(t, fmaf(t, 0.5307027145f, -0.7265760135f), 0.7107068705f), -0.142248368f), 0.127414796f);
   }
 }
 
@@ -70,7 +70,10 @@ __device__ __forceinline__ float act_value(float z, int act) {
   switch (act) {
     case FW_ACT_RELU: return z > 0.f ? z : (z != z ? z : 0.f);
     case FW_ACT_SILU: return z * sigmoid(z);
-    case FW_ACT_GELU: return z * normal_cdf<T>(z, e);
+    case FW_ACT_GELU: {  // z Phi(z) from the tail on z's own side: no difference of near numbers
+      const float q = normal_tail<T>(z, e);
+      return fmaf(-fminf(fabsf(z), 64.f), q, fmaxf(z, 0.f));  // (an infinity times no tail is no tail)
+    }
     case FW_ACT_TANH: return tanh_fast(z);
   }
   return z;
@@ -85,8 +88,8 @@ __device__ __forceinline__ float act_slope(float z, int act) {
     }
     case FW_ACT_GELU: {
       float e;
-      const float c = normal_cdf<T>(z, e);
-      return fmaf(z * 0.39894228f, e, c);
+      const float q = normal_tail<T>(z, e);
+      return fmaf(z * 0.39894228f, e, z < 0.f ? q : 1.f - q);
     }
     case FW_ACT_TANH: {
       const float t = tanh_fast(z);
@@ -99,6 +102,13 @@ __device__ __forceinline__ float act_slope(float z, int act) {
 __device__ __forceinline__ float inv_sqrt(float x) {
   const float r = __builtin_amdgcn_rsqf(x);
   return x < 1e-30f ? 1.f / sqrtf(x) : r * fmaf(-0.5f * x * r, r, 1.5f);
+}
+
+// (x - mean) r, with shift = -mean r.  A 16-bit x resolves its mean to 2^-12 at best, so the fused form's 2^-24 of
+// mean r is nothing beside x's own half step.
+template <typename T>
+__device__ __forceinline__ float normed(float x, float mean, float r, float shift) {
+  return sizeof(T) == 2 ? fmaf(x, r, shift) : (x - mean) * r;
 }
 
 // ------------------------------------------------------------------ units of a few lanes
@@ -240,25 +250,43 @@ __device__ __forceinline__ void block_sum(float* v, float (*lds)[NV]) {  // ever
   }
 }
 
-// Sums v over the threads of equal column (thread = row * cols + column, `rows` rows), result on row 0.
-template <int VW>
-__device__ __forceinline__ void column_sum(float* v, int t, int rows, int cols, bool on, float* lds) {
+// Per channel (VW of a column, thread = row * cols + column, `rows` rows): the sums of NA values over its rows, in a fixed
+// order, each handed to sink(channel, sums) by one thread.  Many rows: a wave per channel; few: a thread.  (Against a tree
+// over the rows with a barrier a step: map of 64 x 900 x 320 bfloat16, forward 48 -> 41 us.)
+template <int VW, int NA, typename Sink>
+__device__ __forceinline__ void channel_sums(const float (&v)[NA][VW], int t, int rows, int cols, bool on, float* lds, Sink sink) {
+  const int threads = (int)blockDim.x, lane = t & 63;
   __syncthreads();
   if (on)
 #pragma unroll
-    for (int k = 0; k < VW; k++) lds[k * 1024 + t] = v[k];
+    for (int a = 0; a < NA; a++)
+#pragma unroll
+      for (int k = 0; k < VW; k++) lds[(a * VW + k) * threads + t] = v[a][k];
   __syncthreads();
-  while (rows > 1) {
-    const int half = (rows + 1) >> 1;
-    if (on && t < (rows - half) * cols)
+  float s[NA];
+  if (rows >= 32) {
+    for (int ch = __builtin_amdgcn_readfirstlane(t >> 6); ch < cols * VW; ch += threads >> 6) {
 #pragma unroll
-      for (int k = 0; k < VW; k++) lds[k * 1024 + t] += lds[k * 1024 + t + half * cols];
-    rows = half;
-    __syncthreads();
+      for (int a = 0; a < NA; a++) s[a] = 0.f;
+      for (int r = lane; r < rows; r += 64)
+#pragma unroll
+        for (int a = 0; a < NA; a++) s[a] += lds[(a * VW + ch % VW) * threads + r * cols + ch / VW];
+#pragma unroll
+      for (int m = 1; m < 64; m <<= 1)
+#pragma unroll
+        for (int a = 0; a < NA; a++) s[a] += __shfl_xor(s[a], m);
+      if (lane == 0) sink(ch, s);
+    }
+  } else {
+    for (int ch = t; ch < cols * VW; ch += threads) {
+#pragma unroll
+      for (int a = 0; a < NA; a++) s[a] = 0.f;
+      for (int r = 0; r < rows; r++)
+#pragma unroll
+        for (int a = 0; a < NA; a++) s[a] += lds[(a * VW + ch % VW) * threads + r * cols + ch / VW];
+      sink(ch, s);
+    }
   }
-  if (on && t < cols)
-#pragma unroll
-    for (int k = 0; k < VW; k++) v[k] = lds[k * 1024 + t];
 }
 
 // Blocks are dealt to the 8 XCDs in turn; neighbouring groups share memory lines, so they are given to one XCD.
@@ -276,7 +304,7 @@ constexpr int max_hold(bool bwd, int vw) { return vw == 8 ? (bwd ? 6 : 8) : bwd 
 template <typename T, int VW, int VPT, bool BWD>
 __global__ __launch_bounds__(max_threads(BWD, VW)) void k_gn_block(GnArgs A) {
   __shared__ float red[16][2];
-  extern __shared__ float cols[];  // VW * 1024 floats in the backward kernel
+  extern __shared__ float cols[];  // 2 VW floats a thread in the backward kernel
   const int64_t u = xcd_unit(blockIdx.x, A.N * A.G);
   const int64_t n = u / A.G;
   const int g = (int)(u % A.G), t = threadIdx.x;
@@ -294,6 +322,12 @@ __global__ __launch_bounds__(max_threads(BWD, VW)) void k_gn_block(GnArgs A) {
     }
   }
   auto have = [&](int i) { return on && r0 + (int64_t)rp * i < A.L; };
+  float w[VW], b[VW];
+#pragma unroll
+  for (int k = 0; k < VW; k++) {
+    w[k] = param(A.w, A.wdt, c + k, 1.f);
+    b[k] = param(A.b, A.wdt, c + k, 0.f);
+  }
   float v[2] = {0.f, 0.f}, mean, r;
   if (BWD && A.stats) {
     mean = A.stats[2 * u];
@@ -322,61 +356,56 @@ __global__ __launch_bounds__(max_threads(BWD, VW)) void k_gn_block(GnArgs A) {
       A.stats[2 * u + 1] = r;
     }
   }
-  float w[VW], b[VW];
-#pragma unroll
-  for (int k = 0; k < VW; k++) {
-    w[k] = param(A.w, A.wdt, c + k, 1.f);
-    b[k] = param(A.b, A.wdt, c + k, 0.f);
-  }
+  const float shift = -mean * r;
   if constexpr (!BWD) {
+#pragma unroll
+    for (int k = 0; k < VW; k++) {  // z = (x - mean) (r w) + b
+      w[k] *= r;
+      if (sizeof(T) == 2) b[k] = fmaf(-mean, w[k], b[k]);
+    }
 #pragma unroll
     for (int i = 0; i < VPT; i++)
       if (have(i)) {
         float y[VW];
 #pragma unroll
-        for (int k = 0; k < VW; k++) y[k] = act_value<T>(fmaf((to_f32(xv[i].e[k]) - mean) * r, w[k], b[k]), A.act);
+        for (int k = 0; k < VW; k++)
+          y[k] = act_value<T>(fmaf(to_f32(xv[i].e[k]) - (sizeof(T) == 2 ? 0.f : mean), w[k], b[k]), A.act);
         store_vec<T, VW>((T*)A.y.p + n * A.y.sn + (r0 + (int64_t)rp * i) * A.y.sl + c, y);
       }
   } else {
-    float dw[VW], db[VW], d[VPT][VW];
+    float sum[2][VW], d[VPT][VW];  // of dweight and dbias
 #pragma unroll
-    for (int k = 0; k < VW; k++) dw[k] = db[k] = 0.f;
+    for (int k = 0; k < VW; k++) sum[0][k] = sum[1][k] = 0.f;
     v[0] = v[1] = 0.f;
 #pragma unroll
     for (int i = 0; i < VPT; i++)
       if (have(i))
 #pragma unroll
         for (int k = 0; k < VW; k++) {
-          const float xh = (to_f32(xv[i].e[k]) - mean) * r;
+          const float xh = normed<T>(to_f32(xv[i].e[k]), mean, r, shift);
           const float dz = to_f32(dv[i].e[k]) * act_slope<T>(fmaf(xh, w[k], b[k]), A.act);
-          db[k] += dz;
-          dw[k] = fmaf(dz, xh, dw[k]);
+          sum[1][k] += dz;
+          sum[0][k] = fmaf(dz, xh, sum[0][k]);
           d[i][k] = dz * w[k];
           v[0] += d[i][k];
           v[1] = fmaf(d[i][k], xh, v[1]);
         }
     block_sum<2>(v, red);
-    const float s1 = v[0] * inv, s2 = v[1] * inv;
+    const float s1 = -r * (v[0] * inv), s2 = -r * (v[1] * inv);
 #pragma unroll
     for (int i = 0; i < VPT; i++)
       if (have(i)) {
         float y[VW];
 #pragma unroll
-        for (int k = 0; k < VW; k++) y[k] = r * (d[i][k] - s1 - (to_f32(xv[i].e[k]) - mean) * r * s2);
+        for (int k = 0; k < VW; k++)
+          y[k] = fmaf(d[i][k], r, fmaf(normed<T>(to_f32(xv[i].e[k]), mean, r, shift), s2, s1));
         store_vec<T, VW>((T*)A.dx.p + n * A.dx.sn + (r0 + (int64_t)rp * i) * A.dx.sl + c, y);
       }
-    if (A.dw) {
-      column_sum<VW>(dw, t, rp, cgv, on, cols);
-      if (t < cgv)
-#pragma unroll
-        for (int k = 0; k < VW; k++) A.dw[u * A.cg + col + k] = dw[k];
-    }
-    if (A.db) {
-      column_sum<VW>(db, t, rp, cgv, on, cols);
-      if (t < cgv)
-#pragma unroll
-        for (int k = 0; k < VW; k++) A.db[u * A.cg + col + k] = db[k];
-    }
+    if (A.dw || A.db)
+      channel_sums<VW, 2>(sum, t, rp, cgv, on, cols, [&](int ch, const float* s) {
+        if (A.dw) A.dw[u * A.cg + ch] = s[0];
+        if (A.db) A.db[u * A.cg + ch] = s[1];
+      });
   }
 }
 
@@ -387,7 +416,7 @@ __global__ __launch_bounds__(max_threads(BWD, VW)) void k_gn_block(GnArgs A) {
 template <typename T, int VPT, bool BWD>
 __global__ __launch_bounds__(max_threads(BWD, 16 / sizeof(T))) void k_gn_bundle(GnArgs A, int bundle) {
   constexpr int VW = 16 / sizeof(T);
-  extern __shared__ float lds[];  // VW * 1024 for the column sums
+  extern __shared__ float lds[];  // VW (backward 2 VW) floats a thread
   __shared__ float chan[2][1024], group[2][64];
   const int64_t u = xcd_unit(blockIdx.x, A.N * A.G / bundle);
   const int64_t n = u / (A.G / bundle);
@@ -408,21 +437,29 @@ __global__ __launch_bounds__(max_threads(BWD, 16 / sizeof(T))) void k_gn_bundle(
   int gi[VW];
 #pragma unroll
   for (int k = 0; k < VW; k++) gi[k] = (col + k) / A.cg;
-  // per group, on every thread: the sum over the group's channels of v's sums over the rows, times scale[channel]
-  auto group_sums = [&](float* v, int which, const float* scale) {
-    column_sum<VW>(v, t, rp, cols, on, lds);
-    if (t < cols)
+  // the channels' sums, and on every thread the groups' from them (weighted: of w times the channel's)
+  auto group_sums = [&](const auto& v, int first, bool weighted) {
+    constexpr int NA = std::extent_v<std::remove_reference_t<decltype(v)>, 0>;
+    channel_sums<VW, NA>(v, t, rp, cols, on, lds, [&](int ch, const float* s) {
 #pragma unroll
-      for (int k = 0; k < VW; k++) chan[which][col + k] = scale ? v[k] * scale[k] : v[k];
+      for (int a = 0; a < NA; a++) chan[first + a][ch] = s[a];
+    });
     __syncthreads();
-    if (t < bundle) {
+    if (t < bundle * NA) {
+      const int a = first + t / bundle, g = t % bundle;
       float s = 0.f;
-      for (int k = 0; k < A.cg; k++) s += chan[which][t * A.cg + k];
-      group[which][t] = s;
+      for (int k = g * A.cg; k < (g + 1) * A.cg; k++)
+        s = fmaf(chan[a][k], weighted ? param(A.w, A.wdt, g0 * A.cg + k, 1.f) : 1.f, s);
+      group[a][g] = s;
     }
     __syncthreads();
   };
-  float v[VW], mean[VW], r[VW], w[VW], b[VW];
+  float v[1][VW], mean[VW], r[VW], w[VW], b[VW];
+#pragma unroll
+  for (int k = 0; k < VW; k++) {
+    w[k] = param(A.w, A.wdt, c + k, 1.f);
+    b[k] = param(A.b, A.wdt, c + k, 0.f);
+  }
   if (BWD && A.stats) {
 #pragma unroll
     for (int k = 0; k < VW; k++) {
@@ -431,17 +468,17 @@ __global__ __launch_bounds__(max_threads(BWD, 16 / sizeof(T))) void k_gn_bundle(
     }
   } else {
 #pragma unroll
-    for (int k = 0; k < VW; k++) v[k] = 0.f;
+    for (int k = 0; k < VW; k++) v[0][k] = 0.f;
 #pragma unroll
     for (int i = 0; i < VPT; i++)
       if (have(i))
 #pragma unroll
-        for (int k = 0; k < VW; k++) v[k] += to_f32(xv[i].e[k]);
-    group_sums(v, 0, nullptr);
+        for (int k = 0; k < VW; k++) v[0][k] += to_f32(xv[i].e[k]);
+    group_sums(v, 0, false);
 #pragma unroll
     for (int k = 0; k < VW; k++) {
       mean[k] = group[0][gi[k]] * inv;
-      v[k] = 0.f;
+      v[0][k] = 0.f;
     }
 #pragma unroll
     for (int i = 0; i < VPT; i++)
@@ -449,9 +486,9 @@ __global__ __launch_bounds__(max_threads(BWD, 16 / sizeof(T))) void k_gn_bundle(
 #pragma unroll
         for (int k = 0; k < VW; k++) {
           const float d = to_f32(xv[i].e[k]) - mean[k];
-          v[k] = fmaf(d, d, v[k]);
+          v[0][k] = fmaf(d, d, v[0][k]);
         }
-    group_sums(v, 1, nullptr);
+    group_sums(v, 1, false);
 #pragma unroll
     for (int k = 0; k < VW; k++) r[k] = inv_sqrt(group[1][gi[k]] * inv + A.eps);
     if (A.stats && t < bundle) {
@@ -459,51 +496,57 @@ __global__ __launch_bounds__(max_threads(BWD, 16 / sizeof(T))) void k_gn_bundle(
       A.stats[2 * (n * A.G + g0 + t) + 1] = inv_sqrt(group[1][t] * inv + A.eps);
     }
   }
-#pragma unroll
-  for (int k = 0; k < VW; k++) {
-    w[k] = param(A.w, A.wdt, c + k, 1.f);
-    b[k] = param(A.b, A.wdt, c + k, 0.f);
-  }
   if constexpr (!BWD) {
+#pragma unroll
+    for (int k = 0; k < VW; k++) {  // z = (x - mean) (r w) + b
+      w[k] *= r[k];
+      if (sizeof(T) == 2) b[k] = fmaf(-mean[k], w[k], b[k]);
+    }
 #pragma unroll
     for (int i = 0; i < VPT; i++)
       if (have(i)) {
         float y[VW];
 #pragma unroll
-        for (int k = 0; k < VW; k++) y[k] = act_value<T>(fmaf((to_f32(xv[i].e[k]) - mean[k]) * r[k], w[k], b[k]), A.act);
+        for (int k = 0; k < VW; k++)
+          y[k] = act_value<T>(fmaf(to_f32(xv[i].e[k]) - (sizeof(T) == 2 ? 0.f : mean[k]), w[k], b[k]), A.act);
         store_vec<T, VW>((T*)A.y.p + n * A.y.sn + (r0 + (int64_t)rp * i) * A.y.sl + c, y);
       }
   } else {
-    float dw[VW], db[VW], d[VPT][VW];
+    float sum[2][VW], shift[VW], d[VPT][VW];  // of dbias and dweight
 #pragma unroll
-    for (int k = 0; k < VW; k++) dw[k] = db[k] = 0.f;
+    for (int k = 0; k < VW; k++) {
+      sum[0][k] = sum[1][k] = 0.f;
+      shift[k] = -mean[k] * r[k];
+    }
 #pragma unroll
     for (int i = 0; i < VPT; i++)
       if (have(i))
 #pragma unroll
         for (int k = 0; k < VW; k++) {
-          const float xh = (to_f32(xv[i].e[k]) - mean[k]) * r[k];
+          const float xh = normed<T>(to_f32(xv[i].e[k]), mean[k], r[k], shift[k]);
           d[i][k] = to_f32(dv[i].e[k]) * act_slope<T>(fmaf(xh, w[k], b[k]), A.act);
-          db[k] += d[i][k];
-          dw[k] = fmaf(d[i][k], xh, dw[k]);
+          sum[0][k] += d[i][k];
+          sum[1][k] = fmaf(d[i][k], xh, sum[1][k]);
         }
-    group_sums(db, 0, w);  // sum dxh = sum w db, sum dxh xh = sum w dw
-    group_sums(dw, 1, w);
-    if (t < cols)
+    group_sums(sum, 0, true);  // sum dxh = sum w db, sum dxh xh = sum w dw
+    for (int ch = t; ch < width; ch += (int)blockDim.x) {
+      if (A.db) A.db[n * A.G * A.cg + g0 * A.cg + ch] = chan[0][ch];
+      if (A.dw) A.dw[n * A.G * A.cg + g0 * A.cg + ch] = chan[1][ch];
+    }
+    float s1[VW], s2[VW];
 #pragma unroll
-      for (int k = 0; k < VW; k++) {
-        if (A.dw) A.dw[n * A.G * A.cg + c + k] = dw[k];
-        if (A.db) A.db[n * A.G * A.cg + c + k] = db[k];
-      }
+    for (int k = 0; k < VW; k++) {
+      s1[k] = -r[k] * (group[0][gi[k]] * inv);
+      s2[k] = -r[k] * (group[1][gi[k]] * inv);
+      w[k] *= r[k];
+    }
 #pragma unroll
     for (int i = 0; i < VPT; i++)
       if (have(i)) {
         float y[VW];
 #pragma unroll
-        for (int k = 0; k < VW; k++) {
-          const float xh = (to_f32(xv[i].e[k]) - mean[k]) * r[k];
-          y[k] = r[k] * (d[i][k] * w[k] - group[0][gi[k]] * inv - xh * (group[1][gi[k]] * inv));
-        }
+        for (int k = 0; k < VW; k++)
+          y[k] = fmaf(d[i][k], w[k], fmaf(normed<T>(to_f32(xv[i].e[k]), mean[k], r[k], shift[k]), s2[k], s1[k]));
         store_vec<T, VW>((T*)A.dx.p + n * A.dx.sn + (r0 + (int64_t)rp * i) * A.dx.sl + c, y);
       }
   }
@@ -672,6 +715,7 @@ __global__ __launch_bounds__(256) void k_gn_stream_apply(GnArgs A) {
       m[k] = A.stats[2 * g];
       w[k] = A.stats[2 * g + 1] * param(A.w, A.wdt, c + k, 1.f);
       b[k] = param(A.b, A.wdt, c + k, 0.f);
+      if (sizeof(T) == 2) b[k] = fmaf(-m[k], w[k], b[k]);
     }
     const T* x = (const T*)A.x.p + p.n * A.x.sn + c;
     T* y = (T*)A.y.p + p.n * A.y.sn + c;
@@ -684,7 +728,8 @@ __global__ __launch_bounds__(256) void k_gn_stream_apply(GnArgs A) {
       for (int i = 0; i < B; i++)
         if (l + (int64_t)at.rp * i < p.l1) {
 #pragma unroll
-          for (int k = 0; k < VW; k++) v[i][k] = act_value<T>(fmaf(v[i][k] - m[k], w[k], b[k]), A.act);
+          for (int k = 0; k < VW; k++)
+            v[i][k] = act_value<T>(fmaf(v[i][k] - (sizeof(T) == 2 ? 0.f : m[k]), w[k], b[k]), A.act);
           store_vec<T, VW>(y + (l + (int64_t)at.rp * i) * A.y.sl, v[i]);
         }
     }
@@ -947,14 +992,14 @@ int launch(const GnArgs& A, const Plan& p, hipStream_t s) {
     else
       hipLaunchKernelGGL((k_gn_wave<T, VW, 4, BWD>), grid, dim3(256), lds, s, A);
   } else if (p.kind == BLOCK) {
-    const size_t lds = BWD ? VW * 1024 * sizeof(float) : 0;
+    const size_t lds = BWD ? 2 * VW * p.threads * sizeof(float) : 0;  // at most 48 KB
     constexpr int HOLD = max_hold(BWD, VW);
     if (p.per < HOLD)
       hipLaunchKernelGGL((k_gn_block<T, VW, HOLD / 2, BWD>), grid, dim3(p.threads), lds, s, A);
     else
       hipLaunchKernelGGL((k_gn_block<T, VW, HOLD, BWD>), grid, dim3(p.threads), lds, s, A);
   } else if (p.kind == BUNDLE) {
-    const size_t lds = 16 / sizeof(T) * 1024 * sizeof(float);
+    const size_t lds = (BWD ? 2 : 1) * 16 / sizeof(T) * p.threads * sizeof(float);  // at most 48 KB
     constexpr int HOLD = BWD && sizeof(T) == 2 ? 6 : 8;
     if (p.per < HOLD)
       hipLaunchKernelGGL((k_gn_bundle<T, HOLD / 2, BWD>), grid, dim3(p.threads), lds, s, A, p.bundle);
