@@ -1234,9 +1234,11 @@ __global__ __launch_bounds__(256) void k_token_narrow(TokenArgs A) {
 // ------------------------------------------------------------------ host side
 int tiles(int d) { return d <= 16 ? 1 : d <= 32 ? 2 : d <= 64 ? 4 : 8; }
 // value tiles of one wave: the state is KT x VT tiles of registers
-int slice_tiles(int dtype, int Dk, int Dv) { return std::min(tiles(Dv), dtype == FW_DT_BF16 && tiles(Dk) == 8 ? 2 : 4); }
-int slices(int dtype, int Dk, int Dv) {
-  const int cols = 16 * slice_tiles(dtype, Dk, Dv);
+int slice_tiles(int dtype, int Dk, int Dv, bool narrow) {
+  return narrow ? 1 : std::min(tiles(Dv), dtype == FW_DT_BF16 && tiles(Dk) == 8 ? 2 : 4);
+}
+int slices(int dtype, int Dk, int Dv, bool narrow) {
+  const int cols = 16 * slice_tiles(dtype, Dk, Dv, narrow);
   return (Dv + cols - 1) / cols;
 }
 
@@ -1245,18 +1247,22 @@ int slices(int dtype, int Dk, int Dv) {
 // Two segments cost more than they bring unless all their waves have a SIMD each (measured, us; 1000 waves of 500 tokens:
 // 1 segment 111 forward and 250 backward, 2 segments 125 and 291; 400 waves of 512, backward: 1 segment 75, 2: 102, 4: 111;
 // 256 waves of 2048: forward 4 segments 109, 8: 104, backward 4 segments 213, 8: 251).
+// Where one segment is left and there are few waves still, each takes one tile of value columns, as long as each has a
+// SIMD to itself: its blocks are then shorter (100 tokens of 4 heads of 64 x 64 bfloat16: 16.6 -> 11 us).
 constexpr int SEG_WAVES = 2048;
 constexpr int SEG_MIN = 128;  // tokens
 struct Plan {
   int64_t seg_len;
   int n_seg;
+  bool narrow;
 };
 Plan plan(int dtype, int64_t T, int64_t N, int H, int Dk, int Dv, bool backward) {
-  const int64_t waves = std::max<int64_t>(1, N * H * slices(dtype, Dk, Dv));
+  const int64_t waves = std::max<int64_t>(1, N * H * slices(dtype, Dk, Dv, false));
+  const int64_t most = N * H * (backward ? slices(dtype, Dk, Dv, true) + 2 * slices(dtype, Dv, Dk, true) : slices(dtype, Dk, Dv, true));
   const int64_t segs = std::min<int64_t>((backward ? SEG_WAVES / 2 : SEG_WAVES) / waves, T / SEG_MIN);
-  if (segs < 2 || (segs == 2 && (backward ? 3 : 1) * 2 * waves > SEG_WAVES / 2)) return {std::max<int64_t>(T, 1), 1};
+  if (segs < 2 || (segs == 2 && (backward ? 3 : 1) * 2 * waves > SEG_WAVES / 2)) return {std::max<int64_t>(T, 1), 1, most <= SEG_WAVES / 2};
   const int64_t len = ((T + segs - 1) / segs + 31) / 32 * 32;
-  return {len, (int)((T + len - 1) / len)};
+  return {len, (int)((T + len - 1) / len), false};
 }
 int quads(int Dk) { return (Dk + 3) / 4 * 4; }
 // a state per segment and what a segment multiplies a state with; the backward pass has two directions of them
@@ -1320,13 +1326,13 @@ int launch_scan(ScanArgs A, int kt, int vt, hipStream_t s) {
 }
 
 // Passes of equal tiles and slices go in one launch.
-int launch_passes(int dtype, ScanArgs A, const Pass* pass, int n_pass, hipStream_t s) {
+int launch_passes(int dtype, bool narrow, ScanArgs A, const Pass* pass, int n_pass, hipStream_t s) {
   for (int i = 0; i < n_pass; i += A.n_pass) {
-    const int kt = tiles(pass[i].Dk), vt = slice_tiles(dtype, pass[i].Dk, pass[i].Dv);
-    A.n_slice = slices(dtype, pass[i].Dk, pass[i].Dv);
+    const int kt = tiles(pass[i].Dk), vt = slice_tiles(dtype, pass[i].Dk, pass[i].Dv, narrow);
+    A.n_slice = slices(dtype, pass[i].Dk, pass[i].Dv, narrow);
     A.n_pass = 0;
-    for (int j = i; j < n_pass && tiles(pass[j].Dk) == kt && slice_tiles(dtype, pass[j].Dk, pass[j].Dv) == vt &&
-                    slices(dtype, pass[j].Dk, pass[j].Dv) == A.n_slice; j++)
+    for (int j = i; j < n_pass && tiles(pass[j].Dk) == kt && slice_tiles(dtype, pass[j].Dk, pass[j].Dv, narrow) == vt &&
+                    slices(dtype, pass[j].Dk, pass[j].Dv, narrow) == A.n_slice; j++)
       A.pass[A.n_pass++] = pass[j];
     const int rc = dtype == FW_DT_F32    ? launch_scan<float>(A, kt, vt, s)
                    : dtype == FW_DT_BF16 ? launch_scan<bf16>(A, kt, vt, s)
@@ -1343,7 +1349,7 @@ int segment_states(int dtype, ScanArgs A, const Pass* add, const State* in, int 
   const int64_t E = (int64_t)quads(Dk) * Dv;
   A.factor = ws + dirs * A.N * A.H * A.n_seg * E;
   A.run_seg = A.n_seg - 1;  // the last segment adds to nothing
-  if (int rc = launch_passes(dtype, A, add, dirs, s)) return rc;
+  if (int rc = launch_passes(dtype, false, A, add, dirs, s)) return rc;
   JoinArgs J{};
   for (int d = 0; d < dirs; d++) J.in[d] = in[d];
   J.ws = ws;
@@ -1434,7 +1440,7 @@ int fw_linattn_forward(const fw_linattn* a, void* stream) {
     if (int rc = segment_states(a->dtype, A, &add, &p.in, 1, ws, s)) return rc;
     p.in = seg;
   }
-  return launch_passes(a->dtype, A, &p, 1, s);
+  return launch_passes(a->dtype, pl.narrow, A, &p, 1, s);
 }
 
 int fw_linattn_backward(const fw_linattn* a, void* stream) {
@@ -1460,7 +1466,7 @@ int fw_linattn_backward(const fw_linattn* a, void* stream) {
       {in(a, a->dout), in(a, a->v), in(a, a->k), in(a, a->dq), turned(S), State{}, 0, a->Dv, a->Dk},
       {in(a, a->v), in(a, a->dout), in(a, a->q), in(a, a->dk), turned(R), State{}, 1, a->Dv, a->Dk},
       {in(a, a->k), in(a, a->q), in(a, a->dout), in(a, a->dv), R, straight(a, a->dstate_in), 1, a->Dk, a->Dv}};
-  return launch_passes(a->dtype, A, main, 3, s);
+  return launch_passes(a->dtype, pl.narrow, A, main, 3, s);
 }
 
 int fw_linattn_step(const fw_linattn_token* a, void* stream_) {
