@@ -1,8 +1,9 @@
 // fw_sequence.hip -- linear attention with a decay per head over rollout columns (include/fwrollout.h):
 //
 //   k_scan        one wave runs one sequence, head and slice of value columns through time in blocks of C tokens
+//   k_scan16      the same on the 16-bit matrix products (bfloat16)
 //   k_scan_join   joins the states of time segments when there are few sequences
-//   k_token       the single-token form: reads the state once, writes it once
+//   k_token       the single-token form: reads the state once, writes it once (k_token_narrow: fewer than 4 columns)
 //
 // The mathematics.  With g = exp(log_decay) and S the state before a block of C tokens,
 //   out_t = g^(t+1) S^T q_t + sum_{s<=t} g^(t-s) (q_t . k_s) v_s        S <- g^C S + sum_s g^(C-1-s) k_s v_s^T
@@ -20,7 +21,7 @@ using namespace fwseq;
 namespace {
 
 constexpr int MAXDIM = 128;
-constexpr int SCAN_WAVES = 4;  // waves per block; each is on its own (no barrier, no LDS)
+constexpr int SCAN_WAVES = 4;  // waves per block; each is on its own, with its own share of LDS and no barrier
 
 struct Operand {
   const void* p;
@@ -327,6 +328,12 @@ __device__ __forceinline__ f32x4 mma(float a, float b, f32x4 c) {
 // O[f] = out^T: value columns down the rows, tokens along the columns.
 // Blocks are copied to LDS by the load unit, NB of them ahead (no registers; the wait is for the oldest alone), in
 // processing order, so that a reversed pass is causal too: its rows run from the last token to the first.
+//
+// float32 runs here because its products have to be float32; float16 because its states leave its range.  A wave owns a
+// sequence rather than a block of tokens because the recurrence then never leaves its registers.  Small heads are bound
+// by memory: 2048 tokens x 512 x 4 heads of 16 x 16, 287 us, 3750 GB/s (403 us with the loads by way of registers, none
+// ahead).  Larger ones are bound by the products, which a padded head wastes: 500 x 250 x 4 heads of 20 x 40 in tiles of
+// 32 x 64, 112 us.
 template <typename T, int KT, int VT>
 struct Ring {
   using K = Tile<T, KT, 16>;
@@ -658,6 +665,12 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, KT * VT <= 16 ? 2 : 1) void k_scan
 // Products of the inputs are exact in the float32 accumulators.  What is not an input is split into bfloat16 terms:
 // weighted scores and the state into two (2^-16 of a term, far below the output's own half step), the weighted operand
 // of the state's product into three (exact to float32: the state is a float32 result).
+//
+// 32 tokens a block: the depth of the product, and half as many splits of the state per token as 16.  Measured at 16
+// heads of 128 x 128 over 16384 tokens: 88 us of outputs after 57 us of segment states (on the float32 products 460 us in
+// all).  In the 88 us the matrix units are busy for 30 % of the time and issue 3.3 million products beside 22 million
+// vector instructions, the splits and weights; two waves a SIMD hide what they wait for only in part.  Three (the outputs
+// in the values' room), the copies given out between the products, and splits by dot products were no faster.
 __device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
@@ -1016,7 +1029,8 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, 2) void k_scan16(ScanArgs A) {
 
 // ws[seg] holds what segment seg adds to a state; rewritten as the state that enters segment seg:
 //   c_0 = in;  c_{s+1} = factor_s c_s + ws_s
-// One thread per four keys of a value column; the loads of all segments are independent of the recurrence.
+// One thread per four keys of a value column; the loads of all segments are independent of the recurrence.  Bound by
+// memory: 32 segments of 16 heads of 128 x 128, 34 MB in and out, 14 us.
 struct JoinArgs {
   State in[2];  // p NULL: zeros
   float* ws;    // [dirs][N][H][n_seg][ceil(Dk / 4)][Dv][4]
@@ -1234,11 +1248,11 @@ __global__ __launch_bounds__(256) void k_token_narrow(TokenArgs A) {
 // ------------------------------------------------------------------ host side
 int tiles(int d) { return d <= 16 ? 1 : d <= 32 ? 2 : d <= 64 ? 4 : 8; }
 // value tiles of one wave: the state is KT x VT tiles of registers
-int slice_tiles(int dtype, int Dk, int Dv, bool narrow) {
-  return narrow ? 1 : std::min(tiles(Dv), dtype == FW_DT_BF16 && tiles(Dk) == 8 ? 2 : 4);
+int slice_tiles(int dtype, int Dk, int Dv, int most) {
+  return std::min({most, tiles(Dv), dtype == FW_DT_BF16 && tiles(Dk) == 8 ? 2 : 4});
 }
-int slices(int dtype, int Dk, int Dv, bool narrow) {
-  const int cols = 16 * slice_tiles(dtype, Dk, Dv, narrow);
+int slices(int dtype, int Dk, int Dv, int most) {
+  const int cols = 16 * slice_tiles(dtype, Dk, Dv, most);
   return (Dv + cols - 1) / cols;
 }
 
@@ -1247,22 +1261,30 @@ int slices(int dtype, int Dk, int Dv, bool narrow) {
 // Two segments cost more than they bring unless all their waves have a SIMD each (measured, us; 1000 waves of 500 tokens:
 // 1 segment 111 forward and 250 backward, 2 segments 125 and 291; 400 waves of 512, backward: 1 segment 75, 2: 102, 4: 111;
 // 256 waves of 2048: forward 4 segments 109, 8: 104, backward 4 segments 213, 8: 251).
-// Where one segment is left and there are few waves still, each takes one tile of value columns, as long as each has a
-// SIMD to itself: its blocks are then shorter (100 tokens of 4 heads of 64 x 64 bfloat16: 16.6 -> 11 us).
+// Where one segment is left, a wave takes fewer value columns as long as each wave has a SIMD to itself (two waves a SIMD
+// with two tiles of float32 products, which are further from the memory's rate): its blocks are shorter and the scores
+// are computed once more per slice.  100 tokens of 4 heads of 64 x 64 bfloat16, one tile against four: 11 against 17 us;
+// 500 x 250 x 4 heads of 20 x 40 float32, two against four: 88 against 102; one against two at 1680 waves: 112 against 100.
 constexpr int SEG_WAVES = 2048;
 constexpr int SEG_MIN = 128;  // tokens
 struct Plan {
   int64_t seg_len;
   int n_seg;
-  bool narrow;
+  int tiles;  // of value columns per wave, at most
 };
 Plan plan(int dtype, int64_t T, int64_t N, int H, int Dk, int Dv, bool backward) {
-  const int64_t waves = std::max<int64_t>(1, N * H * slices(dtype, Dk, Dv, false));
-  const int64_t most = N * H * (backward ? slices(dtype, Dk, Dv, true) + 2 * slices(dtype, Dv, Dk, true) : slices(dtype, Dk, Dv, true));
+  const int64_t waves = std::max<int64_t>(1, N * H * slices(dtype, Dk, Dv, 4));
   const int64_t segs = std::min<int64_t>((backward ? SEG_WAVES / 2 : SEG_WAVES) / waves, T / SEG_MIN);
-  if (segs < 2 || (segs == 2 && (backward ? 3 : 1) * 2 * waves > SEG_WAVES / 2)) return {std::max<int64_t>(T, 1), 1, most <= SEG_WAVES / 2};
+  if (segs < 2 || (segs == 2 && (backward ? 3 : 1) * 2 * waves > SEG_WAVES / 2)) {
+    int vt = 1;
+    for (; vt < 4; vt *= 2) {
+      const int n = backward ? slices(dtype, Dk, Dv, vt) + 2 * slices(dtype, Dv, Dk, vt) : slices(dtype, Dk, Dv, vt);
+      if (N * H * n <= (vt == 2 && dtype != FW_DT_BF16 ? SEG_WAVES : SEG_WAVES / 2)) break;
+    }
+    return {std::max<int64_t>(T, 1), 1, vt};
+  }
   const int64_t len = ((T + segs - 1) / segs + 31) / 32 * 32;
-  return {len, (int)((T + len - 1) / len), false};
+  return {len, (int)((T + len - 1) / len), 4};
 }
 int quads(int Dk) { return (Dk + 3) / 4 * 4; }
 // a state per segment and what a segment multiplies a state with; the backward pass has two directions of them
@@ -1326,13 +1348,13 @@ int launch_scan(ScanArgs A, int kt, int vt, hipStream_t s) {
 }
 
 // Passes of equal tiles and slices go in one launch.
-int launch_passes(int dtype, bool narrow, ScanArgs A, const Pass* pass, int n_pass, hipStream_t s) {
+int launch_passes(int dtype, int most, ScanArgs A, const Pass* pass, int n_pass, hipStream_t s) {
   for (int i = 0; i < n_pass; i += A.n_pass) {
-    const int kt = tiles(pass[i].Dk), vt = slice_tiles(dtype, pass[i].Dk, pass[i].Dv, narrow);
-    A.n_slice = slices(dtype, pass[i].Dk, pass[i].Dv, narrow);
+    const int kt = tiles(pass[i].Dk), vt = slice_tiles(dtype, pass[i].Dk, pass[i].Dv, most);
+    A.n_slice = slices(dtype, pass[i].Dk, pass[i].Dv, most);
     A.n_pass = 0;
-    for (int j = i; j < n_pass && tiles(pass[j].Dk) == kt && slice_tiles(dtype, pass[j].Dk, pass[j].Dv, narrow) == vt &&
-                    slices(dtype, pass[j].Dk, pass[j].Dv, narrow) == A.n_slice; j++)
+    for (int j = i; j < n_pass && tiles(pass[j].Dk) == kt && slice_tiles(dtype, pass[j].Dk, pass[j].Dv, most) == vt &&
+                    slices(dtype, pass[j].Dk, pass[j].Dv, most) == A.n_slice; j++)
       A.pass[A.n_pass++] = pass[j];
     const int rc = dtype == FW_DT_F32    ? launch_scan<float>(A, kt, vt, s)
                    : dtype == FW_DT_BF16 ? launch_scan<bf16>(A, kt, vt, s)
@@ -1349,7 +1371,7 @@ int segment_states(int dtype, ScanArgs A, const Pass* add, const State* in, int 
   const int64_t E = (int64_t)quads(Dk) * Dv;
   A.factor = ws + dirs * A.N * A.H * A.n_seg * E;
   A.run_seg = A.n_seg - 1;  // the last segment adds to nothing
-  if (int rc = launch_passes(dtype, false, A, add, dirs, s)) return rc;
+  if (int rc = launch_passes(dtype, 4, A, add, dirs, s)) return rc;
   JoinArgs J{};
   for (int d = 0; d < dirs; d++) J.in[d] = in[d];
   J.ws = ws;
@@ -1440,7 +1462,7 @@ int fw_linattn_forward(const fw_linattn* a, void* stream) {
     if (int rc = segment_states(a->dtype, A, &add, &p.in, 1, ws, s)) return rc;
     p.in = seg;
   }
-  return launch_passes(a->dtype, pl.narrow, A, &p, 1, s);
+  return launch_passes(a->dtype, pl.tiles, A, &p, 1, s);
 }
 
 int fw_linattn_backward(const fw_linattn* a, void* stream) {
@@ -1466,7 +1488,7 @@ int fw_linattn_backward(const fw_linattn* a, void* stream) {
       {in(a, a->dout), in(a, a->v), in(a, a->k), in(a, a->dq), turned(S), State{}, 0, a->Dv, a->Dk},
       {in(a, a->v), in(a, a->dout), in(a, a->q), in(a, a->dk), turned(R), State{}, 1, a->Dv, a->Dk},
       {in(a, a->k), in(a, a->q), in(a, a->dout), in(a, a->dv), R, straight(a, a->dstate_in), 1, a->Dk, a->Dv}};
-  return launch_passes(a->dtype, pl.narrow, A, main, 3, s);
+  return launch_passes(a->dtype, pl.tiles, A, main, 3, s);
 }
 
 int fw_linattn_step(const fw_linattn_token* a, void* stream_) {
