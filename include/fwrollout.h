@@ -202,12 +202,15 @@ typedef struct fw_seq_tensor {
  *   out_t = S_t^T q_t                                       state_out = S_{len-1}
  * for t < len = clamp(lengths[n], 0, T) (NULL: T); out rows t >= len are written as zeros.
  * state_in / state_out: float [N][H][Dk][Dv], contiguous; they may be the same buffer.
- * log_decay: float [H] (<= 0 for a decay).  starts: uint8 with element strides, or NULL.
+ * log_decay: float [H] (<= 0 for a decay; -infinity: g = 0).  starts: uint8 with element strides, 0 <= starts_st < 2^26,
+ * or NULL.
  * Backward (fw_linattn_backward): given dout and dstate (the gradient of state_out, NULL: zeros) writes
  * dq, dk, dv (rows t >= len: zeros) and dstate_in (may be NULL); q, k, v are read again, no state is
  * kept from the forward call.  Limits: 1 <= Dk, Dv <= 128.  A non-finite input reaches exactly the
  * outputs the recurrence would let it reach; there it comes out as an infinity or a NaN.
- * workspace: fw_linattn_workspace_bytes(...) bytes of device memory (may be 0), used on `stream`. */
+ * workspace: fw_linattn_workspace_bytes(...) bytes of device memory (may be 0), 16-byte aligned, used on `stream`;
+ * calls that may run at the same time need their own.  At most 2^24 blocks of four waves, one wave per sequence, head
+ * and slice of value columns, in a call. */
 typedef struct fw_linattn {
   int64_t T, N;
   int32_t H, Dk, Dv, dtype;
@@ -252,7 +255,8 @@ int fw_linattn_step(const fw_linattn_token* a, void* stream);
  * (dtype or float32), either may be NULL (1 / 0).  Statistics are float32, by deviations from the mean.
  * Backward: dx, and dweight, dbias [C] of wdtype (either may be NULL), summed in a fixed order.
  * stats: float [N][G][2] (m, r), written by the forward call and read by the backward call; it is needed where
- * fw_group_norm_stats says 1 (elsewhere NULL: the statistics are rebuilt from x, which is in registers anyway). */
+ * fw_group_norm_stats says 1 (elsewhere NULL: the statistics are rebuilt from x, which is in registers anyway).  A
+ * forward call needs a workspace only where fw_group_norm_stats says 1.  At most 2^32 threads in a call. */
 #define FW_ACT_NONE 0
 #define FW_ACT_RELU 1
 #define FW_ACT_SILU 2
