@@ -1261,30 +1261,18 @@ int slices(int dtype, int Dk, int Dv, int most) {
 // Two segments cost more than they bring unless all their waves have a SIMD each (measured, us; 1000 waves of 500 tokens:
 // 1 segment 111 forward and 250 backward, 2 segments 125 and 291; 400 waves of 512, backward: 1 segment 75, 2: 102, 4: 111;
 // 256 waves of 2048: forward 4 segments 109, 8: 104, backward 4 segments 213, 8: 251).
-// Where one segment is left, a wave takes fewer value columns as long as each wave has a SIMD to itself (two waves a SIMD
-// with two tiles of float32 products, which are further from the memory's rate): its blocks are shorter and the scores
-// are computed once more per slice.  100 tokens of 4 heads of 64 x 64 bfloat16, one tile against four: 11 against 17 us;
-// 500 x 250 x 4 heads of 20 x 40 float32, two against four: 88 against 102; one against two at 1680 waves: 112 against 100.
 constexpr int SEG_WAVES = 2048;
 constexpr int SEG_MIN = 128;  // tokens
 struct Plan {
   int64_t seg_len;
   int n_seg;
-  int tiles;  // of value columns per wave, at most
 };
 Plan plan(int dtype, int64_t T, int64_t N, int H, int Dk, int Dv, bool backward) {
   const int64_t waves = std::max<int64_t>(1, N * H * slices(dtype, Dk, Dv, 4));
   const int64_t segs = std::min<int64_t>((backward ? SEG_WAVES / 2 : SEG_WAVES) / waves, T / SEG_MIN);
-  if (segs < 2 || (segs == 2 && (backward ? 3 : 1) * 2 * waves > SEG_WAVES / 2)) {
-    int vt = 1;
-    for (; vt < 4; vt *= 2) {
-      const int n = backward ? slices(dtype, Dk, Dv, vt) + 2 * slices(dtype, Dv, Dk, vt) : slices(dtype, Dk, Dv, vt);
-      if (N * H * n <= (vt == 2 && dtype != FW_DT_BF16 ? SEG_WAVES : SEG_WAVES / 2)) break;
-    }
-    return {std::max<int64_t>(T, 1), 1, vt};
-  }
+  if (segs < 2 || (segs == 2 && (backward ? 3 : 1) * 2 * waves > SEG_WAVES / 2)) return {std::max<int64_t>(T, 1), 1};
   const int64_t len = ((T + segs - 1) / segs + 31) / 32 * 32;
-  return {len, (int)((T + len - 1) / len), 4};
+  return {len, (int)((T + len - 1) / len)};
 }
 int quads(int Dk) { return (Dk + 3) / 4 * 4; }
 // a state per segment and what a segment multiplies a state with; the backward pass has two directions of them
@@ -1348,14 +1336,26 @@ int launch_scan(ScanArgs A, int kt, int vt, hipStream_t s) {
 }
 
 // Passes of equal tiles and slices go in one launch.
-int launch_passes(int dtype, int most, ScanArgs A, const Pass* pass, int n_pass, hipStream_t s) {
+// Where there is one segment, a wave takes fewer value columns as long as each wave has a SIMD to itself (two waves a SIMD
+// with two tiles of float32 products, which are further from the memory's rate): its blocks are shorter and the scores
+// are computed once more per slice.  100 tokens of 4 heads of 64 x 64 bfloat16, one tile against four: 11 against 17 us;
+// 500 x 250 x 4 heads of 20 x 40 float32, two against four: 88 against 102; one against two at 1680 waves: 112 against 100.
+int launch_passes(int dtype, ScanArgs A, const Pass* pass, int n_pass, hipStream_t s) {
   for (int i = 0; i < n_pass; i += A.n_pass) {
-    const int kt = tiles(pass[i].Dk), vt = slice_tiles(dtype, pass[i].Dk, pass[i].Dv, most);
-    A.n_slice = slices(dtype, pass[i].Dk, pass[i].Dv, most);
-    A.n_pass = 0;
-    for (int j = i; j < n_pass && tiles(pass[j].Dk) == kt && slice_tiles(dtype, pass[j].Dk, pass[j].Dv, most) == vt &&
-                    slices(dtype, pass[j].Dk, pass[j].Dv, most) == A.n_slice; j++)
-      A.pass[A.n_pass++] = pass[j];
+    const int kt = tiles(pass[i].Dk);
+    auto alike = [&](const Pass& p, int most) {
+      return tiles(p.Dk) == kt && slice_tiles(dtype, p.Dk, p.Dv, most) == slice_tiles(dtype, pass[i].Dk, pass[i].Dv, most) &&
+             slices(dtype, p.Dk, p.Dv, most) == slices(dtype, pass[i].Dk, pass[i].Dv, most);
+    };
+    int most = A.n_seg > 1 ? 4 : 1;
+    for (;; most *= 2) {
+      A.n_slice = slices(dtype, pass[i].Dk, pass[i].Dv, most);
+      A.n_pass = 0;
+      for (int j = i; j < n_pass && alike(pass[j], most); j++) A.pass[A.n_pass++] = pass[j];
+      const int64_t limit = most == 2 && dtype != FW_DT_BF16 ? SEG_WAVES : SEG_WAVES / 2;
+      if (most == 4 || A.N * A.H * A.n_pass * A.n_slice <= limit) break;
+    }
+    const int vt = slice_tiles(dtype, pass[i].Dk, pass[i].Dv, most);
     const int rc = dtype == FW_DT_F32    ? launch_scan<float>(A, kt, vt, s)
                    : dtype == FW_DT_BF16 ? launch_scan<bf16>(A, kt, vt, s)
                                          : launch_scan<f16>(A, kt, vt, s);
@@ -1371,7 +1371,7 @@ int segment_states(int dtype, ScanArgs A, const Pass* add, const State* in, int 
   const int64_t E = (int64_t)quads(Dk) * Dv;
   A.factor = ws + dirs * A.N * A.H * A.n_seg * E;
   A.run_seg = A.n_seg - 1;  // the last segment adds to nothing
-  if (int rc = launch_passes(dtype, 4, A, add, dirs, s)) return rc;
+  if (int rc = launch_passes(dtype, A, add, dirs, s)) return rc;
   JoinArgs J{};
   for (int d = 0; d < dirs; d++) J.in[d] = in[d];
   J.ws = ws;
@@ -1462,7 +1462,7 @@ int fw_linattn_forward(const fw_linattn* a, void* stream) {
     if (int rc = segment_states(a->dtype, A, &add, &p.in, 1, ws, s)) return rc;
     p.in = seg;
   }
-  return launch_passes(a->dtype, pl.tiles, A, &p, 1, s);
+  return launch_passes(a->dtype, A, &p, 1, s);
 }
 
 int fw_linattn_backward(const fw_linattn* a, void* stream) {
@@ -1488,7 +1488,7 @@ int fw_linattn_backward(const fw_linattn* a, void* stream) {
       {in(a, a->dout), in(a, a->v), in(a, a->k), in(a, a->dq), turned(S), State{}, 0, a->Dv, a->Dk},
       {in(a, a->v), in(a, a->dout), in(a, a->q), in(a, a->dk), turned(R), State{}, 1, a->Dv, a->Dk},
       {in(a, a->k), in(a, a->q), in(a, a->dout), in(a, a->dv), R, straight(a, a->dstate_in), 1, a->Dk, a->Dv}};
-  return launch_passes(a->dtype, pl.tiles, A, main, 3, s);
+  return launch_passes(a->dtype, A, main, 3, s);
 }
 
 int fw_linattn_step(const fw_linattn_token* a, void* stream_) {
