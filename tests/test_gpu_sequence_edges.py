@@ -196,3 +196,53 @@ def test_step_rows_of_any_length(N, H, Dk, Dv, dtype):
     out = s.linear_attention_step(d["q"][0], d["k"][0], d["v"][0], d["log_decay"], d["state"], d["starts"][0])
     _close("out", out, ref[0][0], bulk[0][0], Dk + 16)
     _close("state", d["state"], ref[1], bulk[1], 16)
+
+
+def test_second_derivatives_are_refused():
+    """A graph of the gradients can be asked for (another term of the loss may want one), but not run through them."""
+    s = _seq()
+    d = _dev(_case(20, 2, 2, 8, 8, torch.float32, seed=60))
+    q = d["q"].requires_grad_()
+    out, _ = s.linear_attention(q, d["k"], d["v"], d["log_decay"])
+    plain, = torch.autograd.grad(out, q, d["dout"], retain_graph=True)
+    g, = torch.autograd.grad(out, q, d["dout"].requires_grad_(), create_graph=True)
+    assert torch.equal(g, plain)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(g.sum(), d["dout"])
+    x = torch.randn(6, 16, device=DEV, requires_grad=True)
+    dy = torch.randn(6, 16, device=DEV)
+    y = s.group_norm_act(x, 4)
+    plain, = torch.autograd.grad(y, x, dy, retain_graph=True)
+    g, = torch.autograd.grad(y, x, dy.requires_grad_(), create_graph=True)
+    assert torch.equal(g, plain)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(g.sum(), dy)
+
+
+@pytest.mark.parametrize("backward", [False, True])
+def test_accumulated_gradients_and_a_captured_step(backward):
+    """Leaves that an eager step gave gradients, its graph gone: a captured forward (and backward) on them replays right."""
+    s = _seq()
+    d = _dev(_case(64, 2, 2, 16, 16, torch.float32, seed=61))
+    leaves = [d[n].requires_grad_() for n in ("q", "k", "v")]
+
+    def step():
+        out, final = s.linear_attention(*leaves, d["log_decay"], d["state"], None)
+        if not backward:
+            return [out.detach(), final.detach()]
+        return list(torch.autograd.grad([out, final], leaves, [d["dout"], d["dfinal"]]))
+    out, final = s.linear_attention(*leaves, d["log_decay"], d["state"], None)
+    torch.autograd.backward([out, final], [d["dout"], d["dfinal"]])
+    del out, final
+    want = step()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = step()
+    for _ in range(3):
+        for t in got:
+            t.zero_()
+        g.replay()
+        again = step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        assert all(torch.equal(a, b) for a, b in zip(again, want))
