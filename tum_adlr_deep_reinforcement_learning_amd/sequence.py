@@ -115,7 +115,7 @@ def _decay(who, log_decay, H, device):
         raise ValueError("%s: log_decay must be a float32 [H] tensor on the operands' device" % who)
     if log_decay.requires_grad and torch.is_grad_enabled():
         raise ValueError("%s: log_decay is a fixed schedule and has no gradient; detach it" % who)
-    return log_decay.contiguous()
+    return log_decay if log_decay.is_contiguous() else log_decay.contiguous()
 
 
 def _starts(who, x, shape, device):
@@ -132,6 +132,13 @@ def _state(who, x, shape, device, name):
     if not isinstance(x, torch.Tensor) or x.shape != shape or x.dtype != torch.float32 or x.device != device:
         raise ValueError("%s: %s must be a float32 %s tensor on the operands' device" % (who, name, list(shape)))
     return x
+
+
+def _step_state(who, x, shape, device, name):
+    p = _state(who, x, shape, device, name).data_ptr()
+    if p % 16 or not x.is_contiguous():
+        raise ValueError("%s: %s must be contiguous and 16-byte aligned" % (who, name))
+    return p
 
 
 @functools.lru_cache(maxsize=256)
@@ -244,25 +251,25 @@ def linear_attention_step(q, k, v, log_decay, state, episode_starts=None, state_
     _heads(who, q, k, v, 3)
     N, H, Dk = q.shape
     dev = q.device
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, state) if isinstance(t, torch.Tensor)):
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or
+                                    (isinstance(state, torch.Tensor) and state.requires_grad)):
         raise ValueError("%s has no gradient: use linear_attention, or torch.no_grad()" % who)
     log_decay = _decay(who, log_decay, H, dev)
     starts = _starts(who, episode_starts, (N,), dev)
     shape = (N, H, Dk, v.shape[2])
     new = state if state_out is None else state_out
-    for name, t in (("state", state), ("state_out", new))[:1 if new is state else 2]:
-        _state(who, t, shape, dev, name)
-        if not t.is_contiguous() or t.data_ptr() % 16:
-            raise ValueError("%s: %s must be contiguous and 16-byte aligned" % (who, name))
-    if new is not state and new.data_ptr() != state.data_ptr() and \
-            abs(new.data_ptr() - state.data_ptr()) < new.numel() * 4:
-        raise ValueError("%s: state_out overlaps state" % who)
+    at = _step_state(who, state, shape, dev, "state")
+    to = at
+    if new is not state:
+        to = _step_state(who, new, shape, dev, "state_out")
+        if to != at and abs(to - at) < new.numel() * 4:
+            raise ValueError("%s: state_out overlaps state" % who)
     q, k, v = _dense(q), _dense(k), _dense(v)
     out = v.new_empty((N, H, shape[3]))
     _launch("fw_linattn_step",
             _pack_token(N, H, Dk, shape[3], _DT[q.dtype], *_rows3(q), *_rows3(k), *_rows3(v), *_rows3(out),
                         log_decay.data_ptr(), _ptr(starts), starts.stride(0) if starts is not None else 0,
-                        state.data_ptr(), new.data_ptr()), dev)
+                        at, to), dev)
     return out
 
 
@@ -325,6 +332,15 @@ class _GroupNormAct(torch.autograd.Function):
         return dx, dw, db, None, None, None
 
 
+def _channels(name, p, x, C):
+    if p is None:
+        return None
+    if not isinstance(p, torch.Tensor) or p.shape != (C,) or p.get_device() != x.get_device() or \
+            (p.dtype is not torch.float32 and p.dtype is not x.dtype):
+        raise ValueError("group_norm_act: %s must be a [C] tensor of x's dtype or float32 on its device" % name)
+    return p if p.is_contiguous() else p.contiguous()
+
+
 def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, activation="silu"):
     """``activation(group_norm(x))``, channels last: x [N, ..., C] of float32, bfloat16 or float16.
 
@@ -346,10 +362,7 @@ def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, activation="
         raise ValueError("group_norm_act: activation must be one of %s" % ", ".join(_ACT))
     if not float(eps) >= 0.0:
         raise ValueError("group_norm_act: eps must be >= 0")
-    for name, p in (("weight", weight), ("bias", bias)):
-        if p is not None and (not isinstance(p, torch.Tensor) or p.shape != (C,) or p.device != x.device or
-                              p.dtype not in (x.dtype, torch.float32)):
-            raise ValueError("group_norm_act: %s must be a [C] tensor of x's dtype or float32 on its device" % name)
+    weight, bias = _channels("weight", weight, x, C), _channels("bias", bias, x, C)
     if weight is not None and bias is not None and weight.dtype != bias.dtype:
         raise ValueError("group_norm_act: weight and bias must share a dtype")
     shape = x.shape
@@ -359,8 +372,6 @@ def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, activation="
             rows *= d
         x = x.reshape(shape[0], rows, C)
     x = _dense(x)
-    weight = weight.contiguous() if weight is not None else None
-    bias = bias.contiguous() if bias is not None else None
     if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or
                                     (bias is not None and bias.requires_grad)):
         y = _GroupNormAct.apply(x, weight, bias, groups, float(eps), _ACT[activation])
