@@ -333,7 +333,7 @@ __device__ __forceinline__ f32x4 mma(float a, float b, f32x4 c) {
 // sequence rather than a block of tokens because the recurrence then never leaves its registers.  Small heads are bound
 // by memory: 2048 tokens x 512 x 4 heads of 16 x 16, 287 us, 3750 GB/s (403 us with the loads by way of registers, none
 // ahead).  Larger ones are bound by the products, which a padded head wastes: 500 x 250 x 4 heads of 20 x 40 in tiles of
-// 32 x 64, 112 us.
+// 32 x 32 and two slices, 88 us, of which 39 % of the products count.
 template <typename T, int KT, int VT>
 struct Ring {
   using K = Tile<T, KT, 16>;
