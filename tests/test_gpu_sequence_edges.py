@@ -11,6 +11,13 @@ from test_gpu_sequence import DEV, DTYPES, _case, _check, _close, _dev, _oracle,
 pytestmark = pytest.mark.gpu
 
 
+@pytest.fixture
+def large():
+    """Gives the memory of a test with large allocations back to the other tests."""
+    yield
+    torch.cuda.empty_cache()
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("what", ["q", "k", "v", "dout"])
 @pytest.mark.parametrize("at", [0, 20, 31, 45])
@@ -60,7 +67,7 @@ def test_strides_of_single_rows_mean_nothing(dtype):
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("strides", ["tokens", "tokens far apart", "tokens at the limit", "tokens beyond it", "sequences"])
-def test_offsets_beyond_32_bits(strides, dtype):
+def test_offsets_beyond_32_bits(strides, dtype, large):
     """Views whose rows lie gigabytes apart (a block's rows are addressed by 32-bit offsets up to 2^26 elements apart)."""
     T, N, H, D = 70, 2, 2, 32
     st, sn = {"tokens": (2 ** 24 - 64, H * D), "tokens far apart": (2 ** 25 + 64, H * D), "sequences": (H * D, 2 ** 31),
@@ -75,7 +82,7 @@ def test_offsets_beyond_32_bits(strides, dtype):
     _check(_case(T, N, H, D, D, dtype, seed=43, starts=0.05), view=view)
 
 
-def test_states_beyond_32_bits():
+def test_states_beyond_32_bits(large):
     """70 000 states of 64 KB, in place; the last ones against the oracle."""
     N, D = 70000, 128
     gen = torch.Generator(device=DEV).manual_seed(1)
@@ -98,7 +105,7 @@ def test_states_beyond_32_bits():
     _close("state", final[pick], ref[1], bulk[1], 80)
 
 
-def test_norm_offsets_beyond_32_bits():
+def test_norm_offsets_beyond_32_bits(large):
     def view(x):
         N, L, C = x.shape
         room = torch.empty((N - 1) * 2 ** 31 + L * C, dtype=x.dtype, device=DEV)
