@@ -1,0 +1,54 @@
+"""GPU: the sequence operators where a result hangs on few bits: terms that cancel.  Expected values are exact sums."""
+import pytest
+import torch
+
+from test_gpu_sequence import DEV, DTYPES, _seq
+
+pytestmark = pytest.mark.gpu
+SIZES = [(8, 8), (16, 16), (20, 40), (64, 64), (128, 128), (128, 24)]
+BIT = 2.0 ** -17  # 1 + 2^-9 + BIT has three runs of bits, each a bfloat16 of its own
+# Two terms of size 1 meet: products and weights of 1 are exact, and the sum is rounded at most four times.
+TOL = 4 * 2 * 2.0 ** -24
+
+
+def _zeros(T, Dk, Dv, dtype):
+    z = lambda d: torch.zeros(T, 1, 1, d, dtype=dtype, device=DEV)
+    return z(Dk), z(Dk), z(Dv), torch.zeros(1, device=DEV)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("Dk,Dv", SIZES)
+@pytest.mark.parametrize("T", [1, 40])
+def test_states_that_cancel(T, Dk, Dv, dtype):
+    """q picks the difference of two state rows that agree to 2^-17."""
+    q, k, v, ld = _zeros(T, Dk, Dv, dtype)
+    q[..., :2] = 1
+    state = torch.zeros(1, 1, Dk, Dv, device=DEV)
+    state[..., 0, :] = 1 + 2.0 ** -9 + BIT
+    state[..., 1, :] = -(1 + 2.0 ** -9)
+    out, final = _seq().linear_attention(q, k, v, ld, state)
+    assert torch.equal(final, state)
+    assert float((out.double() - BIT).abs().max()) <= TOL
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("Dk,Dv", SIZES)
+@pytest.mark.parametrize("at", [(0, 1), (3, 20), (17, 30)])
+def test_scores_that_cancel(at, Dk, Dv, dtype):
+    """Two tokens' scores agree to 2^-17 and their values are opposite; the gradient of the values likewise."""
+    q, k, v, ld = _zeros(40, Dk, Dv, dtype)
+    q[..., :3] = 1
+    k[at[0], ..., 0] = k[at[1], ..., 0] = 1
+    k[at[0], ..., 1] = k[at[1], ..., 1] = 2.0 ** -9
+    k[at[0], ..., 2] = BIT
+    v[at[0]], v[at[1]] = 1, -1
+    out, _ = _seq().linear_attention(q, k, v, ld)
+    assert float((out[at[1]:].double() - BIT).abs().max()) <= TOL
+    # reversed in time: dv_0 = sum_t (q_t . k_0) dout_t, with the roles of q and k and the order of tokens turned around
+    k, q = q.flip(0), k.flip(0)
+    v = torch.zeros_like(v).requires_grad_()
+    dout = torch.zeros_like(v)
+    dout[39 - at[0]], dout[39 - at[1]] = 1, -1
+    out, _ = _seq().linear_attention(q, k, v, ld)
+    dv, = torch.autograd.grad(out, v, dout)
+    assert float((dv[:40 - at[1]].double() - BIT).abs().max()) <= TOL

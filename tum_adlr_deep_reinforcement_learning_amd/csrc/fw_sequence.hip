@@ -662,9 +662,9 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, KT * VT <= 16 ? 2 : 1) void k_scan
 //                + 4 (f % 2) + i down: a lane has VC neighbours together
 // Operands with tokens as depth (keys and values of the state's product, values of the output's) are read from LDS by
 // the transposing read: 4 lanes x 4 columns of one row each become 4 rows x 1 column per lane.
-// Products of the inputs are exact in the float32 accumulators.  What is not an input is split into bfloat16 terms:
-// weighted scores and the state into two (2^-16 of a term, far below the output's own half step), the weighted operand
-// of the state's product into three (exact to float32: the state is a float32 result).
+// Products of the inputs are exact in the float32 accumulators.  What is not an input (weighted scores, the state, the
+// weighted operand of the state's product) is split into three bfloat16 terms, so that every product is a float32 one: with
+// two, terms that cancel leave 2^-16 of their size, and more outputs fall to the neighbouring bfloat16.
 //
 // 32 tokens a block: the depth of the product, and half as many splits of the state per token as 16.  Measured at 16
 // heads of 128 x 128 over 16384 tokens: 88 us of outputs after 57 us of segment states (on the float32 products 460 us in
@@ -673,6 +673,15 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, KT * VT <= 16 ? 2 : 1) void k_scan
 // in the values' room), the copies given out between the products, and splits by dot products were no faster.
 __device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+// a pair of floats as three pairs of bfloat16: 8 bits each, so together exact
+__device__ __forceinline__ void split(float x0, float x1, uint32_t& a, uint32_t& b, uint32_t& c) {
+  a = pack_bf16(x0, x1);
+  x0 -= lo_f32(a);
+  x1 -= hi_f32(a);
+  b = pack_bf16(x0, x1);
+  c = pack_bf16(x0 - lo_f32(b), x1 - hi_f32(b));
 }
 
 // Operands from the tiles.  Depth step s of rows 16 z + r: columns 4 NT g + 8 s ..
@@ -842,18 +851,18 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, 2) void k_scan16(ScanArgs A) {
         P[2] = mma(kf[1], qf[1], P[2]);
 #pragma unroll
         for (int f = 0; f < VT; f++) {
-          u32x4 hi{0, 0, 0, 0}, lo{0, 0, 0, 0};
+          u32x4 t[3] = {};
 #pragma unroll
           for (int m = 0; m < (KT < 2 ? 2 : 4); m++) {
-            const float x0 = S[2 * s + m / 2][f][2 * (m & 1)], x1 = S[2 * s + m / 2][f][2 * (m & 1) + 1];
-            hi[m] = pack_bf16(x0, x1);
-            lo[m] = pack_bf16(x0 - lo_f32(hi[m]), x1 - hi_f32(hi[m]));
+            uint32_t y[3];
+            split(S[2 * s + m / 2][f][2 * (m & 1)], S[2 * s + m / 2][f][2 * (m & 1) + 1], y[0], y[1], y[2]);
+#pragma unroll
+            for (int x = 0; x < 3; x++) t[x][m] = y[x];
           }
 #pragma unroll
-          for (int z = 0; z < 2; z++) {
-            O[f][z] = mma(hi, qf[z], O[f][z]);
-            O[f][z] = mma(lo, qf[z], O[f][z]);
-          }
+          for (int z = 0; z < 2; z++)
+#pragma unroll
+            for (int x = 0; x < 3; x++) O[f][z] = mma(t[x], qf[z], O[f][z]);
         }
       }
     }
@@ -926,22 +935,23 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, 2) void k_scan16(ScanArgs A) {
             if (s < t && ((cut >> s) >> 1 & ((1ull << (t - s)) - 1)) != 0) P[x][i] = 0.f;
           }
       }
-      u32x2 Ph[3], Pl[3];
+      u32x2 Ps[3][3];  // term, tile
 #pragma unroll
       for (int x = 0; x < 3; x++)
 #pragma unroll
         for (int m = 0; m < 2; m++) {
-          const float x0 = P[x][2 * m], x1 = P[x][2 * m + 1];
-          Ph[x][m] = pack_bf16(x0, x1);
-          Pl[x][m] = pack_bf16(x0 - lo_f32(Ph[x][m]), x1 - hi_f32(Ph[x][m]));
+          uint32_t t[3];
+          split(P[x][2 * m], P[x][2 * m + 1], t[0], t[1], t[2]);
+#pragma unroll
+          for (int y = 0; y < 3; y++) Ps[y][x][m] = t[y];
         }
 #pragma unroll
-      for (int f = 0; f < VT; f++) {
-        O[f][0] = mma(vf[f], u32x4{Ph[0][0], Ph[0][1], 0, 0}, O[f][0]);
-        O[f][1] = mma(vf[f], u32x4{Ph[1][0], Ph[1][1], Ph[2][0], Ph[2][1]}, O[f][1]);
-        O[f][0] = mma(vf[f], u32x4{Pl[0][0], Pl[0][1], 0, 0}, O[f][0]);
-        O[f][1] = mma(vf[f], u32x4{Pl[1][0], Pl[1][1], Pl[2][0], Pl[2][1]}, O[f][1]);
-      }
+      for (int f = 0; f < VT; f++)
+#pragma unroll
+        for (int y = 0; y < 3; y++) {
+          O[f][0] = mma(vf[f], u32x4{Ps[y][0][0], Ps[y][0][1], 0, 0}, O[f][0]);
+          O[f][1] = mma(vf[f], u32x4{Ps[y][1][0], Ps[y][1][1], Ps[y][2][0], Ps[y][2][1]}, O[f][1]);
+        }
       // through LDS, so that neighbouring lanes store neighbouring columns
 #pragma unroll
       for (int z = 0; z < 2; z++) {
@@ -983,12 +993,10 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, 2) void k_scan16(ScanArgs A) {
     auto weigh = [&](u32x4 x, u32x4(&t)[3]) {
 #pragma unroll
       for (int m = 0; m < 4; m++) {
-        float x0 = lo_f32(x[m]) * wu[m / 2][2 * (m & 1)], x1 = hi_f32(x[m]) * wu[m / 2][2 * (m & 1) + 1];
-        t[0][m] = pack_bf16(x0, x1);
-        x0 -= lo_f32(t[0][m]);
-        x1 -= hi_f32(t[0][m]);
-        t[1][m] = pack_bf16(x0, x1);
-        t[2][m] = pack_bf16(x0 - lo_f32(t[1][m]), x1 - hi_f32(t[1][m]));
+        uint32_t y[3];
+        split(lo_f32(x[m]) * wu[m / 2][2 * (m & 1)], hi_f32(x[m]) * wu[m / 2][2 * (m & 1) + 1], y[0], y[1], y[2]);
+#pragma unroll
+        for (int i = 0; i < 3; i++) t[i][m] = y[i];
       }
     };
     u32x4 t[3];
