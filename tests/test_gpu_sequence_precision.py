@@ -52,3 +52,37 @@ def test_scores_that_cancel(at, Dk, Dv, dtype):
     out, _ = _seq().linear_attention(q, k, v, ld)
     dv, = torch.autograd.grad(out, v, dout)
     assert float((dv[:40 - at[1]].double() - BIT).abs().max()) <= TOL
+
+
+# ------------------------------------------------------------------ bad numbers over a long time
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("start", [None, 600])
+@pytest.mark.parametrize("what", ["state", "q", "k", "v", "dout", "dfinal"])
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+def test_bad_numbers_over_time_segments(bad, what, start, dtype):
+    """1100 tokens of one sequence run in time segments; with these decays what a segment multiplies a state with is less
+    than float32 holds.  An infinity or a NaN still reaches every later token (earlier, in the gradients) up to an episode
+    start, as the recurrence has it, and nothing else."""
+    from oracle import sequence_oracle as R
+    T = 1100
+    gen = torch.Generator().manual_seed(3)
+    rn = lambda *s: torch.randn(*s, generator=gen)
+    c = dict(q=rn(T, 1, 2, 16).to(dtype), k=rn(T, 1, 2, 16).to(dtype), v=rn(T, 1, 2, 16).to(dtype), state=rn(1, 2, 16, 16),
+             dout=rn(T, 1, 2, 16).to(dtype), dfinal=rn(1, 2, 16, 16))
+    if what in ("state", "dfinal"):
+        c[what][0, 1, 3, 5] = bad
+    else:
+        c[what][5 if what in "kv" else 1093, 0, 1, 3] = bad
+    ld = torch.tensor([-1.3, -0.9])
+    starts = torch.zeros(T, 1, dtype=torch.uint8)
+    if start:
+        starts[start] = 1
+    d = {n: x.to(DEV) for n, x in c.items()}
+    leaves = [d[n].requires_grad_() for n in ("q", "k", "v", "state")]
+    out, final = _seq().linear_attention(*leaves[:3], ld.to(DEV), leaves[3], starts.to(DEV))
+    got = (out, final) + torch.autograd.grad([out, final], leaves, [d["dout"], d["dfinal"]])
+    ref = R.linear_attention(c["q"], c["k"], c["v"], ld, c["state"], starts, None, c["dout"], c["dfinal"])
+    for name, g, r in zip(("out", "final", "dq", "dk", "dv", "dstate"), got, ref):
+        wrong = g.cpu().isfinite() != r.isfinite()
+        assert not bool(wrong.any()), "%s: %d of %d, first at %s" % (name, int(wrong.sum()), wrong.numel(),
+                                                                     wrong.nonzero()[0].tolist())

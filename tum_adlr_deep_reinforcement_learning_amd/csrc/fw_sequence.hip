@@ -49,7 +49,9 @@ struct ScanArgs {
   const uint8_t* starts;
   int64_t starts_st, starts_sn;
   const int32_t* lengths;
-  float* factor;  // [n_pass][N][H][n_seg]: what a segment multiplies a state with, or NULL
+  // [n_pass][N][H][n_seg]: what a segment multiplies a state with (a weight too small for float32 is 0, and 0 x inf a NaN as
+  // it should be), negative where an episode start cuts it off; or NULL
+  float* factor;
 };
 
 // What one wave works on: unit = ((n H + h) n_slice + slice) n_pass + pass of segment blockIdx.y, so that the waves of a block share
@@ -643,7 +645,7 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, KT * VT <= 16 ? 2 : 1) void k_scan
   if (p.out.p && (seg == A.n_seg - 1 || p.out.sg))
     store_state<MODE, true>(S, p.out, p.out.p + n * p.out.sn + h * p.out.sh + seg * p.out.sg, Dk, Dv, g, column);
   if (A.factor && U.slice == 0 && lane == 0)
-    A.factor[((U.pass * A.N + n) * A.H + h) * A.n_seg + seg] = fresh ? 0.f : (L == 0 ? 1.f : expf(ld * (float)L));
+    A.factor[((U.pass * A.N + n) * A.H + h) * A.n_seg + seg] = fresh ? -1.f : (L == 0 ? 1.f : expf(ld * (float)L));
   if (want_out) {  // rows behind the sequence's end
     for (int i = lane * 16; i < V::BYTES; i += 1024) *(u32x4*)(ring + i) = u32x4{0, 0, 0, 0};
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -1025,7 +1027,7 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, 2) void k_scan16(ScanArgs A) {
   if (p.out.p && (seg == A.n_seg - 1 || p.out.sg))
     store_state<MODE, false>(S, p.out, p.out.p + n * p.out.sn + h * p.out.sh + seg * p.out.sg, Dk, Dv, g, column);
   if (A.factor && U.slice == 0 && lane == 0)
-    A.factor[((U.pass * A.N + n) * A.H + h) * A.n_seg + seg] = fresh ? 0.f : (L == 0 ? 1.f : expf(ld * (float)L));
+    A.factor[((U.pass * A.N + n) * A.H + h) * A.n_seg + seg] = fresh ? -1.f : (L == 0 ? 1.f : expf(ld * (float)L));
   if (want_out) {  // rows behind the sequence's end
 #pragma unroll
     for (int i = 0; i < Out::NI; i++) *(u32x4*)(lo_ + (i * 64 + lane) * 16) = u32x4{0, 0, 0, 0};
@@ -1036,7 +1038,7 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, 2) void k_scan16(ScanArgs A) {
 }
 
 // ws[seg] holds what segment seg adds to a state; rewritten as the state that enters segment seg:
-//   c_0 = in;  c_{s+1} = factor_s c_s + ws_s
+//   c_0 = in;  c_{s+1} = factor_s c_s + ws_s  (factor_s negative: ws_s alone)
 // One thread per four keys of a value column; the loads of all segments are independent of the recurrence.  Bound by
 // memory: 32 segments of 16 heads of 128 x 128, 34 MB in and out, 14 us.
 struct JoinArgs {
@@ -1078,7 +1080,7 @@ __global__ __launch_bounds__(256) void k_scan_join(JoinArgs A) {
         w[(int64_t)(s0 + k) * E] = c;
         if (s0 + k < A.n_seg - 1)
 #pragma unroll
-          for (int i = 0; i < 4; i++) c[i] = fac[k] != 0.f ? fmaf(fac[k], c[i], add[k][i]) : add[k][i];
+          for (int i = 0; i < 4; i++) c[i] = fac[k] < 0.f ? add[k][i] : fmaf(fac[k], c[i], add[k][i]);
       }
   }
 }
