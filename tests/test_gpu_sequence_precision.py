@@ -54,6 +54,55 @@ def test_scores_that_cancel(at, Dk, Dv, dtype):
     assert float((dv[:40 - at[1]].double() - BIT).abs().max()) <= TOL
 
 
+# ------------------------------------------------------------------ decays
+DECAYS = [-1e-4, -0.3, -0.5, -1.1, -2.0, -18.0]
+
+
+def _decayed(T, ld, state):
+    return state.double() * torch.exp(ld.double() * T)[None, :, None, None]
+
+
+def _near(got, want, rel, ld):
+    # what float32 cannot hold any more may be anything up to its smallest normal number
+    err, tol = (got.double() - want).abs(), rel * want.abs() + torch.finfo(got.dtype).tiny
+    worst = (err / tol).amax((0, 2, 3)) if got.dim() == 4 else (err / tol).max()
+    assert bool((err <= tol).all()), "log_decay %s: %s times the tolerance" % (ld.tolist(), worst.tolist())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("Dk,Dv", [(16, 16), (33, 20), (64, 64), (128, 128)])
+@pytest.mark.parametrize("T,N", [(1, 2), (16, 2), (33, 2), (70, 2), (520, 1)])  # the last in time segments
+def test_a_state_that_only_decays(T, N, Dk, Dv, dtype):
+    """No keys: the final state, and the gradient of the initial one, are the state given times g^T.  Per block of 16
+    tokens (and per segment) the weight may be off by two units of float32's exponential and one rounding, and its product
+    with the state by another: 2^-22 together.  The float32 exponent log_decay x c is off by 2^-24 of itself besides."""
+    H = len(DECAYS)
+    z = lambda d: torch.zeros(T, N, H, d, dtype=dtype, device=DEV)
+    ld = torch.tensor(DECAYS, device=DEV)
+    state = (torch.rand(N, H, Dk, Dv, device=DEV) + 0.5) * 1e6
+    dfinal = torch.rand(N, H, Dk, Dv, device=DEV) + 0.5
+    state.requires_grad_()
+    _, final = _seq().linear_attention(z(Dk), z(Dk), z(Dv), ld, state)
+    dstate, = torch.autograd.grad(final, state, dfinal)
+    rel = ((T // 16 + 4) * 2.0 ** -22 + 2.0 ** -23 * T * ld.double().abs())[None, :, None, None]
+    _near(final.detach(), _decayed(T, ld, state.detach()), rel, ld)
+    _near(dstate, _decayed(T, ld, dfinal), rel, ld)
+
+
+@pytest.mark.parametrize("N,Dk,Dv", [(3, 16, 16), (3, 128, 128), (700, 64, 64), (3, 20, 3), (5, 9, 33)])
+def test_a_step_that_only_decays(N, Dk, Dv):
+    H = len(DECAYS)
+    z = lambda d: torch.zeros(N, H, d, device=DEV)
+    ld = torch.tensor(DECAYS, device=DEV)
+    state = (torch.rand(N, H, Dk, Dv, device=DEV) + 0.5) * 1e6
+    want = _decayed(1, ld, state)
+    q = z(Dk)
+    q[..., 0] = 1
+    out = _seq().linear_attention_step(q, z(Dk), z(Dv), ld, state)
+    _near(state, want, 2.0 ** -22, ld)
+    _near(out, want[:, :, 0], 2.0 ** -22, ld)
+
+
 # ------------------------------------------------------------------ bad numbers over a long time
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("start", [None, 600])

@@ -103,6 +103,19 @@ __device__ __forceinline__ f32x4 quad_turn(f32x4 y, int x) {
   return y;
 }
 
+// S becomes g^c S + D, D the sum of what a block adds: near g^c = 1 as S + (S (g^c - 1) + D), rounded once at the size of S, so
+// that a long memory does not gather an error per token; below 1/2 with g^c itself, of which g^c - 1 holds too little (at
+// g^c = 1e-4, three digits).  One form for both, without a branch: keep is 1 or 0.
+struct Decay {
+  float keep, by;
+  __device__ __forceinline__ void set(float x) {  // x = log(g^c)
+    const bool near = x > -0.69f;
+    keep = near ? 1.f : 0.f;
+    by = near ? expm1f(x) : expf(x);
+  }
+  __device__ __forceinline__ float operator()(float s, float d) const { return fmaf(s, keep, fmaf(s, by, d)); }
+};
+
 // The state as a wave holds it: lane 16 g + r, key column 4 KT g + e, value column dv(f), in S[e % KT][f][e / KT] (WIDE)
 // or S[e / 4][f][e % 4].  Four keys move as one access where they lie together.
 template <int MODE, bool WIDE, int KT, int VT, typename Col>
@@ -445,7 +458,8 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, KT * VT <= 16 ? 2 : 1) void k_scan
   // Weights.  A reversed pass carries g x the state of the row before: its first weight is 1, and its final state is
   // the gradient of the initial one.
   const int e = rev ? 0 : 1;
-  float wp[4], wi = power(r + e), wu[TPL], em1 = 0.f;
+  float wp[4], wi = power(r + e), wu[TPL];
+  Decay decay;
   int cur = 0;
 #pragma unroll
   for (int i = 0; i < 4; i++) wp[i] = r >= 4 * g + i ? power(r - 4 * g - i) : 0.f;
@@ -561,7 +575,7 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, KT * VT <= 16 ? 2 : 1) void k_scan
       const int g4 = here(4 * g);
 #pragma unroll
       for (int j = 0; j < TPL; j++) wu[j] = power(max(c - e - (g4 + j), 0));
-      em1 = expm1f(ld * (float)c);
+      decay.set(ld * (float)c);
     }
     if (M != 0 || c < C) {
       const int g4 = here(4 * g);
@@ -611,7 +625,6 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, KT * VT <= 16 ? 2 : 1) void k_scan
     }
     if (MODE != ANY && more) fetch_v(lq, t2, c2);
 
-    // the state: g^c S as S + S (g^c - 1), whose rounding does not add up over the blocks of a long memory
     if (M != 0) {
 #pragma unroll
       for (int a = 0; a < KT; a++)
@@ -625,19 +638,19 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, KT * VT <= 16 ? 2 : 1) void k_scan
           for (int f = 0; f < VT; f++) Vr[j][f] = 0.f;
     }
 #pragma unroll
-    for (int a = 0; a < KT; a++)
+    for (int a = 0; a < KT; a++) {
+      f32x4 D[VT];
+#pragma unroll
+      for (int f = 0; f < VT; f++) D[f] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < TPL; j++)
+#pragma unroll
+        for (int f = 0; f < VT; f++) D[f] = mma(K2[j][a] * wu[j], Vr[j][f], D[f]);
 #pragma unroll
       for (int f = 0; f < VT; f++)
 #pragma unroll
-        for (int i = 0; i < 4; i++) S[a][f][i] = fmaf(S[a][f][i], em1, S[a][f][i]);
-#pragma unroll
-    for (int j = 0; j < TPL; j++)
-#pragma unroll
-      for (int a = 0; a < KT; a++) {
-        const float kw = K2[j][a] * wu[j];
-#pragma unroll
-        for (int f = 0; f < VT; f++) S[a][f] = mma(kw, Vr[j][f], S[a][f]);
-      }
+        for (int i = 0; i < 4; i++) S[a][f][i] = decay(S[a][f][i], D[f][i]);
+    }
     done += c;
     if (single) single--;
   }
@@ -792,7 +805,8 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, 2) void k_scan16(ScanArgs A) {
   // Weights.  A reversed pass carries g x the state of the row before: its first weight is 1, and its final state is
   // the gradient of the initial one.
   const int e = rev ? 0 : 1;
-  float wd[4], wo[4], wi[2], wu[2][4], em1 = 0.f;  // scores on and off the diagonal tile; state out; state in
+  float wd[4], wo[4], wi[2], wu[2][4];  // scores on and off the diagonal tile; state out; state in
+  Decay decay;
   int cur = 0;
 #pragma unroll
   for (int i = 0; i < 4; i++) {
@@ -831,7 +845,7 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, 2) void k_scan16(ScanArgs A) {
       for (int z = 0; z < 2; z++)
 #pragma unroll
         for (int i = 0; i < 4; i++) wu[z][i] = power(max(c - e - (16 * z + g4 + i), 0));
-      em1 = expm1f(ld * (float)c);
+      decay.set(ld * (float)c);
     }
 
     const f32x4 zero{0.f, 0.f, 0.f, 0.f};
@@ -974,7 +988,6 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, 2) void k_scan16(ScanArgs A) {
       Out::template put<MODE>(lo_, ob + t0 * p.o.st, p.o.st, Dv - v0, c, rev, lane);
     }
 
-    // the state: g^c S as S + S (g^c - 1), whose rounding does not add up over the blocks of a long memory
     if (M != 0) {
 #pragma unroll
       for (int a = 0; a < KT; a++)
@@ -985,12 +998,6 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, 2) void k_scan16(ScanArgs A) {
 #pragma unroll
         for (int f = 0; f < VT; f++) vf[f] = u32x4{0, 0, 0, 0};
     }
-#pragma unroll
-    for (int a = 0; a < KT; a++)
-#pragma unroll
-      for (int f = 0; f < VT; f++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) S[a][f][i] = fmaf(S[a][f][i], em1, S[a][f][i]);
     // the weights go to the operand of fewer tiles
     auto weigh = [&](u32x4 x, u32x4(&t)[3]) {
 #pragma unroll
@@ -1005,20 +1012,34 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, 2) void k_scan16(ScanArgs A) {
     if constexpr (KT < VT) {
 #pragma unroll
       for (int a = 0; a < KT; a++) {
+        f32x4 D[VT];
         weigh(k2[a], t);
 #pragma unroll
         for (int x = 0; x < 3; x++)
 #pragma unroll
-          for (int f = 0; f < VT; f++) S[a][f] = mma(t[x], vf[f], S[a][f]);
+          for (int f = 0; f < VT; f++) D[f] = mma(t[x], vf[f], x ? D[f] : zero);
+#pragma unroll
+        for (int f = 0; f < VT; f++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) S[a][f][i] = decay(S[a][f][i], D[f][i]);
       }
     } else {
+      constexpr int AT = KT < 4 ? KT : 4;  // tiles at a time
 #pragma unroll
       for (int f = 0; f < VT; f++) {
         weigh(vf[f], t);
 #pragma unroll
-        for (int x = 0; x < 3; x++)
+        for (int a0 = 0; a0 < KT; a0 += AT) {
+          f32x4 D[AT];
 #pragma unroll
-          for (int a = 0; a < KT; a++) S[a][f] = mma(k2[a], t[x], S[a][f]);
+          for (int x = 0; x < 3; x++)
+#pragma unroll
+            for (int a = 0; a < AT; a++) D[a] = mma(k2[a0 + a], t[x], x ? D[a] : zero);
+#pragma unroll
+          for (int a = 0; a < AT; a++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) S[a0 + a][f][i] = decay(S[a0 + a][f][i], D[a][i]);
+        }
       }
     }
     done += c;
@@ -1124,7 +1145,8 @@ __global__ __launch_bounds__(256) void k_token(TokenArgs A, int nv, int rows, in
   const int E = A.Dk * A.Dv;
   const T *q[B], *k[B], *v[B];
   T* o[B];
-  float vv[B][4], acc[B][4], em1[B];
+  float vv[B][4], acc[B][4], ld[B];
+  Decay decay[B];
   bool start[B];
   {
     uint32_t n = u0 / (uint32_t)A.H, h = u0 - n * (uint32_t)A.H;
@@ -1135,7 +1157,7 @@ __global__ __launch_bounds__(256) void k_token(TokenArgs A, int nv, int rows, in
       v[b] = (const T*)A.v.p + n * A.v.sn + h * A.v.sh;
       o[b] = (T*)A.o.p + n * A.o.sn + h * A.o.sh;
       start[b] = A.starts && A.starts[n * A.starts_sn] != 0;
-      em1[b] = A.log_decay[h];
+      ld[b] = A.log_decay[h];
       if (u0 + b + 1 < units) {  // (the last pair again, where the wave has more places than there are pairs)
         h = h + 1 == (uint32_t)A.H ? 0 : h + 1;
         n += h == 0;
@@ -1172,7 +1194,7 @@ __global__ __launch_bounds__(256) void k_token(TokenArgs A, int nv, int rows, in
 #pragma unroll
           for (int x = 0; x < 4; x++) vv[b][x] = to_f32(v[b][c + x]);
         }
-        em1[b] = expm1f(em1[b]);
+        decay[b].set(ld[b]);
       }
 #pragma unroll
     for (int b = 0; b < B; b++)
@@ -1182,8 +1204,7 @@ __global__ __launch_bounds__(256) void k_token(TokenArgs A, int nv, int rows, in
         if (d < A.Dk && on && b < live) {
 #pragma unroll
           for (int x = 0; x < 4; x++) {
-            const float old = start[b] ? 0.f : fmaf(s[b][i][x], em1[b], s[b][i][x]);
-            s[b][i][x] = fmaf(kd[b][i], vv[b][x], old);
+            s[b][i][x] = decay[b](start[b] ? 0.f : s[b][i][x], kd[b][i] * vv[b][x]);
             acc[b][x] = fmaf(qd[b][i], s[b][i][x], acc[b][x]);
           }
           f32x4_any* so = (f32x4_any*)(out0 + b * E + d * A.Dv + c);
@@ -1238,14 +1259,15 @@ __global__ __launch_bounds__(256) void k_token_narrow(TokenArgs A) {
   const T* v = (const T*)A.v.p + n * A.v.sn + h * A.v.sh;
   T* o = (T*)A.o.p + n * A.o.sn + h * A.o.sh;
   const bool start = A.starts && A.starts[n * A.starts_sn] != 0;
-  const float em1 = expm1f(A.log_decay[h]);
+  Decay decay;
+  decay.set(A.log_decay[h]);
   const int64_t at = (int64_t)u * A.Dk * A.Dv;
   for (int c = 0; c < A.Dv; c++) {
     const float vc = to_f32(v[c]);
     float acc = 0.f;
     for (int d = lane; d < A.Dk; d += 64) {
       const float s = A.in[at + d * A.Dv + c];
-      const float y = fmaf(to_f32(k[d]), vc, start ? 0.f : fmaf(s, em1, s));
+      const float y = decay(start ? 0.f : s, to_f32(k[d]) * vc);
       A.out[at + d * A.Dv + c] = y;
       acc = fmaf(to_f32(q[d]), y, acc);
     }
