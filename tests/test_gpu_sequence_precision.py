@@ -103,6 +103,44 @@ def test_a_step_that_only_decays(N, Dk, Dv):
     _near(out, want[:, :, 0], 2.0 ** -22, ld)
 
 
+@pytest.mark.parametrize("Dk,Dv", [(16, 16), (64, 64), (128, 128), (20, 40)])
+def test_weights_of_a_block(Dk, Dv):
+    """One key and one query at a time: out_t = g^(t+1) S + g^t v, relative to 2^-21 at every distance: the weight's
+    exponent is carried beyond float32 (its rounding alone would be 2^-24 of an exponent of up to 30)."""
+    T, ld = 16, torch.tensor([-0.37, -1.13, -1.9], device=DEV)
+    q = torch.zeros(T, 1, 3, Dk, device=DEV)
+    k, v = torch.zeros_like(q), torch.ones(T, 1, 3, Dv, device=DEV)
+    q[..., 0] = 1
+    k[0, ..., 0] = 1
+    d = torch.exp(ld.double() * torch.arange(T + 1, device=DEV, dtype=torch.double)[:, None])[:, None, :, None]
+    out, final = _seq().linear_attention(q, k, v, ld)
+    _near(out, d[:T].expand(out.shape), 2.0 ** -21, ld)
+    _near(final[:, :, :1], d[T - 1][..., None].expand(final[:, :, :1].shape), 2.0 ** -21, ld)
+    state = torch.zeros(1, 3, Dk, Dv, device=DEV)
+    state[:, :, 0] = 1
+    out, final = _seq().linear_attention(q, torch.zeros_like(k), v, ld, state)
+    _near(out, d[1:].expand(out.shape), 2.0 ** -21, ld)
+    _near(final[:, :, :1], d[T][..., None].expand(final[:, :, :1].shape), 2.0 ** -21, ld)
+    # reversed: dv_0 = sum_t g^t dout_t, one at a time
+    for t in (1, 7, 15):
+        x = torch.zeros(T, 1, 3, Dv, device=DEV).requires_grad_()
+        dout = torch.zeros_like(x)
+        dout[t] = 1
+        out, _ = _seq().linear_attention(q, k, x, ld)
+        dv, = torch.autograd.grad(out, x, dout)
+        _near(dv[:1], d[t:t + 1].expand(dv[:1].shape), 2.0 ** -21, ld)
+
+
+@pytest.mark.parametrize("Dv", [16, 3])
+def test_steps_without_decay_and_without_memory(Dv):
+    z = lambda d: torch.zeros(2, 2, d, device=DEV)
+    state = torch.randn(2, 2, 16, Dv, device=DEV)
+    want = state.clone()
+    want[:, 1] = 0
+    _seq().linear_attention_step(z(16), z(16), z(Dv), torch.tensor([0.0, -float("inf")], device=DEV), state)
+    assert torch.equal(state, want)
+
+
 # ------------------------------------------------------------------ bad numbers over a long time
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("start", [None, 600])

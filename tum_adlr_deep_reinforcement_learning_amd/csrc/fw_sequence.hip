@@ -103,15 +103,24 @@ __device__ __forceinline__ f32x4 quad_turn(f32x4 y, int x) {
   return y;
 }
 
+__device__ __forceinline__ float finite_decay(float ld) { return ld < -1e30f ? -1e30f : ld; }  // g^0 = 1 for g = 0 too
+// exp(ld m).  The product's rounding, 2^-24 of an exponent of up to 100, would be an error of the weight: it is carried along.
+__device__ __forceinline__ float exponent_rest(float ld, float m) { return fmaf(ld, m, -(ld * m)); }
+__device__ __forceinline__ float power_of(float ld, float m) {
+  const float x = expf(ld * m);
+  return fmaf(x, exponent_rest(ld, m), x);
+}
+
 // S becomes g^c S + D, D the sum of what a block adds: near g^c = 1 as S + (S (g^c - 1) + D), rounded once at the size of S, so
 // that a long memory does not gather an error per token; below 1/2 with g^c itself, of which g^c - 1 holds too little (at
 // g^c = 1e-4, three digits).  One form for both, without a branch: keep is 1 or 0.
 struct Decay {
   float keep, by;
-  __device__ __forceinline__ void set(float x) {  // x = log(g^c)
-    const bool near = x > -0.69f;
+  __device__ __forceinline__ void set(float ld, float c) {
+    const bool near = ld * c > -0.69f;
     keep = near ? 1.f : 0.f;
-    by = near ? expm1f(x) : expf(x);
+    const float x = near ? expm1f(ld * c) : expf(ld * c);
+    by = fmaf(keep + x, exponent_rest(ld, c), x);
   }
   __device__ __forceinline__ float operator()(float s, float d) const { return fmaf(s, keep, fmaf(s, by, d)); }
 };
@@ -386,9 +395,8 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, KT * VT <= 16 ? 2 : 1) void k_scan
   T* ob = (T*)p.o.p + n * p.o.sn + h * p.o.sh + U.seg0 * p.o.st + v0;
   const bool want_out = p.o.p != nullptr;
   const uint8_t* xb = A.starts ? A.starts + n * A.starts_sn + U.seg0 * A.starts_st : nullptr;
-  float ld = A.log_decay[h];
-  ld = ld < -1e30f ? -1e30f : ld;  // g^0 = 1 for g = 0 too
-  auto power = [&](int m) { return expf(ld * (float)m); };
+  const float ld = finite_decay(A.log_decay[h]);
+  auto power = [&](int m) { return power_of(ld, (float)m); };
 
   // rows t0 .. t0 + c - 1 of the segment to a place of the ring: queries, keys and starts, then values
   auto fetch_k = [&](char* to, int64_t t0, int c) {
@@ -575,7 +583,7 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, KT * VT <= 16 ? 2 : 1) void k_scan
       const int g4 = here(4 * g);
 #pragma unroll
       for (int j = 0; j < TPL; j++) wu[j] = power(max(c - e - (g4 + j), 0));
-      decay.set(ld * (float)c);
+      decay.set(ld, (float)c);
     }
     if (M != 0 || c < C) {
       const int g4 = here(4 * g);
@@ -658,7 +666,7 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, KT * VT <= 16 ? 2 : 1) void k_scan
   if (p.out.p && (seg == A.n_seg - 1 || p.out.sg))
     store_state<MODE, true>(S, p.out, p.out.p + n * p.out.sn + h * p.out.sh + seg * p.out.sg, Dk, Dv, g, column);
   if (A.factor && U.slice == 0 && lane == 0)
-    A.factor[((U.pass * A.N + n) * A.H + h) * A.n_seg + seg] = fresh ? -1.f : (L == 0 ? 1.f : expf(ld * (float)L));
+    A.factor[((U.pass * A.N + n) * A.H + h) * A.n_seg + seg] = fresh ? -1.f : power_of(ld, (float)L);
   if (want_out) {  // rows behind the sequence's end
     for (int i = lane * 16; i < V::BYTES; i += 1024) *(u32x4*)(ring + i) = u32x4{0, 0, 0, 0};
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -754,9 +762,8 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, 2) void k_scan16(ScanArgs A) {
   bf16* ob = (bf16*)p.o.p + n * p.o.sn + h * p.o.sh + U.seg0 * p.o.st + v0;
   const bool want_out = p.o.p != nullptr;
   const uint8_t* xb = A.starts ? A.starts + n * A.starts_sn + U.seg0 * A.starts_st : nullptr;
-  float ld = A.log_decay[h];
-  ld = ld < -1e30f ? -1e30f : ld;  // g^0 = 1 for g = 0 too
-  auto power = [&](int m) { return expf(ld * (float)m); };
+  const float ld = finite_decay(A.log_decay[h]);
+  auto power = [&](int m) { return power_of(ld, (float)m); };
 
   auto fetch = [&](int64_t t0, int c) {
     auto go = [&](auto whole) {
@@ -845,7 +852,7 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, 2) void k_scan16(ScanArgs A) {
       for (int z = 0; z < 2; z++)
 #pragma unroll
         for (int i = 0; i < 4; i++) wu[z][i] = power(max(c - e - (16 * z + g4 + i), 0));
-      decay.set(ld * (float)c);
+      decay.set(ld, (float)c);
     }
 
     const f32x4 zero{0.f, 0.f, 0.f, 0.f};
@@ -1048,7 +1055,7 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, 2) void k_scan16(ScanArgs A) {
   if (p.out.p && (seg == A.n_seg - 1 || p.out.sg))
     store_state<MODE, false>(S, p.out, p.out.p + n * p.out.sn + h * p.out.sh + seg * p.out.sg, Dk, Dv, g, column);
   if (A.factor && U.slice == 0 && lane == 0)
-    A.factor[((U.pass * A.N + n) * A.H + h) * A.n_seg + seg] = fresh ? -1.f : (L == 0 ? 1.f : expf(ld * (float)L));
+    A.factor[((U.pass * A.N + n) * A.H + h) * A.n_seg + seg] = fresh ? -1.f : power_of(ld, (float)L);
   if (want_out) {  // rows behind the sequence's end
 #pragma unroll
     for (int i = 0; i < Out::NI; i++) *(u32x4*)(lo_ + (i * 64 + lane) * 16) = u32x4{0, 0, 0, 0};
@@ -1194,7 +1201,7 @@ __global__ __launch_bounds__(256) void k_token(TokenArgs A, int nv, int rows, in
 #pragma unroll
           for (int x = 0; x < 4; x++) vv[b][x] = to_f32(v[b][c + x]);
         }
-        decay[b].set(ld[b]);
+        decay[b].set(finite_decay(ld[b]), 1.f);
       }
 #pragma unroll
     for (int b = 0; b < B; b++)
@@ -1260,7 +1267,7 @@ __global__ __launch_bounds__(256) void k_token_narrow(TokenArgs A) {
   T* o = (T*)A.o.p + n * A.o.sn + h * A.o.sh;
   const bool start = A.starts && A.starts[n * A.starts_sn] != 0;
   Decay decay;
-  decay.set(A.log_decay[h]);
+  decay.set(finite_decay(A.log_decay[h]), 1.f);
   const int64_t at = (int64_t)u * A.Dk * A.Dv;
   for (int c = 0; c < A.Dv; c++) {
     const float vc = to_f32(v[c]);
