@@ -599,6 +599,8 @@ class RolloutCollector:
                 g0.replay()
                 self.env.step_exchange()  # the RCCL all-gather of the moment records
                 g1.replay()
+        if self._recurrent():
+            sequence.written(self.memory)
         self.last_obs = self.s_obs.clone().reshape(self.last_obs.shape)
         self.last_dones = self._dsrc.clone()
         buf.pos, buf.full = n, n == buf.buffer_size

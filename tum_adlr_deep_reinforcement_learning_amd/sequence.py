@@ -244,9 +244,9 @@ def linear_attention_step(q, k, v, log_decay, state, episode_starts=None, state_
     """One token per environment of ``linear_attention``: q, k [N, H, Dk], v [N, H, Dv] -> out [N, H, Dv].
 
     ``state`` (float32 [N, H, Dk, Dv], contiguous) is read once and the new state written once, in place or into
-    ``state_out``, which must not overlap it otherwise.  A row with episode_starts [N] set begins from zeros.  Has no
-    gradient (the training form is ``linear_attention``): inputs that require one are refused outside
-    ``torch.no_grad()``."""
+    ``state_out``, which must not overlap it otherwise; autograd sees it as written in place.  A row with
+    episode_starts [N] set begins from zeros.  Has no gradient (the training form is ``linear_attention``): inputs that
+    require one are refused outside ``torch.no_grad()``."""
     who = "linear_attention_step"
     _heads(who, q, k, v, 3)
     N, H, Dk = q.shape
@@ -270,7 +270,14 @@ def linear_attention_step(q, k, v, log_decay, state, episode_starts=None, state_
             _pack_token(N, H, Dk, shape[3], _DT[q.dtype], *_rows3(q), *_rows3(k), *_rows3(v), *_rows3(out),
                         log_decay.data_ptr(), _ptr(starts), starts.stride(0) if starts is not None else 0,
                         at, to), dev)
+    written(new)
     return out
+
+
+def written(t):
+    """Tells autograd that a kernel has written into ``t``, so that a backward pass that saved it refuses to run."""
+    if not t.is_inference():  # (those have no version, and nothing saves them)
+        torch.autograd.graph.increment_version(t)
 
 
 # ------------------------------------------------------------------ group norm
