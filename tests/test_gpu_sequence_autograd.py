@@ -1,6 +1,7 @@
-"""GPU: what autograd has to know of the sequence operators: writes in place."""
+"""GPU: what autograd has to know of the sequence operators: writes in place, tangents."""
 import pytest
 import torch
+import torch.autograd.forward_ad as fwd
 
 from test_gpu_sequence import DEV, _case, _dev, _seq
 
@@ -52,3 +53,39 @@ def test_a_collection_on_a_saved_memory_is_seen(graph):
     with pytest.raises(RuntimeError, match="inplace"):
         (values.sum() + log_probs.sum()).backward()
     env.close()
+
+
+def test_tangents_are_refused():
+    """The operators have no forward-mode derivative; without one their results would be constants."""
+    d = _dev(_case(6, 2, 2, 16, 16, torch.float32))
+    s = _seq()
+    with fwd.dual_level():
+        for n in ("q", "k", "v", "state"):
+            a = dict(d, **{n: fwd.make_dual(d[n], torch.ones_like(d[n]))})
+            for grad in (False, True):
+                with torch.set_grad_enabled(grad):
+                    with pytest.raises(ValueError, match="forward-mode"):
+                        s.linear_attention(a["q"], a["k"], a["v"], a["log_decay"], a["state"])
+            with torch.no_grad(), pytest.raises(ValueError, match="forward-mode"):
+                _step(a, a["state"])
+            with torch.no_grad(), pytest.raises(ValueError, match="forward-mode"):
+                _step(d, d["state"], state_out=fwd.make_dual(torch.zeros_like(d["state"]), torch.ones_like(d["state"])))
+        ld = fwd.make_dual(d["log_decay"], torch.ones_like(d["log_decay"]))
+        with pytest.raises(ValueError, match="forward-mode"):
+            s.linear_attention(d["q"], d["k"], d["v"], ld, d["state"])
+        x, w = torch.randn(4, 8, device=DEV), torch.ones(8, device=DEV)
+        dual = lambda t: fwd.make_dual(t, torch.ones_like(t))
+        for a in ((dual(x), w, w), (x, dual(w), w), (x, w, dual(w))):
+            with pytest.raises(ValueError, match="forward-mode"):
+                s.group_norm_act(a[0], 2, a[1], a[2])
+        s.linear_attention(d["q"], d["k"], d["v"], d["log_decay"], d["state"])  # without a tangent: as ever
+        s.group_norm_act(x, 2, w, w)
+        # a gradient that carries one
+        q = d["q"].detach().requires_grad_()
+        out, _ = s.linear_attention(q, d["k"], d["v"], d["log_decay"], d["state"])
+        with pytest.raises(ValueError, match="forward-mode"):
+            torch.autograd.grad(out, q, dual(torch.ones_like(out)))
+        x.requires_grad_()
+        y = s.group_norm_act(x, 2, w, w)
+        with pytest.raises(ValueError, match="forward-mode"):
+            torch.autograd.grad(y, x, dual(torch.ones_like(y)))

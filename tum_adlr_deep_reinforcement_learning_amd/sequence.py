@@ -16,6 +16,7 @@ import functools
 import struct
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _native
@@ -62,8 +63,16 @@ def _once(backward):
     guarded = once_differentiable(backward)
 
     def run(ctx, *grads):
+        if forward_ad._current_level >= 0:
+            _no_tangents("the backward pass", *grads)
         return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
     return run
+
+
+def _no_tangents(who, *tensors):
+    """A tensor with a forward-mode tangent does not require a gradient: it would come out as a constant."""
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise ValueError("%s has no forward-mode derivative" % who)
 
 
 def _rows4(t):
@@ -217,8 +226,9 @@ def linear_attention(q, k, v, log_decay, initial_state=None, episode_starts=None
     [N, H, Dk, Dv].  episode_starts: uint8 or bool [T, N].  lengths: int [N]; rows behind a column's length are not
     read, come out as zeros and get zero gradients (values are clamped to 0..T).  out has v's shape and dtype.
 
-    Differentiable in q, k, v and initial_state; nothing but the inputs is kept for the backward pass, which is
-    deterministic.  A non-finite input reaches the outputs that the recurrence lets it reach, and no others."""
+    Differentiable in q, k, v and initial_state (in reverse, once); nothing but the inputs is kept for the backward
+    pass, which is deterministic.  A non-finite input reaches the outputs that the recurrence lets it reach, and no
+    others."""
     _heads("linear_attention", q, k, v, 4)
     T, N, H, Dk = q.shape
     dev = q.device
@@ -233,6 +243,8 @@ def linear_attention(q, k, v, log_decay, initial_state=None, episode_starts=None
             raise ValueError("linear_attention: lengths must be an int32 or int64 [N] tensor on the operands' device")
         lengths = lengths.clamp(0, T).to(torch.int32).contiguous() if lengths.dtype == torch.int64 \
             else lengths.contiguous()
+    if forward_ad._current_level >= 0:
+        _no_tangents("linear_attention", q, k, v, log_decay, state)
     q, k, v = _dense(q), _dense(k), _dense(v)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or
                                     (state is not None and state.requires_grad)):
@@ -264,6 +276,8 @@ def linear_attention_step(q, k, v, log_decay, state, episode_starts=None, state_
         to = _step_state(who, new, shape, dev, "state_out")
         if to != at and abs(to - at) < new.numel() * 4:
             raise ValueError("%s: state_out overlaps state" % who)
+    if forward_ad._current_level >= 0:
+        _no_tangents(who, q, k, v, log_decay, state, new)
     q, k, v = _dense(q), _dense(k), _dense(v)
     out = v.new_empty((N, H, shape[3]))
     _launch("fw_linattn_step",
@@ -355,7 +369,7 @@ def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, activation="
     and over every dimension between the first and the last (none of them: per row, as for a policy's features).
     weight, bias: [C] in x's dtype or float32 (both the same), or None.  activation: "none", "relu", "silu", "gelu" (by
     erf) or "tanh".  Returns a contiguous tensor of x's shape and dtype.  Any strides with unit channel stride are
-    read in place.  Differentiable in x, weight and bias; deterministic."""
+    read in place.  Differentiable in x, weight and bias (in reverse, once); deterministic."""
     if not isinstance(x, torch.Tensor) or x.dim() < 2:
         raise ValueError("group_norm_act: x must be an [N, ..., C] tensor")
     if not x.is_cuda:
@@ -372,6 +386,8 @@ def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, activation="
     weight, bias = _channels("weight", weight, x, C), _channels("bias", bias, x, C)
     if weight is not None and bias is not None and weight.dtype != bias.dtype:
         raise ValueError("group_norm_act: weight and bias must share a dtype")
+    if forward_ad._current_level >= 0:
+        _no_tangents("group_norm_act", x, weight, bias)
     shape = x.shape
     if len(shape) != 3:
         rows = 1
