@@ -1,4 +1,4 @@
-"""GPU: what autograd has to know of the sequence operators: writes in place, tangents."""
+"""GPU: what autograd has to know of the sequence operators: writes in place, tangents, traces."""
 import pytest
 import torch
 import torch.autograd.forward_ad as fwd
@@ -89,3 +89,18 @@ def test_tangents_are_refused():
         y = s.group_norm_act(x, 2, w, w)
         with pytest.raises(ValueError, match="forward-mode"):
             torch.autograd.grad(y, x, dual(torch.ones_like(y)))
+
+
+def test_traces_are_refused():
+    """A trace would hold the allocation of the results and no operator."""
+    d = _dev(_case(6, 2, 2, 16, 16, torch.float32))
+    s = _seq()
+    calls = [(lambda q: s.linear_attention(q, d["k"], d["v"], d["log_decay"])[0], d["q"]),
+             (lambda q: s.linear_attention_step(q, d["k"][0], d["v"][0], d["log_decay"], d["state"]), d["q"][0]),
+             (lambda x: s.group_norm_act(x, 4), torch.randn(4, 8, device=DEV))]
+    for f, x in calls:
+        with pytest.raises(RuntimeError, match="trac"):
+            torch.jit.trace(f, (x,), check_trace=False)
+    x = torch.randn(4, 8, device=DEV, requires_grad=True)
+    with pytest.raises(RuntimeError, match="trac"):
+        torch.jit.trace(lambda x: s.group_norm_act(x, 4), (x,), check_trace=False)

@@ -6,8 +6,9 @@
   group_norm_act         group norm with an activation over channels-last rows or maps, with gradients
 
 Every function launches on the current stream of its tensors' device, takes its workspace from torch's allocator on
-that stream and never synchronises.  Tensors are float32, bfloat16 or float16; states, statistics, sums and the
-gradients of parameters are float32.  There is no CPU path: CPU tensors are refused.
+that stream and never synchronises.  They may be captured into HIP graphs; torch.jit.trace is refused.  Tensors are
+float32, bfloat16 or float16; states, statistics, sums and the gradients of parameters are float32.  There is no CPU
+path: CPU tensors are refused.
 
 The reference's policies are memoryless; these have no counterpart there.
 """
@@ -48,6 +49,8 @@ def _ptr(t):
 
 def _launch(name, args, device):
     """lib.<name>(args, current stream) with `device` current, which it mostly is."""
+    if torch._C._is_tracing():  # a trace would hold the allocation of the results and not what writes them
+        raise RuntimeError("%s cannot be traced" % name)
     fn, i = getattr(_native.load(), name), device.index
     if torch._C._cuda_getDevice() == i:
         rc = fn(args, torch._C._cuda_getCurrentRawStream(i))
