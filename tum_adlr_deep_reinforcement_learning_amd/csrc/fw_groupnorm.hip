@@ -107,13 +107,6 @@ __device__ __forceinline__ float inv_sqrt(float x) {
   return x < 1e-30f ? 1.f / sqrtf(x) : r * fmaf(-0.5f * x * r, r, 1.5f);
 }
 
-// (x - mean) r, with shift = -mean r.  A 16-bit x resolves its mean to 2^-12 at best, so the fused form's 2^-24 of
-// mean r is nothing beside x's own half step.
-template <typename T>
-__device__ __forceinline__ float normed(float x, float mean, float r, float shift) {
-  return sizeof(T) == 2 ? fmaf(x, r, shift) : (x - mean) * r;
-}
-
 // ------------------------------------------------------------------ units of a few lanes
 // Slot = a run of 2^lanes_log2 lanes.  The number of slots is a multiple of G, so a slot keeps its group (and its
 // weights, and its weight gradients) while n runs.
@@ -125,7 +118,7 @@ __global__ __launch_bounds__(256) void k_gn_wave(GnArgs A) {
   const int g = (int)(slot % A.G);
   const int64_t dn = slots / A.G;
   const int cgv = A.cg / VW, total = (int)A.L * cgv;
-  const float inv = 1.f / (float)(A.L * A.cg);
+  const float count = (float)(A.L * A.cg), inv = 1.f / count;
   bool ok[VPL];
   int row[VPL], col[VPL];
   float w[VPL][VW], b[VPL][VW], dw[VPL][VW], db[VPL][VW];
@@ -160,7 +153,7 @@ __global__ __launch_bounds__(256) void k_gn_wave(GnArgs A) {
     for (int i = 0; i < VPL; i++)
 #pragma unroll
       for (int k = 0; k < VW; k++) s += ok[i] ? x[i][k] : 0.f;
-    const float mean = total_of(s) * inv;
+    const float mean = total_of(s) / count;  // (of equal numbers: that number)
     s = 0.f;
 #pragma unroll
     for (int i = 0; i < VPL; i++)
@@ -314,7 +307,7 @@ __global__ __launch_bounds__(max_threads(BWD, VW)) void k_gn_block(GnArgs A) {
   const int cgv = A.cg / VW, rp = (int)blockDim.x / cgv;
   const bool on = t < rp * cgv;
   const int r0 = t / cgv, col = (on ? t - r0 * cgv : 0) * VW, c = g * A.cg + col;
-  const float inv = 1.f / ((float)A.L * (float)A.cg);
+  const float count = (float)A.L * (float)A.cg, inv = 1.f / count;
   Pack<T, VW> xv[VPT], dv[VPT];
 #pragma unroll
   for (int i = 0; i < VPT; i++) {
@@ -342,7 +335,7 @@ __global__ __launch_bounds__(max_threads(BWD, VW)) void k_gn_block(GnArgs A) {
 #pragma unroll
         for (int k = 0; k < VW; k++) v[0] += to_f32(xv[i].e[k]);
     block_sum<2>(v, red);
-    mean = v[0] * inv;
+    mean = v[0] / count;  // (of equal numbers: that number)
     v[0] = v[1] = 0.f;
 #pragma unroll
     for (int i = 0; i < VPT; i++)
@@ -359,20 +352,16 @@ __global__ __launch_bounds__(max_threads(BWD, VW)) void k_gn_block(GnArgs A) {
       A.stats[2 * u + 1] = r;
     }
   }
-  const float shift = -mean * r;
-  if constexpr (!BWD) {
+  if constexpr (!BWD) {  // z = (x - mean) (r w) + b; never x (r w) + (b - mean r w): r is up to 1 / sqrt(eps)
 #pragma unroll
-    for (int k = 0; k < VW; k++) {  // z = (x - mean) (r w) + b
-      w[k] *= r;
-      if (sizeof(T) == 2) b[k] = fmaf(-mean, w[k], b[k]);
-    }
+    for (int k = 0; k < VW; k++) w[k] *= r;
 #pragma unroll
     for (int i = 0; i < VPT; i++)
       if (have(i)) {
         float y[VW];
 #pragma unroll
         for (int k = 0; k < VW; k++)
-          y[k] = act_value<T>(fmaf(to_f32(xv[i].e[k]) - (sizeof(T) == 2 ? 0.f : mean), w[k], b[k]), A.act);
+          y[k] = act_value<T>(fmaf(to_f32(xv[i].e[k]) - mean, w[k], b[k]), A.act);
         store_vec<T, VW>((T*)A.y.p + n * A.y.sn + (r0 + (int64_t)rp * i) * A.y.sl + c, y);
       }
   } else {
@@ -385,7 +374,7 @@ __global__ __launch_bounds__(max_threads(BWD, VW)) void k_gn_block(GnArgs A) {
       if (have(i))
 #pragma unroll
         for (int k = 0; k < VW; k++) {
-          const float xh = normed<T>(to_f32(xv[i].e[k]), mean, r, shift);
+          const float xh = (to_f32(xv[i].e[k]) - mean) * r;
           const float dz = to_f32(dv[i].e[k]) * act_slope<T>(fmaf(xh, w[k], b[k]), A.act);
           sum[1][k] += dz;
           sum[0][k] = fmaf(dz, xh, sum[0][k]);
@@ -401,7 +390,7 @@ __global__ __launch_bounds__(max_threads(BWD, VW)) void k_gn_block(GnArgs A) {
         float y[VW];
 #pragma unroll
         for (int k = 0; k < VW; k++)
-          y[k] = fmaf(d[i][k], r, fmaf(normed<T>(to_f32(xv[i].e[k]), mean, r, shift), s2, s1));
+          y[k] = fmaf(d[i][k], r, fmaf((to_f32(xv[i].e[k]) - mean) * r, s2, s1));
         store_vec<T, VW>((T*)A.dx.p + n * A.dx.sn + (r0 + (int64_t)rp * i) * A.dx.sl + c, y);
       }
     if (A.dw || A.db)
@@ -427,7 +416,7 @@ __global__ __launch_bounds__(max_threads(BWD, 16 / sizeof(T))) void k_gn_bundle(
   const int cols = width / VW, rp = (int)blockDim.x / cols;
   const bool on = t < rp * cols;
   const int r0 = t / cols, col = (on ? t - r0 * cols : 0) * VW, c = g0 * A.cg + col;
-  const float inv = 1.f / ((float)A.L * (float)A.cg);
+  const float count = (float)A.L * (float)A.cg, inv = 1.f / count;
   auto have = [&](int i) { return on && r0 + (int64_t)rp * i < A.L; };
   Pack<T, VW> xv[VPT], dv[VPT];
 #pragma unroll
@@ -480,7 +469,7 @@ __global__ __launch_bounds__(max_threads(BWD, 16 / sizeof(T))) void k_gn_bundle(
     group_sums(v, 0, false);
 #pragma unroll
     for (int k = 0; k < VW; k++) {
-      mean[k] = group[0][gi[k]] * inv;
+      mean[k] = group[0][gi[k]] / count;  // (of equal numbers: that number)
       v[0][k] = 0.f;
     }
 #pragma unroll
@@ -495,38 +484,32 @@ __global__ __launch_bounds__(max_threads(BWD, 16 / sizeof(T))) void k_gn_bundle(
 #pragma unroll
     for (int k = 0; k < VW; k++) r[k] = inv_sqrt(group[1][gi[k]] * inv + A.eps);
     if (A.stats && t < bundle) {
-      A.stats[2 * (n * A.G + g0 + t)] = group[0][t] * inv;
+      A.stats[2 * (n * A.G + g0 + t)] = group[0][t] / count;
       A.stats[2 * (n * A.G + g0 + t) + 1] = inv_sqrt(group[1][t] * inv + A.eps);
     }
   }
   if constexpr (!BWD) {
 #pragma unroll
-    for (int k = 0; k < VW; k++) {  // z = (x - mean) (r w) + b
-      w[k] *= r[k];
-      if (sizeof(T) == 2) b[k] = fmaf(-mean[k], w[k], b[k]);
-    }
+    for (int k = 0; k < VW; k++) w[k] *= r[k];  // z = (x - mean) (r w) + b
 #pragma unroll
     for (int i = 0; i < VPT; i++)
       if (have(i)) {
         float y[VW];
 #pragma unroll
         for (int k = 0; k < VW; k++)
-          y[k] = act_value<T>(fmaf(to_f32(xv[i].e[k]) - (sizeof(T) == 2 ? 0.f : mean[k]), w[k], b[k]), A.act);
+          y[k] = act_value<T>(fmaf(to_f32(xv[i].e[k]) - mean[k], w[k], b[k]), A.act);
         store_vec<T, VW>((T*)A.y.p + n * A.y.sn + (r0 + (int64_t)rp * i) * A.y.sl + c, y);
       }
   } else {
-    float sum[2][VW], shift[VW], d[VPT][VW];  // of dbias and dweight
+    float sum[2][VW], d[VPT][VW];  // of dbias and dweight
 #pragma unroll
-    for (int k = 0; k < VW; k++) {
-      sum[0][k] = sum[1][k] = 0.f;
-      shift[k] = -mean[k] * r[k];
-    }
+    for (int k = 0; k < VW; k++) sum[0][k] = sum[1][k] = 0.f;
 #pragma unroll
     for (int i = 0; i < VPT; i++)
       if (have(i))
 #pragma unroll
         for (int k = 0; k < VW; k++) {
-          const float xh = normed<T>(to_f32(xv[i].e[k]), mean[k], r[k], shift[k]);
+          const float xh = (to_f32(xv[i].e[k]) - mean[k]) * r[k];
           d[i][k] = to_f32(dv[i].e[k]) * act_slope<T>(fmaf(xh, w[k], b[k]), A.act);
           sum[0][k] += d[i][k];
           sum[1][k] = fmaf(d[i][k], xh, sum[1][k]);
@@ -549,7 +532,7 @@ __global__ __launch_bounds__(max_threads(BWD, 16 / sizeof(T))) void k_gn_bundle(
         float y[VW];
 #pragma unroll
         for (int k = 0; k < VW; k++)
-          y[k] = fmaf(d[i][k], w[k], fmaf(normed<T>(to_f32(xv[i].e[k]), mean[k], r[k], shift[k]), s2[k], s1[k]));
+          y[k] = fmaf(d[i][k], w[k], fmaf((to_f32(xv[i].e[k]) - mean[k]) * r[k], s2[k], s1[k]));
         store_vec<T, VW>((T*)A.dx.p + n * A.dx.sn + (r0 + (int64_t)rp * i) * A.dx.sl + c, y);
       }
   }
@@ -718,7 +701,6 @@ __global__ __launch_bounds__(256) void k_gn_stream_apply(GnArgs A) {
       m[k] = A.stats[2 * g];
       w[k] = A.stats[2 * g + 1] * param(A.w, A.wdt, c + k, 1.f);
       b[k] = param(A.b, A.wdt, c + k, 0.f);
-      if (sizeof(T) == 2) b[k] = fmaf(-m[k], w[k], b[k]);
     }
     const T* x = (const T*)A.x.p + p.n * A.x.sn + c;
     T* y = (T*)A.y.p + p.n * A.y.sn + c;
@@ -732,7 +714,7 @@ __global__ __launch_bounds__(256) void k_gn_stream_apply(GnArgs A) {
         if (l + (int64_t)at.rp * i < p.l1) {
 #pragma unroll
           for (int k = 0; k < VW; k++)
-            v[i][k] = act_value<T>(fmaf(v[i][k] - (sizeof(T) == 2 ? 0.f : m[k]), w[k], b[k]), A.act);
+            v[i][k] = act_value<T>(fmaf(v[i][k] - m[k], w[k], b[k]), A.act);
           store_vec<T, VW>(y + (l + (int64_t)at.rp * i) * A.y.sl, v[i]);
         }
     }
