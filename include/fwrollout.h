@@ -252,7 +252,8 @@ int fw_linattn_step(const fw_linattn_token* a, void* stream);
 /* Group norm with an activation, channels last.  Per sample n and group of C / G channels, over its L rows:
  *   m = mean, r = 1 / sqrt(var + eps),  z = weight (x - m) r + bias,  y = act(z)
  * x, y, dy, dx: [N][L][C] of dtype with element strides sn, sl and unit channel stride; weight, bias [C] of wdtype
- * (dtype or float32), either may be NULL (1 / 0).  Statistics are float32, by deviations from the mean.
+ * (dtype or float32), either may be NULL (1 / 0).  Statistics are float32, by deviations from the mean; a variance beyond
+ * float32 (deviations above 1e19) is infinite, r = 0.
  * Backward: dx, and dweight, dbias [C] of wdtype (either may be NULL), summed in a fixed order.
  * stats: float [N][G][2] (m, r), written by the forward call and read by the backward call; it is needed where
  * fw_group_norm_stats says 1 (elsewhere NULL: the statistics are rebuilt from x, which is in registers anyway).  A

@@ -1,8 +1,10 @@
-"""GPU: group norm where few bits or small numbers decide: groups without spread."""
+"""GPU: group norm where few bits or small numbers decide: groups without spread, variances that float32
+does not hold."""
 import pytest
 import torch
 
-from test_gpu_groupnorm import DEV, DTYPES, _seq
+from oracle import sequence_oracle as R
+from test_gpu_groupnorm import ACTS, DEV, DTYPES, _seq
 
 pytestmark = pytest.mark.gpu
 # lanes, a block, a bundle of groups, streams
@@ -22,3 +24,20 @@ def test_groups_without_spread(shape, value, dtype):
     assert torch.equal(y.detach(), b.to(dtype).expand(N, L, C))
     dw, = torch.autograd.grad(y, w, torch.randn_like(y))
     assert not bool(dw.any())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("shape", SHAPES)
+def test_variances_beyond_float32(shape, act, dtype):
+    """Deviations of 1e20: their squares are infinite in float32, 1 / sqrt of that is 0, and what follows is finite."""
+    N, L, C, G = shape
+    x = (torch.arange(N * L * C, device=DEV).reshape(N, L, C) % 3 - 1.0).mul_(1e20).to(dtype).requires_grad_()
+    w, b = torch.linspace(0.5, 1.5, C, device=DEV).requires_grad_(), torch.linspace(-1, 1, C, device=DEV).requires_grad_()
+    y = _seq().group_norm_act(x, G, w, b, activation=act)
+    want = R.activation(b.detach().cpu().double(), act)[0]
+    # the activation's own roundings and half a step
+    tol = 2.0 ** -20 + torch.finfo(dtype).eps / 2 * want.abs()
+    assert bool(((y.detach().cpu().double() - want).abs() <= tol).all())
+    dx, dw, db = torch.autograd.grad(y, [x, w, b], torch.ones_like(y))
+    assert not bool(dx.any()) and not bool(dw.any()) and bool(db.isfinite().all())

@@ -101,10 +101,11 @@ __device__ __forceinline__ float act_slope(float z, int act) {
   }
   return 1.f;
 }
-// 1 / sqrt(x): the hardware's estimate and one step of Newton's
+// 1 / sqrt(x): the hardware's estimate and one step of Newton's, which small numbers and an infinite one (a variance beyond
+// float32: 0, so that y is the bias) would leave with 0 x inf
 __device__ __forceinline__ float inv_sqrt(float x) {
   const float r = __builtin_amdgcn_rsqf(x);
-  return x < 1e-30f ? 1.f / sqrtf(x) : r * fmaf(-0.5f * x * r, r, 1.5f);
+  return x < 1e-30f || x > 1e38f ? 1.f / sqrtf(x) : r * fmaf(-0.5f * x * r, r, 1.5f);
 }
 
 // ------------------------------------------------------------------ units of a few lanes
@@ -548,7 +549,7 @@ __device__ __forceinline__ void join(float& n, float& m, float& q, float n2, flo
   if (n2 == 0.f) return;
   const float t = n + n2, d = m2 - m, f = n2 * __builtin_amdgcn_rcpf(t);
   m = fmaf(d, f, m);
-  q += q2 + d * d * (n * f);
+  q += q2 + d * (d * (n * f));  // (n may be 0, and d d infinite)
   n = t;
 }
 
