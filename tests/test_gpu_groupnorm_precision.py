@@ -1,5 +1,5 @@
 """GPU: group norm where few bits or small numbers decide: groups without spread, variances that float32
-does not hold."""
+does not hold, the activations' far sides."""
 import pytest
 import torch
 
@@ -41,3 +41,36 @@ def test_variances_beyond_float32(shape, act, dtype):
     assert bool(((y.detach().cpu().double() - want).abs() <= tol).all())
     dx, dw, db = torch.autograd.grad(y, [x, w, b], torch.ones_like(y))
     assert not bool(dx.any()) and not bool(dw.any()) and bool(db.isfinite().all())
+
+
+def _activated(z, act, dtype):
+    """act(z) and its slope, through groups of two channels -1 and 1: no mean, a spread of 1 (eps = 0), z the weight."""
+    w = torch.stack([z, z], 1).reshape(-1).to(DEV)
+    x = torch.tensor([-1.0, 1.0], device=DEV).repeat(len(z))[None].to(dtype)
+    b = torch.zeros_like(w).requires_grad_()
+    y = _seq().group_norm_act(x, len(z), w, b, eps=0.0, activation=act)
+    slope, = torch.autograd.grad(y, b, torch.ones_like(y))
+    signed = (w * x[0].float()).cpu().double()
+    return signed, y.detach()[0].cpu().double(), slope.cpu().double()
+
+
+def _held(got, want, tol):
+    err = (got - want).abs()
+    worst = int((err / tol).argmax())
+    assert bool((err <= tol).all()), "%g for %g, %.3g times the tolerance" % (got[worst], want[worst], err[worst] / tol[worst])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_gelu_far_from_zero_in_16_bits(dtype):
+    """Half a step of the type, relative to the value itself also where it is small.  The tail's polynomial is off by
+    2^-18, the exponential's argument z^2 / 2 by two roundings: 123 x 2^-23 where float32 ends; a few roundings more:
+    2^-15 together."""
+    z, y, slope = _activated(torch.linspace(0.01, 13.0, 1300), "gelu", dtype)
+    want, dwant = R.activation(z, "gelu")
+    half, least = torch.finfo(dtype).eps / 2, torch.finfo(dtype).tiny
+    # below the smallest normal number: half of float16's last step; bfloat16's numbers there may be 0
+    least = least * torch.finfo(dtype).eps / 2 if dtype == torch.float16 else least
+    _held(y, want, 2.0 ** -15 * want.abs() + half * want.abs() * (1 + 2.0 ** -15) + least)
+    q, p = 0.5 * torch.erfc(z.abs() * 0.5 ** 0.5), torch.exp(-0.5 * z * z) / (2 * torch.pi) ** 0.5 * z.abs()
+    # the slope in float32: its terms' errors, and a rounding of the sum
+    _held(slope, dwant, 2.0 ** -15 * (q + p) + 2.0 ** -23 * dwant.abs() + 1e-37)

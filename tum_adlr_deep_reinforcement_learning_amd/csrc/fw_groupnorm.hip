@@ -53,17 +53,18 @@ __device__ __forceinline__ float tanh_fast(float z) {
   const float q = fmaf(-2.f, __builtin_amdgcn_rcpf(1.f + exp_fast(2.f * z)), 1.f);
   return fabsf(z) < 0.25f ? p : q;
 }
-// Phi(-|z|), and e = exp(-z^2 / 2) beside it.  16-bit types: Abramowitz and Stegun 7.1.26 for erfc (absolute error 1.5e-7
-// of it, against 5e-4 of the types' own step); float32: the library's erfc.
+// Phi(-|z|), and e = exp(-z^2 / 2) beside it.  float32: the library's erfc.  16-bit types: e times a polynomial in t = 1 / (1 +
+// 0.3078 |z|), fitted to Phi(-|z|) / e so that its largest relative error up to z = 13.6 (where float32 ends) is least:
+// 4e-6, and 1e-5 with the exponential's argument, against 5e-4 (float16) and 4e-3 (bfloat16) of half a step.
 template <typename T>
 __device__ __forceinline__ float normal_tail(float z, float& e) {
   e = __builtin_amdgcn_exp2f(z * -0.72134752f * z);
   if constexpr (sizeof(T) == 4) {
     return 0.5f * erfcf(fabsf(z) * 0.70710678f);
   } else {
-    const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f * 0.70710678f, fabsf(z), 1.f));
-    return t * e *
-           fmaf(t, fmaf(t, fmaf(t, fmaf(t, 0.5307027145f, -0.7265760135f), 0.7107068705f), -0.142248368f), 0.127414796f);
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.3078f, fabsf(z), 1.f));
+    const float p = fmaf(t, fmaf(t, fmaf(t, fmaf(t, -0.0756963279f, 0.190882708f), 0.00603458086f), 0.13704883f), 0.118674806f);
+    return t * e * fmaf(t, p, 0.123053535f);
   }
 }
 
