@@ -74,3 +74,11 @@ def test_gelu_far_from_zero_in_16_bits(dtype):
     q, p = 0.5 * torch.erfc(z.abs() * 0.5 ** 0.5), torch.exp(-0.5 * z * z) / (2 * torch.pi) ** 0.5 * z.abs()
     # the slope in float32: its terms' errors, and a rounding of the sum
     _held(slope, dwant, 2.0 ** -15 * (q + p) + 2.0 ** -23 * dwant.abs() + 1e-37)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_gelu_slopes_near_zero_in_16_bits(dtype):
+    """The slopes are summed in float32 over all rows: their own error adds up.  The tail's 9e-8 of at most 1/2, its
+    exponential's argument (4.5 at most, 2^-22 of it, of values below 1/4), and a few roundings of numbers up to 1.2: 2^-20."""
+    z, _, slope = _activated(torch.linspace(0.001, 3.0, 1500), "gelu", dtype)
+    _held(slope, R.activation(z, "gelu")[1], torch.full_like(slope, 2.0 ** -20))
