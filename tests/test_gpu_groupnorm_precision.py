@@ -82,3 +82,21 @@ def test_gelu_slopes_near_zero_in_16_bits(dtype):
     exponential's argument (4.5 at most, 2^-22 of it, of values below 1/4), and a few roundings of numbers up to 1.2: 2^-20."""
     z, _, slope = _activated(torch.linspace(0.001, 3.0, 1500), "gelu", dtype)
     _held(slope, R.activation(z, "gelu")[1], torch.full_like(slope, 2.0 ** -20))
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu", "tanh"])
+def test_activations_in_float32(act):
+    """Relative to the value at every z.  A handful of roundings and units of the hardware's exponential and reciprocal, 2^-23
+    each: 2^-20.  What is below float32's normal numbers may be 0."""
+    z, y, slope = _activated(torch.cat([torch.linspace(0.003, 1.5, 1000), torch.linspace(1.5, 13, 1000)] +
+                                       ([torch.linspace(13, 100, 500)] if act != "gelu" else [])), act, torch.float32)
+    want, dwant = R.activation(z, act)
+    _held(y, want, 2.0 ** -20 * want.abs() + 100 * 2.0 ** -126)
+    if act == "silu":
+        s = torch.sigmoid(z)
+        size = s * (1 + z.abs())
+    elif act == "gelu":
+        size = 0.5 * torch.erfc(-z * 0.5 ** 0.5) + z.abs() * torch.exp(-0.5 * z * z) / (2 * torch.pi) ** 0.5
+    else:
+        size = torch.ones_like(z)
+    _held(slope, dwant, 2.0 ** -20 * size + 100 * 2.0 ** -126)

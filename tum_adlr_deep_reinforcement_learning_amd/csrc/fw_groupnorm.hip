@@ -43,15 +43,33 @@ __device__ __forceinline__ float param(const void* p, int dt, int c, float none)
   return to_f32(((const f16*)p)[c]);
 }
 
-// Activations from the hardware's exp2 and reciprocal (an ulp each), with no division and no branch.
-__device__ __forceinline__ float exp_fast(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504f); }
-__device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.f + exp_fast(-z)); }
+// Activations from the hardware's exp2 and reciprocal (an ulp each), with no division and no branch.  In float32 what the
+// exponent rounds off is carried along and the reciprocal gets a step of Newton's; the 16-bit types do not see either.
+template <typename T>
+__device__ __forceinline__ float exp_fast(float x) {
+  const float h = x * 1.44269504f;
+  if constexpr (sizeof(T) == 2) return __builtin_amdgcn_exp2f(h);
+  const float rest = fmaf(x, 1.92596299e-8f, fmaf(x, 1.44269504f, -h));  // log2(e) in two parts
+  return __builtin_amdgcn_exp2f(h) * fmaf(fabsf(h) < 256.f ? rest : 0.f, 0.693147181f, 1.f);
+}
+template <typename T>
+__device__ __forceinline__ float reciprocal(float x) {  // x >= 1
+  const float r = __builtin_amdgcn_rcpf(x);
+  if constexpr (sizeof(T) == 2) return r;
+  return x < 1e38f ? fmaf(fmaf(-x, r, 1.f), r, r) : r;
+}
+template <typename T>
+__device__ __forceinline__ float sigmoid(float z) {
+  return reciprocal<T>(1.f + exp_fast<T>(-z));
+}
+template <typename T>
 __device__ __forceinline__ float tanh_fast(float z) {
-  // near 0 the difference below loses what it has; there the series to z^9 (next term 9e-9 of z at 1/4)
+  // near 0 the difference below loses what it has; there z + z^3 times a polynomial in z^2, fitted to tanh up to 5/8 (4e-9)
   const float t = z * z;
-  const float p = fmaf(t, fmaf(t, fmaf(t, fmaf(t, 62.f / 2835.f, -17.f / 315.f), 2.f / 15.f), -1.f / 3.f), 1.f) * z;
-  const float q = fmaf(-2.f, __builtin_amdgcn_rcpf(1.f + exp_fast(2.f * z)), 1.f);
-  return fabsf(z) < 0.25f ? p : q;
+  const float p = fmaf(t * z, fmaf(t, fmaf(t, fmaf(t, fmaf(t, -0.00570498453f, 0.0206390843f), -0.0537397154f), 0.133314416f),
+                                   -0.333332807f), z);
+  const float q = fmaf(-2.f, reciprocal<T>(1.f + exp_fast<T>(2.f * z)), 1.f);
+  return fabsf(z) < 0.625f ? p : q;
 }
 // Phi(-|z|), and e = exp(-z^2 / 2) beside it.  float32: the library's erfc.  16-bit types: e times a polynomial in t = 1 / (1 +
 // 0.3041 |z|), fitted to Phi(-|z|) / e so that its largest relative error up to z = 13.6 (where float32 ends) is least:
@@ -59,10 +77,14 @@ __device__ __forceinline__ float tanh_fast(float z) {
 // half a step of 5e-4 (float16) and 4e-3 (bfloat16).
 template <typename T>
 __device__ __forceinline__ float normal_tail(float z, float& e) {
-  e = __builtin_amdgcn_exp2f(z * -0.72134752f * z);
   if constexpr (sizeof(T) == 4) {
-    return 0.5f * erfcf(fabsf(z) * 0.70710678f);
+    // z^2 / 2 and |z| / sqrt(2) round to 2^-24 of numbers that the tail has as exponents: what they lose is carried along
+    const float a = fabsf(z) > 64.f ? 64.f : fabsf(z), s = a * a, x = a * 0.707106769f;
+    e = exp_fast<T>(-0.5f * s) * fmaf(-0.5f, fmaf(a, a, -s), 1.f);
+    const float rest = fmaf(a, 1.21016175e-8f, fmaf(a, 0.707106769f, -x));  // 1 / sqrt(2) in two parts
+    return fmaf(-0.564189584f * rest, e, 0.5f * erfcf(x));
   } else {
+    e = __builtin_amdgcn_exp2f(z * -0.72134752f * z);
     const float t = __builtin_amdgcn_rcpf(fmaf(0.3041f, fabsf(z), 1.f));
     const float p = fmaf(t, fmaf(t, fmaf(t, fmaf(t, 0.0368336476f, -0.1550304f), 0.191474333f), -0.0425504558f), 0.123265989f);
     return t * e * fmaf(t, fmaf(t, fmaf(t, p, 0.102532998f), 0.122198641f), 0.121275306f);
@@ -74,12 +96,12 @@ __device__ __forceinline__ float act_value(float z, int act) {
   float e;
   switch (act) {
     case FW_ACT_RELU: return z > 0.f ? z : (z != z ? z : 0.f);
-    case FW_ACT_SILU: return z * sigmoid(z);
+    case FW_ACT_SILU: return z * sigmoid<T>(z);
     case FW_ACT_GELU: {  // z Phi(z) from the tail on z's own side: no difference of near numbers
       const float q = normal_tail<T>(z, e);
       return fmaf(-fminf(fabsf(z), 64.f), q, fmaxf(z, 0.f));  // (an infinity times no tail is no tail)
     }
-    case FW_ACT_TANH: return tanh_fast(z);
+    case FW_ACT_TANH: return tanh_fast<T>(z);
   }
   return z;
 }
@@ -88,7 +110,7 @@ __device__ __forceinline__ float act_slope(float z, int act) {
   switch (act) {
     case FW_ACT_RELU: return z > 0.f ? 1.f : 0.f;
     case FW_ACT_SILU: {
-      const float s = sigmoid(z);
+      const float s = sigmoid<T>(z);
       return s * fmaf(z, 1.f - s, 1.f);
     }
     case FW_ACT_GELU: {
@@ -97,8 +119,8 @@ __device__ __forceinline__ float act_slope(float z, int act) {
       return fmaf(z * 0.39894228f, e, z < 0.f ? q : 1.f - q);
     }
     case FW_ACT_TANH: {
-      const float t = tanh_fast(z);
-      return fmaf(-t, t, 1.f);
+      const float s = sigmoid<T>(-2.f * fabsf(z));  // 1 - tanh^2, without the difference
+      return 4.f * s * (1.f - s);
     }
   }
   return 1.f;
