@@ -476,12 +476,13 @@ class RolloutCollector:
 
     def graph_key(self):
         """Everything a captured step bakes in: the env's host-side choices, the split around the collective,
-        the buffer, and the policy -- which module, where its parameters live (the launch reads them in
+        the buffer, and the policy -- which module, where its parameters and buffers live (the launch reads them in
         place, so optimiser steps are seen but a replaced tensor is not), whether it explores."""
         env_key = self.env.graph_key() if hasattr(self.env, "graph_key") else None
         pol = self.policy
         pol_key = (id(pol), bool(getattr(pol, "deterministic_rollout", False)),
-                   tuple(p.data_ptr() for p in pol.parameters()) if isinstance(pol, nn.Module) else None,
+                   tuple(t.data_ptr() for ts in (pol.parameters(), pol.buffers()) for t in ts)
+                   if isinstance(pol, nn.Module) else None,
                    self.memory.data_ptr() if self._recurrent() else None)
         return (env_key, self._split(), self.buffer.slab.data_ptr(), self.buffer.buffer_size, pol_key,
                 self.capture_collective, self.steps_per_graph, self.defer_final_merge)
