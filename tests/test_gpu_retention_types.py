@@ -1,4 +1,7 @@
-"""GPU: the policy with a memory whose constants are replaced."""
+"""GPU: the policy with a memory whose constants are replaced, and in 16 bits.
+
+Tolerance of the 16-bit runs: a chain of about ten roundings to the type, half a step each, on values of size up to about 10,
+a norm between them: 30 steps relative to the largest value."""
 import pytest
 import torch
 
@@ -21,4 +24,35 @@ def test_replaced_decays_are_seen(graph):
     _same(values, buf.values)
     _same(log_probs, buf.log_probs)
     assert old is not policy.log_decay
+    env.close()
+
+
+def _same16(a, b, dtype):
+    assert bool(b.isfinite().all())
+    assert float((a.detach().float() - b).abs().max()) < 30 * torch.finfo(dtype).eps * (1 + float(b.abs().max()))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_a_step_captured_under_autocast(dtype):
+    """It makes its own casts of the weights: those of the capture's context are gone after it and know no later update.
+    Outside of autocast it is captured anew."""
+    env, policy, buf, col = _setup(64, 20)
+    col.collect()
+    with torch.autocast("cuda", dtype=dtype):
+        col.collect()
+        col.collect(graph=True)
+        _same16(_replay(policy, buf, col.rollout_memory)[0], buf.values, dtype)
+    old = buf.values.clone()
+    with torch.no_grad():
+        policy.value_net.weight.mul_(-3.0)
+        policy.value_net.bias.add_(1.0)
+    with torch.autocast("cuda", dtype=dtype):
+        col.collect(graph=True)
+        _same16(_replay(policy, buf, col.rollout_memory)[0], buf.values, dtype)
+    assert float((old - buf.values).abs().max()) > 0.5
+    col.collect(graph=True)
+    with torch.no_grad():
+        values, log_probs, _ = _replay(policy, buf, col.rollout_memory)
+    _same(values, buf.values)
+    _same(log_probs, buf.log_probs)
     env.close()

@@ -477,13 +477,15 @@ class RolloutCollector:
     def graph_key(self):
         """Everything a captured step bakes in: the env's host-side choices, the split around the collective,
         the buffer, and the policy -- which module, where its parameters and buffers live (the launch reads them in
-        place, so optimiser steps are seen but a replaced tensor is not), whether it explores."""
+        place, so optimiser steps are seen but a replaced tensor is not), whether it explores, and in which type
+        autocast runs it."""
         env_key = self.env.graph_key() if hasattr(self.env, "graph_key") else None
         pol = self.policy
         pol_key = (id(pol), bool(getattr(pol, "deterministic_rollout", False)),
                    tuple(t.data_ptr() for ts in (pol.parameters(), pol.buffers()) for t in ts)
                    if isinstance(pol, nn.Module) else None,
-                   self.memory.data_ptr() if self._recurrent() else None)
+                   self.memory.data_ptr() if self._recurrent() else None,
+                   torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda") else None)
         return (env_key, self._split(), self.buffer.slab.data_ptr(), self.buffer.buffer_size, pol_key,
                 self.capture_collective, self.steps_per_graph, self.defer_final_merge)
 
@@ -563,15 +565,19 @@ class RolloutCollector:
                           "fw_rollout_store")
 
         self._graphs = [torch.cuda.CUDAGraph()]
-        if split:
-            self._graphs.append(torch.cuda.CUDAGraph())
-            with torch.cuda.graph(self._graphs[0]):
-                head()
-            with torch.cuda.graph(self._graphs[1]):
-                tail(None)
-        else:
-            with torch.cuda.graph(self._graphs[0]):
-                tail(head())
+        # autocast's cache holds casts of the weights until its context ends: a captured step has to make its own, or it
+        # would read freed memory afterwards and never see an optimiser step
+        with torch.autocast("cuda", enabled=torch.is_autocast_enabled("cuda"), dtype=torch.get_autocast_dtype("cuda"),
+                            cache_enabled=False):
+            if split:
+                self._graphs.append(torch.cuda.CUDAGraph())
+                with torch.cuda.graph(self._graphs[0]):
+                    head()
+                with torch.cuda.graph(self._graphs[1]):
+                    tail(None)
+            else:
+                with torch.cuda.graph(self._graphs[0]):
+                    tail(head())
         self._key = self.graph_key()
 
     def _collect_graphed(self, n):
