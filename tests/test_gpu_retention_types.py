@@ -56,3 +56,19 @@ def test_a_step_captured_under_autocast(dtype):
     _same(values, buf.values)
     _same(log_probs, buf.log_probs)
     env.close()
+
+
+@pytest.mark.parametrize("graph", [False, True])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_collection_and_update_in_one_autocast(dtype, graph):
+    """The collection's casts of the weights carry no gradient; the update makes its own."""
+    env, policy, buf, col = _setup(64, 20)
+    with torch.autocast("cuda", dtype=dtype):
+        col.collect()
+        col.collect(graph=graph)
+        values, _, _ = _replay(policy, buf, col.rollout_memory)
+    _same16(values, buf.values, dtype)
+    values.float().sum().backward()
+    for p in (policy.embed.weight, policy.qkv.weight, policy.mix.weight, policy.value_net.weight):
+        assert bool(p.grad.any()) and bool(p.grad.isfinite().all())
+    env.close()

@@ -400,16 +400,24 @@ class RolloutCollector:
         step reads the policy's parameters in place, so optimiser steps between collections are seen; it
         is recaptured when a host-side choice it baked in changes (``graph_key``: VecNormalize training /
         norm flags, the engine's lanes and configuration, the buffer)."""
-        buf, env = self.buffer, self.env
+        buf = self.buffer
         n = n_rollout_steps or buf.buffer_size
         if self.last_obs is None:
-            self.last_obs = env.reset()
+            self.last_obs = self.env.reset()
         if self._recurrent():
             if self.memory is None:
                 self.memory = self.policy.new_memory(buf.n_envs)
             self.rollout_memory = self.memory.clone()
-        if graph and self._graph_ok():
-            return self._collect_graphed(n)
+        try:
+            if graph and self._graph_ok():
+                return self._collect_graphed(n)
+            return self._collect_eager(n)
+        finally:
+            if torch.is_autocast_enabled("cuda"):  # casts without a gradient, which an update in the same context would use
+                torch.clear_autocast_cache()
+
+    def _collect_eager(self, n):
+        buf, env = self.buffer, self.env
         buf.reset()
         fused = self._fused(buf.observations[0])
         noise = self._draw_noise(n) if fused else None
