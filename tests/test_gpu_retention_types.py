@@ -72,3 +72,22 @@ def test_collection_and_update_in_one_autocast(dtype, graph):
     for p in (policy.embed.weight, policy.qkv.weight, policy.mix.weight, policy.value_net.weight):
         assert bool(p.grad.any()) and bool(p.grad.isfinite().all())
     env.close()
+
+
+@pytest.mark.parametrize("graph", [False, True])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_a_policy_cast_to_16_bits(dtype, graph):
+    env, policy, buf, col = _setup(64, 20)
+    decay = policy.log_decay.clone()
+    assert policy.to(dtype) is policy
+    assert torch.equal(policy.log_decay, decay) and policy.embed.weight.dtype == dtype
+    assert "log_decay" in policy.state_dict()
+    col.collect()
+    col.collect(graph=graph)
+    assert col.memory.dtype == torch.float32
+    values, _, _ = _replay(policy, buf, col.rollout_memory)
+    _same16(values, buf.values, dtype)
+    values.float().sum().backward()
+    for p in (policy.embed.weight, policy.qkv.weight, policy.mix.weight, policy.value_net.weight):
+        assert bool(p.grad.any()) and bool(p.grad.isfinite().all())
+    env.close()

@@ -279,7 +279,8 @@ class RetentionActorCritic(nn.Module):
     environment (``forward``, with ``sequence.linear_attention_step``); an update runs it over whole columns of the
     rollout, all of them or some (``evaluate_actions``, with ``sequence.linear_attention``), from the memory the
     collection began with (``RolloutCollector.rollout_memory``) and with the buffer's episode starts
-    (``RolloutBuffer.dones``)."""
+    (``RolloutBuffer.dones``).  It runs in float32, under ``torch.autocast``, or cast to a 16-bit type; its memory and its
+    decays are float32 in each."""
 
     recurrent = True
     deterministic_rollout = False  # forward() without exploration noise (actions = mean)
@@ -301,13 +302,22 @@ class RetentionActorCritic(nn.Module):
         tau = lo * (hi / lo) ** (torch.arange(heads) / max(1, heads - 1))
         self.register_buffer("log_decay", (-1.0 / tau).float())
 
+    def _apply(self, fn, recurse=True):
+        """``bfloat16()``, ``half()`` and ``to(dtype)`` cast the parameters; the decays stay float32, which the operators
+        ask for (1 - g of a long memory is less than a 16-bit step)."""
+        decay = self.log_decay
+        super()._apply(fn, recurse)
+        if self.log_decay.dtype in (torch.bfloat16, torch.float16):
+            self.log_decay = decay.to(self.log_decay.device)
+        return self
+
     def new_memory(self, n_envs):
         """An empty memory, [n_envs][heads][D][D] float32."""
         return torch.zeros(n_envs, self.heads, self.head_dim, self.head_dim, dtype=torch.float32,
                            device=self.log_decay.device)
 
     def _project(self, obs):
-        x = torch.tanh(self.embed(obs))
+        x = torch.tanh(self.embed(obs.to(self.embed.weight.dtype)))
         q, k, v = self.qkv(x).unflatten(-1, (3, self.heads, self.head_dim)).unbind(-3)
         return x, q * self.head_dim ** -0.5, k, v
 
