@@ -1,4 +1,4 @@
-"""GPU: the policy with a memory whose constants are replaced, and in 16 bits.
+"""GPU: the policy with a memory whose constants are replaced, in 16 bits, and in a collector that starts over.
 
 Tolerance of the 16-bit runs: a chain of about ten roundings to the type, half a step each, on values of size up to about 10,
 a norm between them: 30 steps relative to the largest value."""
@@ -90,4 +90,19 @@ def test_a_policy_cast_to_16_bits(dtype, graph):
     values.float().sum().backward()
     for p in (policy.embed.weight, policy.qkv.weight, policy.mix.weight, policy.value_net.weight):
         assert bool(p.grad.any()) and bool(p.grad.isfinite().all())
+    env.close()
+
+
+def test_a_collector_started_over_has_no_memory():
+    """last_obs = None resets the environments with the next collection: what they remembered goes with their episodes."""
+    env, policy, buf, col = _setup(16, 8)
+    col.collect()
+    assert bool(col.memory.any())
+    at = col.memory.data_ptr()
+    col.last_obs = None
+    col.collect()
+    assert not bool(col.rollout_memory.any()) and col.memory.data_ptr() == at
+    with torch.no_grad():
+        values, _, _ = _replay(policy, buf, None)
+    _same(values, buf.values)
     env.close()

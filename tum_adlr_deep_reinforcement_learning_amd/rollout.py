@@ -376,7 +376,8 @@ class RolloutCollector:
     value / log-prob.  No host synchronisation inside the loop.
 
     A ``recurrent`` policy (``RetentionActorCritic``) is also given the environments' ``memory``, which it advances, and
-    the episode starts, eager and captured; ``rollout_memory`` is a copy of the memory before the first stored row."""
+    the episode starts, eager and captured; ``rollout_memory`` is a copy of the memory before the first stored row.
+    ``last_obs`` set to None lets the next collection begin with a reset of the environments, and an empty memory."""
 
     def __init__(self, env, policy, buffer):
         self.env, self.policy, self.buffer = env, policy, buffer
@@ -414,6 +415,8 @@ class RolloutCollector:
         n = n_rollout_steps or buf.buffer_size
         if self.last_obs is None:
             self.last_obs = self.env.reset()
+            if self._recurrent() and self.memory is not None:  # its episodes have ended with the reset
+                self.memory.zero_()
         if self._recurrent():
             if self.memory is None:
                 self.memory = self.policy.new_memory(buf.n_envs)
