@@ -198,7 +198,9 @@ __device__ __forceinline__ void store_state(const f32x4 (&S)[KT][VT], const Stat
 // Each active lane copies 16 bytes (or 1) from base + off to its own place behind `lds`: lane x 16 (x 4) bytes.  base and
 // lds are the same on all lanes.  There is no result to wait for by register: the reader waits on the count of memory
 // operations.  Written as asm because a copy known to the compiler makes it wait for ALL copies before any LDS read; the
-// five wait states are those between a VALU write of the base and its use (the compiler does not look into asm).
+// five wait states are those between a VALU write of the base and its use (the compiler does not look into asm).  m0 is a
+// register that the compiler never keeps anything in from one statement to the next (it warns where one is said to
+// overwrite it), so none is named.
 __device__ __forceinline__ uint64_t uniform(const void* p) {
   const uint64_t x = (uint64_t)p;
   return (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32 |
@@ -226,6 +228,12 @@ __device__ __forceinline__ int here(int x) {
 
 typedef u32x4 __attribute__((aligned(4))) u32x4_any4;
 typedef u32x4 __attribute__((aligned(2))) u32x4_any2;
+
+// x is computed here, not later: without it the compiler puts off a block's sums until registers run out
+template <bool ON>
+__device__ __forceinline__ void pin(f32x4& x) {
+  if (ON) asm volatile("" : "+v"(x));
+}
 
 // ROWS rows of 16 NT columns in LDS, as 16-byte chunks; chunk c of a row is stored at c ^ turn(row), so that the 16
 // lanes that are served together meet in no bank: 16 rows of one chunk, or (TRANSPOSED) 4 rows of 4 half chunks
@@ -379,6 +387,7 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, KT * VT <= 16 ? 2 : 1) void k_scan
   using K = typename R::K;
   using V = typename R::V;
   constexpr int NB = MODE == ANY ? 1 : R::NB;
+  constexpr bool LATE = MODE == ANY && KT == 8 && VT == 2;  // no registers to hold the next block's rows beside this one's
   __shared__ alignas(16) char smem[SCAN_WAVES][NB * R::BYTES];
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
   char* const ring = smem[__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)];
@@ -553,7 +562,7 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, KT * VT <= 16 ? 2 : 1) void k_scan
     const int64_t t2 = rev ? L - asked - c2 : asked;
     if constexpr (MODE == ANY) {
       held = false;
-      if (more) hold(t2, c2);
+      if (!LATE && more) hold(t2, c2);
     } else {
       if (more) {
         fetch_k(lq, t2, c2);
@@ -658,7 +667,11 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, KT * VT <= 16 ? 2 : 1) void k_scan
       for (int f = 0; f < VT; f++)
 #pragma unroll
         for (int i = 0; i < 4; i++) S[a][f][i] = decay(S[a][f][i], D[f][i]);
+#pragma unroll
+      for (int f = 0; f < VT; f++) pin<KT * VT <= 16>(S[a][f]);
     }
+    if constexpr (LATE)
+      if (more) hold(t2, c2);
     done += c;
     if (single) single--;
   }
@@ -1031,7 +1044,7 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, 2) void k_scan16(ScanArgs A) {
           for (int i = 0; i < 4; i++) S[a][f][i] = decay(S[a][f][i], D[f][i]);
       }
     } else {
-      constexpr int AT = KT < 4 ? KT : 4;  // tiles at a time
+      constexpr int AT = KT < 2 ? KT : 2;  // tiles at a time
 #pragma unroll
       for (int f = 0; f < VT; f++) {
         weigh(vf[f], t);
@@ -1046,6 +1059,8 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, 2) void k_scan16(ScanArgs A) {
           for (int a = 0; a < AT; a++)
 #pragma unroll
             for (int i = 0; i < 4; i++) S[a0 + a][f][i] = decay(S[a0 + a][f][i], D[a][i]);
+#pragma unroll
+          for (int a = 0; a < AT; a++) pin<true>(S[a0 + a][f]);
         }
       }
     }
