@@ -100,3 +100,9 @@ def test_activations_in_float32(act):
     else:
         size = torch.ones_like(z)
     _held(slope, dwant, 2.0 ** -20 * size + 100 * 2.0 ** -126)
+
+
+@pytest.mark.parametrize("groups", [2.5, "2", float("nan")])
+def test_groups_are_a_whole_number(groups):
+    with pytest.raises(ValueError):
+        _seq().group_norm_act(torch.zeros(4, 8, device=DEV), groups)

@@ -380,6 +380,8 @@ def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, activation="
     if x.dtype not in _DT:
         raise ValueError("group_norm_act: x must be float32, bfloat16 or float16")
     C, groups = x.shape[-1], int(num_groups)
+    if groups != num_groups:
+        raise ValueError("group_norm_act: num_groups must be a whole number")
     if groups < 1 or C < 1 or C % groups:
         raise ValueError("group_norm_act: %d channels do not form %d groups" % (C, groups))
     if activation not in _ACT:
