@@ -1216,8 +1216,19 @@ __global__ __launch_bounds__(256) void k_token(TokenArgs A, int nv, int rows, in
 #pragma unroll
           for (int x = 0; x < 4; x++) vv[b][x] = to_f32(v[b][c + x]);
         }
-        decay[b].set(finite_decay(ld[b]), 1.f);
       }
+    if (d0 == first) {  // the pairs' decays, one per lane, at the price of one
+      float x = ld[0];
+#pragma unroll
+      for (int b = 1; b < B; b++) x = lane % B == b ? ld[b] : x;
+      Decay mine;
+      mine.set(finite_decay(x), 1.f);
+#pragma unroll
+      for (int b = 0; b < B; b++) {
+        decay[b].keep = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(mine.keep), b));
+        decay[b].by = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(mine.by), b));
+      }
+    }
 #pragma unroll
     for (int b = 0; b < B; b++)
 #pragma unroll
