@@ -34,6 +34,18 @@ def test_a_step_on_a_saved_state_is_seen(out):
     torch.autograd.grad(y, q, d["dout"])
 
 
+def test_a_state_out_that_requires_a_gradient_is_refused():
+    """What autograd knows of such a tensor would not be what it holds."""
+    d = _dev(_case(1, 2, 2, 16, 16, torch.float32))
+    leaf = torch.zeros_like(d["state"]).requires_grad_()
+    for out in (leaf, leaf * 2):
+        with pytest.raises(ValueError, match="no gradient"):
+            _step(d, d["state"], state_out=out)
+    with torch.no_grad():
+        _step(d, d["state"], state_out=leaf)
+    assert bool(leaf.detach().any())
+
+
 def test_steps_in_inference_mode():
     d = _dev(_case(1, 2, 2, 16, 16, torch.float32))
     want = _step(d, d["state"].clone())

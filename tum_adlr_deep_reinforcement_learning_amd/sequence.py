@@ -260,14 +260,14 @@ def linear_attention_step(q, k, v, log_decay, state, episode_starts=None, state_
 
     ``state`` (float32 [N, H, Dk, Dv], contiguous) is read once and the new state written once, in place or into
     ``state_out``, which must not overlap it otherwise; autograd sees it as written in place.  A row with
-    episode_starts [N] set begins from zeros.  Has no gradient (the training form is ``linear_attention``): inputs that
+    episode_starts [N] set begins from zeros.  Has no gradient (the training form is ``linear_attention``): tensors that
     require one are refused outside ``torch.no_grad()``."""
     who = "linear_attention_step"
     _heads(who, q, k, v, 3)
     N, H, Dk = q.shape
     dev = q.device
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or
-                                    (isinstance(state, torch.Tensor) and state.requires_grad)):
+                                    any(isinstance(t, torch.Tensor) and t.requires_grad for t in (state, state_out))):
         raise ValueError("%s has no gradient: use linear_attention, or torch.no_grad()" % who)
     log_decay = _decay(who, log_decay, H, dev)
     starts = _starts(who, episode_starts, (N,), dev)
