@@ -267,7 +267,8 @@ def linear_attention_step(q, k, v, log_decay, state, episode_starts=None, state_
     N, H, Dk = q.shape
     dev = q.device
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or
-                                    any(isinstance(t, torch.Tensor) and t.requires_grad for t in (state, state_out))):
+                                    getattr(state, "requires_grad", False) or
+                                    getattr(state_out, "requires_grad", False)):
         raise ValueError("%s has no gradient: use linear_attention, or torch.no_grad()" % who)
     log_decay = _decay(who, log_decay, H, dev)
     starts = _starts(who, episode_starts, (N,), dev)
