@@ -3,11 +3,11 @@
 // A unit is one sample's group: L rows of cg = C / G adjacent channels, read as vectors of VW channels.  The kernels, by a unit's size:
 //   k_gn_wave   a unit fits 64 lanes x 4 vectors: 2^k lanes per unit, several units per wave; for one row per sample
 //               (a policy's features) this is a plain stream over the tensor (524288 x 64 float32 in 4 groups, tanh:
-//               forward 46 us, 5800 GB/s; backward 82 us, 4900 GB/s)
+//               forward 52 us, 5100 GB/s; backward 86 us, 4700 GB/s)
 //   k_gn_block  a unit fits a block's registers: read once, written once (16 x 4096 x 512 bfloat16 in 32 groups, silu:
-//               38 us, 3500 GB/s; all blocks run at once, so loading, sums and storing follow each other)
+//               39 us, 3500 GB/s; all blocks run at once, so loading, sums and storing follow each other)
 //   k_gn_bundle several neighbouring units do, where one has too few channels for 16-byte accesses (64 x 900 x 320
-//               bfloat16 in 32 groups, gelu: forward 41 us, 1800 GB/s, backward 62 us)
+//               bfloat16 in 32 groups, gelu: forward 44 us, 1700 GB/s, backward 67 us)
 //   k_gn_stream_*  larger: two passes over the tensor
 // All statistics are sums of deviations from a mean, so a large mean does not cancel.  Memory bound: x in, y out (and
 // dy in, dx out); the gradients of weight and bias are column sums of per-unit partial sums, in a fixed order.
@@ -272,8 +272,8 @@ __device__ __forceinline__ void block_sum(float* v, float (*lds)[NV]) {  // ever
 }
 
 // Per channel (VW of a column, thread = row * cols + column, `rows` rows): the sums of NA values over its rows, in a fixed
-// order, each handed to sink(channel, sums) by one thread.  Many rows: a wave per channel; few: a thread.  (Against a tree
-// over the rows with a barrier a step: map of 64 x 900 x 320 bfloat16, forward 48 -> 41 us.)
+// order, each handed to sink(channel, sums) by one thread.  Many rows: a wave per channel; few: a thread.  (A tree over
+// the rows with a barrier a step takes 7 us more: map of 64 x 900 x 320 bfloat16, forward.)
 template <int VW, int NA, typename Sink>
 __device__ __forceinline__ void channel_sums(const float (&v)[NA][VW], int t, int rows, int cols, bool on, float* lds, Sink sink) {
   const int threads = (int)blockDim.x, lane = t & 63;
@@ -318,7 +318,8 @@ __device__ __forceinline__ int64_t xcd_unit(int64_t b, int64_t total) {
 
 // ------------------------------------------------------------------ units held by one block
 // A thread holds up to `hold` vectors; with 8 channels a vector the backward kernel needs 6 x (4 + 4 + 8) registers and
-// as much for the channels' constants and sums, which 768 threads have and 1024 do not.
+// as much for the channels' constants and sums: a few more than the 168 that 768 threads have (it spills 40 bytes a lane, the
+// bundles' 80), and far more than the 128 of 1024.
 constexpr int max_threads(bool bwd, int vw) { return bwd && vw == 8 ? 768 : 1024; }
 constexpr int max_hold(bool bwd, int vw) { return vw == 8 ? (bwd ? 6 : 8) : bwd ? 8 : 16; }
 

@@ -54,8 +54,9 @@ struct ScanArgs {
   float* factor;
 };
 
-// What one wave works on: unit = ((n H + h) n_slice + slice) n_pass + pass of segment blockIdx.y, so that the waves of a block share
-// rows (slices and passes the same ones, heads neighbouring ones).
+// What one wave works on: unit = ((n H + h) n_slice + slice) n_pass + pass of segment blockIdx.y, so that the waves of a block
+// want the same rows (slices and passes) or neighbouring ones (heads).  They are not in step, and little of that meets in the
+// caches: the three backward passes over 2048 x 16 ragged x 16 heads of 64 x 64 bfloat16 read 386 MB, of 427 without any of it.
 struct Unit {
   int pass, slice, h, seg;  // seg in processing order
   int64_t n, seg0, seg1, L;  // the segment's tokens [seg0, seg1), of which the first L are live
@@ -363,9 +364,9 @@ __device__ __forceinline__ f32x4 mma(float a, float b, f32x4 c) {
 //
 // float32 runs here because its products have to be float32; float16 because its states leave its range.  A wave owns a
 // sequence rather than a block of tokens because the recurrence then never leaves its registers.  Small heads are bound
-// by memory: 2048 tokens x 512 x 4 heads of 16 x 16, 287 us, 3750 GB/s (403 us with the loads by way of registers, none
+// by memory: 2048 tokens x 512 x 4 heads of 16 x 16, 285 us, 3790 GB/s (403 us with the loads by way of registers, none
 // ahead).  Larger ones are bound by the products, which a padded head wastes: 500 x 250 x 4 heads of 20 x 40 in tiles of
-// 32 x 32 and two slices, 88 us, of which 39 % of the products count.
+// 32 x 32 and two slices, 96 us, of which 39 % of the products count.
 template <typename T, int KT, int VT>
 struct Ring {
   using K = Tile<T, KT, 16>;
@@ -703,10 +704,11 @@ __global__ __launch_bounds__(64 * SCAN_WAVES, KT * VT <= 16 ? 2 : 1) void k_scan
 // two, terms that cancel leave 2^-16 of their size, and more outputs fall to the neighbouring bfloat16.
 //
 // 32 tokens a block: the depth of the product, and half as many splits of the state per token as 16.  Measured at 16
-// heads of 128 x 128 over 16384 tokens: 88 us of outputs after 57 us of segment states (on the float32 products 460 us in
-// all).  In the 88 us the matrix units are busy for 30 % of the time and issue 3.3 million products beside 22 million
-// vector instructions, the splits and weights; two waves a SIMD hide what they wait for only in part.  Three (the outputs
-// in the values' room), the copies given out between the products, and splits by dot products were no faster.
+// heads of 128 x 128 over 16384 tokens: 108 us of outputs after 63 us of segment states (88 and 57 with two terms and the
+// products added to the state one by one; on the float32 products 460 us in all).  In the 108 us the matrix units are busy for
+// 30 % of the time and issue 4.0 million products beside 33 million vector instructions, the splits and weights; two waves a
+// SIMD hide what they wait for only in part.  Three (the outputs in the values' room), the copies given out between the
+// products, and splits by dot products were no faster.
 __device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
@@ -1323,9 +1325,10 @@ int slices(int dtype, int Dk, int Dv, int most) {
 
 // Time segments: with few waves the card is not full, so the time axis is cut, at the price of reading k and v twice and
 // of a state per segment.  SEG_WAVES is two waves per SIMD; the backward pass runs three passes at once and wants fewer.
-// Two segments cost more than they bring unless all their waves have a SIMD each (measured, us; 1000 waves of 500 tokens:
-// 1 segment 111 forward and 250 backward, 2 segments 125 and 291; 400 waves of 512, backward: 1 segment 75, 2: 102, 4: 111;
-// 256 waves of 2048: forward 4 segments 109, 8: 104, backward 4 segments 213, 8: 251).
+// Two segments cost more than they bring unless all their waves have a SIMD each (measured, us; 1000 waves of 500 tokens, 20 x
+// 40 float32: 1 segment 108 forward and 243 backward, 2 segments 132 and 279; 400 waves of 512, 32 x 32 float32, backward: 1
+// segment 84, 2: 104, 4: 106; 256 waves of 2048, 64 x 64 bfloat16: forward 4 segments 120, 8: 111, backward 4 segments 224,
+// 8: 242).
 constexpr int SEG_WAVES = 2048;
 constexpr int SEG_MIN = 128;  // tokens
 struct Plan {
@@ -1403,8 +1406,9 @@ int launch_scan(ScanArgs A, int kt, int vt, hipStream_t s) {
 // Passes of equal tiles and slices go in one launch.
 // Where there is one segment, a wave takes fewer value columns as long as each wave has a SIMD to itself (two waves a SIMD
 // with two tiles of float32 products, which are further from the memory's rate): its blocks are shorter and the scores
-// are computed once more per slice.  100 tokens of 4 heads of 64 x 64 bfloat16, one tile against four: 11 against 17 us;
-// 500 x 250 x 4 heads of 20 x 40 float32, two against four: 88 against 102; one against two at 1680 waves: 112 against 100.
+// are computed once more per slice.  100 tokens of 4 heads of 64 x 64 bfloat16, one tile against four: 12 against
+// 19 us; 500 x 250 x 4 heads of 20 x 40 float32, two against four: 96 against 107; 500 x 420 x 4 heads of 20 x 20 float32, one
+// (3360 waves) against two: 133 against 97.
 int launch_passes(int dtype, ScanArgs A, const Pass* pass, int n_pass, hipStream_t s) {
   for (int i = 0; i < n_pass; i += A.n_pass) {
     const int kt = tiles(pass[i].Dk);
