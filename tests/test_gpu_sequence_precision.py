@@ -173,3 +173,34 @@ def test_bad_numbers_over_time_segments(bad, what, start, dtype):
         wrong = g.cpu().isfinite() != r.isfinite()
         assert not bool(wrong.any()), "%s: %d of %d, first at %s" % (name, int(wrong.sum()), wrong.numel(),
                                                                      wrong.nonzero()[0].tolist())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("Dk,Dv,T", [(20, 40, 75), (24, 72, 75), (63, 63, 75), (101, 97, 75), (127, 20, 75), (3, 5, 75),
+                                     (128, 120, 75), (63, 63, 600), (101, 97, 600), (24, 72, 600)])
+@pytest.mark.parametrize("what", ["state", "q", "k", "v", "dout", "dfinal"])
+def test_bad_numbers_in_heads_of_any_size(what, Dk, Dv, T, dtype):
+    """Heads that do not fill their tiles, rows that are no whole vectors, the last key and value column: as the oracle."""
+    from oracle import sequence_oracle as R
+    gen = torch.Generator().manual_seed(4)
+    rn = lambda *s: torch.randn(*s, generator=gen)
+    c = dict(q=rn(T, 1, 2, Dk).to(dtype), k=rn(T, 1, 2, Dk).to(dtype), v=rn(T, 1, 2, Dv).to(dtype), state=rn(1, 2, Dk, Dv),
+             dout=rn(T, 1, 2, Dv).to(dtype), dfinal=rn(1, 2, Dk, Dv))
+    if what in ("state", "dfinal"):
+        c[what][0, 1, -1, -1] = float("inf")
+        c[what][0, 0, 0, -2] = float("nan")
+    else:
+        c[what][T // 2, 0, 1, -1] = float("inf")
+        c[what][T // 2 + 3, 0, 0, 0] = float("nan")
+    ld = torch.tensor([-0.3, -0.01])
+    starts = torch.zeros(T, 1, dtype=torch.uint8)
+    starts[T // 4] = starts[3 * T // 4] = 1
+    d = {n: x.to(DEV) for n, x in c.items()}
+    leaves = [d[n].requires_grad_() for n in ("q", "k", "v", "state")]
+    out, final = _seq().linear_attention(*leaves[:3], ld.to(DEV), leaves[3], starts.to(DEV))
+    got = (out, final) + torch.autograd.grad([out, final], leaves, [d["dout"], d["dfinal"]])
+    ref = R.linear_attention(c["q"], c["k"], c["v"], ld, c["state"], starts, None, c["dout"], c["dfinal"])
+    for name, g, r in zip(("out", "final", "dq", "dk", "dv", "dstate"), got, ref):
+        wrong = g.cpu().isfinite() != r.isfinite()
+        assert not bool(wrong.any()), "%s: %d of %d, first at %s" % (name, int(wrong.sum()), wrong.numel(),
+                                                                     wrong.nonzero()[0].tolist())
